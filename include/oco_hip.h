@@ -297,6 +297,38 @@ int oco_add_norm_mx_split(void *x, const void *y, const float *norm_w, void *out
 int oco_matmul_mx_split(const void *w, const void *split, uint64_t split_bytes, void *y, oco_dtype y_dtype,
                         const float *bias, const oco_matrix *p, oco_stream stream);
 
+/* ---- 8-bit floating point rows and products --------------------------------- */
+
+/* No counterpart in the reference, whose 8-bit formats are integers with
+ * 32-column blocks: the products of checkpoints that store e4m3 weights (OCP
+ * 8-bit floating point) with an f32 scale per block of 128 x 128.
+ *
+ * Rows to e4m3 with an f32 scale per 128 columns: scale = max|x| / 448, code =
+ * e4m3(448 x / max|x|) to nearest even, the quotient rounded to f32 first
+ * (exact on borders between codes for 16-bit x).  Blocks whose maximum is
+ * under 448 * 2^-126 take scale 2^-126 (codes of an all-zero block are 0); a
+ * block with a NaN or an infinity has a NaN scale and NaN codes, so every
+ * product of that row is NaN.
+ *   x: rows of k values of x_dtype, x_stride elements apart (0: k)
+ *   codes: [rows, k] bytes, 16-byte aligned, k % 16 == 0
+ *   scales: f32 [ceil(k / 128)][rows] -- by block, then row */
+int oco_fp8_quantize(const void *x, oco_dtype x_dtype, uint32_t rows, uint32_t k, uint64_t x_stride, uint8_t *codes,
+                     float *scales, oco_stream stream);
+
+/* Y[m, n] = X[m, k] W^T (+ bf16(bias)) of e4m3 operands with f32
+ * accumulation: the exact products of a block of 128 columns are summed on the
+ * matrix cores and enter the f32 sum times both scales.
+ *   w: [n, k] bytes, 16-byte aligned; w_scales: f32 [ceil(n / 128)][ceil(k / 128)]
+ *   codes, scales: rows as oco_fp8_quantize or oco_block_norm writes them
+ *   p: k (a multiple of 16), n, m, has_bias (0 or 1); dense only
+ *   y: f32, bf16 or f16; workspace: oco_fp8_matmul_workspace(p) bytes, 16-byte
+ *      aligned (NULL if that is 0); calls sharing one must be ordered on one
+ *      stream, two captured graphs that share one included. */
+uint64_t oco_fp8_matmul_workspace(const oco_matrix *p);
+int oco_fp8_matmul(const uint8_t *w, const float *w_scales, const uint8_t *codes, const float *scales, void *y,
+                   oco_dtype y_dtype, const float *bias, const oco_matrix *p, void *workspace, uint64_t workspace_bytes,
+                   oco_stream stream);
+
 /* ---- routing ------------------------------------------------------------ */
 
 /* Per token: top-k of `experts` logits (ties to the lowest index, non-finite
@@ -314,6 +346,41 @@ int oco_route_select(const float *logits, uint32_t tokens, uint32_t experts, uin
 int oco_router(const void *x, oco_dtype x_dtype, const float *w, const float *bias,
                uint32_t tokens, uint32_t hidden, uint32_t experts, uint32_t k, float *logits,
                uint32_t *ids, float *probs, oco_stream stream);
+
+/* Experts chosen by scores (the sigmoid form is the reference's Nemotron-H
+ * router, shaders/nemotron.metal:148-212; bias, groups and the softmax over
+ * all experts have no counterpart there).  Per token, with s the softmax or
+ * the sigmoid of its logits and c = s + bias:
+ *   - with groups > 1, only the groups_kept groups of the highest rank take
+ *     part (experts / groups consecutive experts each); a group's rank is its
+ *     largest c or the sum of its two largest;
+ *   - the k largest c are chosen, in that order; ties, of experts and of
+ *     groups, go to the lowest index.  c is formed in 64 bits; without a bias
+ *     the order is that of the logits;
+ *   - weight = scale * s, divided by the sum of the chosen s if renormalize
+ *     (0 where that sum is 0).
+ * A logit of -Inf is an expert that is not available: its score is 0, it
+ * ranks behind every other (whatever its bias), and it is chosen, with weight
+ * 0, only where fewer than k others are left.  A NaN or +Inf logit makes the
+ * token's weights NaN (its own expert ranks as not available).  A NaN bias
+ * ranks its expert behind the others too.
+ *   logits: [tokens, experts] of dtype; bias: f32 [experts] or NULL
+ *   ids: u32 [tokens, k]; weights: f32 [tokens, k], as oco_experts_apply
+ *   takes them (there k <= 8). */
+typedef enum oco_score { OCO_SCORE_SOFTMAX = 0, OCO_SCORE_SIGMOID = 1 } oco_score;
+typedef enum oco_group_rank { OCO_GROUP_MAX = 0, OCO_GROUP_TOP2 = 1 } oco_group_rank;
+#define OCO_ROUTING_EXPERTS 1024u
+#define OCO_ROUTING_K 32u
+typedef struct oco_routing {
+    uint32_t experts, k;
+    uint32_t score;               /* oco_score */
+    uint32_t groups, groups_kept; /* groups 0 or 1: no limit; at most 64, experts % groups == 0 */
+    uint32_t group_rank;          /* oco_group_rank */
+    uint32_t renormalize;
+    float scale;
+} oco_routing;
+int oco_route_scores(const void *logits, oco_dtype dtype, const float *bias, uint32_t tokens, const oco_routing *p,
+                     uint32_t *ids, float *weights, oco_stream stream);
 
 /* Words of a route plan for `routes` routes over `experts` experts
  * (src/weights/gpt_oss.rs:63-74). */
@@ -436,6 +503,32 @@ int oco_norm(const void *x, const float *w, void *y, uint32_t rows, uint32_t n, 
 int oco_add_norm(void *x, const void *y, const float *w, void *out, uint32_t rows, uint32_t n,
                  float epsilon, int full_layer, oco_stream stream);
 
+/* The step between two blocks of a layer, in one pass (the reference has
+ * add_norm, elementwise.metal:32-58, without the norm after the block, the
+ * gate and the scale): per row
+ *   v     = y / sqrt(mean(y^2) + epsilon) * (post_w + weight_offset), or y without post_w
+ *   x_out = x + scale * g * v, rounded to x_dtype; g = 1, gate, sigmoid(gate) or tanh(gate)
+ *   out   = x_out / sqrt(mean(x_out^2) + epsilon) * (pre_w + weight_offset), of the rounded x_out
+ * in f32.  pre_w comes with `out`, with `codes` and `scales`, or with all
+ * three; without it only x_out is written.  codes / scales: the rows of
+ * oco_fp8_quantize, of the f32 values that `out` rounds (n % 16 == 0).
+ *   x, x_out: rows of x_dtype, x_stride elements apart (x_out may be x)
+ *   y, out: rows of dtype (out may be y where their strides agree)
+ *   gate: rows of dtype; gate_rows consecutive rows share one (0: all rows do)
+ *   post_w, pre_w: f32 [n] or NULL
+ * x_dtype is F32, or equal to dtype.  Strides of 0 mean n. */
+typedef enum oco_gate { OCO_GATE_NONE = 0, OCO_GATE_LINEAR = 1, OCO_GATE_SIGMOID = 2, OCO_GATE_TANH = 3 } oco_gate;
+typedef struct oco_block {
+    uint32_t rows, n;
+    uint32_t x_dtype, dtype; /* oco_dtype */
+    uint32_t gate;           /* oco_gate */
+    uint32_t gate_rows;
+    uint32_t x_stride, y_stride, gate_stride, out_stride; /* elements */
+    float scale, epsilon, weight_offset;
+} oco_block;
+int oco_block_norm(const void *x, const void *y, void *x_out, const void *gate, const float *post_w, const float *pre_w,
+                   void *out, uint8_t *codes, float *scales, const oco_block *p, oco_stream stream);
+
 /* oco_matvec whose bf16 input rows are RMS-normalised on the way in (the
  * norm fused into the matvec's activation staging): the result equals
  * oco_norm followed by oco_matvec with bf16 x, bit for bit, without the
@@ -474,6 +567,47 @@ int oco_argmax_f32(const float *logits, uint32_t n, uint32_t *out, oco_stream st
 uint64_t oco_argmax_workspace(uint32_t n);
 int oco_argmax_f32_ws(const float *logits, uint32_t n, uint32_t *out, void *workspace,
                       uint64_t workspace_bytes, oco_stream stream);
+
+/* Verification of drafted tokens from given random numbers (no counterpart in
+ * the reference, which decodes greedily token by token).  A sequence has
+ * L = lengths[s] drafted tokens (NULL, or more than drafts: drafts), L + 1 rows of the target
+ * and, unless draft is NULL, L rows of the distributions that its tokens were
+ * drawn from.  With p_i and q_i those distributions and u the sequence's
+ * random numbers in [0, 1):
+ *   - token i is accepted while u[i] q_i(token) < p_i(token) (draft NULL:
+ *     q_i is 1 at the token, as for drafts looked up in the prompt);
+ *   - after n accepted ones, one more token is drawn: from max(p_n - q_n, 0)
+ *     if token n was refused (from p_n where that is 0 everywhere), else from
+ *     p_L; it is the first whose running sum in index order passes u[drafts]
+ *     times the whole sum.
+ * Rows hold logits, p = softmax(row / temperature), where -Inf is probability
+ * 0, or probabilities (temperature does not apply to them).  Temperature 0
+ * is greedy: p_i is 1 at the row's first largest value, draft and uniforms
+ * are not read.  Decisions are made in 64 bits.  A row without a
+ * distribution (a NaN or +Inf, or nothing above zero) ends its sequence
+ * there: the token is 0xffffffff and its probability NaN.  A drafted id past
+ * the vocabulary is refused.
+ *   target: [sequences][drafts + 1] rows of vocabulary values, target_stride apart
+ *   draft: [sequences][drafts] rows or NULL; draft_ids: u32 [sequences][drafts]
+ *   uniforms: f32 [sequences][drafts + 1]
+ *   accepted: u32 [sequences], n; tokens: u32 [sequences][drafts + 1]: the n
+ *   accepted tokens, the drawn one, then 0xffffffff
+ *   probabilities: f32 [sequences][drafts + 1] or NULL: p_i(tokens[i]), 0 past them
+ *   workspace: oco_draft_verify_workspace bytes (0 for a description that is
+ *   refused), 16-byte aligned; calls sharing one must be ordered. */
+typedef enum oco_draft_values { OCO_DRAFT_LOGITS = 0, OCO_DRAFT_PROBABILITIES = 1 } oco_draft_values;
+#define OCO_DRAFT_MAX 64u
+typedef struct oco_draft {
+    uint32_t sequences, drafts, vocabulary;  /* drafts: per sequence, at most OCO_DRAFT_MAX */
+    uint32_t target_values, draft_values;    /* oco_draft_values */
+    uint32_t target_dtype, draft_dtype;      /* oco_dtype */
+    float temperature;
+    uint64_t target_stride, draft_stride;    /* row strides in elements, 0: vocabulary */
+} oco_draft;
+uint64_t oco_draft_verify_workspace(const oco_draft *p);
+int oco_draft_verify(const void *target, const void *draft, const uint32_t *draft_ids, const uint32_t *lengths,
+                     const float *uniforms, uint32_t *accepted, uint32_t *tokens, float *probabilities, const oco_draft *p,
+                     void *workspace, uint64_t workspace_bytes, oco_stream stream);
 
 /* ---- GGUF checkpoints and residency (src/gguf.rs) ------------------------- */
 

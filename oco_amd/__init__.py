@@ -67,6 +67,34 @@ class Activation(enum.IntEnum):
     SWIGLU = 1
 
 
+class Gate(enum.IntEnum):
+    """oco_gate."""
+    NONE = 0
+    LINEAR = 1
+    SIGMOID = 2
+    TANH = 3
+
+
+class Score(enum.IntEnum):
+    """oco_score."""
+    SOFTMAX = 0
+    SIGMOID = 1
+
+
+class GroupRank(enum.IntEnum):
+    """oco_group_rank."""
+    MAX = 0
+    TOP2 = 1
+
+
+class DraftValues(enum.IntEnum):
+    """oco_draft_values."""
+    LOGITS = 0
+    PROBABILITIES = 1
+
+
+NO_TOKEN = 0xFFFFFFFF  # oco_draft_verify's places without a token
+
 _BLOCKS = {0: (1, 4), 1: (1, 2), 30: (1, 2), 2: (32, 18), 3: (32, 20), 8: (32, 34),
            12: (256, 144), 13: (256, 176), 14: (256, 210), 39: (32, 17)}
 
@@ -112,6 +140,26 @@ class ExpertsDesc(ctypes.Structure):
                 ("gate", ctypes.c_void_p), ("up", ctypes.c_void_p), ("down", ctypes.c_void_p),
                 ("gate_bias", ctypes.c_void_p), ("up_bias", ctypes.c_void_p),
                 ("down_bias", ctypes.c_void_p)]
+
+
+class Block(ctypes.Structure):
+    """oco_block: the step between two blocks of a layer."""
+    _fields_ = ([(n, ctypes.c_uint32) for n in ("rows", "n", "x_dtype", "dtype", "gate", "gate_rows", "x_stride",
+                                                "y_stride", "gate_stride", "out_stride")] +
+                [(n, ctypes.c_float) for n in ("scale", "epsilon", "weight_offset")])
+
+
+class Routing(ctypes.Structure):
+    """oco_routing: how experts are chosen from their scores."""
+    _fields_ = [(n, ctypes.c_uint32) for n in ("experts", "k", "score", "groups", "groups_kept", "group_rank",
+                                               "renormalize")] + [("scale", ctypes.c_float)]
+
+
+class Draft(ctypes.Structure):
+    """oco_draft: the rows of a verification of drafted tokens."""
+    _fields_ = ([(n, ctypes.c_uint32) for n in ("sequences", "drafts", "vocabulary", "target_values", "draft_values",
+                                                "target_dtype", "draft_dtype")] +
+                [("temperature", ctypes.c_float), ("target_stride", ctypes.c_uint64), ("draft_stride", ctypes.c_uint64)])
 
 
 class GgufEntry(ctypes.Structure):
@@ -166,6 +214,13 @@ SIGNATURES = {
     "oco_norm_mx_split": (_i32, [_vp, _vp, _vp, _u32, _u32, ctypes.c_float, _i32, _vp, _u64, _vp]),
     "oco_add_norm_mx_split": (_i32, [_vp, _vp, _vp, _vp, _u32, _u32, ctypes.c_float, _i32, _vp, _u64, _vp]),
     "oco_matmul_mx_split": (_i32, [_vp, _vp, _u64, _vp, _i32, _vp, _MP, _vp]),
+    "oco_fp8_quantize": (_i32, [_vp, _i32, _u32, _u32, _u64, _vp, _vp, _vp]),
+    "oco_fp8_matmul_workspace": (_u64, [_MP]),
+    "oco_fp8_matmul": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _vp, _MP, _vp, _u64, _vp]),
+    "oco_route_scores": (_i32, [_vp, _i32, _vp, _u32, ctypes.POINTER(Routing), _vp, _vp, _vp]),
+    "oco_block_norm": (_i32, [_vp] * 9 + [ctypes.POINTER(Block), _vp]),
+    "oco_draft_verify_workspace": (_u64, [ctypes.POINTER(Draft)]),
+    "oco_draft_verify": (_i32, [_vp] * 8 + [ctypes.POINTER(Draft), _vp, _u64, _vp]),
     "oco_route_select": (_i32, [_vp, _u32, _u32, _u32, _vp, _vp, _vp]),
     "oco_router": (_i32, [_vp, _i32, _vp, _vp, _u32, _u32, _u32, _u32, _vp, _vp, _vp, _vp]),
     "oco_route_plan_words": (_u64, [_u32, _u32]),
@@ -501,6 +556,50 @@ def matmul_mx_split(w, split, split_bytes: int, y, p: Matrix, y_dtype=DType.F32,
                                               _addr(bias), ctypes.byref(as_matrix(p)), _stream(stream)))
 
 
+def fp8_quantize(x, rows: int, k: int, codes, scales, x_dtype=DType.BF16, x_stride: int = 0, stream=None):
+    """oco_fp8_quantize: rows to e4m3 codes [rows, k] and f32 scales [ceil(k / 128)][rows]."""
+    _check(load_library().oco_fp8_quantize(_addr(x), int(x_dtype), rows, k, x_stride, _addr(codes), _addr(scales),
+                                           _stream(stream)))
+
+
+def fp8_matmul_workspace(p: Matrix) -> int:
+    return int(load_library().oco_fp8_matmul_workspace(ctypes.byref(as_matrix(p))))
+
+
+def fp8_matmul(w, w_scales, codes, scales, y, p: Matrix, y_dtype=DType.F32, bias=None, workspace=None,
+               workspace_bytes: int = 0, stream=None):
+    """oco_fp8_matmul: e4m3 rows times e4m3 weights with a scale per block of 128 x 128."""
+    _check(load_library().oco_fp8_matmul(_addr(w), _addr(w_scales), _addr(codes), _addr(scales), _addr(y), int(y_dtype),
+                                         _addr(bias), ctypes.byref(as_matrix(p)), _addr(workspace), int(workspace_bytes),
+                                         _stream(stream)))
+
+
+def block_norm(x, y, p: Block, x_out=None, gate=None, post_w=None, pre_w=None, out=None, codes=None, scales=None,
+               stream=None):
+    """oco_block_norm: x_out (x itself by default) = x + scale gate norm(y), out = norm(x_out)."""
+    _check(load_library().oco_block_norm(_addr(x), _addr(y), _addr(x if x_out is None else x_out), _addr(gate),
+                                         _addr(post_w), _addr(pre_w), _addr(out), _addr(codes), _addr(scales),
+                                         ctypes.byref(p), _stream(stream)))
+
+
+def route_scores(logits, tokens: int, p: Routing, ids, weights, dtype=DType.F32, bias=None, stream=None):
+    """oco_route_scores: experts by softmax or sigmoid scores, a balance bias and groups."""
+    _check(load_library().oco_route_scores(_addr(logits), int(dtype), _addr(bias), tokens, ctypes.byref(p), _addr(ids),
+                                           _addr(weights), _stream(stream)))
+
+
+def draft_verify_workspace(p: Draft) -> int:
+    return int(load_library().oco_draft_verify_workspace(ctypes.byref(p)))
+
+
+def draft_verify(target, draft, draft_ids, uniforms, accepted, tokens, p: Draft, lengths=None, probabilities=None,
+                 workspace=None, workspace_bytes: int = 0, stream=None):
+    """oco_draft_verify: drafted tokens against the target's distribution, from given random numbers."""
+    _check(load_library().oco_draft_verify(_addr(target), _addr(draft), _addr(draft_ids), _addr(lengths), _addr(uniforms),
+                                           _addr(accepted), _addr(tokens), _addr(probabilities), ctypes.byref(p),
+                                           _addr(workspace), int(workspace_bytes), _stream(stream)))
+
+
 def route_select(logits, tokens: int, experts: int, k: int, ids, probs, stream=None):
     _check(load_library().oco_route_select(_addr(logits), tokens, experts, k, _addr(ids),
                                            _addr(probs), _stream(stream)))
@@ -708,6 +807,26 @@ class Output(DenseMatrix):
     def apply_row(self, x, y, x_dtype=DType.F32, y_dtype=DType.F32, bias=None, rows: int = 1,
                   stream=None):
         super().apply_row(x, y, x_dtype, DType.F32, bias, rows, stream)
+
+
+class Fp8Matrix:
+    """A learned linear map in e4m3 with an f32 scale per block of 128 x 128:
+    the counterpart of DenseMatrix for rows in 8-bit floating point."""
+
+    def __init__(self, values, scales, input: int, output: int):
+        if input % 16:
+            raise ValueError(f"input={input} is not whole groups of 16")
+        self.values, self.scales, self.input, self.output = values, scales, input, output
+        self._workspace = None
+
+    def apply(self, codes, scales, y, rows: int, y_dtype=DType.F32, bias=None, stream=None):
+        """Y = X W^T for rows of oco_fp8_quantize or oco_block_norm."""
+        p = Matrix(self.input, self.output, rows, 0, 1, 1, 1 if bias is not None else 0)
+        need = fp8_matmul_workspace(p)
+        if need and (self._workspace is None or self._workspace.nbytes < need):
+            self._workspace = DeviceBuffer(need)
+        fp8_matmul(self.values, self.scales, codes, scales, y, p, y_dtype, bias, self._workspace if need else None, need,
+                   stream)
 
 
 class ExpertBank:

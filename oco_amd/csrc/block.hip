@@ -1,0 +1,222 @@
+// The step between two blocks of a layer in one pass over its rows: the norm
+// after a block, its gate, its scale, the residual add, the norm before the
+// next block, and that block's input rows in 8-bit floating point.  With v
+// the block's output row y, post-normed where there is a weight for it,
+//
+//     v  = y / sqrt(mean(y^2) + epsilon) * (post_w + offset)
+//     x' = x + scale * g * v,  g = 1, gate, sigmoid(gate) or tanh(gate)
+//     out = x' / sqrt(mean(x'^2) + epsilon) * (pre_w + offset)
+//
+// x' is rounded to the residual's type and the second norm reads the rounded
+// values, as oco_add_norm does.  Everything between is f32.
+//
+// Bound by memory: x, y and the gate are read once, x' and out written once.
+// A row stays in its threads' registers (runs of eight columns per thread,
+// 16-byte accesses for 16-bit types) from its only read to its last write.
+#include "fp8.h"
+#include "rows.h"
+
+namespace oco {
+
+struct BlockArgs {
+    const void *x, *y, *gate;
+    const float *post_w, *pre_w;
+    void *x_out, *out;
+    uint8_t *codes;
+    float *scales;
+    uint32_t rows, n, kind, gate_rows;
+    uint64_t x_stride, y_stride, gate_stride, out_stride;
+    float scale, epsilon, offset;
+};
+
+// The sum over a row's T threads, in every one of them (fixed order).
+template <int T>
+__device__ __forceinline__ float row_sum(float s, float *part) {
+    s = wave_sum(s);
+    if constexpr (T > 64) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+        __syncthreads();
+        s = part[0];
+#pragma unroll
+        for (int w = 1; w < T / 64; w++) s += part[w];
+    }
+    return s;
+}
+
+__device__ __forceinline__ float gate_value(float g, uint32_t kind) {
+    if (kind == OCO_GATE_SIGMOID) return 1.0f / (1.0f + expf(-g));
+    if (kind == OCO_GATE_TANH) return tanhf(g);
+    return g;
+}
+
+// x' of one run of columns (rounded), from the run's v.
+template <class XT, class YT>
+__device__ __forceinline__ void block_add(const BlockArgs &a, const float *xv, float *v, const YT *gate, uint32_t c0, float inv) {
+    float w[8];
+    if (a.post_w) {
+        load_run(a.post_w, c0, a.n, w);
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = v[j] * inv * (w[j] + a.offset);
+    }
+    if (a.kind != OCO_GATE_NONE) {
+        load_run(gate, c0, a.n, w);
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] *= gate_value(w[j], a.kind);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = RowIO<XT>::round(fmaf(a.scale, v[j], xv[j]));
+}
+
+// out (and its 8-bit form) of one run of columns of x'.
+template <class YT>
+__device__ __forceinline__ void block_out(const BlockArgs &a, const float *v, uint64_t row, uint32_t c0, float inv) {
+    float w[8], o[8];
+    load_run(a.pre_w, c0, a.n, w);
+#pragma unroll
+    for (int j = 0; j < 8; j++) o[j] = c0 + j < a.n ? v[j] * inv * (w[j] + a.offset) : 0.f;
+    if (a.out) store_run((YT *)a.out + row * a.out_stride, c0, a.n, o);
+    if (a.codes) {  // 16 consecutive threads hold a block of 128 columns
+        float scale;
+        const uint2 q = fp8_block(o, scale);
+        if (c0 < a.n) {
+            *reinterpret_cast<uint2 *>(a.codes + row * a.n + c0) = q;
+            if (c0 % FP8_BLOCK == 0) a.scales[(uint64_t)(c0 / FP8_BLOCK) * a.rows + row] = scale;
+        }
+    }
+}
+
+// T threads per row (64: four rows per workgroup), P runs of eight columns
+// per thread; P == 0: any n, a row read again for each of its three passes.
+template <class XT, class YT, int T, int P>
+__global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
+    __shared__ float part[2][T / 64];
+    const uint32_t t = T == 64 ? threadIdx.x & 63 : threadIdx.x;
+    const uint64_t row = T == 64 ? blockIdx.x * 4ull + (threadIdx.x >> 6) : blockIdx.x;
+    if (T == 64 && row >= a.rows) return;
+    const XT *x = (const XT *)a.x + row * a.x_stride;
+    const YT *y = (const YT *)a.y + row * a.y_stride;
+    const YT *gate = (const YT *)a.gate + (a.gate_rows ? row / a.gate_rows : 0) * a.gate_stride;
+    XT *x_out = (XT *)a.x_out + row * a.x_stride;
+    if constexpr (P > 0) {
+        float xv[P][8], v[P][8], s = 0.f, inv = 1.f;
+#pragma unroll
+        for (int p = 0; p < P; p++) load_run(y, 8 * (t + T * p), a.n, v[p]);
+#pragma unroll
+        for (int p = 0; p < P; p++) load_run(x, 8 * (t + T * p), a.n, xv[p]);
+        if (a.post_w) {
+#pragma unroll
+            for (int p = 0; p < P; p++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) s = fmaf(v[p][j], v[p][j], s);
+            inv = 1.0f / sqrtf(row_sum<T>(s, part[0]) / (float)a.n + a.epsilon);
+        }
+        s = 0.f;
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            const uint32_t c0 = 8 * (t + T * p);
+            block_add<XT>(a, xv[p], v[p], gate, c0, inv);
+            store_run(x_out, c0, a.n, v[p]);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (c0 + j < a.n) s = fmaf(v[p][j], v[p][j], s);
+        }
+        if (!a.pre_w) return;
+        inv = 1.0f / sqrtf(row_sum<T>(s, part[1]) / (float)a.n + a.epsilon);
+#pragma unroll
+        for (int p = 0; p < P; p++) block_out<YT>(a, v[p], row, 8 * (t + T * p), inv);
+    } else {
+        float xv[8], v[8], s = 0.f, inv = 1.f;
+        if (a.post_w) {
+            for (uint32_t c0 = 8 * t; c0 < a.n; c0 += 8 * T) {
+                load_run(y, c0, a.n, v);
+#pragma unroll
+                for (int j = 0; j < 8; j++) s = fmaf(v[j], v[j], s);
+            }
+            inv = 1.0f / sqrtf(row_sum<T>(s, part[0]) / (float)a.n + a.epsilon);
+        }
+        s = 0.f;
+        for (uint32_t c0 = 8 * t; c0 < a.n; c0 += 8 * T) {
+            load_run(y, c0, a.n, v);
+            load_run(x, c0, a.n, xv);
+            block_add<XT>(a, xv, v, gate, c0, inv);
+            store_run(x_out, c0, a.n, v);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (c0 + j < a.n) s = fmaf(v[j], v[j], s);
+        }
+        if (!a.pre_w) return;
+        inv = 1.0f / sqrtf(row_sum<T>(s, part[1]) / (float)a.n + a.epsilon);
+        // every thread of a block of 128 columns takes part in its maximum
+        for (uint32_t c0 = 8 * t; c0 - c0 % FP8_BLOCK < a.n; c0 += 8 * T) {
+            load_run((const XT *)x_out, c0, a.n, v);  // this thread's own columns
+            block_out<YT>(a, v, row, c0, inv);
+        }
+    }
+}
+
+typedef void (*BlockFn)(BlockArgs);
+
+// Threads per row and runs per thread: the row in registers up to 32768
+// columns; few rows take twice the threads, for latency.
+template <class XT, class YT>
+static BlockFn block_pick(uint32_t n, uint32_t rows, int &threads) {
+    const bool few = rows <= 256;
+#define PICK(T, P) (threads = T, block_kernel<XT, YT, T, P>)
+    if (n <= 512) return PICK(64, 1);
+    if (n <= 1024 && !few) return PICK(64, 2);
+    if (n <= 2048) return PICK(256, 1);
+    if (n <= 4096) return few ? PICK(512, 1) : PICK(256, 2);
+    if (n <= 8192) return few ? PICK(1024, 1) : PICK(512, 2);
+    if (n <= 16384) return PICK(1024, 2);
+    if (n <= 32768) return PICK(1024, 4);
+    return PICK(1024, 0);
+#undef PICK
+}
+
+}  // namespace oco
+
+using namespace oco;
+
+extern "C" int oco_block_norm(const void *x, const void *y, void *x_out, const void *gate, const float *post_w,
+                              const float *pre_w, void *out, uint8_t *codes, float *scales, const oco_block *p,
+                              oco_stream stream) {
+    if (!p) return fail(OCO_ERR_INVALID, "oco_block_norm: null description");
+    if (p->gate > OCO_GATE_TANH) return fail(OCO_ERR_INVALID, "oco_block_norm: gate %u", p->gate);
+    if (p->rows == 0 || p->n == 0) return OCO_OK;
+    if (!x || !y || !x_out) return fail(OCO_ERR_INVALID, "oco_block_norm: null pointer");
+    if (p->gate != OCO_GATE_NONE && !gate) return fail(OCO_ERR_INVALID, "oco_block_norm: a gate kind without gate rows");
+    if (p->rows > 0x7fffffffu || p->n > 0x7fffff00u)
+        return fail(OCO_ERR_INVALID, "oco_block_norm: %u rows of %u", p->rows, p->n);
+    if (!codes != !scales) return fail(OCO_ERR_INVALID, "oco_block_norm: codes and scales come together");
+    if (!pre_w != !(out || codes)) return fail(OCO_ERR_INVALID, "oco_block_norm: the second norm needs its weight and an output");
+    if (codes && (p->n % 16 || ((uintptr_t)codes & 15u)))
+        return fail(OCO_ERR_INVALID, "oco_block_norm: 8-bit rows need n %% 16 == 0 and 16-byte aligned codes (n = %u)", p->n);
+    const uint32_t strides[4] = {p->x_stride, p->y_stride, p->gate_stride, p->out_stride};
+    for (uint32_t s : strides)
+        if (s && s < p->n) return fail(OCO_ERR_INVALID, "oco_block_norm: a row stride of %u under n = %u", s, p->n);
+    BlockArgs a;
+    a.x = x; a.y = y; a.gate = gate;
+    a.post_w = post_w; a.pre_w = pre_w;
+    a.x_out = x_out; a.out = out;
+    a.codes = codes; a.scales = scales;
+    a.rows = p->rows; a.n = p->n;
+    a.kind = p->gate; a.gate_rows = p->gate_rows;
+    a.x_stride = p->x_stride ? p->x_stride : p->n;
+    a.y_stride = p->y_stride ? p->y_stride : p->n;
+    a.gate_stride = p->gate_stride ? p->gate_stride : p->n;
+    a.out_stride = p->out_stride ? p->out_stride : p->n;
+    a.scale = p->scale; a.epsilon = p->epsilon; a.offset = p->weight_offset;
+    int threads = 0;
+    BlockFn fn = nullptr;
+    if (p->x_dtype == OCO_DT_F32 && p->dtype == OCO_DT_F32) fn = block_pick<float, float>(p->n, p->rows, threads);
+    else if (p->x_dtype == OCO_DT_F32 && p->dtype == OCO_DT_BF16) fn = block_pick<float, bf16_t>(p->n, p->rows, threads);
+    else if (p->x_dtype == OCO_DT_F32 && p->dtype == OCO_DT_F16) fn = block_pick<float, f16_t>(p->n, p->rows, threads);
+    else if (p->x_dtype == OCO_DT_BF16 && p->dtype == OCO_DT_BF16) fn = block_pick<bf16_t, bf16_t>(p->n, p->rows, threads);
+    else if (p->x_dtype == OCO_DT_F16 && p->dtype == OCO_DT_F16) fn = block_pick<f16_t, f16_t>(p->n, p->rows, threads);
+    else
+        return fail(OCO_ERR_UNSUPPORTED, "oco_block_norm: residual type %u with rows of type %u (an f32 residual, or both alike)",
+                    p->x_dtype, p->dtype);
+    const uint32_t grid = threads == 64 ? (p->rows + 3) / 4 : p->rows;
+    hipLaunchKernelGGL(fn, dim3(grid), dim3(threads < 256 ? 256 : threads), 0, (hipStream_t)stream, a);
+    return launch_check("oco_block_norm");
+}

@@ -1,0 +1,59 @@
+// Rows in 8-bit floating point (OCP e4m3: four exponent bits, three mantissa
+// bits, largest value 448) with one f32 scale per 128 columns, and their
+// products.
+#pragma once
+#include "common.h"
+
+namespace oco {
+
+constexpr uint32_t FP8_BLOCK = 128;
+constexpr float FP8_FLOOR = 0x1.cp-118f;  // 448 * 2^-126: the least block maximum, so that scales are normal
+
+// Maximum over the 16 lanes of a DPP row, in every lane.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp16(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
+}
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
+    v = max(v, dpp16<0xB1>(v));
+    v = max(v, dpp16<0x4E>(v));
+    v = max(v, dpp16<0x124>(v));
+    return max(v, dpp16<0x128>(v));
+}
+
+// The codes and the scale of a block of 128 columns, eight in each of 16
+// consecutive lanes (all of them active): scale = max|v| / 448, code =
+// e4m3(448 v / max|v|), nearest even.  The quotient is formed as
+// (0.875 v) / (max|v| / 512), whose operands are exact for 16-bit v, and is
+// rounded to f32 once: reciprocal, product, and one residual step, which
+// returns the rounded quotient where the reciprocal is itself rounded
+// correctly (Markstein).  A quotient on the border between two codes thus
+// stays on it.  A block that holds a NaN or an infinity has a NaN scale (its
+// row's products are NaN) and NaN codes.
+// |v| orders by its bits: finite values, then infinity, then NaN.
+__device__ __forceinline__ uint2 fp8_block(const float *v, float &scale) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+    m = row16_max(m);
+    const float top = fmaxf(__uint_as_float(m), FP8_FLOOR);
+    if (m >= 0x7f800000u) {
+        scale = __uint_as_float(0x7fc00000u);
+        return make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+    }
+    scale = top / 448.0f;
+    const float den = top * 0x1p-9f, inv = 1.0f / den;
+    float q[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float num = v[j] * 0.875f, first = num * inv;
+        q[j] = copysignf(fmaf(fmaf(-first, den, num), inv, first), first);  // -0 stays -0
+    }
+    int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
+    int hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], hi, true);
+    return make_uint2((uint32_t)lo, (uint32_t)hi);
+}
+
+}  // namespace oco

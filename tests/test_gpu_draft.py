@@ -1,0 +1,249 @@
+"""oco_draft_verify against the rule in 64 bits: counts and tokens exactly,
+probabilities within an f32 rounding."""
+import numpy as np
+import pytest
+
+from _ops import CODE, dev, stored
+from _util import Guarded, say
+
+pytestmark = pytest.mark.gpu
+NONE = 0xFFFFFFFF
+
+
+def distribution(row, logits, temperature):
+    if temperature == 0:
+        if np.isnan(row).any() or (row == np.inf).any() or not (row > -np.inf).any():
+            return None
+        p = np.zeros_like(row)
+        p[int(np.argmax(row))] = 1
+        return p
+    if not logits:
+        return row
+    if np.isnan(row).any() or (row == np.inf).any() or not (row > -np.inf).any():
+        return None
+    e = np.exp((row - row.max()) / np.float64(np.float32(temperature)))
+    return e / e.sum()
+
+
+def verify(target, draft, ids, lengths, u, t_logits, d_logits, temperature):
+    S, D1, V = target.shape
+    D = D1 - 1
+    accepted, tokens, probs = np.zeros(S, np.int64), np.full((S, D1), NONE, np.int64), np.zeros((S, D1))
+    for s in range(S):
+        L = D if lengths is None else min(int(lengths[s]), D)
+        n, rest, p = 0, None, None
+        while True:
+            p, rest = distribution(target[s, n], t_logits, temperature), None
+            if n == L or p is None:
+                break
+            d = int(ids[s, n])
+            if draft is None or temperature == 0:
+                q = np.zeros(V)
+                if d < V:
+                    q[d] = 1
+            else:
+                q = distribution(draft[s, n], d_logits, temperature)
+            pd, qd = (p[d] if d < V else 0.0), (1.0 if d >= V else np.nan if q is None else q[d])
+            if (0 if temperature == 0 else np.float64(u[s, n])) * qd < pd and (temperature > 0 or pd == 1):
+                tokens[s, n], probs[s, n] = d, pd
+                n += 1
+                continue
+            rest = None if q is None else np.maximum(p - q, 0)
+            if q is None or np.isnan(rest).any():
+                p = None
+            break
+        accepted[s] = n
+        if p is not None:
+            rest = np.maximum(p, 0) if rest is None or rest.sum() <= 0 else rest
+            sums = np.cumsum(rest)
+            if not (sums[-1] > 0 and np.isfinite(sums[-1])):
+                p = None
+        if p is None:
+            probs[s, n] = np.nan
+            continue
+        passed = np.nonzero((sums > (0 if temperature == 0 else np.float64(u[s, D])) * sums[-1]) & (rest > 0))[0]
+        token = int(passed[0]) if len(passed) else int(np.nonzero(rest > 0)[0][-1])
+        tokens[s, n], probs[s, n] = token, p[token]
+    return accepted, tokens, probs
+
+
+def run(lib, target, draft, ids, lengths, u, t_logits=True, d_logits=True, temperature=1.0, t_dtype="f32", d_dtype="f32", pad=(0, 0), stream=None,
+        want_probs=True):
+    """target [S, D+1, V], draft [S, D, V] or None as f64; the library's (accepted, tokens, probabilities) and the rule's."""
+    S, D1, V = target.shape
+    say("draft_verify", S, D1 - 1, V, t_logits, d_logits, temperature, t_dtype, d_dtype, draft is not None, lengths is not None)
+    grown = [np.concatenate([a, np.full(a.shape[:2] + (x,), 77.0)], 2) if a is not None else None for a, x in ((target, pad[0]), (draft, pad[1]))]
+    tb, tv = stored(grown[0], t_dtype)
+    db, dv = stored(grown[1], d_dtype) if draft is not None else (None, None)
+    p = lib.Draft(sequences=S, drafts=D1 - 1, vocabulary=V, target_values=0 if t_logits else 1, draft_values=0 if d_logits else 1,
+                  target_dtype=CODE[t_dtype], draft_dtype=CODE[d_dtype], temperature=temperature, target_stride=V + pad[0] if pad[0] else 0,
+                  draft_stride=V + pad[1] if pad[1] else 0)
+    need = lib.draft_verify_workspace(p)
+    work, acc, tok, prob = Guarded(lib, need), Guarded(lib, S * 4), Guarded(lib, S * D1 * 4), Guarded(lib, S * D1 * 4)
+    u, ids = np.asarray(u, np.float32), np.asarray(ids)
+    hold = [dev(lib, tb), dev(lib, db) if db is not None and db.size else None, dev(lib, np.asarray(ids, np.uint32)) if D1 > 1 else None, dev(lib, u),
+            dev(lib, np.asarray(lengths, np.uint32)) if lengths is not None else None]
+    lib.draft_verify(hold[0], hold[1], hold[2], hold[3], acc.ptr, tok.ptr, p, lengths=hold[4], probabilities=prob.ptr if want_probs else None,
+                     workspace=work.ptr, workspace_bytes=need, stream=stream)
+    lib.synchronize(stream)
+    work.read(np.uint8)
+    got = acc.read(np.uint32).astype(np.int64), tok.read(np.uint32).astype(np.int64).reshape(S, D1), prob.read(np.float32).reshape(S, D1)
+    want = verify(tv[:, :, :V], dv[:, :, :V] if draft is not None else None, ids, lengths, u, t_logits, d_logits, temperature)
+    np.testing.assert_array_equal(got[0], want[0])
+    np.testing.assert_array_equal(got[1], want[1])
+    if want_probs:
+        np.testing.assert_allclose(got[2], want[2], rtol=2.0 ** -23, atol=2.0 ** -140)
+    return got
+
+
+def sample(rng, S, D, V, noise=0.7, sharp=3.0):
+    target = rng.normal(size=(S, D + 1, V)) * sharp
+    draft = target[:, :D] + rng.normal(size=(S, D, V)) * noise
+    ids = (draft + rng.gumbel(size=draft.shape)).argmax(2) if D else np.zeros((S, 0), np.int64)
+    return target, draft, ids, rng.random((S, D + 1))
+
+
+def softmax(z):
+    e = np.exp(z - z.max(2, keepdims=True))
+    return e / e.sum(2, keepdims=True)
+
+
+@pytest.mark.parametrize("V", [1, 2, 7, 100, 4095, 4096, 4097, 8200, 32001])
+@pytest.mark.parametrize("S,D", [(1, 1), (3, 4), (2, 0)])
+def test_vocabularies(lib, S, D, V):
+    rng = np.random.default_rng(V + D)
+    t, d, ids, u = sample(rng, S, D, V)
+    run(lib, t, d, ids, None, u)
+    run(lib, t, None, ids, None, u, temperature=0.8)
+    run(lib, t, d, ids, None, u, temperature=0.0)
+    run(lib, softmax(t), softmax(d) if D else d, ids, None, u, False, False)
+
+
+@pytest.mark.parametrize("t_dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("d_dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("t_logits,d_logits", [(True, True), (True, False), (False, False), (False, True)])
+def test_types_and_kinds(lib, t_dtype, d_dtype, t_logits, d_logits):
+    rng = np.random.default_rng(11)
+    t, d, ids, u = sample(rng, 5, 3, 5000)
+    run(lib, t if t_logits else softmax(t), d if d_logits else softmax(d), ids, [3, 0, 2, 1, 900], u, t_logits, d_logits, 1.0, t_dtype, d_dtype, pad=(3, 5))
+
+
+@pytest.mark.parametrize("temperature", [0.01, 0.3, 1.0, 7.5])
+def test_temperatures(lib, temperature):
+    rng = np.random.default_rng(int(temperature * 100))
+    t, d, ids, u = sample(rng, 6, 5, 9000)
+    got = run(lib, t, d, ids, None, u, temperature=temperature)
+    assert got[0].max() > 0 or temperature < 1
+
+
+def test_accepts_everything_where_the_drafter_is_the_target(lib):
+    rng = np.random.default_rng(1)
+    t, _, ids, u = sample(rng, 4, 64, 300)
+    got = run(lib, t, t[:, :64], ids, None, u)
+    assert np.all(got[0] == 64) and np.all(got[1] != NONE)
+
+
+def test_refused_with_nothing_left_draws_from_the_target(lib):
+    """p == q as probabilities, but a drafted id of probability 0: refused,
+    max(p - q, 0) is 0 everywhere, and the token comes from p."""
+    p = np.zeros((1, 2, 10))
+    p[:, :, 3], p[:, :, 7] = 0.25, 0.75
+    for u, token in ((0.1, 3), (0.24, 3), (0.26, 7), (0.9999999, 7)):
+        got = run(lib, p, p[:, :1], [[5]], None, [[0.0, u]], False, False)
+        assert got[0][0] == 0 and got[1][0, 0] == token and got[1][0, 1] == NONE
+
+
+def test_random_numbers_at_their_ends(lib):
+    """u = 0 takes the first token with any probability, the largest u below
+    1 the last one; acceptance is strict."""
+    last = np.float32(1) - np.float32(2.0 ** -24)
+    p = np.zeros((1, 2, 6000))
+    p[0, :, 100], p[0, :, 5000] = 0.5, 0.5
+    q = np.zeros((1, 1, 6000))
+    q[0, 0, 100] = 1.0
+    for u0, u1, want in ((0.0, 0.0, (1, 100, 100)), (0.5, 0.0, (0, 5000, NONE)), (0.49999997, last, (1, 100, 5000)), (last, last, (0, 5000, NONE))):
+        got = run(lib, p, q, [[100]], None, [[u0, u1]], False, False)
+        assert (got[0][0], got[1][0, 0], got[1][0, 1]) == want
+
+
+def test_masked_tokens_and_ids_past_the_vocabulary(lib):
+    rng = np.random.default_rng(3)
+    t, d, ids, u = sample(rng, 6, 3, 9000)
+    t[:, :, :5000] = -np.inf  # a whole chunk of 4096 and part of the next
+    d[0, :, ::2] = -np.inf
+    ids[1, 0], ids[2, 1], ids[3, 2] = 9000, 0x7FFFFFFF, 100  # past the vocabulary; masked in the target
+    run(lib, t, d, ids, None, u)
+    run(lib, t, None, ids, None, u)
+    run(lib, t, None, ids, None, u, temperature=0.0)
+    t[4] = -np.inf
+    t[4, :, 8999] = -3.0  # one token left
+    run(lib, t, d, ids, None, u)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, None])
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_rows_without_a_distribution_end_their_sequence(lib, bad, temperature):
+    rng = np.random.default_rng(4)
+    t, _, ids, u = sample(rng, 5, 3, 4100)
+    d = t[:, :3].copy()
+    for s, i in ((0, 0), (1, 2), (2, 3)):
+        if bad is None:
+            t[s, i] = -np.inf
+        else:
+            t[s, i, 4099] = bad
+    ids[:, :] = np.where(np.isfinite(d), d, -9e9).argmax(2)
+    got = run(lib, t, d, ids, None, u, temperature=temperature)
+    assert got[1][0, 0] == NONE and np.isnan(got[2][0, 0])
+    if temperature > 0 and bad is not None:
+        d2 = rng.normal(size=d.shape)
+        d2[3, 1, 7] = bad
+        run(lib, t, d2, ids, None, u)
+
+
+def test_greedy_takes_the_first_of_equal_values(lib):
+    t = np.zeros((1, 3, 5000))
+    t[0, 0, [4500, 300]] = 2.0
+    t[0, 1, [10, 11]] = -0.0
+    got = run(lib, t, None, [[300, 0]], None, [[0, 0, 0]], temperature=0.0)
+    assert list(got[1][0]) == [300, 0, 0] and got[0][0] == 2
+    t[0, 0, 200] = 2.0
+    got = run(lib, t, None, [[300, 0]], None, [[0, 0, 0]], temperature=0.0)
+    assert list(got[1][0]) == [200, NONE, NONE] and got[0][0] == 0
+
+
+def test_large_vocabulary_and_batch(lib):
+    rng = np.random.default_rng(5)
+    t, d, ids, u = sample(rng, 3, 2, 151936)
+    run(lib, t, d, ids, [2, 1, 0], u)
+    run(lib, t, d, ids, None, u, temperature=0.5, t_dtype="bf16", want_probs=False)
+    t, d, ids, u = sample(rng, 33, 2, 150)
+    run(lib, t, d, ids, None, u)
+
+
+def test_more_chunks_than_lanes(lib):
+    """A vocabulary of more than 64 chunks of 4096, flat, so that the drawn
+    token lies anywhere."""
+    rng = np.random.default_rng(6)
+    V = 300001
+    t = rng.normal(size=(4, 1, V)) * 0.01
+    got = run(lib, t, np.zeros((4, 0, V)), np.zeros((4, 0), int), None, [[0.0], [0.3], [0.9], [0.9999999]])
+    assert got[1][1, 0] > 64 * 1000 and got[1][2, 0] > 64 * 4096
+
+
+def test_the_result_is_distributed_as_the_target(lib):
+    """Over a grid of random numbers the emitted first token's frequencies
+    are the target's probabilities, whatever the drafter: with G equal steps
+    of u for each of the two draws, each of the V thresholds of either draw
+    shifts a frequency by at most 1 / G."""
+    rng = np.random.default_rng(7)
+    V, G = 6, 40
+    p, q = softmax(rng.normal(size=(1, 1, V)))[0, 0], softmax(rng.normal(size=(1, 1, V)))[0, 0]
+    freq = np.zeros(V)
+    grid = (np.arange(G) + 0.5) / G
+    u = np.stack(np.meshgrid(grid, grid, indexing="ij"), -1).reshape(-1, 2)
+    for d in range(V):  # the drafter proposes d with probability q[d]
+        S = len(u)
+        target = np.broadcast_to(p, (S, 2, V)).copy()
+        got = run(lib, target, np.broadcast_to(q, (S, 1, V)).copy(), np.full((S, 1), d), None, u, False, False)
+        freq += q[d] * np.bincount(got[1][:, 0], minlength=V)[:V] / S
+    assert np.all(np.abs(freq - p) <= 2.0 / G)

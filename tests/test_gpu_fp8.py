@@ -1,0 +1,204 @@
+"""Rows in 8-bit floating point and their products against 64-bit forms."""
+import numpy as np
+import pytest
+
+from _ops import CODE, HALF, LEAST, SIZE, U, dev, e4m3, quantized, stored, values
+from _util import Guarded, say
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,k,pad", [(1, 16, 0), (3, 128, 0), (5, 144, 3), (17, 2880, 0), (2, 4096, 8), (1, 12288, 0)])
+def test_quantize_is_exact(lib, dtype, rows, k, pad):
+    """Codes and scales bit for bit: 16-bit rows by the real quotient, f32
+    rows by the quotient of the two f32 operands."""
+    say("quantize", dtype, rows, k, pad)
+    rng = np.random.default_rng(rows + k)
+    x = rng.normal(size=(rows, k + pad)) * np.where(rng.random(k + pad) < 0.02, 30.0, 1.0)
+    x[0, :8] = [448, 1, 1.0625, 1.1875, 17, 19, 0, -0.0]  # quotients on borders between codes
+    xb, x = stored(x, dtype)
+    codes, scales = Guarded(lib, rows * k), Guarded(lib, -(-k // 128) * rows * 4)
+    lib.fp8_quantize(dev(lib, xb), rows, k, codes.ptr, scales.ptr, CODE[dtype], k + pad if pad else 0)
+    lib.synchronize()
+    want_codes, want_scales = quantized(x[:, :k], dtype != "f32")
+    np.testing.assert_array_equal(scales.read(np.float32).reshape(-1, rows), want_scales)
+    np.testing.assert_array_equal(codes.read(np.uint8).reshape(rows, k), want_codes)
+
+
+def test_quantize_extremes(lib):
+    """Zeros, subnormal and largest values, and blocks that are not finite."""
+    rows, k = 6, 256
+    x = np.ones((rows, k), np.float32)
+    x[0] = 0
+    x[1, :128] = 2.0 ** -140
+    x[2] = np.float32(3.0e38)
+    x[3, 5] = np.nan
+    x[4, 200] = np.inf
+    x[5, :] = np.float32(2.0 ** -118) * np.arange(k)
+    codes, scales = Guarded(lib, rows * k), Guarded(lib, 2 * rows * 4)
+    lib.fp8_quantize(dev(lib, x), rows, k, codes.ptr, scales.ptr, CODE["f32"])
+    lib.synchronize()
+    s, c = scales.read(np.float32).reshape(2, rows), e4m3(codes.read(np.uint8), (rows, k))
+    assert np.all(s[:, 0] == 2.0 ** -126) and not c[0].any()
+    assert s[0, 1] == 2.0 ** -126 and s[1, 1] == np.float32(1) / np.float32(448)
+    assert np.all(c[2] == 448) and np.all(np.isfinite(s[:, 2]))
+    assert np.isnan(s[0, 3]) and np.all(np.isnan(c[3, :128])) and np.all(c[3, 128:] == 448)
+    assert np.isnan(s[1, 4]) and np.all(np.isnan(c[4, 128:])) and np.all(c[4, :128] == 448)
+    q = x[5].astype(np.float64) / np.repeat(s[:, 5].astype(np.float64), 128)
+    assert np.all(np.abs(c[5] - q) <= np.maximum(np.abs(q) * 2.0 ** -4, 2.0 ** -10) * 1.001)
+
+
+def operands(rng, m, n, k):
+    """Random codes over the whole finite range of e4m3, and scales over several powers of two."""
+    x, w = (rng.integers(0, 256, size=s).astype(np.uint8) for s in ((m, k), (n, k)))
+    for a in (x, w):
+        a[(a & 0x7F) == 0x7F] = 0x38  # NaN codes
+    xs = (2.0 ** rng.uniform(-6, 2, size=(-(-k // 128), m))).astype(np.float32)
+    ws = (2.0 ** rng.uniform(-8, 0, size=(-(-n // 128), -(-k // 128)))).astype(np.float32)
+    return x, w, xs, ws
+
+
+def product(x, w, xs, ws):
+    """(sum, sum of magnitudes) in 64 bits."""
+    (m, k), n = x.shape, w.shape[0]
+    xv, wv = e4m3(x, x.shape), e4m3(w, w.shape)
+    y, mag = np.zeros((m, n)), np.zeros((m, n))
+    for b in range(len(xs)):
+        c = slice(128 * b, 128 * b + 128)
+        s = xs[b].astype(np.float64)[:, None] * ws[np.arange(n) // 128, b].astype(np.float64)
+        y += (xv[:, c] @ wv[:, c].T) * s
+        mag += (np.abs(xv[:, c]) @ np.abs(wv[:, c]).T) * s
+    return y, mag
+
+
+def dropped(x, w, xs, ws):
+    """What the 8-bit matrix instruction may drop: in each group of eight
+    consecutive k, seven products each lose under 2^-13 of the largest one's
+    binade (codes of k, of the same group: |x| |w| at most)."""
+    (m, k), n = x.shape, w.shape[0]
+    xv, wv, out = np.abs(e4m3(x, x.shape)), np.abs(e4m3(w, w.shape)), np.zeros((m, n))
+    for g in range(0, k, 8):
+        s = xs[g // 128].astype(np.float64)[:, None] * ws[np.arange(n) // 128, g // 128].astype(np.float64)
+        most = np.zeros((m, n))
+        for j in range(g, min(g + 8, k)):
+            np.maximum(most, xv[:, j:j + 1] * wv[:, j], out=most)
+        out += 7 * 2.0 ** -13 * most * s
+    return out
+
+
+def check(lib, m, n, k, y_dtype="f32", bias=False, seed=0):
+    say("fp8_matmul", m, n, k, y_dtype, bias)
+    rng = np.random.default_rng(seed + m * 31 + n * 7 + k)
+    x, w, xs, ws = operands(rng, m, n, k)
+    b = rng.normal(size=n).astype(np.float32) if bias else None
+    p = lib.Matrix(k, n, m, 0, 1, 1, 1 if bias else 0)
+    need = lib.fp8_matmul_workspace(p)
+    ws_buf = lib.DeviceBuffer(need) if need else None
+    out = Guarded(lib, m * n * SIZE[y_dtype])
+    bufs = [dev(lib, a) for a in (w, ws, x, xs)]
+    bb = dev(lib, b) if bias else None
+    lib.fp8_matmul(*bufs, out.ptr, p, CODE[y_dtype], bb, ws_buf, need)
+    lib.synchronize()
+    got = values(out.read(np.uint8), y_dtype, (m, n))
+    want, mag = product(x, w, xs, ws)
+    if bias:
+        br = stored(b, "bf16")[1]
+        want, mag = want + br, mag + np.abs(br)
+    # a block's 128 exact products summed in f32 (two half steps each: the
+    # matrix core may truncate), one FMA per block, the K parts, the scales' product and the bias
+    bound = (2 * 128 + len(xs) + 12) * U * mag + HALF[y_dtype] * 1.01 * np.abs(want) + LEAST[y_dtype]
+    if y_dtype != "f32":  # 16-bit outputs may take 8-bit matrix instructions
+        bound = bound + dropped(x, w, xs, ws)
+    if y_dtype == "f16":
+        fits = np.abs(want) < 65000
+        assert fits.any()
+        got, want, bound = got[fits], want[fits], bound[fits]
+    assert np.all(np.abs(got - want) <= bound), float(np.max(np.abs(got - want) / bound))
+    return out.read(np.uint8)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1, 16), (1, 16, 128), (1, 17, 144), (2, 33, 272), (7, 129, 2880), (15, 100, 4096), (16, 31, 112),
+                                   (1, 2880, 4096), (8, 1000, 1024)])
+def test_few_rows(lib, m, n, k):
+    check(lib, m, n, k)
+
+
+@pytest.mark.parametrize("m,n,k", [(17, 40, 144), (31, 257, 1040), (32, 128, 128), (33, 129, 16), (63, 300, 2880), (64, 64, 4096), (65, 500, 400),
+                                   (100, 127, 2064), (127, 256, 128), (129, 511, 640), (200, 1000, 1280), (257, 260, 4096), (300, 700, 96),
+                                   (511, 513, 528), (1030, 255, 272)])
+def test_many_rows(lib, m, n, k):
+    check(lib, m, n, k)
+
+
+@pytest.mark.parametrize("y_dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("m", [1, 40, 130, 600])
+def test_outputs_and_bias(lib, m, y_dtype):
+    """Odd output widths: rows of y that are not 16-byte aligned."""
+    check(lib, m, 333, 272, y_dtype, bias=True)
+    check(lib, m, 336, 272, y_dtype, bias=True)
+
+
+@pytest.mark.parametrize("m", [3, 70, 300])
+def test_same_call_same_bits(lib, m):
+    np.testing.assert_array_equal(check(lib, m, 200, 2880), check(lib, m, 200, 2880))
+
+
+@pytest.mark.parametrize("m,bad", [(9, 4), (9, 0), (150, 149)])
+def test_a_row_that_is_not_finite_stays_alone(lib, m, bad):
+    """A NaN scale makes its row NaN and no other; so do NaN codes."""
+    rng = np.random.default_rng(m)
+    n, k = 144, 400
+    x, w, xs, ws = operands(rng, m, n, k)
+    xs[1, bad] = np.nan
+    x[bad, 130] = 0x7F
+    p = lib.Matrix(k, n, m, 0, 1, 1, 0)
+    need = lib.fp8_matmul_workspace(p)
+    out = Guarded(lib, m * n * 4)
+    lib.fp8_matmul(dev(lib, w), dev(lib, ws), dev(lib, x), dev(lib, xs), out.ptr, p, 0, workspace=lib.DeviceBuffer(max(need, 16)), workspace_bytes=need)
+    lib.synchronize()
+    got = out.read(np.float32).reshape(m, n)
+    assert np.all(np.isnan(got[bad])) and np.all(np.isfinite(got[np.arange(m) != bad]))
+
+
+@pytest.mark.parametrize("m,k", [(1, 144), (20, 144), (140, 144), (300, 272)])
+def test_what_lies_behind_a_row_is_not_read(lib, m, k):
+    """K ends inside a block of 128: NaN codes in the next rows' place (the
+    next weights row, and behind the last rows) do not reach a sum."""
+    rng = np.random.default_rng(k)
+    n = 64
+    x, w, xs, ws = operands(rng, m, n, k)
+    say("fp8 behind", m, k)
+    x[1:], w[1:] = 0x7F, 0x7F  # every row but the first is NaN throughout
+    pad = np.full(4096, 0x7F, np.uint8)
+    p = lib.Matrix(k, n, m, 0, 1, 1, 0)
+    need = lib.fp8_matmul_workspace(p)
+    out = lib.DeviceBuffer(m * n * 4)
+    lib.fp8_matmul(dev(lib, np.concatenate([w.ravel(), pad])), dev(lib, ws), dev(lib, np.concatenate([x.ravel(), pad])), dev(lib, xs), out, p, 0,
+                   workspace=lib.DeviceBuffer(max(need, 16)), workspace_bytes=need)
+    lib.synchronize()
+    got = out.download(np.float32).reshape(m, n)
+    want = product(x[:1], w[:1], xs[:, :1], ws)[0]
+    assert abs(got[0, 0] - want[0, 0]) <= 300 * U * product(x[:1], w[:1], xs[:, :1], ws)[1][0, 0]
+    assert np.all(np.isnan(got[0, 1:])) and np.all(np.isnan(got[1:]))
+
+
+def test_quantized_rows_of_a_matrix(lib):
+    """Fp8Matrix over quantised bf16 rows is near the product of the rows
+    themselves: each value is off by at most 2^-4 of itself or 2^-10 of its
+    block's scale."""
+    rng = np.random.default_rng(8)
+    m, n, k = 37, 96, 1296
+    xb, x = stored(rng.normal(size=(m, k)), "bf16")
+    _, w, _, ws = operands(rng, 1, n, k)
+    codes, scales, y = lib.DeviceBuffer(m * k), lib.DeviceBuffer(-(-k // 128) * m * 4), lib.DeviceBuffer(m * n * 4)
+    lib.fp8_quantize(dev(lib, xb), m, k, codes, scales)
+    lib.Fp8Matrix(dev(lib, w), dev(lib, ws), k, n).apply(codes, scales, y, m)
+    lib.synchronize()
+    c, s = quantized(x, True)
+    want, mag = product(c, w, s, ws)
+    got = y.download(np.float32).reshape(m, n)
+    assert np.all(np.abs(got - want) <= (2 * 128 + 11 + 12) * U * mag)
+    wv = e4m3(w, w.shape) * np.repeat(np.repeat(ws.astype(np.float64), 128, 0), 128, 1)[:n, :k]
+    step = np.maximum(np.abs(x) * 2.0 ** -4, np.repeat(s.T.astype(np.float64), 128, 1)[:, :k] * 2.0 ** -10)
+    assert np.all(np.abs(got - x @ wv.T) <= (step @ np.abs(wv).T) * 1.01)
