@@ -70,12 +70,23 @@ struct Fp8Args {
 __device__ __forceinline__ void fp8_put4(void *y, uint32_t dtype, uint64_t at, const float *v, uint32_t live) {
     if (dtype == OCO_DT_F32) {
         float *p = (float *)y + at;
-        for (uint32_t j = 0; j < 4; j++)
-            if (j < live) p[j] = v[j];
+        if (live >= 4)
+            *reinterpret_cast<u32x4_u *>(p) = u32x4_u{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+        else
+#pragma unroll
+            for (uint32_t j = 0; j < 3; j++)
+                if (j < live) p[j] = v[j];
     } else {
         uint16_t *p = (uint16_t *)y + at;
-        for (uint32_t j = 0; j < 4; j++)
-            if (j < live) p[j] = dtype == OCO_DT_BF16 ? f32_to_bf16_bits(v[j]) : (uint16_t)RowIO<f16_t>::bits(v[j]);
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) h[j] = dtype == OCO_DT_BF16 ? f32_to_bf16_bits(v[j]) : RowIO<f16_t>::bits(v[j]);
+        if (live >= 4)
+            *reinterpret_cast<u32x2_u *>(p) = u32x2_u{h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
+        else
+#pragma unroll
+            for (uint32_t j = 0; j < 3; j++)
+                if (j < live) p[j] = (uint16_t)h[j];
     }
 }
 
@@ -171,6 +182,177 @@ __global__ __launch_bounds__(64 * FP8_WAVES) void fp8_rows_kernel(Fp8Args a) {
     }
 }
 
+// ---- many rows: tiles through LDS ------------------------------------------------------
+//
+// BM activation rows x BN weight rows per workgroup of WM x WN wavefronts.  A
+// stage is one block of K: both operands' 128 bytes per row go from global
+// memory straight to LDS (16 bytes per lane), two stages deep, one barrier
+// per stage.  Row r's 16-byte chunk c lies in slot c ^ (r % 8), so that the
+// fragment reads (16 rows, one chunk each) fall on all banks.
+// HALF: the f16 matrix instruction on converted codes (f32 outputs), else the
+// 8-bit one, whose dropped bits (2^-13 of a group of eight products, at most)
+// lie under the rounding of the 16-bit outputs it is used for.
+
+// 16 bytes per lane from a buffer to LDS at `to` + 16 lane (uniform).
+__device__ __forceinline__ void fp8_to_lds(__amdgpu_buffer_rsrc_t rs, void *to, uint32_t at, uint32_t base) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void *)to, 16, at, base, 0, 0);
+}
+
+struct Fp8TileArgs {
+    Fp8Args p;
+    uint32_t mt, nt, parts;
+    float *sums;  // parts > 1: f32 [part][m][n]
+};
+
+template <int BM, int BN, int WM, int WN, bool HALF>
+__global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8TileArgs ta) {
+    const Fp8Args &a = ta.p;
+    constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
+    constexpr int XL = BM / 8 / WAVES, WL = BN / 8 / WAVES;  // 1 KB loads per wavefront and stage
+    constexpr uint32_t XB = BM * FP8_BLOCK, STAGE = (BM + BN) * FP8_BLOCK;
+    static_assert(XL * 8 * WAVES == BM && WL * 8 * WAVES == BN && FP8_BLOCK % (BN / WN) == 0, "whole loads, one weight scale per wavefront");
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    float *const xs_lds = reinterpret_cast<float *>(lds + 2 * STAGE);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    // tiles in groups of four columns, rows within: neighbours share operands in one L2
+    const uint32_t tiles = ta.mt * ta.nt, lin = xcd_order(blockIdx.x, tiles);
+    const uint32_t per = 4 * ta.mt, g = lin / per, wide = min(4u, ta.nt - 4 * g), in = lin - g * per;
+    const uint32_t m0 = in / wide * BM, n0 = (4 * g + in % wide) * BN;
+    const uint32_t b0 = (uint32_t)((uint64_t)a.blocks * blockIdx.y / ta.parts), b1 = (uint32_t)((uint64_t)a.blocks * (blockIdx.y + 1) / ta.parts);
+
+    const uint32_t xrows = min(a.m - m0, (uint32_t)BM), wrows = min(a.n - n0, (uint32_t)BN);
+    const __amdgpu_buffer_rsrc_t xr = uniform_rsrc(a.x + (uint64_t)m0 * a.k, xrows * a.k);
+    const __amdgpu_buffer_rsrc_t wr = uniform_rsrc(a.w + (uint64_t)n0 * a.k, wrows * a.k);
+    const uint32_t chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+    uint32_t xo[XL], wo[WL];  // rows past the last read the last one (their results are not written)
+#pragma unroll
+    for (int i = 0; i < XL; i++) xo[i] = min((wave * XL + i) * 8 + (lane >> 3), xrows - 1) * a.k + chunk;
+#pragma unroll
+    for (int i = 0; i < WL; i++) wo[i] = min((wave * WL + i) * 8 + (lane >> 3), wrows - 1) * a.k + chunk;
+    const float *xsrc = a.xs + min(m0 + threadIdx.x, a.m - 1);
+    auto fetch = [&](uint32_t b, uint32_t s) {
+        // columns past k: the row's first chunk, cleared before it is read
+        const uint32_t back = FP8_BLOCK * b + chunk < a.k ? 0 : chunk;
+#pragma unroll
+        for (int i = 0; i < XL; i++)
+            fp8_to_lds(xr, lds + s * STAGE + (wave * XL + i) * 1024, xo[i] - back, FP8_BLOCK * b);
+#pragma unroll
+        for (int i = 0; i < WL; i++)
+            fp8_to_lds(wr, lds + s * STAGE + XB + (wave * WL + i) * 1024, wo[i] - back, FP8_BLOCK * b);
+        if (wave < BM / 64)
+            __builtin_amdgcn_global_load_lds((const GLOBAL void *)(xsrc + (uint64_t)b * a.m),
+                                             (__attribute__((address_space(3))) void *)(xs_lds + s * BM + wave * 64), 4, 0, 0);
+    };
+
+    const uint32_t wm = wave / WN * TM * 16, wn = wave % WN * TN * 16;
+    f32x4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int t = 0; t < TN; t++) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float *wsrc = a.ws + (uint64_t)(min(n0 + wn, a.n - 1) / FP8_BLOCK) * a.blocks;
+    const uint32_t lo = (q ^ (r & 7)) * 16, hi = ((4 + q) ^ (r & 7)) * 16;
+    auto frag = [&](const uint8_t *row) {
+        const u32x4 u = *reinterpret_cast<const u32x4 *>(row + lo), v = *reinterpret_cast<const u32x4 *>(row + hi);
+        return i32x8{(int)u.x, (int)u.y, (int)u.z, (int)u.w, (int)v.x, (int)v.y, (int)v.z, (int)v.w};
+    };
+
+    if (b0 < b1) fetch(b0, 0);
+    for (uint32_t b = b0; b < b1; b++) {
+        const uint32_t s = (b - b0) & 1;
+        const float ws = wsrc[b];
+        __syncthreads();  // this stage has arrived; the other buffer is read no more
+        if (FP8_BLOCK * (b + 1) > a.k) {
+            const uint32_t left = (a.k - FP8_BLOCK * b) / 16;
+            for (uint32_t c = threadIdx.x; c < (BM + BN) * 8; c += 64 * WAVES)
+                if (((c & 7) ^ ((c >> 3) & 7)) >= left) *reinterpret_cast<u32x4 *>(lds + s * STAGE + c * 16) = u32x4{0, 0, 0, 0};
+            __syncthreads();
+        }
+        if (b + 1 < b1) fetch(b + 1, s ^ 1);
+        const uint8_t *xt = lds + s * STAGE + (wm + r) * FP8_BLOCK, *wt = lds + s * STAGE + XB + (wn + r) * FP8_BLOCK;
+        if constexpr (HALF) {
+            f16x8 wf[TN][4];
+#pragma unroll
+            for (int t = 0; t < TN; t++) {
+                const HalfBlock h(frag(wt + t * 16 * FP8_BLOCK));
+#pragma unroll
+                for (int u = 0; u < 4; u++) wf[t][u] = h.v[u];
+            }
+#pragma unroll
+            for (int i = 0; i < TM; i++) {
+                const HalfBlock x(frag(xt + i * 16 * FP8_BLOCK));
+                const float f = ws * xs_lds[s * BM + wm + 16 * i + r];
+                f32x4 p[TN];
+#pragma unroll
+                for (int t = 0; t < TN; t++) p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+#pragma unroll
+                    for (int t = 0; t < TN; t++) p[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[t][u], x.v[u], p[t], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < TN; t++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) acc[i][t][v] = fmaf(p[t][v], f, acc[i][t][v]);
+            }
+        } else {
+            i32x8 wf[TN];
+#pragma unroll
+            for (int t = 0; t < TN; t++) wf[t] = frag(wt + t * 16 * FP8_BLOCK);
+#pragma unroll
+            for (int i = 0; i < TM; i++) {
+                const i32x8 x = frag(xt + i * 16 * FP8_BLOCK);
+                const float f = ws * xs_lds[s * BM + wm + 16 * i + r];
+#pragma unroll
+                for (int t = 0; t < TN; t++) {
+                    const f32x4 p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[t], x, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+                    for (int v = 0; v < 4; v++) acc[i][t][v] = fmaf(p[v], f, acc[i][t][v]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+        const uint32_t row = m0 + wm + 16 * i + r;
+        if (row >= a.m) continue;
+#pragma unroll
+        for (int t = 0; t < TN; t++) {
+            const uint32_t col = n0 + wn + 16 * t + 4 * q;
+            if (col >= a.n) continue;
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = acc[i][t][j];
+            if (ta.parts > 1) {
+                fp8_put4(ta.sums, OCO_DT_F32, ((uint64_t)blockIdx.y * a.m + row) * a.n + col, v, a.n - col);
+                continue;
+            }
+            if (a.bias)
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[j] += round_bf16(a.bias[min(col + j, a.n - 1)]);
+            fp8_put4(a.y, a.y_dtype, (uint64_t)row * a.n + col, v, a.n - col);
+        }
+    }
+}
+
+// The K parts' sums, in order.
+__global__ __launch_bounds__(256) void fp8_join_kernel(Fp8TileArgs ta) {
+    const Fp8Args &a = ta.p;
+    const uint64_t size = (uint64_t)a.m * a.n;
+    for (uint64_t at = 4 * ((uint64_t)blockIdx.x * 256 + threadIdx.x); at < size; at += 1024ull * gridDim.x) {
+        float v[4];
+        const uint32_t live = (uint32_t)min(size - at, (uint64_t)4);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            v[j] = 0.f;
+            if (j < (int)live) {
+                for (uint32_t p = 0; p < ta.parts; p++) v[j] += ta.sums[p * size + at + j];
+                if (a.bias) v[j] += round_bf16(a.bias[(at + j) % a.n]);
+            }
+        }
+        fp8_put4(a.y, a.y_dtype, at, v, live);
+    }
+}
+
 }  // namespace oco
 
 using namespace oco;
@@ -203,9 +385,40 @@ extern "C" int oco_fp8_quantize(const void *x, oco_dtype x_dtype, uint32_t rows,
     return launch_check("oco_fp8_quantize");
 }
 
+namespace oco {
+
+// How a product runs: the few-row kernel, or tiles with K in parts.
+struct Fp8Plan {
+    uint32_t bm, bn, mt, nt, parts;  // bm 0: few rows
+};
+constexpr uint32_t FP8_FEW = 32;
+static Fp8Plan fp8_plan(uint32_t m, uint32_t n, uint32_t k) {
+    Fp8Plan p = {0, 0, 0, 0, 1};
+    if (m <= FP8_FEW) return p;
+    const uint32_t blocks = (k + FP8_BLOCK - 1) / FP8_BLOCK;
+    p.bm = p.bn = (uint64_t)((m + 255) / 256) * ((n + 255) / 256) >= 256 ? 256 : 128;
+    p.mt = (m + p.bm - 1) / p.bm;
+    p.nt = (n + p.bn - 1) / p.bn;
+    while (p.bm == 128 && (uint64_t)p.mt * p.nt * p.parts < 256 && p.parts < 8 && blocks / (2 * p.parts) >= 4) p.parts *= 2;
+    return p;
+}
+
+template <int BM, int BN, int WM, int WN, bool HALF>
+static int fp8_tiles(const Fp8TileArgs &a, hipStream_t stream) {
+    const size_t lds = 2 * ((BM + BN) * FP8_BLOCK + BM * 4);
+    auto fn = fp8_tile_kernel<BM, BN, WM, WN, HALF>;
+    if (lds > 64 * 1024)
+        OCO_TRY(hip_check(hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), "hipFuncSetAttribute"));
+    hipLaunchKernelGGL(fn, dim3(a.mt * a.nt, a.parts), dim3(64 * WM * WN), lds, stream, a);
+    return launch_check("oco_fp8_matmul (tiles)");
+}
+
+}  // namespace oco
+
 extern "C" uint64_t oco_fp8_matmul_workspace(const oco_matrix *p) {
-    (void)p;
-    return 0;
+    if (!p || p->m == 0 || p->n == 0 || p->k == 0) return 0;
+    const Fp8Plan plan = fp8_plan(p->m, p->n, p->k);
+    return plan.parts > 1 ? (uint64_t)plan.parts * p->m * p->n * 4 : 0;
 }
 
 extern "C" int oco_fp8_matmul(const uint8_t *w, const float *w_scales, const uint8_t *codes, const float *scales, void *y,
@@ -223,8 +436,12 @@ extern "C" int oco_fp8_matmul(const uint8_t *w, const float *w_scales, const uin
     // 32-bit offsets inside a workgroup's rows
     if (p->k > 0x1000000u || p->n > 0x7fffff00u || p->m > 0x7fffff00u)
         return fail(OCO_ERR_INVALID, "oco_fp8_matmul: %u x %u x %u", p->m, p->n, p->k);
-    (void)workspace;
-    (void)workspace_bytes;
+    const Fp8Plan plan = fp8_plan(p->m, p->n, p->k);
+    const uint64_t need = oco_fp8_matmul_workspace(p);
+    if (need && (!workspace || ((uintptr_t)workspace & 15u) || workspace_bytes < need))
+        return fail(OCO_ERR_INVALID, "oco_fp8_matmul: workspace of %llu bytes, need %llu, 16-byte aligned",
+                    (unsigned long long)workspace_bytes, (unsigned long long)need);
+    if ((uint64_t)plan.mt * plan.nt > 0x7fffffffull) return fail(OCO_ERR_INVALID, "oco_fp8_matmul: %u x %u outputs", p->m, p->n);
     Fp8Args a;
     a.w = w;
     a.x = codes;
@@ -237,11 +454,27 @@ extern "C" int oco_fp8_matmul(const uint8_t *w, const float *w_scales, const uin
     a.k = p->k;
     a.blocks = (p->k + FP8_BLOCK - 1) / FP8_BLOCK;
     a.y_dtype = y_dtype;
-    const dim3 grid((p->n + 31) / 32, (p->m + 31) / 32);
-    if (grid.y > 65535) return fail(OCO_ERR_INVALID, "oco_fp8_matmul: %u rows", p->m);
-    if (p->m <= 16)
-        hipLaunchKernelGGL((fp8_rows_kernel<1, 2>), dim3(grid.x, 1), dim3(64 * FP8_WAVES), 0, (hipStream_t)stream, a);
+    hipStream_t st = (hipStream_t)stream;
+    if (!plan.bm) {
+        auto fn = p->m <= 16 ? fp8_rows_kernel<1, 2> : fp8_rows_kernel<2, 2>;
+        hipLaunchKernelGGL(fn, dim3((p->n + 31) / 32), dim3(64 * FP8_WAVES), 0, st, a);
+        return launch_check("oco_fp8_matmul");
+    }
+    Fp8TileArgs t;
+    t.p = a;
+    t.mt = plan.mt;
+    t.nt = plan.nt;
+    t.parts = plan.parts;
+    t.sums = (float *)workspace;
+    const bool half = y_dtype == OCO_DT_F32;
+    if (plan.bm == 256)
+        OCO_TRY(half ? (fp8_tiles<256, 256, 2, 4, true>(t, st)) : (fp8_tiles<256, 256, 2, 4, false>(t, st)));
     else
-        hipLaunchKernelGGL((fp8_rows_kernel<2, 2>), grid, dim3(64 * FP8_WAVES), 0, (hipStream_t)stream, a);
-    return launch_check("oco_fp8_matmul");
+        OCO_TRY(half ? (fp8_tiles<128, 128, 2, 2, true>(t, st)) : (fp8_tiles<128, 128, 2, 2, false>(t, st)));
+    if (plan.parts > 1) {
+        const uint64_t groups = ((uint64_t)p->m * p->n + 1023) / 1024;
+        hipLaunchKernelGGL(fp8_join_kernel, dim3((uint32_t)(groups < 8192 ? groups : 8192)), dim3(256), 0, st, t);
+        return launch_check("oco_fp8_matmul (join)");
+    }
+    return OCO_OK;
 }
