@@ -187,15 +187,29 @@ __global__ __launch_bounds__(64 * FP8_WAVES) void fp8_rows_kernel(Fp8Args a) {
 // BM activation rows x BN weight rows per workgroup of WM x WN wavefronts.  A
 // stage is one block of K: both operands' 128 bytes per row go from global
 // memory straight to LDS (16 bytes per lane), two stages deep, one barrier
-// per stage.  Row r's 16-byte chunk c lies in slot c ^ (r % 8), so that the
-// fragment reads (16 rows, one chunk each) fall on all banks.
-// HALF: the f16 matrix instruction on converted codes (f32 outputs), else the
-// 8-bit one, whose dropped bits (2^-13 of a group of eight products, at most)
-// lie under the rounding of the 16-bit outputs it is used for.
+// per stage.  HALF: the f16 matrix instruction on converted codes (f32
+// outputs), else the 8-bit one, whose dropped bits (2^-13 of a group of eight
+// products, at most) lie under the rounding of the 16-bit outputs it is used for.
+//
+// Which weight row meets which row of the matrix instruction is free: row j
+// of tile t is weight row 4 TN (j / 4) + 4 t + j % 4 of the wavefront's, so
+// that a lane's results are 4 TN consecutive outputs and its four lane groups
+// write whole lines.
+//
+// LDS: a row's 16-byte chunk c lies in slot c ^ swizzle(row), with a swizzle
+// that takes eight values over the rows that lanes r = 0 .. 7 read (r % 8 for
+// the activations; for the weights' order 4 (row / (4 TN) % 2) + row % 4), so
+// that fragment reads run at 256 bytes a clock.
+//
+// Workgroups stay and take tile after tile: the next tile's first stage is
+// requested before this one's results are written.
 
-// 16 bytes per lane from a buffer to LDS at `to` + 16 lane (uniform).
-__device__ __forceinline__ void fp8_to_lds(__amdgpu_buffer_rsrc_t rs, void *to, uint32_t at, uint32_t base) {
+// 16 (4) bytes per lane from a buffer to LDS at `to` + 16 (4) lane (`to` is uniform).
+__device__ __forceinline__ void to_lds16(__amdgpu_buffer_rsrc_t rs, void *to, uint32_t at, uint32_t base) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void *)to, 16, at, base, 0, 0);
+}
+__device__ __forceinline__ void to_lds4(__amdgpu_buffer_rsrc_t rs, void *to, uint32_t at) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void *)to, 4, at, 0, 0, 0);
 }
 
 struct Fp8TileArgs {
@@ -204,133 +218,206 @@ struct Fp8TileArgs {
     float *sums;  // parts > 1: f32 [part][m][n]
 };
 
+// N consecutive outputs (N a multiple of 4), `live` of them inside the row.
+template <int N>
+__device__ __forceinline__ void fp8_put(void *y, uint32_t dtype, uint64_t at, const float *v, uint32_t live) {
+    if (live >= N && dtype != OCO_DT_F32) {
+        uint32_t h[N / 2];
+        if (dtype == OCO_DT_BF16)
+#pragma unroll
+            for (int j = 0; j < N / 2; j++) h[j] = f32_to_bf16_bits(v[2 * j]) | ((uint32_t)f32_to_bf16_bits(v[2 * j + 1]) << 16);
+        else
+#pragma unroll
+            for (int j = 0; j < N / 2; j++) h[j] = RowIO<f16_t>::bits(v[2 * j]) | (RowIO<f16_t>::bits(v[2 * j + 1]) << 16);
+        uint16_t *p = (uint16_t *)y + at;
+        if constexpr (N % 8 == 0) {
+#pragma unroll
+            for (int j = 0; j < N / 8; j++)
+                *reinterpret_cast<u32x4_u *>(p + 8 * j) = u32x4_u{h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]};
+        } else {
+#pragma unroll
+            for (int j = 0; j < N / 4; j++) *reinterpret_cast<u32x2_u *>(p + 4 * j) = u32x2_u{h[2 * j], h[2 * j + 1]};
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < N; j += 4)
+        if (j < (int)live) fp8_put4(y, dtype, at + j, v + j, live - j);
+}
+
 template <int BM, int BN, int WM, int WN, bool HALF>
 __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8TileArgs ta) {
     const Fp8Args &a = ta.p;
-    constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
+    constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, OUT = 4 * TN;
     constexpr int XL = BM / 8 / WAVES, WL = BN / 8 / WAVES;  // 1 KB loads per wavefront and stage
     constexpr uint32_t XB = BM * FP8_BLOCK, STAGE = (BM + BN) * FP8_BLOCK;
-    static_assert(XL * 8 * WAVES == BM && WL * 8 * WAVES == BN && FP8_BLOCK % (BN / WN) == 0, "whole loads, one weight scale per wavefront");
+    static_assert(XL * 8 * WAVES == BM && WL * 8 * WAVES == BN && FP8_BLOCK % (BN / WN) == 0 && BM <= 64 * WAVES, "whole loads, one weight scale per wavefront");
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     float *const xs_lds = reinterpret_cast<float *>(lds + 2 * STAGE);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-    // tiles in groups of four columns, rows within: neighbours share operands in one L2
-    const uint32_t tiles = ta.mt * ta.nt, lin = xcd_order(blockIdx.x, tiles);
-    const uint32_t per = 4 * ta.mt, g = lin / per, wide = min(4u, ta.nt - 4 * g), in = lin - g * per;
-    const uint32_t m0 = in / wide * BM, n0 = (4 * g + in % wide) * BN;
-    const uint32_t b0 = (uint32_t)((uint64_t)a.blocks * blockIdx.y / ta.parts), b1 = (uint32_t)((uint64_t)a.blocks * (blockIdx.y + 1) / ta.parts);
+    const uint32_t wm = wave / WN * TM * 16, wn = wave % WN * TN * 16;
+    const uint32_t tiles = ta.mt * ta.nt, part = blockIdx.y;
+    const uint32_t b0 = (uint32_t)((uint64_t)a.blocks * part / ta.parts), b1 = (uint32_t)((uint64_t)a.blocks * (part + 1) / ta.parts);
+    // the chunk that lane l fetches into slot l % 8 of row l / 8 of eight (the weights': ^ 4 where row / OUT is odd)
+    const uint32_t xchunk = ((lane & 7) ^ (lane >> 3)) * 16, wchunk = ((lane & 7) ^ (lane >> 3 & 3)) * 16;
 
-    const uint32_t xrows = min(a.m - m0, (uint32_t)BM), wrows = min(a.n - n0, (uint32_t)BN);
-    const __amdgpu_buffer_rsrc_t xr = uniform_rsrc(a.x + (uint64_t)m0 * a.k, xrows * a.k);
-    const __amdgpu_buffer_rsrc_t wr = uniform_rsrc(a.w + (uint64_t)n0 * a.k, wrows * a.k);
-    const uint32_t chunk = ((lane & 7) ^ (lane >> 3)) * 16;
-    uint32_t xo[XL], wo[WL];  // rows past the last read the last one (their results are not written)
+    uint32_t m0, n0;
+    __amdgpu_buffer_rsrc_t xr, wr;
+    uint32_t xo[XL], wo[WL];
+    const float *wsrc;
+    // tiles in groups of four columns, rows within: neighbours share operands in one L2
+    auto enter = [&](uint32_t id) {
+        const uint32_t lin = xcd_order(id, tiles), per = 4 * ta.mt, g = lin / per, wide = min(4u, ta.nt - 4 * g), in = lin - g * per;
+        m0 = in / wide * BM;
+        n0 = (4 * g + in % wide) * BN;
+        const uint32_t xrows = min(a.m - m0, (uint32_t)BM), wrows = min(a.n - n0, (uint32_t)BN);
+        xr = uniform_rsrc(a.x + (uint64_t)m0 * a.k, xrows * a.k);
+        wr = uniform_rsrc(a.w + (uint64_t)n0 * a.k, wrows * a.k);
+        // rows past the last read the last one (their results are not written)
 #pragma unroll
-    for (int i = 0; i < XL; i++) xo[i] = min((wave * XL + i) * 8 + (lane >> 3), xrows - 1) * a.k + chunk;
+        for (int i = 0; i < XL; i++) xo[i] = min((wave * XL + i) * 8 + (lane >> 3), xrows - 1) * a.k;
 #pragma unroll
-    for (int i = 0; i < WL; i++) wo[i] = min((wave * WL + i) * 8 + (lane >> 3), wrows - 1) * a.k + chunk;
-    const float *xsrc = a.xs + min(m0 + threadIdx.x, a.m - 1);
+        for (int i = 0; i < WL; i++) wo[i] = min((wave * WL + i) * 8 + (lane >> 3), wrows - 1) * a.k;
+        wsrc = a.ws + (uint64_t)(min(n0 + wn, a.n - 1) / FP8_BLOCK) * a.blocks;
+    };
     auto fetch = [&](uint32_t b, uint32_t s) {
         // columns past k: the row's first chunk, cleared before it is read
-        const uint32_t back = FP8_BLOCK * b + chunk < a.k ? 0 : chunk;
+        const uint32_t base = FP8_BLOCK * b, xc = base + xchunk < a.k ? xchunk : 0;
+        const uint32_t wc[2] = {base + wchunk < a.k ? wchunk : 0, base + (wchunk ^ 64) < a.k ? wchunk ^ 64 : 0};
 #pragma unroll
-        for (int i = 0; i < XL; i++)
-            fp8_to_lds(xr, lds + s * STAGE + (wave * XL + i) * 1024, xo[i] - back, FP8_BLOCK * b);
+        for (int i = 0; i < XL; i++) to_lds16(xr, lds + s * STAGE + (wave * XL + i) * 1024, xo[i] + xc, base);
 #pragma unroll
         for (int i = 0; i < WL; i++)
-            fp8_to_lds(wr, lds + s * STAGE + XB + (wave * WL + i) * 1024, wo[i] - back, FP8_BLOCK * b);
-        if (wave < BM / 64)
-            __builtin_amdgcn_global_load_lds((const GLOBAL void *)(xsrc + (uint64_t)b * a.m),
-                                             (__attribute__((address_space(3))) void *)(xs_lds + s * BM + wave * 64), 4, 0, 0);
+            to_lds16(wr, lds + s * STAGE + XB + (wave * WL + i) * 1024, wo[i] + wc[(wave * WL + i) * 8 / OUT & 1], base);
+        if (wave < BM / 64) {
+            const uint32_t rows = min(a.m - m0, (uint32_t)BM);
+            to_lds4(uniform_rsrc(a.xs + (uint64_t)b * a.m + m0, rows * 4), xs_lds + s * BM + wave * 64, min(wave * 64 + lane, rows - 1) * 4);
+        }
     };
-
-    const uint32_t wm = wave / WN * TM * 16, wn = wave % WN * TN * 16;
-    f32x4 acc[TM][TN];
-#pragma unroll
-    for (int i = 0; i < TM; i++)
-#pragma unroll
-        for (int t = 0; t < TN; t++) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const float *wsrc = a.ws + (uint64_t)(min(n0 + wn, a.n - 1) / FP8_BLOCK) * a.blocks;
-    const uint32_t lo = (q ^ (r & 7)) * 16, hi = ((4 + q) ^ (r & 7)) * 16;
-    auto frag = [&](const uint8_t *row) {
-        const u32x4 u = *reinterpret_cast<const u32x4 *>(row + lo), v = *reinterpret_cast<const u32x4 *>(row + hi);
+    // fragment addresses: chunks q and 4 + q of the lane's rows
+    const uint32_t xlo = (wm + r) * FP8_BLOCK + (q ^ (r & 7)) * 16, wrow = wn + OUT * (r >> 2) + (r & 3);
+    const uint32_t wlo = XB + wrow * FP8_BLOCK + (q ^ ((r & 3) | (wrow / OUT % 2 * 4))) * 16;
+    auto frag = [&](uint32_t at) {
+        const u32x4 u = *reinterpret_cast<const u32x4 *>(lds + at), v = *reinterpret_cast<const u32x4 *>(lds + (at ^ 64));
         return i32x8{(int)u.x, (int)u.y, (int)u.z, (int)u.w, (int)v.x, (int)v.y, (int)v.z, (int)v.w};
     };
 
+    enter(blockIdx.x);
     if (b0 < b1) fetch(b0, 0);
-    for (uint32_t b = b0; b < b1; b++) {
-        const uint32_t s = (b - b0) & 1;
-        const float ws = wsrc[b];
-        __syncthreads();  // this stage has arrived; the other buffer is read no more
-        if (FP8_BLOCK * (b + 1) > a.k) {
-            const uint32_t left = (a.k - FP8_BLOCK * b) / 16;
-            for (uint32_t c = threadIdx.x; c < (BM + BN) * 8; c += 64 * WAVES)
-                if (((c & 7) ^ ((c >> 3) & 7)) >= left) *reinterpret_cast<u32x4 *>(lds + s * STAGE + c * 16) = u32x4{0, 0, 0, 0};
-            __syncthreads();
-        }
-        if (b + 1 < b1) fetch(b + 1, s ^ 1);
-        const uint8_t *xt = lds + s * STAGE + (wm + r) * FP8_BLOCK, *wt = lds + s * STAGE + XB + (wn + r) * FP8_BLOCK;
-        if constexpr (HALF) {
-            f16x8 wf[TN][4];
+    float ws_next = wsrc[min(b0, a.blocks - 1)];
+    for (uint32_t id = blockIdx.x;;) {
+        f32x4 acc[TM][TN];
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+#pragma unroll
+            for (int t = 0; t < TN; t++) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        f32x4 sum[TN];  // the last step's sums and their scale
+        float fs = 0.f;
+#pragma unroll
+        for (int t = 0; t < TN; t++) sum[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (uint32_t b = b0; b < b1; b++) {
+            const uint32_t s = (b - b0) & 1;
+            const float ws = ws_next;
+            __syncthreads();  // this stage has arrived; the other buffer is read no more
+            if (FP8_BLOCK * (b + 1) > a.k) {
+                const uint32_t left = (a.k - FP8_BLOCK * b) / 16;
+                for (uint32_t c = threadIdx.x; c < (BM + BN) * 8; c += 64 * WAVES) {
+                    const uint32_t row = c >> 3, f = row < BM ? row & 7 : (row & 3) | ((row - BM) / OUT % 2 * 4);
+                    if (((c & 7) ^ f) >= left) *reinterpret_cast<u32x4 *>(lds + s * STAGE + c * 16) = u32x4{0, 0, 0, 0};
+                }
+                __syncthreads();
+            }
+            if (b + 1 < b1) {
+                fetch(b + 1, s ^ 1);
+                ws_next = wsrc[b + 1];
+            }
+            const uint32_t xt = s * STAGE + xlo, wt = s * STAGE + wlo;
+            const float *const xsb = xs_lds + s * BM + wm + r;
+            // Fragments of x are read one step of 16 rows ahead, and a step's sums are added while the next
+            // step is on the matrix core.
+            f16x8 wh[HALF ? TN : 1][4];
+            i32x8 w[HALF ? 1 : TN];
 #pragma unroll
             for (int t = 0; t < TN; t++) {
-                const HalfBlock h(frag(wt + t * 16 * FP8_BLOCK));
+                const i32x8 c = frag(wt + t * 4 * FP8_BLOCK);
+                if constexpr (HALF) {
+                    const HalfBlock h(c);
 #pragma unroll
-                for (int u = 0; u < 4; u++) wf[t][u] = h.v[u];
-            }
-#pragma unroll
-            for (int i = 0; i < TM; i++) {
-                const HalfBlock x(frag(xt + i * 16 * FP8_BLOCK));
-                const float f = ws * xs_lds[s * BM + wm + 16 * i + r];
-                f32x4 p[TN];
-#pragma unroll
-                for (int t = 0; t < TN; t++) p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int u = 0; u < 4; u++)
-#pragma unroll
-                    for (int t = 0; t < TN; t++) p[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[t][u], x.v[u], p[t], 0, 0, 0);
-#pragma unroll
-                for (int t = 0; t < TN; t++)
-#pragma unroll
-                    for (int v = 0; v < 4; v++) acc[i][t][v] = fmaf(p[t][v], f, acc[i][t][v]);
-            }
-        } else {
-            i32x8 wf[TN];
-#pragma unroll
-            for (int t = 0; t < TN; t++) wf[t] = frag(wt + t * 16 * FP8_BLOCK);
-#pragma unroll
-            for (int i = 0; i < TM; i++) {
-                const i32x8 x = frag(xt + i * 16 * FP8_BLOCK);
-                const float f = ws * xs_lds[s * BM + wm + 16 * i + r];
-#pragma unroll
-                for (int t = 0; t < TN; t++) {
-                    const f32x4 p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[t], x, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-#pragma unroll
-                    for (int v = 0; v < 4; v++) acc[i][t][v] = fmaf(p[v], f, acc[i][t][v]);
+                    for (int u = 0; u < 4; u++) wh[t][u] = h.v[u];
+                } else {
+                    w[t] = c;
                 }
             }
-        }
-    }
+            i32x8 x = frag(xt);
+            float f = ws * xsb[0];
 #pragma unroll
-    for (int i = 0; i < TM; i++) {
-        const uint32_t row = m0 + wm + 16 * i + r;
-        if (row >= a.m) continue;
+            for (int i = 0; i < TM; i++) {
+                constexpr int LAST = TM - 1;
+                const int before = i ? i - 1 : LAST;
+                i32x8 xn = x;
+                float fn = f;
+                if (i < LAST) {
+                    xn = frag(xt + (i + 1) * 16 * FP8_BLOCK);
+                    fn = ws * xsb[16 * (i + 1)];
+                }
+                f32x4 p[TN];
+                if constexpr (HALF) {
+                    const HalfBlock h(x);
 #pragma unroll
-        for (int t = 0; t < TN; t++) {
-            const uint32_t col = n0 + wn + 16 * t + 4 * q;
-            if (col >= a.n) continue;
-            float v[4];
+                    for (int t = 0; t < TN; t++) p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = acc[i][t][j];
-            if (ta.parts > 1) {
-                fp8_put4(ta.sums, OCO_DT_F32, ((uint64_t)blockIdx.y * a.m + row) * a.n + col, v, a.n - col);
-                continue;
+                    for (int u = 0; u < 4; u++)
+#pragma unroll
+                        for (int t = 0; t < TN; t++) {
+                            p[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[t][u], h.v[u], p[t], 0, 0, 0);
+                            acc[before][t][u] = fmaf(sum[t][u], fs, acc[before][t][u]);
+                        }
+                } else {
+#pragma unroll
+                    for (int t = 0; t < TN; t++) {
+                        p[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[t], x, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+                        for (int v = 0; v < 4; v++) acc[before][t][v] = fmaf(sum[t][v], fs, acc[before][t][v]);
+                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // a product, four FMAs
+                        __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < TN; t++) sum[t] = p[t];
+                fs = f;
+                x = xn;
+                f = fn;
             }
-            if (a.bias)
-#pragma unroll
-                for (int j = 0; j < 4; j++) v[j] += round_bf16(a.bias[min(col + j, a.n - 1)]);
-            fp8_put4(a.y, a.y_dtype, (uint64_t)row * a.n + col, v, a.n - col);
         }
+#pragma unroll
+        for (int t = 0; t < TN; t++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) acc[TM - 1][t][v] = fmaf(sum[t][v], fs, acc[TM - 1][t][v]);
+        // the next tile's first stage, then this one's results
+        const uint32_t row0 = m0 + wm + r, col = n0 + wn + OUT * q;
+        id += gridDim.x;
+        if (id < tiles) {
+            __syncthreads();
+            enter(id);
+            if (b0 < b1) fetch(b0, 0);
+            ws_next = wsrc[min(b0, a.blocks - 1)];
+        }
+        if (col < a.n) {
+            float bias[OUT];
+#pragma unroll
+            for (int j = 0; j < OUT; j++) bias[j] = a.bias && ta.parts == 1 ? round_bf16(a.bias[min(col + j, a.n - 1)]) : 0.f;
+            void *const y = ta.parts > 1 ? (void *)(ta.sums + (uint64_t)part * a.m * a.n) : a.y;
+            const uint32_t dtype = ta.parts > 1 ? (uint32_t)OCO_DT_F32 : a.y_dtype;
+#pragma unroll
+            for (int i = 0; i < TM; i++) {
+                if (row0 + 16 * i >= a.m) break;
+                float v[OUT];
+#pragma unroll
+                for (int j = 0; j < OUT; j++) v[j] = acc[i][j / 4][j % 4] + bias[j];
+                fp8_put<OUT>(y, dtype, (uint64_t)(row0 + 16 * i) * a.n + col, v, a.n - col);
+            }
+        }
+        if (id >= tiles) break;
     }
 }
 
@@ -409,7 +496,9 @@ static int fp8_tiles(const Fp8TileArgs &a, hipStream_t stream) {
     auto fn = fp8_tile_kernel<BM, BN, WM, WN, HALF>;
     if (lds > 64 * 1024)
         OCO_TRY(hip_check(hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), "hipFuncSetAttribute"));
-    hipLaunchKernelGGL(fn, dim3(a.mt * a.nt, a.parts), dim3(64 * WM * WN), lds, stream, a);
+    // workgroups that fill the card once (256 compute units, one or two each by their LDS), the same number for each XCD
+    const uint32_t tiles = a.mt * a.nt, most = lds > 80 * 1024 ? 256 : 512;
+    hipLaunchKernelGGL(fn, dim3(tiles < most ? tiles : most, a.parts), dim3(64 * WM * WN), lds, stream, a);
     return launch_check("oco_fp8_matmul (tiles)");
 }
 
