@@ -583,10 +583,11 @@ int oco_argmax_f32_ws(const float *logits, uint32_t n, uint32_t *out, void *work
  * Rows hold logits, p = softmax(row / temperature), where -Inf is probability
  * 0, or probabilities (temperature does not apply to them).  Temperature 0
  * is greedy: p_i is 1 at the row's first largest value, draft and uniforms
- * are not read.  Decisions are made in 64 bits.  A row without a
- * distribution (a NaN or +Inf, or nothing above zero) ends its sequence
- * there: the token is 0xffffffff and its probability NaN.  A drafted id past
- * the vocabulary is refused.
+ * are not read.  Decisions are made in 64 bits, on rows' sums of f32
+ * exponentials (relative error about 1e-8).  A row without a distribution (a
+ * NaN or +Inf, or nothing above zero) ends its sequence there: the token is
+ * 0xffffffff and its probability NaN.  A drafted id past the vocabulary is
+ * refused.
  *   target: [sequences][drafts + 1] rows of vocabulary values, target_stride apart
  *   draft: [sequences][drafts] rows or NULL; draft_ids: u32 [sequences][drafts]
  *   uniforms: f32 [sequences][drafts + 1]

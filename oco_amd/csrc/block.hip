@@ -32,7 +32,8 @@ struct BlockArgs {
 // The sum over a row's T threads, in every one of them (fixed order).
 template <int T>
 __device__ __forceinline__ float row_sum(float s, float *part) {
-    s = wave_sum(s);
+    s = wave_sum(s);  // one lane's of it: the order of the additions differs between lanes
+    if constexpr (T == 64) s = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(s)));
     if constexpr (T > 64) {
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
         __syncthreads();

@@ -10,9 +10,11 @@
 // drawn from the target one at a time.  Temperature 0 is greedy: p_i is all
 // on the row's largest value (lowest index), and no random number is used.
 //
-// Every decision is made on 64-bit exponentials and sums (relative error
-// about 1e-11), so that it follows from the inputs and not from the order of
-// the sums.
+// A decision must follow from the inputs and not from the order of sums or
+// the rounding of exp: the two rows that a token is drawn from are 64-bit
+// exponentials (7e-12) and 64-bit running sums.  The rows' normalising sums
+// are f32 exponentials added in 64 bits: their error, some 1e-8, shifts a
+// whole row alike, and so a decision only where u is within that of its border.
 //
 // Bound by reading the rows once where they are logits: each chunk of each
 // row gives its maximum and its sum of exponentials; the decisions follow
@@ -79,8 +81,7 @@ __device__ void draft_part(const T *row, uint32_t chunk, const DraftArgs &a, Dra
         bad |= !(v[j] < INFINITY);
         m = fmaxf(m, v[j]);
     }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    m = wave_max_f32(m);
     if (lane == 0) smax[wave] = m;
     __syncthreads();
     m = fmaxf(fmaxf(smax[0], smax[1]), fmaxf(smax[2], smax[3]));
@@ -90,13 +91,21 @@ __device__ void draft_part(const T *row, uint32_t chunk, const DraftArgs &a, Dra
 #pragma unroll
         for (int j = DRAFT_RUN - 1; j >= 0; j--)
             if (v[j] == m) at = chunk * DRAFT_CHUNK + 2048 * (j / 8) + 8 * threadIdx.x + j % 8;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) at = min(at, (uint32_t)__shfl_xor((int)at, o));
+        at = wave_min_u32(at);
         s = bad ? __builtin_nan("") : 0.0;
     } else {
+        // c in two parts: its rounding would shift every term of a row the same way
+        const float c = (float)a.c, rest = (float)(a.c - (double)c);
 #pragma unroll
-        for (int j = 0; j < (int)DRAFT_RUN; j++) s += v[j] > -INFINITY ? exp2_f64<9>(((double)v[j] - (double)m) * a.c) : 0.0;
-        if (bad) s = __builtin_nan("");
+        for (int j = 0; j < (int)DRAFT_RUN; j++) {
+            const float d = fmaxf(v[j] - m, -1e30f);  // -Inf: an exponential of 0, without -Inf * rest
+            v[j] = __builtin_amdgcn_exp2f(fmaf(d, rest, d * c));
+        }
+#pragma unroll
+        for (int w = DRAFT_RUN / 2; w; w /= 2)
+#pragma unroll
+            for (int j = 0; j < w; j++) v[j] += v[j + w];
+        s = bad ? __builtin_nan("") : m > -INFINITY ? (double)v[0] : 0.0;  // a chunk of -Inf alone has sum 0
     }
     s = wave_sum_f64(s);
     if (lane == 0) {
@@ -134,29 +143,33 @@ struct DraftRow {
     double inv;  // 1 / sum of exp((v - max) / T); NaN for a row without a distribution
     uint32_t at;
 };
-// A row from its parts, by one wavefront.
-__device__ __forceinline__ DraftRow draft_row(const DraftPart *parts, const DraftArgs &a) {
+// A row from its parts, by one wavefront; `first`: the lane's part of the first 64.
+__device__ __forceinline__ DraftRow draft_row(const DraftPart *parts, const DraftPart &first, const DraftArgs &a) {
     const uint32_t lane = threadIdx.x & 63;
-    float m = -INFINITY;
-    for (uint32_t i = lane; i < a.chunks; i += 64) m = fmaxf(m, parts[i].max);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-    double s = 0.0;
-    uint32_t at = DRAFT_NONE;
-    for (uint32_t i = lane; i < a.chunks; i += 64) {
+    float m = first.max;
+    for (uint32_t i = 64 + lane; i < a.chunks; i += 64) m = fmaxf(m, parts[i].max);
+    m = wave_max_f32(m);
+    // a NaN or +Inf in the row stays a NaN sum
+    auto scaled = [&](const DraftPart &p) { return p.sum * (p.max > -INFINITY ? exp2_f64<9>(((double)p.max - (double)m) * a.c) : 1.0); };
+    double s = scaled(first);
+    uint32_t at = first.max == m ? first.at : DRAFT_NONE;
+    for (uint32_t i = 64 + lane; i < a.chunks; i += 64) {
         const DraftPart p = parts[i];
         if (p.max == m) at = min(at, p.at);
-        // a chunk of -Inf alone has sum 0, and a NaN or +Inf stays NaN
-        s += p.sum * (p.max > -INFINITY ? exp2_f64<12>(((double)p.max - (double)m) * a.c) : 1.0);
+        s += scaled(p);
     }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) at = min(at, (uint32_t)__shfl_xor((int)at, o));
     s = wave_sum_f64(s);
     DraftRow r;
     r.max = m;
     r.inv = m > -INFINITY ? 1.0 / s : __builtin_nan("");
-    r.at = at;
+    r.at = wave_min_u32(at);
     return r;
+}
+__device__ __forceinline__ DraftPart draft_first(const DraftPart *parts, const DraftArgs &a) {
+    const uint32_t lane = threadIdx.x & 63;
+    DraftPart p = {-INFINITY, DRAFT_NONE, 0.0};
+    if (lane < a.chunks) p = parts[lane];
+    return p;
 }
 
 __device__ __forceinline__ double draft_value(float v, bool logits, float max, double inv, double c) {
@@ -183,7 +196,7 @@ __global__ __launch_bounds__(256) void draft_greedy_kernel(DraftArgs a) {
     const uint32_t s = blockIdx.x, wave = threadIdx.x >> 6, length = draft_length(a, s);
     const DraftRows<float, float> rows{a, s};
     for (uint32_t i = wave; i <= length; i += 4) {
-        const DraftRow r = draft_row(rows.target_parts(i), a);
+        const DraftRow r = draft_row(rows.target_parts(i), draft_first(rows.target_parts(i), a), a);
         if ((threadIdx.x & 63) == 0) best[i] = r.inv == r.inv ? r.at : DRAFT_NONE;
     }
     __syncthreads();
@@ -210,22 +223,45 @@ __global__ __launch_bounds__(256) void draft_rest_kernel(DraftArgs a) {
     const uint32_t s = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const uint32_t length = draft_length(a, s);
     const DraftRows<TT, TD> rows{a, s};
-    for (uint32_t i = wave; i <= length; i += 4) {
-        DraftRow p = {0.f, 1.0, 0}, q = {0.f, 1.0, 0};
-        if (a.target_logits) p = draft_row(rows.target_parts(i), a);
-        if (i < length && a.draft && a.draft_logits) q = draft_row(rows.draft_parts(i), a);
-        if (lane == 0) {
-            prow[i] = p;
-            qrow[i] = q;
+    const bool with_q = a.draft && a.draft_logits;
+    constexpr int AT_ONCE = 2;  // positions whose loads a wavefront has in flight together
+    for (uint32_t base = wave; base <= length; base += 4 * AT_ONCE) {
+        DraftPart pp[AT_ONCE], qp[AT_ONCE];
+        float pd[AT_ONCE], qd[AT_ONCE], u[AT_ONCE];
+        bool known[AT_ONCE];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; j++) {
+            const uint32_t i = base + 4 * j;
+            pp[j] = qp[j] = DraftPart{-INFINITY, DRAFT_NONE, 0.0};
+            pd[j] = qd[j] = u[j] = 0.f;
+            known[j] = false;
+            if (i <= length && a.target_logits) pp[j] = draft_first(rows.target_parts(i), a);
             if (i < length) {
+                if (with_q) qp[j] = draft_first(rows.draft_parts(i), a);
                 const uint32_t id = a.ids[(uint64_t)s * a.drafts + i];
-                double pd = 0.0, qd = 1.0;  // an id past the vocabulary has no probability
-                if (id < a.vocabulary) {
-                    pd = draft_value(RowIO<TT>::one(rows.target(i) + id), a.target_logits, p.max, p.inv, a.c);
-                    if (a.draft) qd = draft_value(RowIO<TD>::one(rows.draft(i) + id), a.draft_logits, q.max, q.inv, a.c);
+                u[j] = a.u[(uint64_t)s * (a.drafts + 1) + i];
+                known[j] = id < a.vocabulary;
+                if (known[j]) {
+                    pd[j] = RowIO<TT>::one(rows.target(i) + id);
+                    if (a.draft) qd[j] = RowIO<TD>::one(rows.draft(i) + id);
                 }
-                good[i] = (double)a.u[(uint64_t)s * (a.drafts + 1) + i] * qd < pd;
-                pid[i] = (float)pd;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; j++) {
+            const uint32_t i = base + 4 * j;
+            if (i > length) break;
+            DraftRow p = {0.f, 1.0, 0}, q = {0.f, 1.0, 0};
+            if (a.target_logits) p = draft_row(rows.target_parts(i), pp[j], a);
+            if (i < length && with_q) q = draft_row(rows.draft_parts(i), qp[j], a);
+            // an id past the vocabulary has no probability
+            const double pr = known[j] ? draft_value(pd[j], a.target_logits, p.max, p.inv, a.c) : 0.0;
+            const double qr = known[j] && a.draft ? draft_value(qd[j], a.draft_logits, q.max, q.inv, a.c) : 1.0;
+            if (lane == 0) {
+                prow[i] = p;
+                qrow[i] = q;
+                pid[i] = (float)pr;
+                good[i] = (double)u[j] * qr < pr;
             }
         }
     }
@@ -290,24 +326,6 @@ __global__ __launch_bounds__(256) void draft_rest_kernel(DraftArgs a) {
             if (a.probabilities) a.probabilities[at] = i < n ? pid[i] : 0.f;
         }
     }
-}
-
-// The inclusive sums of a wavefront's lanes.
-__device__ __forceinline__ double wave_scan_f64(double v) {
-    const uint32_t lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t b = (uint64_t)__double_as_longlong(v);
-        const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)b, o), hi = (uint32_t)__shfl_up((int)(b >> 32), o);
-        const double w = __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
-        if (lane >= (uint32_t)o) v += w;
-    }
-    return v;
-}
-__device__ __forceinline__ double lane_f64(double v, int lane) {
-    const uint64_t b = (uint64_t)__double_as_longlong(v);
-    const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)b, lane), hi = (uint32_t)__shfl((int)(b >> 32), lane);
-    return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
 }
 
 // One workgroup per sequence: the chunk, then the token in it, where the
@@ -392,7 +410,8 @@ __global__ __launch_bounds__(256) void draft_token_kernel(DraftArgs a) {
     if (lane == 63) swave[wave] = scan;
     __syncthreads();
     double before = schunk[0];
-    for (uint32_t w = 0; w < wave; w++) before += swave[w];
+#pragma unroll
+    for (uint32_t w = 0; w < 3; w++) before += w < wave ? swave[w] : 0.0;
     before += scan - sum;
     uint32_t first = DRAFT_NONE, last = 0;
 #pragma unroll
@@ -406,11 +425,14 @@ __global__ __launch_bounds__(256) void draft_token_kernel(DraftArgs a) {
     if (first != DRAFT_NONE) atomicMin(&sat[1], first);
     if (last) atomicMax(&sat[2], last);
     __syncthreads();
-    if (threadIdx.x == 0) {
-        const uint32_t token = sat[1] != DRAFT_NONE ? sat[1] : sat[2] - 1;
+    const uint32_t token = sat[1] != DRAFT_NONE ? sat[1] : sat[2] - 1;
+    if (token - c0 < DRAFT_RUN) {  // the thread that holds it
         a.tokens[out] = token;
-        if (a.probabilities)
-            a.probabilities[out] = (float)draft_value(RowIO<TT>::one(rows.target(n) + token), a.target_logits, st.max_p, st.inv_p, a.c);
+        float value = 0.f;
+#pragma unroll
+        for (int j = 0; j < (int)DRAFT_RUN; j++)
+            if (token - c0 == (uint32_t)j) value = pv[j];
+        if (a.probabilities) a.probabilities[out] = (float)draft_value(value, a.target_logits, st.max_p, st.inv_p, a.c);
     }
 }
 

@@ -25,15 +25,72 @@ __device__ __forceinline__ double exp2_f64(double x) {
     return x < -1000.0 ? 0.0 : x >= 1000.0 ? __builtin_inf() : y;
 }
 
-__device__ __forceinline__ double shfl_xor_f64(double v, int o) {
-    const uint64_t b = __double_as_longlong(v);
-    const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)b, o), hi = (uint32_t)__shfl_xor((int)(b >> 32), o);
-    return __longlong_as_double(((uint64_t)hi << 32) | lo);
+// 64-bit values across a wavefront by DPP and permlane swaps: a step is a few
+// clocks where a shuffle through LDS is over a hundred.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double dpp_f64(double v) {  // 0 where the source is outside, or the row is masked
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, false);
+    return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
 }
-__device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v += shfl_xor_f64(v, o);
+__device__ __forceinline__ double words_f64(uint32_t lo, uint32_t hi) {
+    return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
+}
+// The inclusive sums over the lanes: within rows of 16, then the rows before.
+__device__ __forceinline__ double wave_scan_f64(double v) {
+    v += dpp_f64<0x111>(v);  // row_shr 1, 2, 4, 8
+    v += dpp_f64<0x112>(v);
+    v += dpp_f64<0x114>(v);
+    v += dpp_f64<0x118>(v);
+    v += dpp_f64<0x142, 0xa>(v);  // row_bcast 15 into rows 1 and 3
+    v += dpp_f64<0x143, 0xc>(v);  // row_bcast 31 into rows 2 and 3
     return v;
+}
+// The value of a lane that is the same for all.
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    return words_f64((uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane), (uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), lane));
+}
+
+// The sum in every lane: lane 0's (the rotations add in another order in other lanes).
+__device__ __forceinline__ double wave_sum_f64(double v) {
+    v += dpp_f64<0xB1>(v);
+    v += dpp_f64<0x4E>(v);
+    v += dpp_f64<0x124>(v);
+    v += dpp_f64<0x128>(v);
+    uint64_t b = (uint64_t)__double_as_longlong(v);
+    auto l = __builtin_amdgcn_permlane16_swap((uint32_t)b, (uint32_t)b, false, false);
+    auto h = __builtin_amdgcn_permlane16_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+    v = words_f64(l[0], h[0]) + words_f64(l[1], h[1]);
+    b = (uint64_t)__double_as_longlong(v);
+    l = __builtin_amdgcn_permlane32_swap((uint32_t)b, (uint32_t)b, false, false);
+    h = __builtin_amdgcn_permlane32_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+    return lane_f64(words_f64(l[0], h[0]) + words_f64(l[1], h[1]), 0);
+}
+
+// Maximum and minimum of 32-bit words over a wavefront, in every lane.
+template <class F>
+__device__ __forceinline__ uint32_t wave_reduce_u32(uint32_t v, F f) {
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));
+    auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = f(a[0], a[1]);
+    a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return f(a[0], a[1]);
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    return wave_reduce_u32(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+__device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) {
+    return wave_reduce_u32(v, [](uint32_t a, uint32_t b) { return min(a, b); });
+}
+__device__ __forceinline__ float wave_max_f32(float v) {
+    return __uint_as_float(wave_reduce_u32(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }));
 }
 
 // 64-bit values as integers that order alike (-0 as +0); 0 is below every

@@ -32,12 +32,6 @@ struct ScoresArgs {
 
 constexpr int SCORE_WAVES = 4;
 
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
-    return v;
-}
-
 // 1 / d for d >= 1: the hardware's estimate and two Newton steps.
 __device__ __forceinline__ double recip_f64(double d) {
     double r = __builtin_amdgcn_rcp(d);
@@ -78,8 +72,7 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void scores_kernel(ScoresArgs a) 
         float m = v[0];
 #pragma unroll
         for (int j = 1; j < J; j++) m = fmaxf(m, v[j]);
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+        m = wave_max_f32(m);
         double sum = 0.0;
 #pragma unroll
         for (int j = 0; j < J; j++) {
@@ -122,7 +115,8 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void scores_kernel(ScoresArgs a) 
         }
         uint32_t better = 0;
         for (uint32_t g = 0; g < a.groups; g++) {
-            const uint64_t other = ((uint64_t)(uint32_t)__shfl((int)(rank >> 32), g) << 32) | (uint32_t)__shfl((int)(uint32_t)rank, g);
+            const uint64_t other = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(rank >> 32), g) << 32) |
+                                   (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)rank, g);
             better += other > rank || (other == rank && g < lane);
         }
         const uint64_t kept = __ballot(lane < a.groups && better < a.kept);
@@ -155,7 +149,7 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void scores_kernel(ScoresArgs a) 
             e = wave_max_u32(top && (uint32_t)best == lo ? ~e : 0);
             e = ~e;
         } else {
-            e = (uint32_t)__shfl((int)e, __builtin_ctzll(lanes));
+            e = (uint32_t)__builtin_amdgcn_readlane((int)e, __builtin_ctzll(lanes));
         }
         if (lane == r) chosen = e;
 #pragma unroll
@@ -166,7 +160,7 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void scores_kernel(ScoresArgs a) 
     const float w = lane < a.k ? score_lds[wave][chosen] : 0.f;
     float factor = a.scale;
     if (a.renormalize) {
-        const float sum = wave_sum(w);
+        const float sum = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_sum(w))));
         factor = sum > 0.f ? a.scale / sum : 0.f;
     }
     if (lane < a.k) {
