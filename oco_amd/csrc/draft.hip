@@ -26,6 +26,7 @@
 namespace oco {
 
 constexpr uint32_t DRAFT_CHUNK = 4096, DRAFT_RUN = 16;  // values per workgroup and row; per thread
+constexpr uint32_t DRAFT_STEP = 1024, DRAFT_STEPS = DRAFT_CHUNK / DRAFT_STEP;  // what is left of a row: sums of 1024 values
 constexpr uint32_t DRAFT_NONE = 0xffffffffu;
 
 // A chunk's part of a row: its maximum (and where it first is), and the sum
@@ -35,7 +36,7 @@ struct DraftPart {
     uint32_t at;
     double sum;
 };
-struct DraftRest {  // a chunk's sums of max(p - q, 0) and of p
+struct DraftRest {  // a step's sums of max(p - q, 0) and of p
     double rest, all;
 };
 struct DraftState {  // the row that a token is drawn from
@@ -51,7 +52,7 @@ struct DraftArgs {
     uint32_t *accepted, *tokens;
     float *probabilities;
     DraftPart *parts;  // [sequences * (drafts + 1)][chunks], then [sequences * drafts][chunks]
-    DraftRest *rests;  // [sequences][chunks]
+    DraftRest *rests;  // [sequences][chunks * DRAFT_STEPS]
     DraftState *states;
     uint64_t target_stride, draft_stride;
     uint32_t sequences, drafts, vocabulary, chunks;
@@ -211,177 +212,218 @@ __global__ __launch_bounds__(256) void draft_greedy_kernel(DraftArgs a) {
     }
 }
 
-// One workgroup per (sequence, chunk): every workgroup of a sequence makes
-// its decisions from the rows' parts, then sums its chunk of what is left of
-// the target at the first refused draft.
+// Four values c0 .. c0 + 3 of a row, 16 bytes at once for f32.
+template <class T>
+__device__ __forceinline__ void load_four(const T *row, uint32_t c0, uint32_t n, float *v, float fill) {
+    if (c0 + 4 <= n) {
+        if constexpr (sizeof(T) == 4) {
+            const u32x4_u a = *reinterpret_cast<const u32x4_u *>(row + c0);
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = __uint_as_float(a[j]);
+        } else {
+            const u32x2_u a = *reinterpret_cast<const u32x2_u *>(row + c0);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const T h = {(uint16_t)(a[j / 2] >> (16 * (j % 2)))};
+                v[j] = RowIO<T>::one(&h);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = c0 + j < n ? RowIO<T>::one(row + c0 + j) : fill;
+    }
+}
+
+// What the token is drawn from at four places: x = p, and d = max(p - q, 0)
+// (minus: p - q, else p).  NaN stays.
 template <class TT, class TD>
-__global__ __launch_bounds__(256) void draft_rest_kernel(DraftArgs a) {
-    __shared__ DraftRow prow[DRAFT_MOST + 1], qrow[DRAFT_MOST + 1];
-    __shared__ float pid[DRAFT_MOST + 1];
-    __shared__ uint32_t good[DRAFT_MOST + 1];
-    __shared__ double sums[2][4];
-    const uint32_t s = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const uint32_t length = draft_length(a, s);
+__device__ __forceinline__ void draft_left(const DraftArgs &a, const DraftRows<TT, TD> &rows, const DraftState &st, bool minus, uint32_t id,
+                                           uint32_t c0, float *pv, double *x, double *d) {
+    float qv[4];
+    load_four(rows.target(st.accepted), c0, a.vocabulary, pv, a.target_logits ? -INFINITY : 0.f);
+    if (minus && a.draft) load_four(rows.draft(st.accepted), c0, a.vocabulary, qv, a.draft_logits ? -INFINITY : 0.f);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        x[j] = draft_value(pv[j], a.target_logits, st.max_p, st.inv_p, a.c);
+        double y = 0.0;
+        if (minus) y = a.draft ? draft_value(qv[j], a.draft_logits, st.max_q, st.inv_q, a.c) : c0 + j == id ? 1.0 : 0.0;
+        const double left = x[j] - y;
+        d[j] = left <= 0.0 ? 0.0 : left;
+        x[j] = x[j] <= 0.0 ? 0.0 : x[j];
+    }
+}
+
+// The decisions of a sequence, by 1024 threads: a wavefront per row, then a
+// thread per draft.  `write`: this workgroup stores them.
+template <class TT, class TD>
+__device__ __forceinline__ DraftState draft_decide(const DraftArgs &a, uint32_t s, bool write) {
+    __shared__ DraftRow row_of[2 * DRAFT_MOST + 1];  // the target's rows, then the drafter's
+    __shared__ uint32_t good[DRAFT_MOST];
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63, length = draft_length(a, s), i = threadIdx.x;
     const DraftRows<TT, TD> rows{a, s};
-    const bool with_q = a.draft && a.draft_logits;
-    constexpr int AT_ONCE = 2;  // positions whose loads a wavefront has in flight together
-    for (uint32_t base = wave; base <= length; base += 4 * AT_ONCE) {
-        DraftPart pp[AT_ONCE], qp[AT_ONCE];
-        float pd[AT_ONCE], qd[AT_ONCE], u[AT_ONCE];
-        bool known[AT_ONCE];
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; j++) {
-            const uint32_t i = base + 4 * j;
-            pp[j] = qp[j] = DraftPart{-INFINITY, DRAFT_NONE, 0.0};
-            pd[j] = qd[j] = u[j] = 0.f;
-            known[j] = false;
-            if (i <= length && a.target_logits) pp[j] = draft_first(rows.target_parts(i), a);
-            if (i < length) {
-                if (with_q) qp[j] = draft_first(rows.draft_parts(i), a);
-                const uint32_t id = a.ids[(uint64_t)s * a.drafts + i];
-                u[j] = a.u[(uint64_t)s * (a.drafts + 1) + i];
-                known[j] = id < a.vocabulary;
-                if (known[j]) {
-                    pd[j] = RowIO<TT>::one(rows.target(i) + id);
-                    if (a.draft) qd[j] = RowIO<TD>::one(rows.draft(i) + id);
-                }
-            }
+    // thread i: the drafted token i
+    uint32_t id = DRAFT_NONE;
+    float u = 0.f, pd = 0.f, qd = 0.f;
+    if (i < length) {
+        id = a.ids[(uint64_t)s * a.drafts + i];
+        u = a.u[(uint64_t)s * (a.drafts + 1) + i];
+        if (id < a.vocabulary) {
+            pd = RowIO<TT>::one(rows.target(i) + id);
+            if (a.draft) qd = RowIO<TD>::one(rows.draft(i) + id);
         }
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; j++) {
-            const uint32_t i = base + 4 * j;
-            if (i > length) break;
-            DraftRow p = {0.f, 1.0, 0}, q = {0.f, 1.0, 0};
-            if (a.target_logits) p = draft_row(rows.target_parts(i), pp[j], a);
-            if (i < length && with_q) q = draft_row(rows.draft_parts(i), qp[j], a);
-            // an id past the vocabulary has no probability
-            const double pr = known[j] ? draft_value(pd[j], a.target_logits, p.max, p.inv, a.c) : 0.0;
-            const double qr = known[j] && a.draft ? draft_value(qd[j], a.draft_logits, q.max, q.inv, a.c) : 1.0;
-            if (lane == 0) {
-                prow[i] = p;
-                qrow[i] = q;
-                pid[i] = (float)pr;
-                good[i] = (double)u[j] * qr < pr;
-            }
-        }
+    }
+    const uint32_t first = a.target_logits ? 0 : length + 1, last = a.draft && a.draft_logits ? 2 * length + 1 : length + 1;
+#pragma unroll 1
+    for (uint32_t r = first + wave; r < last; r += 16) {
+        const DraftPart *const parts = r <= length ? rows.target_parts(r) : rows.draft_parts(r - length - 1);
+        const DraftRow row = draft_row(parts, draft_first(parts, a), a);
+        if (lane == 0) row_of[r] = row;
     }
     __syncthreads();
-    uint32_t n = 0;
-    while (n < length && good[n]) n++;
-    const bool refused = n < length;
-    const DraftRow p = prow[n], q = qrow[n];
-    const uint32_t id = refused ? a.ids[(uint64_t)s * a.drafts + n] : DRAFT_NONE;
-
-    float pv[DRAFT_RUN], qv[DRAFT_RUN];
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const uint32_t c0 = chunk * DRAFT_CHUNK + DRAFT_RUN * threadIdx.x + 8 * h;
-        load_run(rows.target(n), c0, a.vocabulary, pv + 8 * h, a.target_logits ? -INFINITY : 0.f);
-        if (refused && a.draft) load_run(rows.draft(n), c0, a.vocabulary, qv + 8 * h, a.draft_logits ? -INFINITY : 0.f);
+    if (i < length) {
+        const DraftRow p = row_of[i], q = row_of[length + 1 + i];
+        // an id past the vocabulary has no probability; without a draft's distribution q is 1
+        const double pr = id < a.vocabulary ? draft_value(pd, a.target_logits, p.max, p.inv, a.c) : 0.0;
+        const double qr = id < a.vocabulary && a.draft ? draft_value(qd, a.draft_logits, q.max, q.inv, a.c) : 1.0;
+        good[i] = (double)u * qr < pr;
+        pd = (float)pr;
     }
-    double rest = 0.0, all = 0.0;
-#pragma unroll
-    for (int j = 0; j < (int)DRAFT_RUN; j++) {
-        const double x = draft_value(pv[j], a.target_logits, p.max, p.inv, a.c);
-        double y = 0.0;
-        if (refused) {
-            if (a.draft)
-                y = draft_value(qv[j], a.draft_logits, q.max, q.inv, a.c);
-            else
-                y = chunk * DRAFT_CHUNK + DRAFT_RUN * threadIdx.x + j == id ? 1.0 : 0.0;
+    __syncthreads();
+    const uint64_t refusals = ~__ballot(lane < length && good[lane]);
+    const uint32_t n = min(length, refusals ? (uint32_t)__builtin_ctzll(refusals) : 64u);
+    const DraftRow &q = row_of[min(length + 1 + n, 2 * length)];
+    DraftState st;
+    st.accepted = n;
+    st.refused = n < length;
+    st.max_p = row_of[n].max;
+    st.inv_p = row_of[n].inv;
+    st.max_q = q.max;
+    st.inv_q = q.inv;
+    if (write) {
+        if (i == 0) {
+            a.states[s] = st;
+            a.accepted[s] = n;
         }
-        const double d = x - y;
-        rest += d <= 0.0 ? 0.0 : d;  // NaN stays
-        all += x <= 0.0 ? 0.0 : x;
+        if (i <= a.drafts && i != n) {  // at n: the token that is drawn next
+            const uint64_t at = (uint64_t)s * (a.drafts + 1) + i;
+            a.tokens[at] = i < n ? id : DRAFT_NONE;
+            if (a.probabilities) a.probabilities[at] = i < n ? pd : 0.f;
+        }
     }
-    rest = wave_sum_f64(rest);
-    all = wave_sum_f64(all);
+    return st;
+}
+
+template <class TT, class TD>
+__global__ __launch_bounds__(1024) void draft_decide_kernel(DraftArgs a) {
+    draft_decide<TT, TD>(a, blockIdx.x, true);
+}
+
+// What is left of the target at the first refused draft, in steps of 1024
+// values: four wavefronts with four values per thread.  FUSED: one workgroup
+// per (sequence, chunk of four steps), each of which makes its sequence's
+// decisions itself; bound by latency, and one launch less.  Else one workgroup per
+// (sequence, step), from decisions that are there.
+template <class TT, class TD, bool FUSED>
+__global__ __launch_bounds__(FUSED ? 1024 : 256) void draft_rest_kernel(DraftArgs a) {
+    constexpr uint32_t STEPS = FUSED ? DRAFT_STEPS : 1;
+    __shared__ double sums[2][4 * STEPS];
+    const uint32_t per = FUSED ? a.chunks : a.chunks * DRAFT_STEPS, s = blockIdx.x / per, part = blockIdx.x % per;
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const DraftRows<TT, TD> rows{a, s};
+    DraftState st;
+    if constexpr (FUSED)
+        st = draft_decide<TT, TD>(a, s, part == 0);
+    else
+        st = a.states[s];
+    const uint32_t id = st.refused ? a.ids[(uint64_t)s * a.drafts + st.accepted] : DRAFT_NONE;
+    float pv[4];
+    double x[4], d[4];
+    draft_left(a, rows, st, st.refused, id, part * STEPS * DRAFT_STEP + 4 * threadIdx.x, pv, x, d);
+    const double rest = wave_sum_f64((d[0] + d[1]) + (d[2] + d[3])), all = wave_sum_f64((x[0] + x[1]) + (x[2] + x[3]));
     if (lane == 0) {
         sums[0][wave] = rest;
         sums[1][wave] = all;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        DraftRest r;
-        r.rest = ((sums[0][0] + sums[0][1]) + sums[0][2]) + sums[0][3];
-        r.all = ((sums[1][0] + sums[1][1]) + sums[1][2]) + sums[1][3];
-        a.rests[(uint64_t)s * a.chunks + chunk] = r;
-    }
-    if (chunk == 0) {
-        if (threadIdx.x == 0) {
-            DraftState st;
-            st.inv_p = p.inv;
-            st.inv_q = q.inv;
-            st.max_p = p.max;
-            st.max_q = q.max;
-            st.accepted = n;
-            st.refused = refused;
-            a.states[s] = st;
-            a.accepted[s] = n;
-        }
-        for (uint32_t i = threadIdx.x; i <= a.drafts; i += 256) {
-            if (i == n) continue;  // the token that is drawn next
-            const uint64_t at = (uint64_t)s * (a.drafts + 1) + i;
-            a.tokens[at] = i < n ? a.ids[(uint64_t)s * a.drafts + i] : DRAFT_NONE;
-            if (a.probabilities) a.probabilities[at] = i < n ? pid[i] : 0.f;
-        }
+    if (threadIdx.x < STEPS) {
+        const double *const r = sums[0] + 4 * threadIdx.x, *const t = sums[1] + 4 * threadIdx.x;
+        a.rests[((uint64_t)s * per + part) * STEPS + threadIdx.x] = DraftRest{((r[0] + r[1]) + r[2]) + r[3], ((t[0] + t[1]) + t[2]) + t[3]};
     }
 }
 
-// One workgroup per sequence: the chunk, then the token in it, where the
-// running sum passes u times the whole.
+// One workgroup per sequence: the step of 1024 values, then the token in it,
+// where the running sum passes u times the whole.
 template <class TT, class TD>
 __global__ __launch_bounds__(256) void draft_token_kernel(DraftArgs a) {
-    __shared__ double schunk[3];
-    __shared__ uint32_t sat[3];
-    __shared__ double swave[4];
-    const uint32_t s = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const DraftRest *rests = a.rests + (uint64_t)s * a.chunks;
+    __shared__ double sat_before, mark_of, swave[4];
+    __shared__ uint32_t sat[3], from_rest;
+    const uint32_t s = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, steps = a.chunks * DRAFT_STEPS;
+    const DraftRest *rests = a.rests + (uint64_t)s * steps;
     const DraftState st = a.states[s];
     const uint32_t n = st.accepted;
+    const double u = (double)a.u[(uint64_t)s * (a.drafts + 1) + a.drafts];
+    const uint32_t refused_id = st.refused ? a.ids[(uint64_t)s * a.drafts + n] : DRAFT_NONE;
     if (wave == 0) {
         double rest = 0.0, all = 0.0;
-        for (uint32_t i = lane; i < a.chunks; i += 64) {
+        constexpr int HELD = 4;  // steps per lane that are read once
+        DraftRest held[HELD];
+#pragma unroll
+        for (int h = 0; h < HELD; h++) {
+            held[h] = DraftRest{0.0, 0.0};
+            if (64 * h + lane < steps) held[h] = rests[64 * h + lane];
+        }
+#pragma unroll
+        for (int h = 0; h < HELD; h++) {
+            rest += held[h].rest;
+            all += held[h].all;
+        }
+        for (uint32_t i = 64 * HELD + lane; i < steps; i += 64) {
             rest += rests[i].rest;
             all += rests[i].all;
         }
         rest = wave_sum_f64(rest);
         all = wave_sum_f64(all);
         const bool left = !(rest <= 0.0);  // nothing left (p == q): draw from p
-        const double whole = left ? rest : all, mark = (double)a.u[(uint64_t)s * (a.drafts + 1) + a.drafts] * whole;
-        // the first chunk whose running sum passes the mark, or the last one that holds anything
-        double before = 0.0, at_before = 0.0, last_before = 0.0;
-        uint32_t found = DRAFT_NONE, last = DRAFT_NONE;
-        for (uint32_t base = 0; base < a.chunks && found == DRAFT_NONE; base += 64) {
+        const double whole = left ? rest : all, mark = u * whole;
+        // the first step whose running sum passes the mark, or the last one that holds anything
+        double before = 0.0, at_before = 0.0;
+        uint32_t found = DRAFT_NONE;
+        bool passed = false;
+#pragma unroll 1
+        for (uint32_t base = 0; base < steps && !passed; base += 64) {
             const uint32_t i = base + lane;
-            const double w = i < a.chunks ? (left ? rests[i].rest : rests[i].all) : 0.0;
+            DraftRest r = {0.0, 0.0};
+            if (base >= 64 * HELD) {
+                if (i < steps) r = rests[i];
+            } else {
+#pragma unroll
+                for (int h = 0; h < HELD; h++)
+                    if (base == 64u * h) r = held[h];
+            }
+            const double w = left ? r.rest : r.all;
             const double sum = before + wave_scan_f64(w);
             const uint64_t pass = __ballot(sum > mark && w > 0.0), some = __ballot(w > 0.0);
-            if (pass) {
-                const int l = __builtin_ctzll(pass);
+            passed = pass != 0;
+            if (some) {
+                const int l = passed ? __builtin_ctzll(pass) : 63 - __builtin_clzll(some);
                 found = base + l;
                 at_before = lane_f64(sum, l) - lane_f64(w, l);
-            } else if (some) {
-                const int l = 63 - __builtin_clzll(some);
-                last = base + l;
-                last_before = lane_f64(sum, l) - lane_f64(w, l);
             }
             before = lane_f64(sum, 63);
         }
         if (lane == 0) {
-            const bool fine = whole > 0.0 && whole < __builtin_inf();
-            sat[0] = !fine ? DRAFT_NONE : found != DRAFT_NONE ? found : last;
+            sat[0] = whole > 0.0 && whole < __builtin_inf() ? found : DRAFT_NONE;
             sat[1] = DRAFT_NONE;
             sat[2] = 0;
-            schunk[0] = found != DRAFT_NONE ? at_before : last_before;
-            schunk[1] = mark;
-            schunk[2] = left ? 1.0 : 0.0;
+            sat_before = at_before;
+            mark_of = mark;
+            from_rest = left;
         }
     }
     __syncthreads();
-    const uint32_t chunk = sat[0];
+    const uint32_t step = sat[0];
     const uint64_t out = (uint64_t)s * (a.drafts + 1) + n;
-    if (chunk == DRAFT_NONE) {  // no distribution: a NaN, an infinity, or nothing but zeros
+    if (step == DRAFT_NONE) {  // no distribution: a NaN, an infinity, or nothing but zeros
         if (threadIdx.x == 0) {
             a.tokens[out] = DRAFT_NONE;
             if (a.probabilities) a.probabilities[out] = __uint_as_float(0x7fc00000u);
@@ -389,36 +431,24 @@ __global__ __launch_bounds__(256) void draft_token_kernel(DraftArgs a) {
         return;
     }
     const DraftRows<TT, TD> rows{a, s};
-    const bool minus = st.refused && schunk[2] != 0.0;
-    const uint32_t id = minus ? a.ids[(uint64_t)s * a.drafts + n] : DRAFT_NONE, c0 = chunk * DRAFT_CHUNK + DRAFT_RUN * threadIdx.x;
-    float pv[DRAFT_RUN], qv[DRAFT_RUN];
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        load_run(rows.target(n), c0 + 8 * h, a.vocabulary, pv + 8 * h, a.target_logits ? -INFINITY : 0.f);
-        if (minus && a.draft) load_run(rows.draft(n), c0 + 8 * h, a.vocabulary, qv + 8 * h, a.draft_logits ? -INFINITY : 0.f);
-    }
-    double r[DRAFT_RUN], sum = 0.0;
-#pragma unroll
-    for (int j = 0; j < (int)DRAFT_RUN; j++) {
-        const double x = draft_value(pv[j], a.target_logits, st.max_p, st.inv_p, a.c);
-        double y = 0.0;
-        if (minus) y = a.draft ? draft_value(qv[j], a.draft_logits, st.max_q, st.inv_q, a.c) : c0 + j == id ? 1.0 : 0.0;
-        r[j] = fmax(x - y, 0.0);
-        sum += r[j];
-    }
-    const double scan = wave_scan_f64(sum);
+    const bool left = from_rest != 0;
+    const uint32_t c0 = step * DRAFT_STEP + 4 * threadIdx.x;
+    float pv[4];
+    double x[4], d[4];
+    draft_left(a, rows, st, st.refused && left, refused_id, c0, pv, x, d);
+    const double sum = (d[0] + d[1]) + (d[2] + d[3]), scan = wave_scan_f64(sum);
     if (lane == 63) swave[wave] = scan;
     __syncthreads();
-    double before = schunk[0];
+    double before = sat_before;
 #pragma unroll
     for (uint32_t w = 0; w < 3; w++) before += w < wave ? swave[w] : 0.0;
     before += scan - sum;
     uint32_t first = DRAFT_NONE, last = 0;
 #pragma unroll
-    for (int j = 0; j < (int)DRAFT_RUN; j++) {
-        before += r[j];
-        if (r[j] > 0.0) {
-            if (before > schunk[1] && first == DRAFT_NONE) first = c0 + j;
+    for (int j = 0; j < 4; j++) {
+        before += d[j];
+        if (d[j] > 0.0) {
+            if (before > mark_of && first == DRAFT_NONE) first = c0 + j;
             last = c0 + j + 1;
         }
     }
@@ -426,13 +456,15 @@ __global__ __launch_bounds__(256) void draft_token_kernel(DraftArgs a) {
     if (last) atomicMax(&sat[2], last);
     __syncthreads();
     const uint32_t token = sat[1] != DRAFT_NONE ? sat[1] : sat[2] - 1;
-    if (token - c0 < DRAFT_RUN) {  // the thread that holds it
+    if (token - c0 < 4) {  // the thread that holds it
         a.tokens[out] = token;
-        float value = 0.f;
+        if (a.probabilities) {
+            double p = 0.0;
 #pragma unroll
-        for (int j = 0; j < (int)DRAFT_RUN; j++)
-            if (token - c0 == (uint32_t)j) value = pv[j];
-        if (a.probabilities) a.probabilities[out] = (float)draft_value(value, a.target_logits, st.max_p, st.inv_p, a.c);
+            for (int j = 0; j < 4; j++)
+                if (token - c0 == (uint32_t)j) p = a.target_logits ? x[j] : (double)pv[j];
+            a.probabilities[out] = (float)p;
+        }
     }
 }
 
@@ -445,7 +477,7 @@ static DraftLayout draft_layout(const oco_draft *p) {
     const uint64_t s = p->sequences;
     l.chunks = (uint32_t)(((uint64_t)p->vocabulary + DRAFT_CHUNK - 1) / DRAFT_CHUNK);
     l.parts = s * (2 * (uint64_t)p->drafts + 1) * l.chunks * sizeof(DraftPart);
-    l.rests = s * l.chunks * sizeof(DraftRest);
+    l.rests = s * l.chunks * DRAFT_STEPS * sizeof(DraftRest);
     l.states = s * sizeof(DraftState);
     l.bytes = l.parts + l.rests + l.states;
     return l;
@@ -467,7 +499,16 @@ static int draft_launch(const DraftArgs &a, bool greedy, hipStream_t stream) {
         hipLaunchKernelGGL(draft_greedy_kernel, dim3(a.sequences), dim3(256), 0, stream, a);
         return launch_check("oco_draft_verify (greedy)");
     }
-    hipLaunchKernelGGL((draft_rest_kernel<TT, TD>), dim3(a.sequences * a.chunks), dim3(256), 0, stream, a);
+    // Decisions in every workgroup while they all run at once (two of 1024 threads per compute unit), in a launch of
+    // their own beyond: 38 workgroups (one sequence of 151936 tokens) 5.8 us; 1216 of them 30.8 us
+    // against 4.7 + 16.7.
+    if ((uint64_t)a.sequences * a.chunks <= 512) {
+        hipLaunchKernelGGL((draft_rest_kernel<TT, TD, true>), dim3(a.sequences * a.chunks), dim3(1024), 0, stream, a);
+    } else {
+        hipLaunchKernelGGL((draft_decide_kernel<TT, TD>), dim3(a.sequences), dim3(1024), 0, stream, a);
+        OCO_TRY(launch_check("oco_draft_verify (decisions)"));
+        hipLaunchKernelGGL((draft_rest_kernel<TT, TD, false>), dim3(a.sequences * a.chunks * DRAFT_STEPS), dim3(256), 0, stream, a);
+    }
     OCO_TRY(launch_check("oco_draft_verify (rest)"));
     hipLaunchKernelGGL((draft_token_kernel<TT, TD>), dim3(a.sequences), dim3(256), 0, stream, a);
     return launch_check("oco_draft_verify (token)");
@@ -482,7 +523,7 @@ static const char *draft_problem(const oco_draft *p) {
     if ((p->target_stride && p->target_stride < p->vocabulary) || (p->draft_stride && p->draft_stride < p->vocabulary))
         return "a row stride under the vocabulary";
     const DraftLayout l = draft_layout(p);
-    if ((uint64_t)p->sequences * (2ull * p->drafts + 1) * l.chunks > 0x7fffffffull) return "too many rows for one call";
+    if ((uint64_t)p->sequences * (2ull * p->drafts + DRAFT_STEPS) * l.chunks > 0x7fffffffull) return "too many rows for one call";
     return nullptr;
 }
 
