@@ -212,28 +212,6 @@ __global__ __launch_bounds__(256) void draft_greedy_kernel(DraftArgs a) {
     }
 }
 
-// Four values c0 .. c0 + 3 of a row, 16 bytes at once for f32.
-template <class T>
-__device__ __forceinline__ void load_four(const T *row, uint32_t c0, uint32_t n, float *v, float fill) {
-    if (c0 + 4 <= n) {
-        if constexpr (sizeof(T) == 4) {
-            const u32x4_u a = *reinterpret_cast<const u32x4_u *>(row + c0);
-#pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = __uint_as_float(a[j]);
-        } else {
-            const u32x2_u a = *reinterpret_cast<const u32x2_u *>(row + c0);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const T h = {(uint16_t)(a[j / 2] >> (16 * (j % 2)))};
-                v[j] = RowIO<T>::one(&h);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = c0 + j < n ? RowIO<T>::one(row + c0 + j) : fill;
-    }
-}
-
 // What the token is drawn from at four places: x = p, and d = max(p - q, 0)
 // (minus: p - q, else p).  NaN stays.
 template <class TT, class TD>
@@ -242,12 +220,28 @@ __device__ __forceinline__ void draft_left(const DraftArgs &a, const DraftRows<T
     float qv[4];
     load_four(rows.target(st.accepted), c0, a.vocabulary, pv, a.target_logits ? -INFINITY : 0.f);
     if (minus && a.draft) load_four(rows.draft(st.accepted), c0, a.vocabulary, qv, a.draft_logits ? -INFINITY : 0.f);
+    // both rows' exponentials side by side
+    double at[8], e[8], y[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        x[j] = draft_value(pv[j], a.target_logits, st.max_p, st.inv_p, a.c);
-        double y = 0.0;
-        if (minus) y = a.draft ? draft_value(qv[j], a.draft_logits, st.max_q, st.inv_q, a.c) : c0 + j == id ? 1.0 : 0.0;
-        const double left = x[j] - y;
+        at[j] = ((double)pv[j] - (double)st.max_p) * a.c;
+        at[4 + j] = minus && a.draft ? ((double)qv[j] - (double)st.max_q) * a.c : 0.0;
+    }
+    if (minus && a.draft)
+        exp2_clamped<9, 8>(at, e);
+    else
+        exp2_clamped<9, 4>(at, e);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        x[j] = a.target_logits ? (at[j] < -1000.0 ? 0.0 : e[j]) * st.inv_p : (double)pv[j];
+        y[j] = 0.0;
+        if (minus) {
+            if (a.draft)
+                y[j] = a.draft_logits ? (at[4 + j] < -1000.0 ? 0.0 : e[4 + j]) * st.inv_q : (double)qv[j];
+            else
+                y[j] = c0 + j == id ? 1.0 : 0.0;
+        }
+        const double left = x[j] - y[j];
         d[j] = left <= 0.0 ? 0.0 : left;
         x[j] = x[j] <= 0.0 ? 0.0 : x[j];
     }

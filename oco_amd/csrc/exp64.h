@@ -8,21 +8,36 @@ constexpr double LOG2E = 1.4426950408889634074;
 
 // 2^x by the Taylor series of e^(f ln 2) about f = 0, f = x - round(x):
 // |f ln 2| <= 0.3466, so the first term left out is at most 0.3466^(D+1) /
-// (D+1)! relative: 7e-12 for D = 9, 1.7e-16 for D = 12.  0 below 2^-1000
-// (and for -Inf), Inf from 2^1000 on, NaN for NaN.
-template <int D>
-__device__ __forceinline__ double exp2_f64(double x) {
+// (D+1)! relative: 7e-12 for D = 9, 1.7e-16 for D = 12.  N at once, term by
+// term: the chains of dependent FMAs run side by side and share their
+// constants.  x is taken into -1000 .. 1000 (a NaN too).
+template <int D, int N>
+__device__ __forceinline__ void exp2_clamped(const double *x, double *y) {
     constexpr double C[13] = {1.0, 0.69314718055994530942, 0.24022650695910071233, 0.055504108664821579953,
                               0.0096181291076284771619, 0.0013333558146428443423, 0.00015403530393381609954,
                               1.5252733804059840280e-5, 1.3215486790144309488e-6, 1.0178086009239699728e-7,
                               7.0549116208011233299e-9, 4.4455382718708114976e-10, 2.5678435993488205142e-11};
-    const double n = __builtin_rint(x), f = x - n;
-    double r = C[D];
+    double n[N], f[N];
 #pragma unroll
-    for (int i = D - 1; i >= 0; i--) r = __builtin_fma(r, f, C[i]);
-    // |n| <= 1000 keeps ldexp's integer in range
-    const double y = __builtin_ldexp(r, (int)fmin(fmax(n, -1000.0), 1000.0));
-    return x < -1000.0 ? 0.0 : x >= 1000.0 ? __builtin_inf() : y;
+    for (int i = 0; i < N; i++) {
+        const double t = fmin(fmax(x[i], -1000.0), 1000.0);
+        n[i] = __builtin_rint(t);
+        f[i] = t - n[i];
+        y[i] = C[D];
+    }
+#pragma unroll
+    for (int d = D - 1; d >= 0; d--)
+#pragma unroll
+        for (int i = 0; i < N; i++) y[i] = __builtin_fma(y[i], f[i], C[d]);
+#pragma unroll
+    for (int i = 0; i < N; i++) y[i] = __builtin_ldexp(y[i], (int)n[i]);
+}
+// The same of one x, with 0 below 2^-1000 (and for -Inf), Inf from 2^1000 on and NaN for NaN.
+template <int D>
+__device__ __forceinline__ double exp2_f64(double x) {
+    double y;
+    exp2_clamped<D, 1>(&x, &y);
+    return x < -1000.0 ? 0.0 : x < 1000.0 ? y : x + __builtin_inf();
 }
 
 // 64-bit values across a wavefront by DPP and permlane swaps: a step is a few

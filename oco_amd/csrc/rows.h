@@ -111,4 +111,26 @@ __device__ __forceinline__ void store_run(T *row, uint32_t c0, uint32_t n, const
     }
 }
 
+// Columns c0 .. c0 + 3 of a row of n.
+template <class T>
+__device__ __forceinline__ void load_four(const T *row, uint32_t c0, uint32_t n, float *v, float fill = 0.f) {
+    if (c0 + 4 <= n) {
+        if constexpr (sizeof(T) == 4) {
+            const u32x4_u a = *reinterpret_cast<const u32x4_u *>(row + c0);
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = __uint_as_float(a[j]);
+        } else {
+            const u32x2_u a = *reinterpret_cast<const u32x2_u *>(row + c0);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const T h = {(uint16_t)(a[j / 2] >> (16 * (j % 2)))};
+                v[j] = RowIO<T>::one(&h);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = c0 + j < n ? RowIO<T>::one(row + c0 + j) : fill;
+    }
+}
+
 }  // namespace oco

@@ -14,10 +14,14 @@
 // them is chosen must not depend on how exp was rounded.  Without a bias
 // c_e orders as z_e does, and the logits' own bits decide.
 //
-// Bound by issue: one wavefront per token; the k rounds (a wave-wide maximum
-// each) and, with a bias or ranked groups, the 64-bit exponentials.
+// Bound by issue: one wavefront per token.  A lane holds J consecutive experts
+// and sorts them once; a round takes the largest head of the 64 lanes.  WIDE
+// (a bias, or groups ranked by sums): 64-bit scores of every expert; else the
+// rounds run on the logits' own 32 bits and only the chosen get a score.
 #include "exp64.h"
 #include "rows.h"
+
+#include <type_traits>
 
 namespace oco {
 
@@ -39,125 +43,245 @@ __device__ __forceinline__ double recip_f64(double d) {
     return __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
 }
 
-template <class T, int J>  // J experts per lane: lane + 64 j
+// Values as integers that order alike (-0 as +0); 0 is below every number, -Inf included.
+__device__ __forceinline__ uint32_t order_f32(float v) {
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return b >> 31 ? ~b : b | 0x80000000u;
+}
+
+// The larger and the smaller of two lanes' pairs (first >= second of disjoint sets).
+template <int CTRL>
+__device__ __forceinline__ void merge_dpp(double &first, double &second) {
+    auto other = [](double v) {
+        const uint64_t b = (uint64_t)__double_as_longlong(v);
+        return words_f64((uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false),
+                         (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xf, 0xf, false));
+    };
+    const double a = other(first), b = other(second);
+    second = fmax(fmin(first, a), fmax(second, b));
+    first = fmax(first, a);
+}
+__device__ __forceinline__ void merge_swap(double &first, double &second, bool wide) {
+    auto pair = [&](double v, double &x, double &y) {
+        const uint64_t b = (uint64_t)__double_as_longlong(v);
+        const uint32_t lo = (uint32_t)b, hi = (uint32_t)(b >> 32);
+        if (wide) {
+            auto l = __builtin_amdgcn_permlane32_swap(lo, lo, false, false), h = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+            x = words_f64(l[0], h[0]);
+            y = words_f64(l[1], h[1]);
+        } else {
+            auto l = __builtin_amdgcn_permlane16_swap(lo, lo, false, false), h = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+            x = words_f64(l[0], h[0]);
+            y = words_f64(l[1], h[1]);
+        }
+    };
+    double a, b, c, d;
+    pair(first, a, b);
+    pair(second, c, d);
+    second = fmax(fmin(a, b), fmax(c, d));
+    first = fmax(a, b);
+}
+
+template <class T, int J, bool WIDE>  // J experts per lane: J lane + j
 __global__ __launch_bounds__(64 * SCORE_WAVES) void scores_kernel(ScoresArgs a) {
-    __shared__ double choice_lds[SCORE_WAVES][64 * J];
-    __shared__ float score_lds[SCORE_WAVES][64 * J];
+    using Key = std::conditional_t<WIDE, uint64_t, uint32_t>;
+    __shared__ double choice_lds[SCORE_WAVES][64 * J];  // groups that are not whole lanes
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const uint64_t token = (uint64_t)blockIdx.x * SCORE_WAVES + wave;
     if (token >= a.tokens) return;
     const T *z = (const T *)a.logits + token * a.experts;
-    const bool ranked = a.groups > 1;
-    const bool wide = a.bias || (ranked && a.top2);  // the choice needs scores, not logits
     float v[J];
-    bool bad = false, open[J];
+    bool bad = false;
+    if constexpr (J % 8 == 0) {
+#pragma unroll
+        for (int h = 0; h < J / 8; h++) load_run(z, J * lane + 8 * h, a.experts, v + 8 * h, -INFINITY);
+    } else if constexpr (J == 4) {
+        load_four(z, 4 * lane, a.experts, v, -INFINITY);
+    } else {
+#pragma unroll
+        for (int j = 0; j < J; j++) v[j] = J * lane + j < a.experts ? RowIO<T>::one(z + J * lane + j) : -INFINITY;
+    }
+    float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < J; j++) {
-        const uint32_t e = lane + 64 * j;
-        v[j] = e < a.experts ? RowIO<T>::one(z + e) : -INFINITY;
         if (!(v[j] < INFINITY)) {  // NaN or +Inf: the token's weights are NaN
             bad = true;
             v[j] = -INFINITY;
         }
-        open[j] = v[j] > -INFINITY;  // -Inf: an expert that is not available
+        m = fmaxf(m, v[j]);
     }
     bad = __ballot(bad) != 0;
 
-    // scores
+    // e = exp(z - max) for the softmax, exp(-z) for the sigmoid; a score of 0 for an expert that is not available
+    double inv = 1.0;  // softmax: the scores' common factor, where it does not cancel
+    if (!a.sigmoid) m = wave_max_f32(m);
+    const double from = a.sigmoid ? 0.0 : (double)m, rate = a.sigmoid ? -LOG2E : LOG2E;
     double s[J];
-    if (a.sigmoid) {
+    if (WIDE || !(a.sigmoid || a.renormalize)) {
+        double x[J];
 #pragma unroll
-        for (int j = 0; j < J; j++) s[j] = open[j] ? recip_f64(1.0 + exp2_f64<12>(fmin((double)v[j] * -LOG2E, 999.0))) : 0.0;
-    } else {
-        float m = v[0];
+        for (int j = 0; j < J; j++) x[j] = ((double)v[j] - from) * rate;
+        exp2_clamped<12, J>(x, s);
+        if (a.sigmoid) {
 #pragma unroll
-        for (int j = 1; j < J; j++) m = fmaxf(m, v[j]);
-        m = wave_max_f32(m);
-        double sum = 0.0;
+            for (int j = 0; j < J; j++) s[j] = v[j] > -INFINITY ? recip_f64(1.0 + s[j]) : 0.0;
+        } else {
+            double sum = 0.0;
 #pragma unroll
-        for (int j = 0; j < J; j++) {
-            s[j] = open[j] ? exp2_f64<12>(((double)v[j] - (double)m) * LOG2E) : 0.0;
-            sum += s[j];
+            for (int j = 0; j < J; j++) {
+                s[j] = v[j] > -INFINITY ? s[j] : 0.0;
+                sum += s[j];
+            }
+            sum = wave_sum_f64(sum);
+            inv = sum > 0.0 ? recip_f64(sum) : 0.0;
+#pragma unroll
+            for (int j = 0; j < J; j++) s[j] *= inv;
         }
-        sum = wave_sum_f64(sum);
-        const double inv = sum > 0.0 ? recip_f64(sum) : 0.0;
-#pragma unroll
-        for (int j = 0; j < J; j++) s[j] *= inv;
     }
+
+    float bias[J];
+#pragma unroll
+    for (int j = 0; j < J; j++) bias[j] = WIDE && a.bias && J * lane + j < a.experts ? a.bias[J * lane + j] : 0.f;
 
     // what is ranked, as integers: 0 for an expert that cannot be chosen
-    uint64_t key[J];
+    Key key[J];
+    double first = -__builtin_inf(), second = -__builtin_inf();
+    const bool ranked = a.groups > 1;
+    const uint32_t size = a.experts / a.groups, span = size / J;
+    const bool in_lanes = size % J == 0 && (span & (span - 1)) == 0;  // a group is 1, 2, 4 .. lanes
 #pragma unroll
     for (int j = 0; j < J; j++) {
-        const uint32_t e = lane + 64 * j;
+        const uint32_t e = J * lane + j;
         double c = (double)v[j];
-        if (wide) {
-            c = s[j] + (a.bias && e < a.experts ? (double)a.bias[e] : 0.0);
-            if (!open[j] || c != c) c = -__builtin_inf();
+        if constexpr (WIDE) {
+            c = s[j] + (double)bias[j];
+            if (!(v[j] > -INFINITY) || c != c) c = -__builtin_inf();
+            key[j] = e < a.experts ? order_f64(c) : 0;
+        } else {
+            key[j] = e < a.experts ? order_f32(v[j]) : 0;
         }
-        key[j] = e < a.experts ? order_f64(c) : 0;
-        score_lds[wave][e] = (float)s[j];
-        if (ranked) choice_lds[wave][e] = c;
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (ranked) {
-        const uint32_t size = a.experts / a.groups;
-        uint64_t rank = 0;
-        if (lane < a.groups) {
-            double first = -__builtin_inf(), second = -__builtin_inf();
-            for (uint32_t i = 0; i < size; i++) {
-                const double c = choice_lds[wave][lane * size + i];
+        if (ranked) {
+            if (in_lanes) {
                 second = fmax(second, fmin(first, c));
                 first = fmax(first, c);
+            } else {
+                choice_lds[wave][e] = c;
             }
-            if (a.top2 && second > -__builtin_inf()) first += second;
-            rank = order_f64(first);
         }
+    }
+    if (ranked) {
+        uint32_t group = lane;
+        if (in_lanes) {  // each lane its own group's two largest
+            group = lane / span;
+            if (span > 1) merge_dpp<0xB1>(first, second);   // lanes ^ 1
+            if (span > 2) merge_dpp<0x4E>(first, second);   // ^ 2
+            if (span > 4) merge_dpp<0x141>(first, second);  // the mirrored half row
+            if (span > 8) merge_dpp<0x140>(first, second);  // the mirrored row
+            if (span > 16) merge_swap(first, second, false);
+            if (span > 32) merge_swap(first, second, true);
+        } else {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (lane < a.groups)
+#pragma unroll 4
+                for (uint32_t i = 0; i < size; i++) {
+                    const double c = choice_lds[wave][lane * size + i];
+                    second = fmax(second, fmin(first, c));
+                    first = fmax(first, c);
+                }
+        }
+        if (a.top2 && second > -__builtin_inf()) first += second;
+        const uint64_t rank = order_f64(first);
         uint32_t better = 0;
         for (uint32_t g = 0; g < a.groups; g++) {
-            const uint64_t other = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(rank >> 32), g) << 32) |
-                                   (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)rank, g);
-            better += other > rank || (other == rank && g < lane);
+            const uint32_t at = in_lanes ? g * span : g;
+            const uint64_t other = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(rank >> 32), at) << 32) |
+                                   (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)rank, at);
+            better += other > rank || (other == rank && g < group);
         }
-        const uint64_t kept = __ballot(lane < a.groups && better < a.kept);
-        const float per = 1.0f / (float)size;
+        if (in_lanes) {
 #pragma unroll
-        for (int j = 0; j < J; j++) {
-            // (e + 1/2) / size is at least 1 / (2 size) from an integer
-            const uint32_t g = (uint32_t)(((float)(lane + 64 * j) + 0.5f) * per);
-            if (!((kept >> (g & 63)) & 1)) key[j] = 0;
+            for (int j = 0; j < J; j++) key[j] = better < a.kept ? key[j] : 0;
+        } else {
+            const uint64_t kept = __ballot(lane < a.groups && better < a.kept);
+            const float per = 1.0f / (float)size;
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                // (e + 1/2) / size is at least 1 / (2 size) from an integer
+                const uint32_t g = (uint32_t)(((float)(J * lane + j) + 0.5f) * per);
+                if (!((kept >> (g & 63)) & 1)) key[j] = 0;
+            }
         }
     }
 
-    // k rounds: the largest high word, then, where several lanes have it, the low words
+    // each lane's experts in order: largest first, equal ones by index (adjacent exchanges that are strict)
+    uint32_t at[J];
+#pragma unroll
+    for (int j = 0; j < J; j++) at[j] = J * lane + j;
+    if constexpr (J <= 4) {
+#pragma unroll
+        for (int r = 0; r < J; r++)
+#pragma unroll
+            for (int j = r % 2; j + 1 < J; j += 2) {
+                const bool swap = key[j + 1] > key[j];
+                const Key k0 = key[j];
+                const uint32_t a0 = at[j];
+                key[j] = swap ? key[j + 1] : k0;
+                key[j + 1] = swap ? k0 : key[j + 1];
+                at[j] = swap ? at[j + 1] : a0;
+                at[j + 1] = swap ? a0 : at[j + 1];
+            }
+    }
+    // k rounds: the largest head; of equal ones the lowest lane's, whose experts come first
     uint32_t chosen = 0;
     for (uint32_t r = 0; r < a.k; r++) {
-        uint64_t best = key[0];
-        uint32_t at = 0;
+        Key best = key[0];
+        uint32_t e = at[0];
+        if constexpr (J > 4) {
 #pragma unroll
-        for (int j = 1; j < J; j++)
-            if (key[j] > best) {
-                best = key[j];
-                at = j;
+            for (int j = 1; j < J; j++) {
+                const bool more = key[j] > best;
+                best = more ? key[j] : best;
+                e = more ? at[j] : e;
             }
-        const uint32_t hi = wave_max_u32((uint32_t)(best >> 32));
-        const bool top = (uint32_t)(best >> 32) == hi;
-        uint64_t lanes = __ballot(top);
-        uint32_t e = lane + 64 * at;
-        if (__popcll(lanes) > 1) {
-            const uint32_t lo = wave_max_u32(top ? (uint32_t)best : 0);
-            e = wave_max_u32(top && (uint32_t)best == lo ? ~e : 0);
-            e = ~e;
-        } else {
-            e = (uint32_t)__builtin_amdgcn_readlane((int)e, __builtin_ctzll(lanes));
         }
-        if (lane == r) chosen = e;
+        uint64_t lanes;
+        if constexpr (WIDE) {
+            const uint32_t hi = wave_max_u32((uint32_t)(best >> 32));
+            const bool top = (uint32_t)(best >> 32) == hi;
+            lanes = __ballot(top);
+            if (__popcll(lanes) > 1) {
+                const uint32_t lo = wave_max_u32(top ? (uint32_t)best : 0);
+                lanes = __ballot(top && (uint32_t)best == lo);
+            }
+        } else {
+            const uint32_t most = wave_max_u32(best);
+            lanes = __ballot(best == most);
+        }
+        const int head = __builtin_ctzll(lanes);
+        const uint32_t winner = (uint32_t)__builtin_amdgcn_readlane((int)e, head);
+        if (lane == r) chosen = winner;
+        if constexpr (J > 4) {
 #pragma unroll
-        for (int j = 0; j < J; j++)
-            if (e == lane + 64 * j) key[j] = 0;
+            for (int j = 0; j < J; j++) key[j] = at[j] == winner ? 0 : key[j];
+        } else {
+            const bool mine = lane == (uint32_t)head;
+#pragma unroll
+            for (int j = 0; j + 1 < J; j++) {
+                key[j] = mine ? key[j + 1] : key[j];
+                at[j] = mine ? at[j + 1] : at[j];
+            }
+            key[J - 1] = mine ? 0 : key[J - 1];
+        }
     }
 
-    const float w = lane < a.k ? score_lds[wave][chosen] : 0.f;
+    float w = 0.f;
+    if (lane < a.k) {
+        const float logit = RowIO<T>::one(z + chosen);
+        const double x = ((double)logit - from) * rate;
+        double e;
+        exp2_clamped<12, 1>(&x, &e);
+        w = logit > -INFINITY && logit < INFINITY ? (float)(a.sigmoid ? recip_f64(1.0 + e) : e * inv) : 0.f;
+    }
     float factor = a.scale;
     if (a.renormalize) {
         const float sum = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_sum(w))));
@@ -170,13 +294,13 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void scores_kernel(ScoresArgs a) 
 }
 
 typedef void (*ScoresFn)(ScoresArgs);
-template <class T>
+template <class T, bool WIDE>
 static ScoresFn scores_pick(uint32_t experts) {
-    if (experts <= 64) return scores_kernel<T, 1>;
-    if (experts <= 128) return scores_kernel<T, 2>;
-    if (experts <= 256) return scores_kernel<T, 4>;
-    if (experts <= 512) return scores_kernel<T, 8>;
-    return scores_kernel<T, 16>;
+    if (experts <= 64) return scores_kernel<T, 1, WIDE>;
+    if (experts <= 128) return scores_kernel<T, 2, WIDE>;
+    if (experts <= 256) return scores_kernel<T, 4, WIDE>;
+    if (experts <= 512) return scores_kernel<T, 8, WIDE>;
+    return scores_kernel<T, 16, WIDE>;
 }
 
 }  // namespace oco
@@ -213,11 +337,12 @@ extern "C" int oco_route_scores(const void *logits, oco_dtype dtype, const float
     a.sigmoid = p->score == OCO_SCORE_SIGMOID;
     a.renormalize = p->renormalize != 0;
     a.scale = p->scale;
+    const bool wide = bias || (a.groups > 1 && a.top2);
     ScoresFn fn;
     switch (dtype) {
-    case OCO_DT_F32: fn = scores_pick<float>(p->experts); break;
-    case OCO_DT_BF16: fn = scores_pick<bf16_t>(p->experts); break;
-    case OCO_DT_F16: fn = scores_pick<f16_t>(p->experts); break;
+    case OCO_DT_F32: fn = wide ? scores_pick<float, true>(p->experts) : scores_pick<float, false>(p->experts); break;
+    case OCO_DT_BF16: fn = wide ? scores_pick<bf16_t, true>(p->experts) : scores_pick<bf16_t, false>(p->experts); break;
+    case OCO_DT_F16: fn = wide ? scores_pick<f16_t, true>(p->experts) : scores_pick<f16_t, false>(p->experts); break;
     default: return fail(OCO_ERR_UNSUPPORTED, "oco_route_scores: logits of type %d", (int)dtype);
     }
     hipLaunchKernelGGL(fn, dim3((uint32_t)(((uint64_t)tokens + SCORE_WAVES - 1) / SCORE_WAVES)), dim3(64 * SCORE_WAVES), 0,
