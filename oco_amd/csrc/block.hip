@@ -50,31 +50,38 @@ __device__ __forceinline__ float gate_value(float g, uint32_t kind) {
     return g;
 }
 
+// A run of weights and gate values, as the formulas use them.
+struct BlockRun {
+    float post[8], gate[8], pre[8];
+};
+template <class YT>
+__device__ __forceinline__ void block_load_add(const BlockArgs &a, const YT *gate, uint32_t c0, BlockRun &w) {
+    if (a.post_w) load_run(a.post_w, c0, a.n, w.post);
+    if (a.kind != OCO_GATE_NONE) load_run(gate, c0, a.n, w.gate);
+}
+__device__ __forceinline__ void block_load_out(const BlockArgs &a, uint32_t c0, BlockRun &w) {
+    if (a.pre_w) load_run(a.pre_w, c0, a.n, w.pre);
+}
+
 // x' of one run of columns (rounded), from the run's v.
-template <class XT, class YT>
-__device__ __forceinline__ void block_add(const BlockArgs &a, const float *xv, float *v, const YT *gate, uint32_t c0, float inv) {
-    float w[8];
-    if (a.post_w) {
-        load_run(a.post_w, c0, a.n, w);
+template <class XT>
+__device__ __forceinline__ void block_add(const BlockArgs &a, const float *xv, float *v, const BlockRun &w, float inv) {
+    if (a.post_w)
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = v[j] * inv * (w[j] + a.offset);
-    }
-    if (a.kind != OCO_GATE_NONE) {
-        load_run(gate, c0, a.n, w);
+        for (int j = 0; j < 8; j++) v[j] = v[j] * inv * (w.post[j] + a.offset);
+    if (a.kind != OCO_GATE_NONE)
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] *= gate_value(w[j], a.kind);
-    }
+        for (int j = 0; j < 8; j++) v[j] *= gate_value(w.gate[j], a.kind);
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] = RowIO<XT>::round(fmaf(a.scale, v[j], xv[j]));
 }
 
 // out (and its 8-bit form) of one run of columns of x'.
 template <class YT>
-__device__ __forceinline__ void block_out(const BlockArgs &a, const float *v, uint64_t row, uint32_t c0, float inv) {
-    float w[8], o[8];
-    load_run(a.pre_w, c0, a.n, w);
+__device__ __forceinline__ void block_out(const BlockArgs &a, const float *v, const BlockRun &w, uint64_t row, uint32_t c0, float inv) {
+    float o[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) o[j] = c0 + j < a.n ? v[j] * inv * (w[j] + a.offset) : 0.f;
+    for (int j = 0; j < 8; j++) o[j] = c0 + j < a.n ? v[j] * inv * (w.pre[j] + a.offset) : 0.f;
     if (a.out) store_run((YT *)a.out + row * a.out_stride, c0, a.n, o);
     if (a.codes) {  // 16 consecutive threads hold a block of 128 columns
         float scale;
@@ -88,6 +95,9 @@ __device__ __forceinline__ void block_out(const BlockArgs &a, const float *v, ui
 
 // T threads per row (64: four rows per workgroup), P runs of eight columns
 // per thread; P == 0: any n, a row read again for each of its three passes.
+// A thread of one run requests its weights and gate with the rows, so that
+// one memory latency stands before the first sum and none behind it; with two
+// runs the registers cost more than that gives (8192 x 4096: 66 us against 61).
 template <class XT, class YT, int T, int P>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
     __shared__ float part[2][T / 64];
@@ -99,11 +109,19 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
     const YT *gate = (const YT *)a.gate + (a.gate_rows ? row / a.gate_rows : 0) * a.gate_stride;
     XT *x_out = (XT *)a.x_out + row * a.x_stride;
     if constexpr (P > 0) {
+        constexpr bool EARLY = P == 1;
         float xv[P][8], v[P][8], s = 0.f, inv = 1.f;
+        BlockRun w[EARLY ? P : 1];
 #pragma unroll
         for (int p = 0; p < P; p++) load_run(y, 8 * (t + T * p), a.n, v[p]);
 #pragma unroll
         for (int p = 0; p < P; p++) load_run(x, 8 * (t + T * p), a.n, xv[p]);
+        if constexpr (EARLY) {
+#pragma unroll
+            for (int p = 0; p < P; p++) block_load_add(a, gate, 8 * (t + T * p), w[p]);
+#pragma unroll
+            for (int p = 0; p < P; p++) block_load_out(a, 8 * (t + T * p), w[p]);
+        }
         if (a.post_w) {
 #pragma unroll
             for (int p = 0; p < P; p++)
@@ -115,7 +133,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
 #pragma unroll
         for (int p = 0; p < P; p++) {
             const uint32_t c0 = 8 * (t + T * p);
-            block_add<XT>(a, xv[p], v[p], gate, c0, inv);
+            if constexpr (!EARLY) block_load_add(a, gate, c0, w[0]);
+            block_add<XT>(a, xv[p], v[p], w[EARLY ? p : 0], inv);
             store_run(x_out, c0, a.n, v[p]);
 #pragma unroll
             for (int j = 0; j < 8; j++)
@@ -124,9 +143,13 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
         if (!a.pre_w) return;
         inv = 1.0f / sqrtf(row_sum<T>(s, part[1]) / (float)a.n + a.epsilon);
 #pragma unroll
-        for (int p = 0; p < P; p++) block_out<YT>(a, v[p], row, 8 * (t + T * p), inv);
+        for (int p = 0; p < P; p++) {
+            if constexpr (!EARLY) block_load_out(a, 8 * (t + T * p), w[0]);
+            block_out<YT>(a, v[p], w[EARLY ? p : 0], row, 8 * (t + T * p), inv);
+        }
     } else {
         float xv[8], v[8], s = 0.f, inv = 1.f;
+        BlockRun w;
         if (a.post_w) {
             for (uint32_t c0 = 8 * t; c0 < a.n; c0 += 8 * T) {
                 load_run(y, c0, a.n, v);
@@ -139,7 +162,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
         for (uint32_t c0 = 8 * t; c0 < a.n; c0 += 8 * T) {
             load_run(y, c0, a.n, v);
             load_run(x, c0, a.n, xv);
-            block_add<XT>(a, xv, v, gate, c0, inv);
+            block_load_add(a, gate, c0, w);
+            block_add<XT>(a, xv, v, w, inv);
             store_run(x_out, c0, a.n, v);
 #pragma unroll
             for (int j = 0; j < 8; j++)
@@ -150,7 +174,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
         // every thread of a block of 128 columns takes part in its maximum
         for (uint32_t c0 = 8 * t; c0 - c0 % FP8_BLOCK < a.n; c0 += 8 * T) {
             load_run((const XT *)x_out, c0, a.n, v);  // this thread's own columns
-            block_out<YT>(a, v, row, c0, inv);
+            block_load_out(a, c0, w);
+            block_out<YT>(a, v, w, row, c0, inv);
         }
     }
 }
@@ -161,7 +186,7 @@ typedef void (*BlockFn)(BlockArgs);
 // columns; few rows take twice the threads, for latency.
 template <class XT, class YT>
 static BlockFn block_pick(uint32_t n, uint32_t rows, int &threads) {
-    const bool few = rows <= 256;
+    const bool few = rows <= 1024;
 #define PICK(T, P) (threads = T, block_kernel<XT, YT, T, P>)
     if (n <= 512) return PICK(64, 1);
     if (n <= 1024 && !few) return PICK(64, 2);

@@ -264,13 +264,15 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void scores_kernel(ScoresArgs a) 
 #pragma unroll
             for (int j = 0; j < J; j++) key[j] = at[j] == winner ? 0 : key[j];
         } else {
-            const bool mine = lane == (uint32_t)head;
+            if (lane == (uint32_t)head) {
+                asm volatile("");  // a branch of moves: as selects by every lane it is four times the instructions
 #pragma unroll
-            for (int j = 0; j + 1 < J; j++) {
-                key[j] = mine ? key[j + 1] : key[j];
-                at[j] = mine ? at[j + 1] : at[j];
+                for (int j = 0; j + 1 < J; j++) {
+                    key[j] = key[j + 1];
+                    at[j] = at[j + 1];
+                }
+                key[J - 1] = 0;
             }
-            key[J - 1] = mine ? 0 : key[J - 1];
         }
     }
 
