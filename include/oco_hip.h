@@ -107,7 +107,9 @@ typedef enum oco_knob {
     OCO_KNOB_MATMUL_VENDOR = 12,  /* f16-operand prefill: value 0 the fused f16 MFMA tiles, 1 the dequantize pass
                                      and the vendor GEMM, 2 with row tiles, column tiles and K parts the panel
                                      kernel (default: by size, among these and the few-row kernel) */
-    OCO_KNOB_COUNT = 13
+    OCO_KNOB_FP8 = 13,            /* 8-bit products: 0 the few-row kernel (up to 64 rows), 128 or 256 tiles of that size;
+                                     second value (optional): K parts of the tiles */
+    OCO_KNOB_COUNT = 14
 } oco_knob;
 int oco_plan_override(uint32_t knob, const int32_t *values, uint32_t count);
 

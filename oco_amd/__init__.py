@@ -54,6 +54,7 @@ class Knob(enum.IntEnum):
     MX_EXPERTS_KS = 10
     STREAM_DIRECT = 11
     MATMUL_VENDOR = 12
+    FP8 = 13
 
 
 class DType(enum.IntEnum):

@@ -95,6 +95,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 struct HalfBlock {
     f16x8 v[4];
+    HalfBlock() = default;
     __device__ __forceinline__ HalfBlock(i32x8 c) {
 #pragma unroll
         for (int s = 0; s < 4; s++) {
@@ -113,73 +114,113 @@ __device__ __forceinline__ f32x4 half_block_sum(const HalfBlock &w, const HalfBl
     return p;
 }
 
-// Few rows: bound by the weight stream.  A workgroup's four wavefronts take
-// every fourth block of K of 16 NT weight rows straight into the registers
-// that the products read, and meet in LDS at the end.  The conversions to f16
-// hide behind the stream.
-constexpr int FP8_WAVES = 4;
+// Few rows: bound by the weight stream.  A workgroup's WAVES wavefronts share
+// the blocks of K of 16 NT weight rows among them, take them straight into
+// the registers that the products read, two blocks ahead, and meet in LDS at
+// the end.  The conversions to f16 hide behind the stream.  Loads keep their
+// lines in the caches: a load instruction takes half a line of each row, and
+// the next one the other half (151936 x 4096, 8 rows: 118 us, 129 with the
+// nontemporal hint).
 constexpr uint32_t FP8_OFF = 0x80000000u;  // past every range: reads zero without touching memory
 
-template <int MT, int NT>
-__global__ __launch_bounds__(64 * FP8_WAVES) void fp8_rows_kernel(Fp8Args a) {
-    __shared__ f32x4 part[FP8_WAVES * MT * NT * 64];
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+template <int MT, int NT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void fp8_rows_kernel(Fp8Args a) {
+    __shared__ f32x4 part[WAVES * MT * NT * 64];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     const uint32_t n0 = blockIdx.x * 16 * NT, rows = min(a.n - n0, 16u * NT);
-    const uint32_t m0 = blockIdx.y * 16 * MT, xrows = min(a.m - m0, 16u * MT);
     const __amdgpu_buffer_rsrc_t wr = uniform_rsrc(a.w + (uint64_t)n0 * a.k, rows * a.k);
-    const __amdgpu_buffer_rsrc_t xr = uniform_rsrc(a.x + (uint64_t)m0 * a.k, xrows * a.k);
-    auto load = [&](const __amdgpu_buffer_rsrc_t &rs, uint32_t row, bool live, uint32_t b) {
-        const uint32_t k0 = FP8_BLOCK * b + 16 * q, at = row * a.k + k0;
-        const u32x4 lo = __builtin_amdgcn_raw_buffer_load_b128(rs, live && k0 < a.k ? at : FP8_OFF, 0, 0);
-        const u32x4 hi = __builtin_amdgcn_raw_buffer_load_b128(rs, live && k0 + 64 < a.k ? at + 64 : FP8_OFF, 0, 0);
-        return i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+    const __amdgpu_buffer_rsrc_t xr = uniform_rsrc(a.x, a.m * a.k);
+    uint32_t wrow[NT], xrow[MT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) wrow[t] = 16 * t + r < rows ? (16 * t + r) * a.k + 16 * q : FP8_OFF;
+#pragma unroll
+    for (int i = 0; i < MT; i++) xrow[i] = 16 * i + r < a.m ? (16 * i + r) * a.k + 16 * q : FP8_OFF;
+    static_assert(FP8_BLOCK % (16 * NT) == 0, "one weight scale per block of K");
+    const float *const wsrc = a.ws + (uint64_t)(n0 / FP8_BLOCK) * a.blocks;
+    struct Buf {
+        i32x8 w[NT], x[MT];
+        float ws, xs[MT];
+    };
+    auto load = [&](Buf &f, uint32_t b) {  // blocks past the last, and chunks past k, read zero
+        const uint32_t k0 = FP8_BLOCK * b;
+        const uint32_t lo = k0 + 16 * q < a.k ? k0 : FP8_OFF, hi = k0 + 64 + 16 * q < a.k ? k0 + 64 : FP8_OFF;
+        auto both = [&](const __amdgpu_buffer_rsrc_t &rs, uint32_t row) {
+            const u32x4 u = __builtin_amdgcn_raw_buffer_load_b128(rs, (row | lo) & FP8_OFF ? FP8_OFF : row + lo, 0, 0);
+            const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rs, (row | hi) & FP8_OFF ? FP8_OFF : row + hi, 0, 0);
+            return i32x8{(int)u.x, (int)u.y, (int)u.z, (int)u.w, (int)v.x, (int)v.y, (int)v.z, (int)v.w};
+        };
+#pragma unroll
+        for (int t = 0; t < NT; t++) f.w[t] = both(wr, wrow[t]);
+#pragma unroll
+        for (int i = 0; i < MT; i++) f.x[i] = both(xr, xrow[i]);
+        const uint32_t at = min(b, a.blocks - 1);
+        f.ws = wsrc[at];
+#pragma unroll
+        for (int i = 0; i < MT; i++) f.xs[i] = a.xs[(uint64_t)at * a.m + min(16 * i + r, a.m - 1)];
     };
     f32x4 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
         for (int t = 0; t < NT; t++) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (uint32_t b = wave; b < a.blocks; b += FP8_WAVES) {
-        i32x8 w[NT], x[MT];
-        float ws[NT], xs[MT];
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-            w[t] = load(wr, 16 * t + r, 16 * t + r < rows, b);
-            ws[t] = a.ws[(uint64_t)(min(n0 + 16 * t, a.n - 1) / FP8_BLOCK) * a.blocks + b];
-        }
+    auto compute = [&](const Buf &f) {
+        HalfBlock x[MT];
+        float s[MT];
 #pragma unroll
         for (int i = 0; i < MT; i++) {
-            x[i] = load(xr, 16 * i + r, 16 * i + r < xrows, b);
-            xs[i] = a.xs[(uint64_t)b * a.m + min(m0 + 16 * i + r, a.m - 1)];
+            x[i] = HalfBlock(f.x[i]);
+            s[i] = f.ws * f.xs[i];
         }
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            const HalfBlock wh(w[t]);
+            const HalfBlock w(f.w[t]);
 #pragma unroll
             for (int i = 0; i < MT; i++) {
-                const f32x4 p = half_block_sum(wh, HalfBlock(x[i]));
-                const float s = ws[t] * xs[i];
+                const f32x4 p = half_block_sum(w, x[i]);
 #pragma unroll
-                for (int v = 0; v < 4; v++) acc[i][t][v] = fmaf(p[v], s, acc[i][t][v]);
+                for (int v = 0; v < 4; v++) acc[i][t][v] = fmaf(p[v], s[i], acc[i][t][v]);
             }
         }
+    };
+    Buf f0, f1;
+    load(f0, wave);
+    load(f1, wave + WAVES);
+    for (uint32_t b = wave; b < a.blocks; b += 2 * WAVES) {
+        compute(f0);
+        load(f0, b + 2 * WAVES);
+        if (b + WAVES < a.blocks) compute(f1);
+        load(f1, b + 3 * WAVES);
     }
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
         for (int t = 0; t < NT; t++) part[(wave * MT * NT + i * NT + t) * 64 + lane] = acc[i][t];
     __syncthreads();
-    for (uint32_t o = threadIdx.x; o < MT * NT * 64; o += 64 * FP8_WAVES) {
+    for (uint32_t o = threadIdx.x; o < MT * NT * 64; o += 64 * WAVES) {
         f32x4 s = part[o];
 #pragma unroll
-        for (int w = 1; w < FP8_WAVES; w++) s += part[w * MT * NT * 64 + o];
-        const uint32_t tile = o / 64, l = o % 64, row = m0 + 16 * (tile / NT) + (l & 15), col = n0 + 16 * (tile % NT) + 4 * (l >> 4);
+        for (int w = 1; w < WAVES; w++) s += part[w * MT * NT * 64 + o];
+        const uint32_t tile = o / 64, l = o % 64, row = 16 * (tile / NT) + (l & 15), col = n0 + 16 * (tile % NT) + 4 * (l >> 4);
         if (row >= a.m || col >= a.n) continue;
         float v[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) v[j] = s[j] + (a.bias ? round_bf16(a.bias[min(col + j, a.n - 1)]) : 0.f);
         fp8_put4(a.y, a.y_dtype, (uint64_t)row * a.n + col, v, a.n - col);
     }
+}
+
+typedef void (*Fp8RowsFn)(Fp8Args);
+// Up to 512 tiles of 16 weight rows, eight wavefronts on one tile, so that the
+// loads in flight fill the card (2880 x 4096, one row: 5.4 us; two tiles and
+// four wavefronts 6.3); beyond, four wavefronts on two tiles, which read the
+// activations half as often (12288 x 4096, 32 rows: 19.8 us against 21.9).
+static Fp8RowsFn fp8_rows_pick(uint32_t m, uint32_t n, uint32_t &cols, uint32_t &waves) {
+    const bool small = n <= 512 * 16;
+    cols = small ? 16 : 32;
+    waves = small ? 8 : 4;
+    if (m <= 16) return small ? fp8_rows_kernel<1, 1, 8> : fp8_rows_kernel<1, 2, 4>;
+    if (m <= 32) return small ? fp8_rows_kernel<2, 1, 8> : fp8_rows_kernel<2, 2, 4>;
+    return small ? fp8_rows_kernel<4, 1, 8> : fp8_rows_kernel<4, 2, 4>;
 }
 
 // ---- many rows: tiles through LDS ------------------------------------------------------
@@ -478,16 +519,50 @@ namespace oco {
 struct Fp8Plan {
     uint32_t bm, bn, mt, nt, parts;  // bm 0: few rows
 };
-constexpr uint32_t FP8_FEW = 32;
-static Fp8Plan fp8_plan(uint32_t m, uint32_t n, uint32_t k) {
-    Fp8Plan p = {0, 0, 0, 0, 1};
-    if (m <= FP8_FEW) return p;
+constexpr uint32_t FP8_FEW = 64;  // the few-row kernel's limit
+// The least of the estimated times, in us, each term fitted to measured calls
+// (n, k of 512 x 2880, 2880 x 4096, 4096 x 4096, 4096 x 12288 and 12288 x
+// 4096, 1 to 1024 rows; the estimates are within about 15% of them):
+//  * few rows: the weight stream at 5.3 TB/s, and 0.2 ns for each product of
+//    16 x 16 x 128 past the first 16 rows' (those hide behind the stream);
+//  * 128-tiles: a block of K takes 0.82 us (f32 outputs, on the f16
+//    instruction: 1.17) with a workgroup per compute unit, 1.08 (1.45) with two;
+//  * 256-tiles (16-bit outputs): 2.15 us, one workgroup per compute unit;
+//  * K parts: a launch, and their sums written and read at 3 TB/s.
+static Fp8Plan fp8_plan(uint32_t m, uint32_t n, uint32_t k, bool half) {
     const uint32_t blocks = (k + FP8_BLOCK - 1) / FP8_BLOCK;
-    p.bm = p.bn = (uint64_t)((m + 255) / 256) * ((n + 255) / 256) >= 256 ? 256 : 128;
-    p.mt = (m + p.bm - 1) / p.bm;
-    p.nt = (n + p.bn - 1) / p.bn;
-    while (p.bm == 128 && (uint64_t)p.mt * p.nt * p.parts < 256 && p.parts < 8 && blocks / (2 * p.parts) >= 4) p.parts *= 2;
-    return p;
+    int32_t knob[4] = {-1, 0, 0, 0};
+    const int set = plan_override(OCO_KNOB_FP8, knob);
+    Fp8Plan best = {0, 0, 0, 0, 1};
+    double least = 1e30;
+    if (m <= FP8_FEW && (!set || knob[0] == 0)) {
+        const double more = m <= 16 ? 0 : m <= 32 ? 1 : 3;
+        least = 4.0 + (double)n * k / 5.3e6 + (more > 0 ? 1.2 + more * ((n + 15) / 16) * blocks * 0.2e-3 : 0.0);
+        if (set) return best;
+    }
+    for (uint32_t tile = 128; tile <= (half ? 128u : 256u); tile *= 2) {
+        if (set && knob[0] == 256 && !half && tile != 256) continue;
+        if (set && knob[0] != 256 && tile != 128) continue;
+        Fp8Plan p = {tile, tile, (m + tile - 1) / tile, (n + tile - 1) / tile, 1};
+        const uint64_t tiles = (uint64_t)p.mt * p.nt;
+        for (p.parts = 1; p.parts <= 16; p.parts++) {  // by the rule: up to 8, powers of two
+            if (set > 1 && p.parts != std::min((uint32_t)std::max(knob[1], 1), std::min(blocks, 16u))) continue;
+            if (!(set > 1) && (p.parts > 8 || p.parts & (p.parts - 1) || (p.parts > 1 && blocks / p.parts < 2))) continue;
+            const uint64_t work = tiles * p.parts;
+            const double stages = (double)((blocks + p.parts - 1) / p.parts);
+            double t = 3.0;
+            if (tile == 256)
+                t += (double)((work + 255) / 256) * stages * 2.15;
+            else
+                t += work <= 256 ? stages * (half ? 1.17 : 0.82) : (double)((work + 511) / 512) * stages * (half ? 1.45 : 1.08);
+            if (p.parts > 1) t += 5.5 + (double)p.parts * m * n * 8.0 / 3e6;
+            if (t < least) {
+                least = t;
+                best = p;
+            }
+        }
+    }
+    return best;
 }
 
 template <int BM, int BN, int WM, int WN, bool HALF>
@@ -504,10 +579,14 @@ static int fp8_tiles(const Fp8TileArgs &a, hipStream_t stream) {
 
 }  // namespace oco
 
+static uint64_t fp8_need(const Fp8Plan &plan, const oco_matrix *p) {
+    return plan.parts > 1 ? (uint64_t)plan.parts * p->m * p->n * 4 : 0;
+}
+
+// For outputs of either kind.
 extern "C" uint64_t oco_fp8_matmul_workspace(const oco_matrix *p) {
     if (!p || p->m == 0 || p->n == 0 || p->k == 0) return 0;
-    const Fp8Plan plan = fp8_plan(p->m, p->n, p->k);
-    return plan.parts > 1 ? (uint64_t)plan.parts * p->m * p->n * 4 : 0;
+    return std::max(fp8_need(fp8_plan(p->m, p->n, p->k, true), p), fp8_need(fp8_plan(p->m, p->n, p->k, false), p));
 }
 
 extern "C" int oco_fp8_matmul(const uint8_t *w, const float *w_scales, const uint8_t *codes, const float *scales, void *y,
@@ -522,11 +601,12 @@ extern "C" int oco_fp8_matmul(const uint8_t *w, const float *w_scales, const uin
     if (!w || !w_scales || !codes || !scales || !y || (p->has_bias && !bias))
         return fail(OCO_ERR_INVALID, "oco_fp8_matmul: null pointer");
     if (((uintptr_t)w | (uintptr_t)codes) & 15u) return fail(OCO_ERR_INVALID, "oco_fp8_matmul: weights and codes are 16-byte aligned");
-    // 32-bit offsets inside a workgroup's rows
-    if (p->k > 0x1000000u || p->n > 0x7fffff00u || p->m > 0x7fffff00u)
+    // 31-bit offsets inside a workgroup's rows
+    if (p->k > 0x400000u || p->n > 0x7fffff00u || p->m > 0x7fffff00u)
         return fail(OCO_ERR_INVALID, "oco_fp8_matmul: %u x %u x %u", p->m, p->n, p->k);
-    const Fp8Plan plan = fp8_plan(p->m, p->n, p->k);
-    const uint64_t need = oco_fp8_matmul_workspace(p);
+    const bool half = y_dtype == OCO_DT_F32;
+    const Fp8Plan plan = fp8_plan(p->m, p->n, p->k, half);
+    const uint64_t need = fp8_need(plan, p);
     if (need && (!workspace || ((uintptr_t)workspace & 15u) || workspace_bytes < need))
         return fail(OCO_ERR_INVALID, "oco_fp8_matmul: workspace of %llu bytes, need %llu, 16-byte aligned",
                     (unsigned long long)workspace_bytes, (unsigned long long)need);
@@ -545,8 +625,9 @@ extern "C" int oco_fp8_matmul(const uint8_t *w, const float *w_scales, const uin
     a.y_dtype = y_dtype;
     hipStream_t st = (hipStream_t)stream;
     if (!plan.bm) {
-        auto fn = p->m <= 16 ? fp8_rows_kernel<1, 2> : fp8_rows_kernel<2, 2>;
-        hipLaunchKernelGGL(fn, dim3((p->n + 31) / 32), dim3(64 * FP8_WAVES), 0, st, a);
+        uint32_t cols = 0, waves = 0;
+        const Fp8RowsFn fn = fp8_rows_pick(p->m, p->n, cols, waves);
+        hipLaunchKernelGGL(fn, dim3((p->n + cols - 1) / cols), dim3(64 * waves), 0, st, a);
         return launch_check("oco_fp8_matmul");
     }
     Fp8TileArgs t;
@@ -555,9 +636,8 @@ extern "C" int oco_fp8_matmul(const uint8_t *w, const float *w_scales, const uin
     t.nt = plan.nt;
     t.parts = plan.parts;
     t.sums = (float *)workspace;
-    const bool half = y_dtype == OCO_DT_F32;
     if (plan.bm == 256)
-        OCO_TRY(half ? (fp8_tiles<256, 256, 2, 4, true>(t, st)) : (fp8_tiles<256, 256, 2, 4, false>(t, st)));
+        OCO_TRY((fp8_tiles<256, 256, 2, 4, false>(t, st)));
     else
         OCO_TRY(half ? (fp8_tiles<128, 128, 2, 2, true>(t, st)) : (fp8_tiles<128, 128, 2, 2, false>(t, st)));
     if (plan.parts > 1) {

@@ -202,3 +202,44 @@ def test_quantized_rows_of_a_matrix(lib):
     wv = e4m3(w, w.shape) * np.repeat(np.repeat(ws.astype(np.float64), 128, 0), 128, 1)[:n, :k]
     step = np.maximum(np.abs(x) * 2.0 ** -4, np.repeat(s.T.astype(np.float64), 128, 1)[:, :k] * 2.0 ** -10)
     assert np.all(np.abs(got - x @ wv.T) <= (step @ np.abs(wv).T) * 1.01)
+
+
+@pytest.mark.parametrize("plan", [(0,), (128, 1), (128, 2), (128, 3), (128, 16), (256, 1), (256, 5)])
+@pytest.mark.parametrize("m,n,k", [(61, 333, 2064), (64, 40, 1296), (300, 520, 400), (513, 260, 144)])
+def test_every_kernel_and_k_split(lib, plan, m, n, k):
+    """Each kernel on sizes that the rule would give to another: the few-row
+    kernel up to its limit, both tiles at ragged edges, K in parts that are
+    not even, of single blocks and of a last block that is not whole."""
+    with lib.overridden(lib.Knob.FP8, plan):
+        for y_dtype in ("f32", "bf16"):
+            check(lib, m, n, k, y_dtype, bias=True)
+
+
+@pytest.mark.parametrize("m,n", [(520, 8900), (2100, 2600)])
+def test_workgroups_that_take_several_tiles(lib, m, n):
+    """More tiles than workgroups: a tile's first stage is requested while the
+    one before is written (every 37th column is checked)."""
+    k = 272
+    say("fp8 several tiles", m, n)
+    rng = np.random.default_rng(m)
+    x, w, xs, ws = operands(rng, m, n, k)
+    p = lib.Matrix(k, n, m, 0, 1, 1, 0)
+    bufs = [dev(lib, a) for a in (w, ws, x, xs)]
+    cols = np.arange(0, n, 37)
+    for plan, y_dtype in (((128, 1), "f32"), ((128, 1), "bf16"), ((256, 1), "bf16")):
+        out = Guarded(lib, m * n * SIZE[y_dtype])
+        with lib.overridden(lib.Knob.FP8, plan):
+            lib.fp8_matmul(*bufs, out.ptr, p, CODE[y_dtype])
+        lib.synchronize()
+        got = values(out.read(np.uint8), y_dtype, (m, n))[:, cols]
+        sub = ws[cols // 128]
+        want, mag, lost = np.zeros((m, len(cols))), np.zeros((m, len(cols))), 0.0
+        xv, wv = e4m3(x, x.shape), e4m3(w, w.shape)[cols]
+        for b in range(len(xs)):
+            c = slice(128 * b, 128 * b + 128)
+            s = xs[b].astype(np.float64)[:, None] * sub[:, b].astype(np.float64)
+            want += (xv[:, c] @ wv[:, c].T) * s
+            mag += (np.abs(xv[:, c]) @ np.abs(wv[:, c]).T) * s
+        if y_dtype != "f32":  # the largest of a group of eight products is at most their sum of magnitudes
+            lost = 7 * 2.0 ** -13 * mag
+        assert np.all(np.abs(got - want) <= (256 + len(xs) + 12) * U * mag + HALF[y_dtype] * 1.01 * np.abs(want) + lost)

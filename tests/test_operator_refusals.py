@@ -70,7 +70,7 @@ def test_fp8():
     refused(product(dt=3), "type 3", 2)
     refused(product(w=ODD), "16-byte")
     refused(product(codes=ODD), "16-byte")
-    refused(product(k=0x2000000), "x 33554432")
+    refused(product(k=0x400010), "x 4194320")
     refused(L.oco_fp8_matmul(FAKE, FAKE, FAKE, FAKE, FAKE, 0, None, None, None, 0, None), "null matrix")
     assert product(m=0, w=None) == 0 and product(n=0, w=None) == 0
     with pytest.raises(ValueError):
