@@ -321,20 +321,28 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8TileArgs t
         for (int i = 0; i < WL; i++) wo[i] = min((wave * WL + i) * 8 + (lane >> 3), wrows - 1) * a.k;
         wsrc = a.ws + (uint64_t)(min(n0 + wn, a.n - 1) / FP8_BLOCK) * a.blocks;
     };
-    auto fetch = [&](uint32_t b, uint32_t s) {
-        // columns past k: the row's first chunk, cleared before it is read
-        const uint32_t base = FP8_BLOCK * b, xc = base + xchunk < a.k ? xchunk : 0;
-        const uint32_t wc[2] = {base + wchunk < a.k ? wchunk : 0, base + (wchunk ^ 64) < a.k ? wchunk ^ 64 : 0};
-#pragma unroll
-        for (int i = 0; i < XL; i++) to_lds16(xr, lds + s * STAGE + (wave * XL + i) * 1024, xo[i] + xc, base);
-#pragma unroll
-        for (int i = 0; i < WL; i++)
-            to_lds16(wr, lds + s * STAGE + XB + (wave * WL + i) * 1024, wo[i] + wc[(wave * WL + i) * 8 / OUT & 1], base);
-        if (wave < BM / 64) {
+    // One of the LOADS requests of a stage.  Columns past k: the row's first chunk, cleared before it is read.
+    constexpr int LOADS = XL + WL + 1;
+    auto fetch_one = [&](uint32_t b, uint32_t s, int i) {
+        const uint32_t base = FP8_BLOCK * b;
+        if (i < XL) {
+            to_lds16(xr, lds + s * STAGE + (wave * XL + i) * 1024, xo[i < XL ? i : 0] + (base + xchunk < a.k ? xchunk : 0), base);
+        } else if (i < XL + WL) {
+            const int j = i < XL + WL ? i - XL : 0;
+            const uint32_t c = wchunk ^ ((wave * WL + j) * 8 / OUT & 1 ? 64 : 0);
+            to_lds16(wr, lds + s * STAGE + XB + (wave * WL + j) * 1024, wo[j] + (base + c < a.k ? c : 0), base);
+        } else if (wave < BM / 64) {
             const uint32_t rows = min(a.m - m0, (uint32_t)BM);
             to_lds4(uniform_rsrc(a.xs + (uint64_t)b * a.m + m0, rows * 4), xs_lds + s * BM + wave * 64, min(wave * 64 + lane, rows - 1) * 4);
         }
     };
+    auto fetch = [&](uint32_t b, uint32_t s) {
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) fetch_one(b, s, i);
+    };
+    // Requests between the products, where registers allow: ahead of them they hold the wavefront up before its
+    // first LDS read (1024 x 4096 x 12288: 88 us against 96).
+    constexpr bool BETWEEN = BM * BN <= 128 * 128;
     // fragment addresses: chunks q and 4 + q of the lane's rows
     const uint32_t xlo = (wm + r) * FP8_BLOCK + (q ^ (r & 7)) * 16, wrow = wn + OUT * (r >> 2) + (r & 3);
     const uint32_t wlo = XB + wrow * FP8_BLOCK + (q ^ ((r & 3) | (wrow / OUT % 2 * 4))) * 16;
@@ -368,10 +376,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8TileArgs t
                 }
                 __syncthreads();
             }
-            if (b + 1 < b1) {
-                fetch(b + 1, s ^ 1);
-                ws_next = wsrc[b + 1];
-            }
+            // behind the last stage, that one again: its place is free until the next tile
+            const uint32_t bn = min(b + 1, b1 - 1);
+            if constexpr (!BETWEEN)
+                if (b + 1 < b1) fetch(b + 1, s ^ 1);
+            ws_next = wsrc[bn];
             const uint32_t xt = s * STAGE + xlo, wt = s * STAGE + wlo;
             const float *const xsb = xs_lds + s * BM + wm + r;
             // Fragments of x are read one step of 16 rows ahead, and a step's sums are added while the next
@@ -401,6 +410,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8TileArgs t
                     xn = frag(xt + (i + 1) * 16 * FP8_BLOCK);
                     fn = ws * xsb[16 * (i + 1)];
                 }
+                if constexpr (BETWEEN)
+#pragma unroll
+                    for (int l = i * LOADS / TM; l < (i + 1) * LOADS / TM; l++) fetch_one(bn, s ^ 1, l);
                 f32x4 p[TN];
                 if constexpr (HALF) {
                     const HalfBlock h(x);
@@ -437,8 +449,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8TileArgs t
         // the next tile's first stage, then this one's results
         const uint32_t row0 = m0 + wm + r, col = n0 + wn + OUT * q;
         id += gridDim.x;
+        __syncthreads();  // nothing is on its way to LDS any more
         if (id < tiles) {
-            __syncthreads();
             enter(id);
             if (b0 < b1) fetch(b0, 0);
             ws_next = wsrc[min(b0, a.blocks - 1)];
@@ -528,7 +540,7 @@ constexpr uint32_t FP8_FEW = 64;  // the few-row kernel's limit
 //  * 128-tiles: a block of K takes 0.82 us (f32 outputs, on the f16
 //    instruction: 1.17) with a workgroup per compute unit, 1.08 (1.45) with two;
 //  * 256-tiles (16-bit outputs): 2.15 us, one workgroup per compute unit;
-//  * K parts: a launch, and their sums written and read at 3 TB/s.
+//  * K parts: a launch, 0.4 us each, and their sums written and read at 3 TB/s.
 static Fp8Plan fp8_plan(uint32_t m, uint32_t n, uint32_t k, bool half) {
     const uint32_t blocks = (k + FP8_BLOCK - 1) / FP8_BLOCK;
     int32_t knob[4] = {-1, 0, 0, 0};
@@ -555,7 +567,7 @@ static Fp8Plan fp8_plan(uint32_t m, uint32_t n, uint32_t k, bool half) {
                 t += (double)((work + 255) / 256) * stages * 2.15;
             else
                 t += work <= 256 ? stages * (half ? 1.17 : 0.82) : (double)((work + 511) / 512) * stages * (half ? 1.45 : 1.08);
-            if (p.parts > 1) t += 5.5 + (double)p.parts * m * n * 8.0 / 3e6;
+            if (p.parts > 1) t += 5.5 + 0.4 * p.parts + (double)p.parts * m * n * 8.0 / 3e6;
             if (t < least) {
                 least = t;
                 best = p;
