@@ -450,8 +450,8 @@ class DeviceBuffer:
 
 
 def _addr(b) -> int | None:
-    if b is None:
-        return None
+    if type(b) is int or b is None:  # the usual case of a serving loop, first
+        return b
     if isinstance(b, DeviceBuffer):
         return b.ptr
     return int(b)

@@ -43,6 +43,7 @@ struct DraftState {  // the row that a token is drawn from
     double inv_p, inv_q;
     float max_p, max_q;
     uint32_t accepted, refused;
+    uint32_t id, pad;  // the refused draft
 };
 
 struct DraftArgs {
@@ -215,8 +216,8 @@ __global__ __launch_bounds__(256) void draft_greedy_kernel(DraftArgs a) {
 // What the token is drawn from at four places: x = p, and d = max(p - q, 0)
 // (minus: p - q, else p).  NaN stays.
 template <class TT, class TD>
-__device__ __forceinline__ void draft_left(const DraftArgs &a, const DraftRows<TT, TD> &rows, const DraftState &st, bool minus, uint32_t id,
-                                           uint32_t c0, float *pv, double *x, double *d) {
+__device__ __forceinline__ void draft_left(const DraftArgs &a, const DraftRows<TT, TD> &rows, const DraftState &st, bool minus, uint32_t c0,
+                                           float *pv, double *x, double *d) {
     float qv[4];
     load_four(rows.target(st.accepted), c0, a.vocabulary, pv, a.target_logits ? -INFINITY : 0.f);
     if (minus && a.draft) load_four(rows.draft(st.accepted), c0, a.vocabulary, qv, a.draft_logits ? -INFINITY : 0.f);
@@ -239,7 +240,7 @@ __device__ __forceinline__ void draft_left(const DraftArgs &a, const DraftRows<T
             if (a.draft)
                 y[j] = a.draft_logits ? (at[4 + j] < -1000.0 ? 0.0 : e[4 + j]) * st.inv_q : (double)qv[j];
             else
-                y[j] = c0 + j == id ? 1.0 : 0.0;
+                y[j] = c0 + j == st.id ? 1.0 : 0.0;
         }
         const double left = x[j] - y[j];
         d[j] = left <= 0.0 ? 0.0 : left;
@@ -252,7 +253,7 @@ __device__ __forceinline__ void draft_left(const DraftArgs &a, const DraftRows<T
 template <class TT, class TD>
 __device__ __forceinline__ DraftState draft_decide(const DraftArgs &a, uint32_t s, bool write) {
     __shared__ DraftRow row_of[2 * DRAFT_MOST + 1];  // the target's rows, then the drafter's
-    __shared__ uint32_t good[DRAFT_MOST];
+    __shared__ uint32_t good[DRAFT_MOST], refused_id;
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63, length = draft_length(a, s), i = threadIdx.x;
     const DraftRows<TT, TD> rows{a, s};
     // thread i: the drafted token i
@@ -285,10 +286,14 @@ __device__ __forceinline__ DraftState draft_decide(const DraftArgs &a, uint32_t 
     __syncthreads();
     const uint64_t refusals = ~__ballot(lane < length && good[lane]);
     const uint32_t n = min(length, refusals ? (uint32_t)__builtin_ctzll(refusals) : 64u);
+    if (i == n && n < length) refused_id = id;
+    __syncthreads();
     const DraftRow &q = row_of[min(length + 1 + n, 2 * length)];
     DraftState st;
     st.accepted = n;
     st.refused = n < length;
+    st.id = n < length ? refused_id : DRAFT_NONE;
+    st.pad = 0;
     st.max_p = row_of[n].max;
     st.inv_p = row_of[n].inv;
     st.max_q = q.max;
@@ -329,10 +334,9 @@ __global__ __launch_bounds__(FUSED ? 1024 : 256) void draft_rest_kernel(DraftArg
         st = draft_decide<TT, TD>(a, s, part == 0);
     else
         st = a.states[s];
-    const uint32_t id = st.refused ? a.ids[(uint64_t)s * a.drafts + st.accepted] : DRAFT_NONE;
     float pv[4];
     double x[4], d[4];
-    draft_left(a, rows, st, st.refused, id, part * STEPS * DRAFT_STEP + 4 * threadIdx.x, pv, x, d);
+    draft_left(a, rows, st, st.refused != 0, part * STEPS * DRAFT_STEP + 4 * threadIdx.x, pv, x, d);
     const double rest = wave_sum_f64((d[0] + d[1]) + (d[2] + d[3])), all = wave_sum_f64((x[0] + x[1]) + (x[2] + x[3]));
     if (lane == 0) {
         sums[0][wave] = rest;
@@ -356,7 +360,6 @@ __global__ __launch_bounds__(256) void draft_token_kernel(DraftArgs a) {
     const DraftState st = a.states[s];
     const uint32_t n = st.accepted;
     const double u = (double)a.u[(uint64_t)s * (a.drafts + 1) + a.drafts];
-    const uint32_t refused_id = st.refused ? a.ids[(uint64_t)s * a.drafts + n] : DRAFT_NONE;
     if (wave == 0) {
         double rest = 0.0, all = 0.0;
         constexpr int HELD = 4;  // steps per lane that are read once
@@ -429,7 +432,7 @@ __global__ __launch_bounds__(256) void draft_token_kernel(DraftArgs a) {
     const uint32_t c0 = step * DRAFT_STEP + 4 * threadIdx.x;
     float pv[4];
     double x[4], d[4];
-    draft_left(a, rows, st, st.refused && left, refused_id, c0, pv, x, d);
+    draft_left(a, rows, st, st.refused && left, c0, pv, x, d);
     const double sum = (d[0] + d[1]) + (d[2] + d[3]), scan = wave_scan_f64(sum);
     if (lane == 63) swave[wave] = scan;
     __syncthreads();
