@@ -318,11 +318,16 @@ int oco_fp8_quantize(const void *x, oco_dtype x_dtype, uint32_t rows, uint32_t k
                      float *scales, oco_stream stream);
 
 /* Y[m, n] = X[m, k] W^T (+ bf16(bias)) of e4m3 operands with f32
- * accumulation: the exact products of a block of 128 columns are summed on the
- * matrix cores and enter the f32 sum times both scales.
+ * accumulation: the products of a block of 128 columns are summed on the
+ * matrix cores and enter the f32 sum times both scales.  f32 outputs, and
+ * products of up to 64 rows where the few-row kernel runs, keep every bit of
+ * the products (1e-8 of the block's sum of magnitudes).  16-bit outputs of
+ * more rows run on the 8-bit matrix instruction, which drops what lies under
+ * 2^-13 of the largest of eight consecutive products: 1.5e-5 on normal data,
+ * 7 * 2^-13 of the largest product of each eight at most.
  *   w: [n, k] bytes, 16-byte aligned; w_scales: f32 [ceil(n / 128)][ceil(k / 128)]
  *   codes, scales: rows as oco_fp8_quantize or oco_block_norm writes them
- *   p: k (a multiple of 16), n, m, has_bias (0 or 1); dense only
+ *   p: k (a multiple of 16, at most 4194304), n, m, has_bias (0 or 1); dense only
  *   y: f32, bf16 or f16; workspace: oco_fp8_matmul_workspace(p) bytes, 16-byte
  *      aligned (NULL if that is 0); calls sharing one must be ordered on one
  *      stream, two captured graphs that share one included. */
@@ -360,7 +365,7 @@ int oco_router(const void *x, oco_dtype x_dtype, const float *w, const float *bi
  *     groups, go to the lowest index.  c is formed in 64 bits; without a bias
  *     the order is that of the logits;
  *   - weight = scale * s, divided by the sum of the chosen s if renormalize
- *     (0 where that sum is 0).
+ *     (0 where that sum is 0), in 64 bits; scores under 2^-1000 count as 0.
  * A logit of -Inf is an expert that is not available: its score is 0, it
  * ranks behind every other (whatever its bias), and it is chosen, with weight
  * 0, only where fewer than k others are left.  A NaN or +Inf logit makes the
@@ -583,13 +588,15 @@ int oco_argmax_f32_ws(const float *logits, uint32_t n, uint32_t *out, void *work
  *     p_L; it is the first whose running sum in index order passes u[drafts]
  *     times the whole sum.
  * Rows hold logits, p = softmax(row / temperature), where -Inf is probability
- * 0, or probabilities (temperature does not apply to them).  Temperature 0
- * is greedy: p_i is 1 at the row's first largest value, draft and uniforms
- * are not read.  Decisions are made in 64 bits, on rows' sums of f32
- * exponentials (relative error about 1e-8).  A row without a distribution (a
- * NaN or +Inf, or nothing above zero) ends its sequence there: the token is
- * 0xffffffff and its probability NaN.  A drafted id past the vocabulary is
- * refused.
+ * 0, or probabilities (temperature does not apply to them, and a value under 0
+ * counts as 0).  The temperature is 2^-126 to 2^64, or 0 for greedy: p_i is 1
+ * at the row's first largest value, draft and uniforms are not read.
+ * Decisions are made in 64 bits, on rows' sums of f32 exponentials (relative
+ * error about 1e-8).  A row without a distribution (a NaN or +Inf, or nothing
+ * above zero) ends its sequence there: the token is 0xffffffff and its
+ * probability NaN; rows of probabilities are read, and so seen, at the drafted
+ * ids and in the rows that the last token is drawn from.  A drafted id past
+ * the vocabulary is refused.
  *   target: [sequences][drafts + 1] rows of vocabulary values, target_stride apart
  *   draft: [sequences][drafts] rows or NULL; draft_ids: u32 [sequences][drafts]
  *   uniforms: f32 [sequences][drafts + 1]
@@ -597,7 +604,8 @@ int oco_argmax_f32_ws(const float *logits, uint32_t n, uint32_t *out, void *work
  *   accepted tokens, the drawn one, then 0xffffffff
  *   probabilities: f32 [sequences][drafts + 1] or NULL: p_i(tokens[i]), 0 past them
  *   workspace: oco_draft_verify_workspace bytes (0 for a description that is
- *   refused), 16-byte aligned; calls sharing one must be ordered. */
+ *   refused), 16-byte aligned; calls sharing one must be ordered
+ *   accepted, tokens and probabilities lie apart from draft_ids, lengths and uniforms. */
 typedef enum oco_draft_values { OCO_DRAFT_LOGITS = 0, OCO_DRAFT_PROBABILITIES = 1 } oco_draft_values;
 #define OCO_DRAFT_MAX 64u
 typedef struct oco_draft {

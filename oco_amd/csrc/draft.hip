@@ -199,7 +199,7 @@ __global__ __launch_bounds__(256) void draft_greedy_kernel(DraftArgs a) {
     const DraftRows<float, float> rows{a, s};
     for (uint32_t i = wave; i <= length; i += 4) {
         const DraftRow r = draft_row(rows.target_parts(i), draft_first(rows.target_parts(i), a), a);
-        if ((threadIdx.x & 63) == 0) best[i] = r.inv == r.inv ? r.at : DRAFT_NONE;
+        if ((threadIdx.x & 63) == 0) best[i] = r.inv == r.inv && (a.target_logits || r.max > 0.f) ? r.at : DRAFT_NONE;
     }
     __syncthreads();
     uint32_t n = 0;  // drafts that are their row's first maximum, from the front
@@ -243,7 +243,7 @@ __device__ __forceinline__ void draft_left(const DraftArgs &a, const DraftRows<T
                 y[j] = c0 + j == st.id ? 1.0 : 0.0;
         }
         const double left = x[j] - y[j];
-        d[j] = left <= 0.0 ? 0.0 : left;
+        d[j] = left <= 0.0 ? left * 0.0 : left;  // an infinite q: NaN
         x[j] = x[j] <= 0.0 ? 0.0 : x[j];
     }
 }
@@ -280,7 +280,7 @@ __device__ __forceinline__ DraftState draft_decide(const DraftArgs &a, uint32_t 
         // an id past the vocabulary has no probability; without a draft's distribution q is 1
         const double pr = id < a.vocabulary ? draft_value(pd, a.target_logits, p.max, p.inv, a.c) : 0.0;
         const double qr = id < a.vocabulary && a.draft ? draft_value(qd, a.draft_logits, q.max, q.inv, a.c) : 1.0;
-        good[i] = (double)u * qr < pr;
+        good[i] = (double)u * qr < pr && pr < __builtin_inf();
         pd = (float)pr;
     }
     __syncthreads();
@@ -516,7 +516,9 @@ static const char *draft_problem(const oco_draft *p) {
     if (p->vocabulary == 0 || p->vocabulary >= 0x80000000u) return "the vocabulary is empty or past 2^31";
     if (p->target_values > OCO_DRAFT_PROBABILITIES || p->draft_values > OCO_DRAFT_PROBABILITIES) return "unknown kind of values";
     if (p->target_dtype > OCO_DT_F16 || p->draft_dtype > OCO_DT_F16) return "unknown type";
-    if (!(p->temperature >= 0.f) || !(p->temperature <= 3.0e38f)) return "the temperature is negative or not finite";
+    // the exponents' factor log2(e) / T and its remainder are f32, and -1e30 of it is an exponential of 0
+    if (p->temperature != 0.f && !(p->temperature >= 0x1p-126f && p->temperature <= 0x1p64f))
+        return "the temperature is neither 0 nor in 2^-126 .. 2^64";
     if ((p->target_stride && p->target_stride < p->vocabulary) || (p->draft_stride && p->draft_stride < p->vocabulary))
         return "a row stride under the vocabulary";
     const DraftLayout l = draft_layout(p);
@@ -541,6 +543,14 @@ extern "C" int oco_draft_verify(const void *target, const void *draft, const uin
     const bool greedy = p->temperature == 0.f;
     if (!target || !accepted || !tokens || (p->drafts && !draft_ids) || (!greedy && !uniforms))
         return fail(OCO_ERR_INVALID, "oco_draft_verify: null pointer");
+    // the first sequences' outputs are there before the last ones' inputs are read
+    const uint64_t counts = (uint64_t)p->sequences * 4, places = counts * (p->drafts + 1);
+    const void *const in[3] = {draft_ids, lengths, greedy ? nullptr : uniforms}, *const out[3] = {accepted, tokens, probabilities};
+    const uint64_t in_bytes[3] = {counts * p->drafts, counts, places}, out_bytes[3] = {counts, places, places};
+    for (int i = 0; i < 3; i++)
+        for (int o = 0; o < 3; o++)
+            if (in[i] && out[o] && (uintptr_t)in[i] < (uintptr_t)out[o] + out_bytes[o] && (uintptr_t)out[o] < (uintptr_t)in[i] + in_bytes[i])
+                return fail(OCO_ERR_INVALID, "oco_draft_verify: an output lies over the drafted ids, the lengths or the random numbers");
     const DraftLayout l = draft_layout(p);
     if (!workspace || ((uintptr_t)workspace & 15u) || workspace_bytes < l.bytes)
         return fail(OCO_ERR_INVALID, "oco_draft_verify: workspace of %llu bytes, need %llu, 16-byte aligned",

@@ -458,7 +458,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8TileArgs t
         if (col < a.n) {
             float bias[OUT];
 #pragma unroll
-            for (int j = 0; j < OUT; j++) bias[j] = a.bias && ta.parts == 1 ? round_bf16(a.bias[min(col + j, a.n - 1)]) : 0.f;
+            for (int j = 0; j < OUT; j++) bias[j] = 0.f;
+            if (a.bias && ta.parts == 1)
+#pragma unroll
+                for (int j = 0; j < OUT; j++) bias[j] = round_bf16(a.bias[min(col + j, a.n - 1)]);
             void *const y = ta.parts > 1 ? (void *)(ta.sums + (uint64_t)part * a.m * a.n) : a.y;
             const uint32_t dtype = ta.parts > 1 ? (uint32_t)OCO_DT_F32 : a.y_dtype;
 #pragma unroll

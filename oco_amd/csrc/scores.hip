@@ -276,22 +276,24 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void scores_kernel(ScoresArgs a) 
         }
     }
 
-    float w = 0.f;
+    // in 64 bits: scores that f32 cannot hold still have ratios
+    double w = 0.0;
     if (lane < a.k) {
         const float logit = RowIO<T>::one(z + chosen);
         const double x = ((double)logit - from) * rate;
         double e;
         exp2_clamped<12, 1>(&x, &e);
-        w = logit > -INFINITY && logit < INFINITY ? (float)(a.sigmoid ? recip_f64(1.0 + e) : e * inv) : 0.f;
+        const bool some = logit > -INFINITY && logit < INFINITY && (a.sigmoid ? x < 1000.0 : x > -1000.0);
+        w = some ? a.sigmoid ? recip_f64(1.0 + e) : e * inv : 0.0;
     }
-    float factor = a.scale;
+    double factor = (double)a.scale;
     if (a.renormalize) {
-        const float sum = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_sum(w))));
-        factor = sum > 0.f ? a.scale / sum : 0.f;
+        const double sum = wave_sum_f64(w);
+        factor = sum > 0.0 ? factor / sum : 0.0;
     }
     if (lane < a.k) {
         a.ids[token * a.k + lane] = chosen;
-        a.weights[token * a.k + lane] = bad ? __uint_as_float(0x7fc00000u) : w * factor;
+        a.weights[token * a.k + lane] = bad ? __uint_as_float(0x7fc00000u) : (float)(w * factor);
     }
 }
 

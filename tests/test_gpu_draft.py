@@ -14,6 +14,8 @@ def distribution(row, logits, temperature):
     if temperature == 0:
         if np.isnan(row).any() or (row == np.inf).any() or not (row > -np.inf).any():
             return None
+        if not logits and not row.max() > 0:
+            return None
         p = np.zeros_like(row)
         p[int(np.argmax(row))] = 1
         return p
@@ -44,11 +46,11 @@ def verify(target, draft, ids, lengths, u, t_logits, d_logits, temperature):
             else:
                 q = distribution(draft[s, n], d_logits, temperature)
             pd, qd = (p[d] if d < V else 0.0), (1.0 if d >= V else np.nan if q is None else q[d])
-            if (0 if temperature == 0 else np.float64(u[s, n])) * qd < pd and (temperature > 0 or pd == 1):
+            if (0 if temperature == 0 else np.float64(u[s, n])) * qd < pd < np.inf and (temperature > 0 or pd == 1):
                 tokens[s, n], probs[s, n] = d, pd
                 n += 1
                 continue
-            rest = None if q is None else np.maximum(p - q, 0)
+            rest = None if q is None else np.where(np.isinf(q), np.nan, np.maximum(p - q, 0))
             if q is None or np.isnan(rest).any():
                 p = None
             break
@@ -202,6 +204,32 @@ def test_rows_without_a_distribution_end_their_sequence(lib, bad, temperature):
         d2 = rng.normal(size=d.shape)
         d2[3, 1, 7] = bad
         run(lib, t, d2, ids, None, u)
+
+
+def test_rows_of_probabilities_without_a_distribution(lib):
+    """Infinite or missing probabilities: at a drafted id, in the row that a
+    token is drawn from, in the drafter's; greedy rows of zeros."""
+    rng = np.random.default_rng(14)
+    t, _, ids, u = sample(rng, 5, 2, 4200)
+    t = softmax(t)
+    d = t[:, :2].copy()
+    t[0, 0, ids[0, 0]] = np.inf
+    t[1, 2, 4199] = np.inf
+    t[2, 2] = 0.0
+    d[3, 1, ids[3, 1]] = np.inf
+    got = run(lib, t, d, ids, None, u, False, False)
+    assert [list(r).index(NONE) for r in got[1][:4]] == [0, 2, 2, 1]
+    t[4, 0] = 0.0
+    got = run(lib, t, None, t.argmax(2)[:, :2], None, u, False, temperature=0.0)
+    assert [int(x) for x in got[0]] == [0, 2, 2, 2, 0] and list(got[1][:, 2]) == [NONE, NONE, NONE, got[1][3, 2], NONE]
+
+
+@pytest.mark.parametrize("temperature", [2.0 ** -126, 2.0 ** 64])
+def test_the_ends_of_the_temperatures(lib, temperature):
+    rng = np.random.default_rng(15)
+    t, d, ids, u = sample(rng, 4, 2, 4200)
+    t[:, :, 4000:] = -np.inf
+    run(lib, t, d, ids, None, u, temperature=temperature)
 
 
 def test_greedy_takes_the_first_of_equal_values(lib):

@@ -147,6 +147,18 @@ def test_extreme_logits(lib):
     check(lib, z[:1], 8, True, renormalize=False)
 
 
+def test_scores_under_the_range_of_f32_keep_their_ratios(lib):
+    rng = np.random.default_rng(10)
+    z = rng.normal(size=(5, 48)) - 120.0
+    check(lib, z, 8, True)  # sigmoids of 1e-52
+    bias = np.zeros(48, np.float32)
+    bias[8:16] = 1.0
+    z[:, 0] = 0.0  # the softmax is all on an expert that the bias leaves out
+    check(lib, z, 8, False, bias=bias)
+    check(lib, z, 8, True, 6, 1, True, bias=bias)
+    check(lib, z, 8, False, bias=bias, renormalize=False)
+
+
 def test_close_scores_are_told_apart(lib):
     """Sums of score and bias that differ by less than an f32 step."""
     z = np.zeros((1, 64))

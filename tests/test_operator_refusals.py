@@ -115,7 +115,7 @@ def draft(**over):
 def test_draft_verify():
     L = oco.load_library()
 
-    def call(p, target=FAKE, rows=FAKE, ids=FAKE, u=FAKE, acc=FAKE, tok=FAKE, work=FAKE, bytes_=1 << 30):
+    def call(p, target=FAKE, rows=FAKE, ids=FAKE, u=FAKE, acc=0x2000, tok=0x3000, work=FAKE, bytes_=1 << 30):
         return L.oco_draft_verify(target, rows, ids, None, u, acc, tok, None, ctypes.byref(p), work, bytes_, None)
     bad = [(dict(drafts=65), "too many drafts"), (dict(vocabulary=0), "vocabulary"), (dict(vocabulary=1 << 31), "vocabulary"),
            (dict(target_values=2), "kind"), (dict(draft_values=2), "kind"), (dict(target_dtype=3), "type"), (dict(draft_dtype=9), "type"),
@@ -133,3 +133,19 @@ def test_draft_verify():
     refused(call(draft(), work=ODD), "workspace")
     refused(L.oco_draft_verify(*[FAKE] * 8, None, FAKE, 1 << 30, None), "null description")
     assert call(draft(sequences=0), target=None) == 0
+
+
+def test_draft_verify_apart():
+    """Outputs over the ids, the lengths or the random numbers; temperatures whose exponents f32 cannot hold."""
+    L = oco.load_library()
+
+    def call(acc, tok, prob, p=None):  # 2 sequences of 3: ids 24 bytes, lengths 8, random numbers 32
+        return L.oco_draft_verify(FAKE, FAKE, 0x10000, 0x20000, 0x30000, acc, tok, prob, ctypes.byref(p or draft()), FAKE, 0, None)
+    for acc, tok, prob in ((0x20000, 0x50000, 0x60000), (0x20004, 0x50000, None), (0x40000, 0x10000, None), (0x40000, 0x10000 - 28, None),
+                           (0x40000, 0x50000, 0x30000), (0x30000 + 28, 0x50000, None), (0x40000, 0x20000, None)):
+        refused(call(acc, tok, prob), "lies over")
+    for acc, tok, prob in ((0x20008, 0x50000, 0x60000), (0x40000, 0x10000 - 32, 0x30020), (0x20000 - 8, 0x10018, None)):
+        refused(call(acc, tok, prob), "workspace")
+    refused(call(0x40000, 0x50000, 0x30000, draft(temperature=0.0)), "workspace")  # greedy reads no random numbers
+    for t in (2.0 ** -127, 2.0 ** 65, 1e-45):
+        refused(call(0x40000, 0x50000, None, draft(temperature=t)), "temperature")
