@@ -41,18 +41,19 @@ struct QuantArgs {
     uint64_t stride;
 };
 
-// 16 threads per block of 128 columns, four consecutive blocks of a row per wavefront.
+// 16 threads per block of 128 columns, four consecutive blocks of a row per
+// wavefront.  Bound by memory: 2048 x 4096 bf16 in 6.8 us (25 MB, 3.7 TB/s);
+// two or four such sets per wavefront with their loads ahead take 7.7 and 8.5.
 template <class T>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs a) {
-    const uint64_t unit = (uint64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const uint64_t row = unit / a.blocks;
-    const uint32_t b = (uint32_t)(unit % a.blocks), c0 = FP8_BLOCK * b + 8 * (threadIdx.x & 15);
+    const uint32_t unit = blockIdx.x * 16 + (threadIdx.x >> 4), row = unit / a.blocks, b = unit - row * a.blocks;
+    const uint32_t c0 = FP8_BLOCK * b + 8 * (threadIdx.x & 15);
     const bool live = row < a.rows;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, scale;
     if (live) load_run((const T *)a.x + row * a.stride, c0, a.k, v);
     const uint2 q = fp8_block(v, scale);
     if (live && c0 < a.k) {
-        *reinterpret_cast<uint2 *>(a.codes + row * a.k + c0) = q;
+        *reinterpret_cast<uint2 *>(a.codes + (uint64_t)row * a.k + c0) = q;
         if ((threadIdx.x & 15) == 0) a.scales[(uint64_t)b * a.rows + row] = scale;
     }
 }
@@ -484,12 +485,14 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(Fp8TileArgs ta) {
     for (uint64_t at = 4 * ((uint64_t)blockIdx.x * 256 + threadIdx.x); at < size; at += 1024ull * gridDim.x) {
         float v[4];
         const uint32_t live = (uint32_t)min(size - at, (uint64_t)4);
+        uint32_t col = a.bias ? (uint32_t)(at % a.n) : 0;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             v[j] = 0.f;
             if (j < (int)live) {
                 for (uint32_t p = 0; p < ta.parts; p++) v[j] += ta.sums[p * size + at + j];
-                if (a.bias) v[j] += round_bf16(a.bias[(at + j) % a.n]);
+                if (a.bias) v[j] += round_bf16(a.bias[col]);
+                col = col + 1 == a.n ? 0 : col + 1;
             }
         }
         fp8_put4(a.y, a.y_dtype, at, v, live);
@@ -515,8 +518,8 @@ extern "C" int oco_fp8_quantize(const void *x, oco_dtype x_dtype, uint32_t rows,
     a.k = k;
     a.blocks = (k + FP8_BLOCK - 1) / FP8_BLOCK;
     a.stride = x_stride ? x_stride : k;
-    const uint64_t groups = ((uint64_t)rows * a.blocks + 15) / 16;
-    if (groups > 0x7fffffffull) return fail(OCO_ERR_INVALID, "oco_fp8_quantize: %u rows of %u", rows, k);
+    const uint64_t units = (uint64_t)rows * a.blocks;
+    if (units > 0xfffff000ull) return fail(OCO_ERR_INVALID, "oco_fp8_quantize: %u rows of %u", rows, k);
     void (*fn)(QuantArgs);
     switch (x_dtype) {
     case OCO_DT_F32: fn = fp8_quantize_kernel<float>; break;
@@ -524,7 +527,7 @@ extern "C" int oco_fp8_quantize(const void *x, oco_dtype x_dtype, uint32_t rows,
     case OCO_DT_F16: fn = fp8_quantize_kernel<f16_t>; break;
     default: return fail(OCO_ERR_UNSUPPORTED, "oco_fp8_quantize: rows of type %d", (int)x_dtype);
     }
-    hipLaunchKernelGGL(fn, dim3((uint32_t)groups), dim3(256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(fn, dim3((uint32_t)((units + 15) / 16)), dim3(256), 0, (hipStream_t)stream, a);
     return launch_check("oco_fp8_quantize");
 }
 
