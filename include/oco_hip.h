@@ -516,9 +516,10 @@ int oco_add_norm(void *x, const void *y, const float *w, void *out, uint32_t row
  *   v     = y / sqrt(mean(y^2) + epsilon) * (post_w + weight_offset), or y without post_w
  *   x_out = x + scale * g * v, rounded to x_dtype; g = 1, gate, sigmoid(gate) or tanh(gate)
  *   out   = x_out / sqrt(mean(x_out^2) + epsilon) * (pre_w + weight_offset), of the rounded x_out
- * in f32.  pre_w comes with `out`, with `codes` and `scales`, or with all
- * three; without it only x_out is written.  codes / scales: the rows of
- * oco_fp8_quantize, of the f32 values that `out` rounds (n % 16 == 0).
+ * in f32, in 64 bits with `codes` (the gate in f32).  pre_w comes with `out`,
+ * with `codes` and `scales`, or with all three; without it only x_out is
+ * written.  codes / scales: rows as oco_fp8_quantize writes them, of the
+ * values that `out` rounds (n % 16 == 0).
  *   x, x_out: rows of x_dtype, x_stride elements apart (x_out may be x)
  *   y, out: rows of dtype (out may be y where their strides agree)
  *   gate: rows of dtype; gate_rows consecutive rows share one (0: all rows do)

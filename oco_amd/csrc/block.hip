@@ -8,7 +8,10 @@
 //     out = x' / sqrt(mean(x'^2) + epsilon) * (pre_w + offset)
 //
 // x' is rounded to the residual's type and the second norm reads the rounded
-// values, as oco_add_norm does.  Everything between is f32.
+// values, as oco_add_norm does.  Everything between is f32; with 8-bit rows
+// the values between and the sums over the threads are 64-bit, since one value
+// in a million lies within the f32 roundings of a border between two codes
+// (512 x 2880 with a gate per row: 10.4 us, 9.3 in f32).
 //
 // Bound by memory: x, y and the gate are read once, x' and out written once.
 // A row stays in its threads' registers (runs of eight columns per thread,
@@ -31,11 +34,15 @@ struct BlockArgs {
     float scale, epsilon, offset;
 };
 
-// The sum over a row's T threads, in every one of them (fixed order).
-template <int T>
-__device__ __forceinline__ float row_sum(float s, float *part) {
-    s = wave_sum(s);  // one lane's of it: the order of the additions differs between lanes
-    if constexpr (T == 64) s = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(s)));
+// 1 / sqrt(mean + epsilon) from the T threads' sums of squares of a row, in every one of them (fixed order).
+template <int T, class V>
+__device__ __forceinline__ V row_inverse(const BlockArgs &a, float mine, V *part) {
+    // one lane's of it: the order of the additions differs between lanes
+    V s;
+    if constexpr (sizeof(V) == 8)
+        s = wave_sum_f64((double)mine);
+    else
+        s = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_sum(mine))));
     if constexpr (T > 64) {
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
         __syncthreads();
@@ -43,7 +50,10 @@ __device__ __forceinline__ float row_sum(float s, float *part) {
 #pragma unroll
         for (int w = 1; w < T / 64; w++) s += part[w];
     }
-    return s;
+    if constexpr (sizeof(V) == 8)
+        return rsqrt_f64(__builtin_fma(s, recip_f64((double)a.n), (double)a.epsilon));
+    else
+        return 1.0f / sqrtf(s / (float)a.n + a.epsilon);
 }
 
 __device__ __forceinline__ float gate_value(float g, uint32_t kind) {
@@ -65,29 +75,32 @@ __device__ __forceinline__ void block_load_out(const BlockArgs &a, uint32_t c0, 
     if (a.pre_w) load_run(a.pre_w, c0, a.n, w.pre);
 }
 
-// x' of one run of columns (rounded), from the run's v.
-template <class XT>
-__device__ __forceinline__ void block_add(const BlockArgs &a, const float *xv, float *v, const BlockRun &w, float inv) {
-    if (a.post_w)
+// x' of one run of columns (rounded), from the run's v; V: the type between.
+template <class XT, class V>
+__device__ __forceinline__ void block_add(const BlockArgs &a, const float *xv, float *v, const BlockRun &w, V inv) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = v[j] * inv * (w.post[j] + a.offset);
-    if (a.kind != OCO_GATE_NONE)
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] *= gate_value(w.gate[j], a.kind);
-#pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = RowIO<XT>::round(fmaf(a.scale, v[j], xv[j]));
+    for (int j = 0; j < 8; j++) {
+        V d = (V)v[j];
+        if (a.post_w) d = d * inv * ((V)w.post[j] + (V)a.offset);
+        if (a.kind != OCO_GATE_NONE) d *= (V)gate_value(w.gate[j], a.kind);
+        v[j] = RowIO<XT>::round((float)__builtin_elementwise_fma((V)a.scale, d, (V)xv[j]));
+    }
 }
 
-// out (and its 8-bit form) of one run of columns of x'.
-template <class YT>
-__device__ __forceinline__ void block_out(const BlockArgs &a, const float *v, const BlockRun &w, uint64_t row, uint32_t c0, float inv) {
+// out of one run of columns of x', and its 8-bit form where V is 64-bit.
+template <class YT, class V>
+__device__ __forceinline__ void block_out(const BlockArgs &a, const float *v, const BlockRun &w, uint64_t row, uint32_t c0, V inv) {
+    V d[8];
     float o[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) o[j] = c0 + j < a.n ? v[j] * inv * (w.pre[j] + a.offset) : 0.f;
+    for (int j = 0; j < 8; j++) {
+        d[j] = c0 + j < a.n ? (V)v[j] * (sizeof(V) == 8 ? (V)1 : inv) * ((V)w.pre[j] + (V)a.offset) : (V)0;
+        o[j] = sizeof(V) == 8 ? c0 + j < a.n ? (float)(d[j] * inv) : 0.f : (float)d[j];
+    }
     if (a.out) store_run((YT *)a.out + row * a.out_stride, c0, a.n, o);
-    if (a.codes) {  // 16 consecutive threads hold a block of 128 columns
+    if constexpr (sizeof(V) == 8) {  // 16 consecutive threads hold a block of 128 columns
         float scale;
-        const uint2 q = fp8_block(o, scale);
+        const uint2 q = fp8_block(d, inv, o, scale);
         if (c0 < a.n) {
             *reinterpret_cast<uint2 *>(a.codes + row * a.n + c0) = q;
             if (c0 % FP8_BLOCK == 0) a.scales[(uint64_t)(c0 / FP8_BLOCK) * a.rows + row] = scale;
@@ -101,19 +114,20 @@ __device__ __forceinline__ void block_out(const BlockArgs &a, const float *v, co
 // one memory latency stands before the first sum and none behind it (8192 x
 // 4096: 56.7 us with one run of 512 threads, 59.9 with two of 256); with two
 // runs the registers cost more than that gives (66 us).
-template <class XT, class YT, int T, int P>
+template <class XT, class YT, class V, int T, int P>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
-    __shared__ float part[2][T / 64];
+    __shared__ V part[2][T / 64];
     const uint32_t t = T == 64 ? threadIdx.x & 63 : threadIdx.x;
     const uint64_t row = T == 64 ? blockIdx.x * 4ull + (threadIdx.x >> 6) : blockIdx.x;
     if (T == 64 && row >= a.rows) return;
     const XT *x = (const XT *)a.x + row * a.x_stride;
     const YT *y = (const YT *)a.y + row * a.y_stride;
-    const YT *gate = (const YT *)a.gate + (a.gate_rows ? row / a.gate_rows : 0) * a.gate_stride;
+    const YT *gate = (const YT *)a.gate + (uint64_t)(a.gate_rows ? (uint32_t)row / a.gate_rows : 0) * a.gate_stride;
     XT *x_out = (XT *)a.x_out + row * a.x_stride;
     if constexpr (P > 0) {
         constexpr bool EARLY = P == 1;
-        float xv[P][8], v[P][8], s = 0.f, inv = 1.f;
+        float xv[P][8], v[P][8], s = 0.f;
+        V inv = 1;
         BlockRun w[EARLY ? P : 1];
 #pragma unroll
         for (int p = 0; p < P; p++) load_run(y, 8 * (t + T * p), a.n, v[p]);
@@ -130,28 +144,29 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
             for (int p = 0; p < P; p++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) s = fmaf(v[p][j], v[p][j], s);
-            inv = 1.0f / sqrtf(row_sum<T>(s, part[0]) / (float)a.n + a.epsilon);
+            inv = row_inverse<T, V>(a, s, part[0]);
         }
         s = 0.f;
 #pragma unroll
         for (int p = 0; p < P; p++) {
             const uint32_t c0 = 8 * (t + T * p);
             if constexpr (!EARLY) block_load_add(a, gate, c0, w[0]);
-            block_add<XT>(a, xv[p], v[p], w[EARLY ? p : 0], inv);
+            block_add<XT, V>(a, xv[p], v[p], w[EARLY ? p : 0], inv);
             store_run(x_out, c0, a.n, v[p]);
 #pragma unroll
             for (int j = 0; j < 8; j++)
                 if (c0 + j < a.n) s = fmaf(v[p][j], v[p][j], s);
         }
         if (!a.pre_w) return;
-        inv = 1.0f / sqrtf(row_sum<T>(s, part[1]) / (float)a.n + a.epsilon);
+        inv = row_inverse<T, V>(a, s, part[1]);
 #pragma unroll
         for (int p = 0; p < P; p++) {
             if constexpr (!EARLY) block_load_out(a, 8 * (t + T * p), w[0]);
-            block_out<YT>(a, v[p], w[EARLY ? p : 0], row, 8 * (t + T * p), inv);
+            block_out<YT, V>(a, v[p], w[EARLY ? p : 0], row, 8 * (t + T * p), inv);
         }
     } else {
-        float xv[8], v[8], s = 0.f, inv = 1.f;
+        float xv[8], v[8], s = 0.f;
+        V inv = 1;
         BlockRun w;
         if (a.post_w) {
             for (uint32_t c0 = 8 * t; c0 < a.n; c0 += 8 * T) {
@@ -159,26 +174,26 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) s = fmaf(v[j], v[j], s);
             }
-            inv = 1.0f / sqrtf(row_sum<T>(s, part[0]) / (float)a.n + a.epsilon);
+            inv = row_inverse<T, V>(a, s, part[0]);
         }
         s = 0.f;
         for (uint32_t c0 = 8 * t; c0 < a.n; c0 += 8 * T) {
             load_run(y, c0, a.n, v);
             load_run(x, c0, a.n, xv);
             block_load_add(a, gate, c0, w);
-            block_add<XT>(a, xv, v, w, inv);
+            block_add<XT, V>(a, xv, v, w, inv);
             store_run(x_out, c0, a.n, v);
 #pragma unroll
             for (int j = 0; j < 8; j++)
                 if (c0 + j < a.n) s = fmaf(v[j], v[j], s);
         }
         if (!a.pre_w) return;
-        inv = 1.0f / sqrtf(row_sum<T>(s, part[1]) / (float)a.n + a.epsilon);
+        inv = row_inverse<T, V>(a, s, part[1]);
         // every thread of a block of 128 columns takes part in its maximum
         for (uint32_t c0 = 8 * t; c0 - c0 % FP8_BLOCK < a.n; c0 += 8 * T) {
             load_run((const XT *)x_out, c0, a.n, v);  // this thread's own columns
             block_load_out(a, c0, w);
-            block_out<YT>(a, v, w, row, c0, inv);
+            block_out<YT, V>(a, v, w, row, c0, inv);
         }
     }
 }
@@ -189,9 +204,9 @@ typedef void (*BlockFn)(BlockArgs);
 // registers up to 32768.  Rows of up to 1024 columns, many of them: a wavefront
 // per row with two runs and no barrier (1024 bf16 columns, 4096 rows: 11.3 us,
 // 13.1 with a workgroup per row; 512 rows: 5.7 against 4.2).
-template <class XT, class YT>
+template <class XT, class YT, class V>
 static BlockFn block_pick(uint32_t n, uint32_t rows, int &threads) {
-#define PICK(T, P) (threads = T, block_kernel<XT, YT, T, P>)
+#define PICK(T, P) (threads = T, block_kernel<XT, YT, V, T, P>)
     if (n <= 512) return PICK(64, 1);
     if (n <= 1024 && rows > 1024) return PICK(64, 2);
     if (n <= 2048) return PICK(256, 1);
@@ -238,11 +253,11 @@ extern "C" int oco_block_norm(const void *x, const void *y, void *x_out, const v
     a.scale = p->scale; a.epsilon = p->epsilon; a.offset = p->weight_offset;
     int threads = 0;
     BlockFn fn = nullptr;
-    if (p->x_dtype == OCO_DT_F32 && p->dtype == OCO_DT_F32) fn = block_pick<float, float>(p->n, p->rows, threads);
-    else if (p->x_dtype == OCO_DT_F32 && p->dtype == OCO_DT_BF16) fn = block_pick<float, bf16_t>(p->n, p->rows, threads);
-    else if (p->x_dtype == OCO_DT_F32 && p->dtype == OCO_DT_F16) fn = block_pick<float, f16_t>(p->n, p->rows, threads);
-    else if (p->x_dtype == OCO_DT_BF16 && p->dtype == OCO_DT_BF16) fn = block_pick<bf16_t, bf16_t>(p->n, p->rows, threads);
-    else if (p->x_dtype == OCO_DT_F16 && p->dtype == OCO_DT_F16) fn = block_pick<f16_t, f16_t>(p->n, p->rows, threads);
+    if (p->x_dtype == OCO_DT_F32 && p->dtype == OCO_DT_F32) fn = codes ? block_pick<float, float, double>(p->n, p->rows, threads) : block_pick<float, float, float>(p->n, p->rows, threads);
+    else if (p->x_dtype == OCO_DT_F32 && p->dtype == OCO_DT_BF16) fn = codes ? block_pick<float, bf16_t, double>(p->n, p->rows, threads) : block_pick<float, bf16_t, float>(p->n, p->rows, threads);
+    else if (p->x_dtype == OCO_DT_F32 && p->dtype == OCO_DT_F16) fn = codes ? block_pick<float, f16_t, double>(p->n, p->rows, threads) : block_pick<float, f16_t, float>(p->n, p->rows, threads);
+    else if (p->x_dtype == OCO_DT_BF16 && p->dtype == OCO_DT_BF16) fn = codes ? block_pick<bf16_t, bf16_t, double>(p->n, p->rows, threads) : block_pick<bf16_t, bf16_t, float>(p->n, p->rows, threads);
+    else if (p->x_dtype == OCO_DT_F16 && p->dtype == OCO_DT_F16) fn = codes ? block_pick<f16_t, f16_t, double>(p->n, p->rows, threads) : block_pick<f16_t, f16_t, float>(p->n, p->rows, threads);
     else
         return fail(OCO_ERR_UNSUPPORTED, "oco_block_norm: residual type %u with rows of type %u (an f32 residual, or both alike)",
                     p->x_dtype, p->dtype);

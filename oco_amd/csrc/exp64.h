@@ -1,4 +1,4 @@
-// 64-bit exponentials for decisions that must not hang on a rounding.
+// 64-bit values for decisions that must not hang on a rounding.
 #pragma once
 #include "common.h"
 
@@ -38,6 +38,21 @@ __device__ __forceinline__ double exp2_f64(double x) {
     double y;
     exp2_clamped<D, 1>(&x, &y);
     return x < -1000.0 ? 0.0 : x < 1000.0 ? y : x + __builtin_inf();
+}
+
+// 1 / d for a normal d whose reciprocal is normal: the hardware's estimate and two Newton steps.
+__device__ __forceinline__ double recip_f64(double d) {
+    double r = __builtin_amdgcn_rcp(d);
+    r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+    return __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+}
+// 1 / sqrt(d) likewise; 0 and Inf give Inf and 0.
+__device__ __forceinline__ double rsqrt_f64(double d) {
+    const double e = __builtin_amdgcn_rsq(d);
+    double r = e;
+#pragma unroll
+    for (int i = 0; i < 2; i++) r = __builtin_fma(0.5 * r, __builtin_fma(-d * r, r, 1.0), r);
+    return d > 0.0 && d < __builtin_inf() ? r : e;
 }
 
 // 64-bit values across a wavefront by DPP and permlane swaps: a step is a few

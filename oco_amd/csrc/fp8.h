@@ -2,7 +2,7 @@
 // bits, largest value 448) with one f32 scale per 128 columns, and their
 // products.
 #pragma once
-#include "common.h"
+#include "exp64.h"
 
 namespace oco {
 
@@ -48,6 +48,45 @@ __device__ __forceinline__ uint2 fp8_block(const float *v, float &scale) {
     for (int j = 0; j < 8; j++) {
         const float num = v[j] * 0.875f, first = num * inv;
         q[j] = copysignf(fmaf(fmaf(-first, den, num), inv, first), first);  // -0 stays -0
+    }
+    int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
+    int hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], hi, true);
+    return make_uint2((uint32_t)lo, (uint32_t)hi);
+}
+
+// The same for f32 rows that were computed in 64 bits, v[j] times `factor`:
+// the codes are those of the 64-bit quotients, so that a value next to a
+// border between two codes does not hang on the roundings of a norm.  Whether
+// all are finite is seen on the f32 values o.
+__device__ __forceinline__ uint2 fp8_block(const double *v, double factor, const float *o, float &scale) {
+    uint32_t m = 0;
+    double top = 0.0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        m = max(m, __float_as_uint(o[j]) & 0x7fffffffu);
+        top = fmax(top, fabs(v[j]));
+    }
+    m = row16_max(m);
+    top = fmax(top, dpp_f64<0xB1>(top));
+    top = fmax(top, dpp_f64<0x4E>(top));
+    top = fmax(top, dpp_f64<0x124>(top));
+    top = fmax(top, dpp_f64<0x128>(top)) * factor;
+    if (m >= 0x7f800000u) {
+        scale = __uint_as_float(0x7fc00000u);
+        return make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+    }
+    top = fmax(top, (double)FP8_FLOOR);
+    scale = (float)(top * (1.0 / 448.0));
+    const double rate = 448.0 * factor * recip_f64(top);
+    float q[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        // to f32 by chopping, with the last bit set where that is inexact: the code is then rounded once
+        const uint64_t b = (uint64_t)__double_as_longlong(v[j] * rate);
+        const uint32_t lo = (uint32_t)b;
+        q[j] = (float)words_f64((lo & 0xe0000000u) | (lo & 0x1fffffffu ? 0x20000000u : 0u), (uint32_t)(b >> 32));
     }
     int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
     lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);

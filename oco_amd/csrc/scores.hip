@@ -36,13 +36,6 @@ struct ScoresArgs {
 
 constexpr int SCORE_WAVES = 4;
 
-// 1 / d for d >= 1: the hardware's estimate and two Newton steps.
-__device__ __forceinline__ double recip_f64(double d) {
-    double r = __builtin_amdgcn_rcp(d);
-    r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
-    return __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
-}
-
 // Values as integers that order alike (-0 as +0); 0 is below every number, -Inf included.
 __device__ __forceinline__ uint32_t order_f32(float v) {
     const uint32_t b = __float_as_uint(v + 0.0f);
