@@ -20,6 +20,9 @@
 // row gives its maximum and its sum of exponentials; the decisions follow
 // from those, and only the two rows at the first refused draft are read
 // again.  Rows of probabilities are read at the drafted tokens and there alone.
+// 32 sequences of 7 drafts, 151936 f32 logits on both sides: rows 47 us (291 MB,
+// 6.2 TB/s), decisions 4.7, what is left 15.5 (64-bit exponentials: bound by
+// issue), token 8.7.  One sequence: three launches of 3.1, 6.2 and 6.2 us, all latency.
 #include "exp64.h"
 #include "rows.h"
 

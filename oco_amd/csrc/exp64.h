@@ -99,17 +99,19 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
     return lane_f64(words_f64(l[0], h[0]) + words_f64(l[1], h[1]), 0);
 }
 
-// Maximum and minimum of 32-bit words over a wavefront, in every lane.
+// Maximum and minimum of 32-bit words over a wavefront, uniform: within rows of
+// 16 by rotations, then each row takes the last lane of the rows before it
+// (f of a value with itself is that value, so lanes without a source keep
+// theirs); lane 63 has it all.
 template <class F>
 __device__ __forceinline__ uint32_t wave_reduce_u32(uint32_t v, F f) {
-    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));
-    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));
-    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
-    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));
-    auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    v = f(a[0], a[1]);
-    a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return f(a[0], a[1]);
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0xB1, 0xf, 0xf, true));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x4E, 0xf, 0xf, true));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x124, 0xf, 0xf, true));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x128, 0xf, 0xf, true));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x142, 0xf, 0xf, false));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x143, 0xf, 0xf, false));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     return wave_reduce_u32(v, [](uint32_t a, uint32_t b) { return max(a, b); });

@@ -245,6 +245,11 @@ static Fp8RowsFn fp8_rows_pick(uint32_t m, uint32_t n, uint32_t &cols, uint32_t 
 //
 // Workgroups stay and take tile after tile: the next tile's first stage is
 // requested before this one's results are written.
+//
+// 4096 x 12288 x 4096 to bf16 on 256-tiles: 196 us, 2.1 PFLOP/s; the matrix
+// cores are busy for 46% of the clocks, the four FMAs behind each product and
+// the waits at the barrier take the rest.  1999 x 4096 x 12288 to f32 on
+// 128-tiles: 190 us, 1.06 PFLOP/s, with the conversions to f16 beside the products.
 
 // 16 (4) bytes per lane from a buffer to LDS at `to` + 16 (4) lane (`to` is uniform).
 __device__ __forceinline__ void to_lds16(__amdgpu_buffer_rsrc_t rs, void *to, uint32_t at, uint32_t base) {

@@ -14,7 +14,9 @@
 // them is chosen must not depend on how exp was rounded.  Without a bias
 // c_e orders as z_e does, and the logits' own bits decide.
 //
-// Bound by issue: one wavefront per token.  A lane holds J consecutive experts
+// Bound by issue, one wavefront per token: 8192 tokens of 256 experts with a
+// bias and groups in 13.0 us, about 800 instructions each (the 8.9 MB would
+// take 1.9); one token of 128 in 2.6.  A lane holds J consecutive experts
 // and sorts them once; a round takes the largest head of the 64 lanes.  WIDE
 // (a bias, or groups ranked by sums): 64-bit scores of every expert; else the
 // rounds run on the logits' own 32 bits and only the chosen get a score.

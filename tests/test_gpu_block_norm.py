@@ -183,3 +183,9 @@ def test_zero_rows_and_extreme_values(lib):
     assert not codes.download(np.uint8).any() and np.all(scales.download(np.float32) == 2.0 ** -126)
     check(lib, 3, 700, "bf16", "bf16", spread=2.0 ** 40)
     check(lib, 3, 700, "bf16", "bf16", spread=2.0 ** -40)
+
+
+@pytest.mark.parametrize("rows,n", [(1, 16), (3, 512), (1030, 1024), (2, 2048), (3, 2064), (2, 4096), (1, 8192), (2, 16384), (1, 32768), (1, 40016)])
+def test_8_bit_rows_at_every_width(lib, rows, n):
+    check(lib, rows, n, "f32", "bf16", kind=1, codes=True)
+    check(lib, rows, n, "bf16", "bf16", codes=True, inplace=True)
