@@ -818,16 +818,24 @@ class Fp8Matrix:
         if input % 16:
             raise ValueError(f"input={input} is not whole groups of 16")
         self.values, self.scales, self.input, self.output = values, scales, input, output
-        self._workspace = None
+        self._workspaces = {}  # by stream, the largest last; none is freed while a captured graph may use it
 
-    def apply(self, codes, scales, y, rows: int, y_dtype=DType.F32, bias=None, stream=None):
-        """Y = X W^T for rows of oco_fp8_quantize or oco_block_norm."""
+    def apply(self, codes, scales, y, rows: int, y_dtype=DType.F32, bias=None, workspace=None, stream=None):
+        """Y = X W^T for rows of oco_fp8_quantize or oco_block_norm.  Without a
+        `workspace` (a DeviceBuffer of fp8_matmul_workspace bytes) the matrix
+        keeps one per stream; a first call that needs one is made outside a
+        capture, and graphs that run on other streams than they were captured
+        on bring their own."""
         p = Matrix(self.input, self.output, rows, 0, 1, 1, 1 if bias is not None else 0)
         need = fp8_matmul_workspace(p)
-        if need and (self._workspace is None or self._workspace.nbytes < need):
-            self._workspace = DeviceBuffer(need)
-        fp8_matmul(self.values, self.scales, codes, scales, y, p, y_dtype, bias, self._workspace if need else None, need,
-                   stream)
+        if need and workspace is None:
+            handle = _stream(stream)
+            kept = self._workspaces.setdefault(getattr(handle, "value", handle), [])
+            if not kept or kept[-1].nbytes < need:
+                kept.append(DeviceBuffer(need))
+            workspace = kept[-1]
+        fp8_matmul(self.values, self.scales, codes, scales, y, p, y_dtype, bias, workspace if need else None,
+                   workspace.nbytes if need else 0, stream)
 
 
 class ExpertBank:

@@ -204,6 +204,43 @@ def test_quantized_rows_of_a_matrix(lib):
     assert np.all(np.abs(got - x @ wv.T) <= (step @ np.abs(wv).T) * 1.01)
 
 
+def test_workspaces_of_a_matrix(lib):
+    """K in parts through Fp8Matrix: a captured call keeps its workspace when
+    a larger eager one follows, two streams have their own, and one that the
+    caller brings is used and checked."""
+    rng = np.random.default_rng(21)
+    n, k = 72, 784
+    x, w, xs, ws = operands(rng, 300, n, k)
+    few = np.ascontiguousarray(xs[:, :70])
+    want_all, mag_all = product(x, w, xs, ws)
+    bound = (256 + len(xs) + 12) * U * mag_all
+    W = lib.Fp8Matrix(dev(lib, w), dev(lib, ws), k, n)
+    xb, xsb, fewb = dev(lib, x), dev(lib, xs), dev(lib, few)
+    y, ya, yb = (lib.DeviceBuffer(m * n * 4) for m in (300, 70, 300))
+    a, b = lib.Stream(), lib.Stream()
+    with lib.overridden(lib.Knob.FP8, (128, 3)):
+        W.apply(xb, fewb, ya, 70, stream=a)
+        a.sync()
+        graph = lib.Graph(a, lambda: W.apply(xb, fewb, ya, 70, stream=a))
+        for _ in range(3):
+            ya.upload(np.zeros(70 * n, np.float32), 0)
+            W.apply(xb, xsb, y, 300, stream=a)  # grows the stream's workspace
+            W.apply(xb, xsb, yb, 300, stream=b)
+            graph.launch()
+            a.sync()
+            b.sync()
+            assert np.all(np.abs(ya.download(np.float32).reshape(70, n) - want_all[:70]) <= bound[:70])
+            for full in (y, yb):
+                assert np.all(np.abs(full.download(np.float32).reshape(300, n) - want_all) <= bound)
+        own = lib.DeviceBuffer(lib.fp8_matmul_workspace(lib.Matrix(k, n, 300, 0, 1, 1, 0)))
+        y.upload(np.zeros(300 * n, np.float32), 0)
+        W.apply(xb, xsb, y, 300, workspace=own)
+        lib.synchronize()
+        assert np.all(np.abs(y.download(np.float32).reshape(300, n) - want_all) <= bound)
+        with pytest.raises(Exception, match="workspace"):
+            W.apply(xb, xsb, y, 300, workspace=lib.DeviceBuffer(1024))
+
+
 @pytest.mark.parametrize("plan", [(0,), (128, 1), (128, 2), (128, 3), (128, 16), (256, 1), (256, 5)])
 @pytest.mark.parametrize("m,n,k", [(61, 333, 2064), (64, 40, 1296), (300, 520, 400), (513, 260, 144)])
 def test_every_kernel_and_k_split(lib, plan, m, n, k):
