@@ -11,7 +11,7 @@
 // values, as oco_add_norm does.  Everything between is f32; with 8-bit rows
 // the values between and the sums over the threads are 64-bit, since one value
 // in a million lies within the f32 roundings of a border between two codes
-// (512 x 2880 with a gate per row: 10.4 us, 9.3 in f32).
+// (512 x 2880 with a gate per row: 10.2 us, 9.3 in f32).
 //
 // Bound by memory: x, y and the gate are read once, x' and out written once.
 // A row stays in its threads' registers (runs of eight columns per thread,
@@ -56,9 +56,25 @@ __device__ __forceinline__ V row_inverse(const BlockArgs &a, float mine, V *part
         return 1.0f / sqrtf(s / (float)a.n + a.epsilon);
 }
 
+// 1 / d for d >= 1 (0 for Inf).
+__device__ __forceinline__ float recip_f32(float d) {
+    const float r = __builtin_amdgcn_rcpf(d);
+    return d < INFINITY ? fmaf(fmaf(-d, r, 1.f), r, r) : r;
+}
+// tanh: its Taylor series to g^21 up to 0.625 (relative remainder 0.16^11), 1 - 2 / (exp(2 |g|) + 1) beyond, within
+// 3 x 2^-24.  A gate row that all rows share is formed again for each row, so its instructions count: 8192 x 4096
+// bf16 70.9 us with tanh and 66.6 with the sigmoid, 73.1 and 72.1 by tanhf and a division, 52.5 without a gate.
 __device__ __forceinline__ float gate_value(float g, uint32_t kind) {
-    if (kind == OCO_GATE_SIGMOID) return 1.0f / (1.0f + expf(-g));
-    if (kind == OCO_GATE_TANH) return tanhf(g);
+    if (kind == OCO_GATE_SIGMOID) return recip_f32(1.0f + expf(-g));
+    if (kind == OCO_GATE_TANH) {
+        constexpr float C[10] = {9.69153796e-05f, -0.000239129114f, 0.000590027441f, -0.00145583439f, 0.00359212804f, -0.00886323553f, 0.0218694885f, -0.053968254f, 0.133333333f, -0.333333333f};
+        const float s = g * g, t = fabsf(g);
+        float p = C[0];
+#pragma unroll
+        for (int i = 1; i < 10; i++) p = fmaf(p, s, C[i]);
+        const float far = fmaf(-2.f, recip_f32(1.f + __builtin_amdgcn_exp2f(t * 2.88539008f)), 1.f);
+        return t < 0.625f ? fmaf(g * s, p, g) : copysignf(far, g);
+    }
     return g;
 }
 
@@ -201,7 +217,9 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
 typedef void (*BlockFn)(BlockArgs);
 
 // Threads per row and runs per thread: one run up to 8192 columns, the row in
-// registers up to 32768.  Rows of up to 1024 columns, many of them: a wavefront
+// registers up to 32768.  The threads fit the row, as those without columns
+// take places on the compute unit (5339 x 2502 bf16: 36 us
+// with 320, 43 with 512; 3855 x 4352: 44 with 640, 49 with 1024).  Rows of up to 1024 columns, many of them: a wavefront
 // per row with two runs and no barrier (1024 bf16 columns, 4096 rows: 11.3 us,
 // 13.1 with a workgroup per row; 512 rows: 5.7 against 4.2).
 template <class XT, class YT, class V>
@@ -209,9 +227,14 @@ static BlockFn block_pick(uint32_t n, uint32_t rows, int &threads) {
 #define PICK(T, P) (threads = T, block_kernel<XT, YT, V, T, P>)
     if (n <= 512) return PICK(64, 1);
     if (n <= 1024 && rows > 1024) return PICK(64, 2);
-    if (n <= 2048) return PICK(256, 1);
-    if (n <= 4096) return PICK(512, 1);
-    if (n <= 8192) return PICK(1024, 1);
+    const uint32_t runs = (n + 7) / 8;
+    if (runs <= 256) return PICK(256, 1);
+    if (runs <= 320) return PICK(320, 1);
+    if (runs <= 448) return PICK(448, 1);
+    if (runs <= 512) return PICK(512, 1);
+    if (runs <= 640) return PICK(640, 1);
+    if (runs <= 768) return PICK(768, 1);
+    if (runs <= 1024) return PICK(1024, 1);
     if (n <= 16384) return PICK(1024, 2);
     if (n <= 32768) return PICK(1024, 4);
     return PICK(1024, 0);

@@ -189,3 +189,9 @@ def test_zero_rows_and_extreme_values(lib):
 def test_8_bit_rows_at_every_width(lib, rows, n):
     check(lib, rows, n, "f32", "bf16", kind=1, codes=True)
     check(lib, rows, n, "bf16", "bf16", codes=True, inplace=True)
+
+
+@pytest.mark.parametrize("n", [2049, 2560, 2561, 3584, 3585, 5120, 5121, 6144, 6145, 8185])
+def test_threads_that_fit_the_row(lib, n):
+    check(lib, 5, n, "bf16", "bf16", kind=3)
+    check(lib, 3, n // 16 * 16, "f32", "f16", kind=2, gate_rows=2, codes=True)
