@@ -218,10 +218,11 @@ typedef void (*BlockFn)(BlockArgs);
 
 // Threads per row and runs per thread: one run up to 8192 columns, the row in
 // registers up to 32768.  The threads fit the row, as those without columns
-// take places on the compute unit (5339 x 2502 bf16: 36 us
-// with 320, 43 with 512; 3855 x 4352: 44 with 640, 49 with 1024).  Rows of up to 1024 columns, many of them: a wavefront
-// per row with two runs and no barrier (1024 bf16 columns, 4096 rows: 11.3 us,
-// 13.1 with a workgroup per row; 512 rows: 5.7 against 4.2).
+// take places on the compute unit (5339 x 2502 bf16: 36 us with 320, 43 with
+// 512; 3855 x 4352: 44 with 640, 49 with 1024).  Rows of up to 1024 columns,
+// many of them: a wavefront per row with two runs and no barrier (1024 bf16
+// columns, 4096 rows: 11.3 us, 13.1 with a workgroup per row; 512 rows: 5.7
+// against 4.2).
 template <class XT, class YT, class V>
 static BlockFn block_pick(uint32_t n, uint32_t rows, int &threads) {
 #define PICK(T, P) (threads = T, block_kernel<XT, YT, V, T, P>)
