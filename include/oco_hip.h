@@ -319,9 +319,9 @@ int oco_fp8_quantize(const void *x, oco_dtype x_dtype, uint32_t rows, uint32_t k
 
 /* Y[m, n] = X[m, k] W^T (+ bf16(bias)) of e4m3 operands with f32
  * accumulation: the products of a block of 128 columns are summed on the
- * matrix cores and enter the f32 sum times both scales.  f32 outputs, and
- * products of up to 64 rows where the few-row kernel runs, keep every bit of
- * the products (1e-8 of the block's sum of magnitudes).  16-bit outputs of
+ * matrix cores and enter the f32 sum times both scales.  f32 and f16 outputs,
+ * and products of up to 64 rows where the few-row kernel runs, keep every bit
+ * of the products (1e-8 of the block's sum of magnitudes).  bf16 outputs of
  * more rows run on the 8-bit matrix instruction, which drops what lies under
  * 2^-13 of the largest of eight consecutive products: 1.5e-5 on normal data,
  * 7 * 2^-13 of the largest product of each eight at most.

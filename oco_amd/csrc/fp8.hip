@@ -229,9 +229,13 @@ static Fp8RowsFn fp8_rows_pick(uint32_t m, uint32_t n, uint32_t &cols, uint32_t 
 // BM activation rows x BN weight rows per workgroup of WM x WN wavefronts.  A
 // stage is one block of K: both operands' 128 bytes per row go from global
 // memory straight to LDS (16 bytes per lane), two stages deep, one barrier
-// per stage.  HALF: the f16 matrix instruction on converted codes (f32
-// outputs), else the 8-bit one, whose dropped bits (2^-13 of a group of eight
-// products, at most) lie under the rounding of the 16-bit outputs it is used for.
+// per stage.  HALF: the f16 matrix instruction on converted codes (f32 and f16
+// outputs), else the 8-bit one, for bf16 outputs alone: of the largest of eight
+// products it drops at most 7 * 2^-13, less than half a bf16 step (2^-9 to 2^-8)
+// but more than half an f16 one (2^-12 to 2^-11).  Where a bf16 output is small
+// because its products cancel, what is dropped can pass its rounding, as the
+// rounding of f32 sums does at 2^-24 of the products.  4096 x 12288 x 4096 to
+// f16: 382 us, where the 8-bit instruction would take 209.
 //
 // Which weight row meets which row of the matrix instruction is free: row j
 // of tile t is weight row 4 TN (j / 4) + 4 t + j % 4 of the wavefront's, so
@@ -548,9 +552,9 @@ constexpr uint32_t FP8_FEW = 64;  // the few-row kernel's limit
 // 4096, 1 to 1024 rows; the estimates are within about 15% of them):
 //  * few rows: the weight stream at 5.3 TB/s, and 0.2 ns for each product of
 //    16 x 16 x 128 past the first 16 rows' (those hide behind the stream);
-//  * 128-tiles: a block of K takes 0.82 us (f32 outputs, on the f16
+//  * 128-tiles: a block of K takes 0.82 us (f32 and f16 outputs, on the f16
 //    instruction: 1.17) with a workgroup per compute unit, 1.08 (1.45) with two;
-//  * 256-tiles (16-bit outputs): 2.15 us, one workgroup per compute unit;
+//  * 256-tiles (bf16 outputs): 2.15 us, one workgroup per compute unit;
 //  * K parts: a launch, 0.4 us each, and their sums written and read at 3 TB/s.
 static Fp8Plan fp8_plan(uint32_t m, uint32_t n, uint32_t k, bool half) {
     const uint32_t blocks = (k + FP8_BLOCK - 1) / FP8_BLOCK;
@@ -627,7 +631,7 @@ extern "C" int oco_fp8_matmul(const uint8_t *w, const float *w_scales, const uin
     // 31-bit offsets inside a workgroup's rows
     if (p->k > 0x400000u || p->n > 0x7fffff00u || p->m > 0x7fffff00u)
         return fail(OCO_ERR_INVALID, "oco_fp8_matmul: %u x %u x %u", p->m, p->n, p->k);
-    const bool half = y_dtype == OCO_DT_F32;
+    const bool half = y_dtype != OCO_DT_BF16;
     const Fp8Plan plan = fp8_plan(p->m, p->n, p->k, half);
     const uint64_t need = fp8_need(plan, p);
     if (need && (!workspace || ((uintptr_t)workspace & 15u) || workspace_bytes < need))

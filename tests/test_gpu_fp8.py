@@ -280,3 +280,25 @@ def test_workgroups_that_take_several_tiles(lib, m, n):
         if y_dtype != "f32":  # the largest of a group of eight products is at most their sum of magnitudes
             lost = 7 * 2.0 ** -13 * mag
         assert np.all(np.abs(got - want) <= (256 + len(xs) + 12) * U * mag + HALF[y_dtype] * 1.01 * np.abs(want) + lost)
+
+
+@pytest.mark.parametrize("m,n,k", [(65, 500, 400), (130, 333, 2880), (300, 129, 1296), (600, 513, 272), (1030, 255, 2064)])
+@pytest.mark.parametrize("plan", [(), (128, 1), (128, 3), (256, 1)])
+def test_f16_outputs_keep_every_bit_of_the_products(lib, m, n, k, plan):
+    """f16 rounds at 2^-11, which the bits that the 8-bit matrix instruction
+    drops can exceed: f16 outputs are those of the f32 sums, at any number of rows."""
+    say("fp8_matmul f16", m, n, k, plan)
+    rng = np.random.default_rng(m + n + k)
+    x, w, xs, ws = operands(rng, m, n, k)
+    xs, ws = xs * np.float32(2.0 ** -8), ws * np.float32(2.0 ** -4)
+    want, mag = product(x, w, xs, ws)
+    with lib.overridden(lib.Knob.FP8, plan):
+        need = lib.fp8_matmul_workspace(lib.Matrix(k, n, m, 0, 1, 1, 0))
+        out = Guarded(lib, m * n * 2)
+        lib.fp8_matmul(dev(lib, w), dev(lib, ws), dev(lib, x), dev(lib, xs), out.ptr, lib.Matrix(k, n, m, 0, 1, 1, 0), CODE["f16"],
+                       workspace=lib.DeviceBuffer(max(need, 16)), workspace_bytes=need)
+        lib.synchronize()
+    got, fits = values(out.read(np.uint8), "f16", (m, n)), np.abs(want) < 65000
+    assert fits.mean() > 0.9
+    bound = (2 * 128 + len(xs) + 12) * U * mag + HALF["f16"] * 1.01 * np.abs(want) + LEAST["f16"]  # as check()'s
+    assert np.all((np.abs(got - want) <= bound)[fits]), float(np.max(np.abs(got - want)[fits] / bound[fits]))
