@@ -177,8 +177,10 @@ __device__ __forceinline__ DraftPart draft_first(const DraftPart *parts, const D
     return p;
 }
 
+// A probability as it counts: 0 for a value under 0 (a NaN stays).
+__device__ __forceinline__ double draft_probability(float v) { return v < 0.f ? 0.0 : (double)v; }
 __device__ __forceinline__ double draft_value(float v, bool logits, float max, double inv, double c) {
-    return logits ? exp2_f64<9>(((double)v - (double)max) * c) * inv : (double)v;
+    return logits ? exp2_f64<9>(((double)v - (double)max) * c) * inv : draft_probability(v);
 }
 
 template <class TT, class TD>
@@ -237,17 +239,16 @@ __device__ __forceinline__ void draft_left(const DraftArgs &a, const DraftRows<T
         exp2_clamped<9, 4>(at, e);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        x[j] = a.target_logits ? (at[j] < -1000.0 ? 0.0 : e[j]) * st.inv_p : (double)pv[j];
+        x[j] = a.target_logits ? (at[j] < -1000.0 ? 0.0 : e[j]) * st.inv_p : draft_probability(pv[j]);
         y[j] = 0.0;
         if (minus) {
             if (a.draft)
-                y[j] = a.draft_logits ? (at[4 + j] < -1000.0 ? 0.0 : e[4 + j]) * st.inv_q : (double)qv[j];
+                y[j] = a.draft_logits ? (at[4 + j] < -1000.0 ? 0.0 : e[4 + j]) * st.inv_q : draft_probability(qv[j]);
             else
                 y[j] = c0 + j == st.id ? 1.0 : 0.0;
         }
         const double left = x[j] - y[j];
         d[j] = left <= 0.0 ? left * 0.0 : left;  // an infinite q: NaN
-        x[j] = x[j] <= 0.0 ? 0.0 : x[j];
     }
 }
 

@@ -1,5 +1,7 @@
 """oco_draft_verify against the rule in 64 bits: counts and tokens exactly,
 probabilities within the roundings of f32 exponentials."""
+import sys
+
 import numpy as np
 import pytest
 
@@ -279,3 +281,37 @@ def test_the_result_is_distributed_as_the_target(lib):
         got = run(lib, target, np.broadcast_to(q, (S, 1, V)).copy(), np.full((S, 1), d), None, u, False, False)
         freq += q[d] * np.bincount(got[1][:, 0], minlength=V)[:V] / S
     assert np.all(np.abs(freq - p) <= 2.0 / G)
+
+
+@pytest.mark.parametrize("t_dtype,d_dtype", [("f32", "f32"), ("bf16", "f16")])
+@pytest.mark.parametrize("S", [4, 300])
+def test_values_under_zero_count_as_zero(lib, monkeypatch, S, t_dtype, d_dtype):
+    """Negative probabilities on both sides, -Inf among them, at drafted ids
+    and elsewhere: the rule on rows whose negative values are 0.  A token that
+    the target gives nothing is neither accepted nor drawn."""
+    zeroed = lambda a: None if a is None else np.where(a < 0, 0.0, a)  # noqa: E731
+    plain = verify
+    monkeypatch.setattr(sys.modules[__name__], "verify", lambda t, d, *rest: plain(zeroed(t), zeroed(d), *rest))
+    rng = np.random.default_rng(16)
+    D, V = 3, 9000
+    t, d, ids, u = sample(rng, S, D, V)
+    t, d = softmax(t), softmax(d)
+    t[:, :, ::5] *= -1
+    d[:, :, ::7] *= -1
+    t[:, :, 11], d[:, :, 13] = -np.inf, -np.inf
+    rows = np.arange(S)
+    ids[:2, 0] = 35, 70  # negative on both sides
+    ids[2, 0], ids[3, 0] = 11, 13
+    u[:2, 0] = 0.0, 0.5
+    run(lib, t, d, ids, None, u, False, False, t_dtype=t_dtype, d_dtype=d_dtype)
+    run(lib, t, None, ids, None, u, False, t_dtype=t_dtype)
+    t[:, :, ids[:, 0]] = 0.0  # refused, unless a negative q lets it in
+    d[rows, 0, ids[:, 0]] = -0.25
+    got = run(lib, t, d, ids, None, u, False, False, t_dtype=t_dtype, d_dtype=d_dtype)
+    assert not got[0].any()
+    t[:, :, :] = 0.0
+    t[:, :, 17] = 1.0
+    d[:, :, :] = -1.0
+    d[:, :, 17] = 1.0  # nothing left but what negative values would add
+    got = run(lib, t, d, np.zeros_like(ids), None, u, False, False, t_dtype=t_dtype, d_dtype=d_dtype)
+    assert np.all(got[1][:, 0] == 17)
