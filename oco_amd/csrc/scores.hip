@@ -17,9 +17,9 @@
 // Bound by issue, one wavefront per token: 8192 tokens of 256 experts with a
 // bias and groups in 12.6 us, about 780 instructions each (the 8.9 MB would
 // take 1.9); one token of 128 in 2.6.  A lane holds J consecutive experts
-// and sorts them once; a round takes the largest head of the 64 lanes.  WIDE
-// (a bias, or groups ranked by sums): 64-bit scores of every expert; else the
-// rounds run on the logits' own 32 bits and only the chosen get a score.
+// and sorts them once; a round takes the largest head of the 64 lanes.  With a
+// bias the rounds run on 64-bit keys, else on the logits' own 32 bits; then
+// scores are formed for groups ranked by sums, or of the chosen alone.
 #include "exp64.h"
 #include "rows.h"
 
@@ -37,6 +37,11 @@ struct ScoresArgs {
 };
 
 constexpr int SCORE_WAVES = 4;
+
+// What is ranked: experts and groups by their logits; groups by scores and
+// experts by their logits (scores that coincide in 64 bits, as sigmoids from
+// 37 on, still have an order); both by biased scores.
+enum class Ranked { LOGITS, GROUPS, BIASED };
 
 // A key and its expert take the next one's place, in their registers; the wait
 // states are those of a DPP read, which the compiler does not add behind asm.
@@ -86,8 +91,9 @@ __device__ __forceinline__ void merge_swap(double &first, double &second, bool w
     first = fmax(a, b);
 }
 
-template <class T, int J, bool WIDE>  // J experts per lane: J lane + j
+template <class T, int J, Ranked BY>  // J experts per lane: J lane + j
 __global__ __launch_bounds__(64 * SCORE_WAVES) void scores_kernel(ScoresArgs a) {
+    constexpr bool SCORED = BY != Ranked::LOGITS, WIDE = BY == Ranked::BIASED;
     using Key = std::conditional_t<WIDE, uint64_t, uint32_t>;
     __shared__ double choice_lds[SCORE_WAVES][64 * J];  // groups that are not whole lanes
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -121,7 +127,7 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void scores_kernel(ScoresArgs a) 
     if (!a.sigmoid) m = wave_max_f32(m);
     const double from = a.sigmoid ? 0.0 : (double)m, rate = a.sigmoid ? -LOG2E : LOG2E;
     double s[J];
-    if (WIDE || !(a.sigmoid || a.renormalize)) {
+    if (SCORED || !(a.sigmoid || a.renormalize)) {
         double x[J];
 #pragma unroll
         for (int j = 0; j < J; j++) x[j] = ((double)v[j] - from) * rate;
@@ -145,7 +151,7 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void scores_kernel(ScoresArgs a) 
 
     float bias[J];
 #pragma unroll
-    for (int j = 0; j < J; j++) bias[j] = WIDE && a.bias && J * lane + j < a.experts ? a.bias[J * lane + j] : 0.f;
+    for (int j = 0; j < J; j++) bias[j] = WIDE && J * lane + j < a.experts ? a.bias[J * lane + j] : 0.f;
 
     // what is ranked, as integers: 0 for an expert that cannot be chosen
     Key key[J];
@@ -157,13 +163,14 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void scores_kernel(ScoresArgs a) 
     for (int j = 0; j < J; j++) {
         const uint32_t e = J * lane + j;
         double c = (double)v[j];
-        if constexpr (WIDE) {
-            c = s[j] + (double)bias[j];
+        if constexpr (SCORED) {
+            c = WIDE ? s[j] + (double)bias[j] : s[j];
             if (!(v[j] > -INFINITY) || c != c) c = -__builtin_inf();
-            key[j] = e < a.experts ? order_f64(c) : 0;
-        } else {
-            key[j] = e < a.experts ? order_f32(v[j]) : 0;
         }
+        if constexpr (WIDE)
+            key[j] = e < a.experts ? order_f64(c) : 0;
+        else
+            key[j] = e < a.experts ? order_f32(v[j]) : 0;
         if (ranked) {
             if (in_lanes) {
                 second = fmax(second, fmin(first, c));
@@ -300,13 +307,19 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void scores_kernel(ScoresArgs a) 
 }
 
 typedef void (*ScoresFn)(ScoresArgs);
-template <class T, bool WIDE>
+template <class T, Ranked BY>
 static ScoresFn scores_pick(uint32_t experts) {
-    if (experts <= 64) return scores_kernel<T, 1, WIDE>;
-    if (experts <= 128) return scores_kernel<T, 2, WIDE>;
-    if (experts <= 256) return scores_kernel<T, 4, WIDE>;
-    if (experts <= 512) return scores_kernel<T, 8, WIDE>;
-    return scores_kernel<T, 16, WIDE>;
+    if (experts <= 64) return scores_kernel<T, 1, BY>;
+    if (experts <= 128) return scores_kernel<T, 2, BY>;
+    if (experts <= 256) return scores_kernel<T, 4, BY>;
+    if (experts <= 512) return scores_kernel<T, 8, BY>;
+    return scores_kernel<T, 16, BY>;
+}
+template <class T>
+static ScoresFn scores_pick(const ScoresArgs &a) {
+    if (a.bias) return scores_pick<T, Ranked::BIASED>(a.experts);
+    if (a.groups > 1 && a.top2) return scores_pick<T, Ranked::GROUPS>(a.experts);
+    return scores_pick<T, Ranked::LOGITS>(a.experts);
 }
 
 }  // namespace oco
@@ -343,12 +356,11 @@ extern "C" int oco_route_scores(const void *logits, oco_dtype dtype, const float
     a.sigmoid = p->score == OCO_SCORE_SIGMOID;
     a.renormalize = p->renormalize != 0;
     a.scale = p->scale;
-    const bool wide = bias || (a.groups > 1 && a.top2);
     ScoresFn fn;
     switch (dtype) {
-    case OCO_DT_F32: fn = wide ? scores_pick<float, true>(p->experts) : scores_pick<float, false>(p->experts); break;
-    case OCO_DT_BF16: fn = wide ? scores_pick<bf16_t, true>(p->experts) : scores_pick<bf16_t, false>(p->experts); break;
-    case OCO_DT_F16: fn = wide ? scores_pick<f16_t, true>(p->experts) : scores_pick<f16_t, false>(p->experts); break;
+    case OCO_DT_F32: fn = scores_pick<float>(a); break;
+    case OCO_DT_BF16: fn = scores_pick<bf16_t>(a); break;
+    case OCO_DT_F16: fn = scores_pick<f16_t>(a); break;
     default: return fail(OCO_ERR_UNSUPPORTED, "oco_route_scores: logits of type %d", (int)dtype);
     }
     hipLaunchKernelGGL(fn, dim3((uint32_t)(((uint64_t)tokens + SCORE_WAVES - 1) / SCORE_WAVES)), dim3(64 * SCORE_WAVES), 0,

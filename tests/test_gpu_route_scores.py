@@ -180,3 +180,53 @@ def test_matches_the_library_s_selection(lib):
     lib.synchronize()
     np.testing.assert_array_equal(ids2.download(np.uint32).reshape(40, 8), ids)
     np.testing.assert_allclose(probs.download(np.float32).reshape(40, 8), w, rtol=2 * 4 * 2.0 ** -8 + 2.0 ** -8 + 2.0 ** -9)
+
+
+def by_logits(z, k, sigmoid, groups, kept):
+    """Without a bias: groups by the sum of their two largest scores, experts by their logits."""
+    ids, size = [], z.shape[1] // groups
+    for row in z:
+        s = 1 / (1 + np.exp(-row)) if sigmoid else np.exp(row - row.max()) / np.exp(row - row.max()).sum()
+        two = -np.sort(-s.reshape(groups, size), 1)[:, :2].sum(1)
+        best = sorted(range(groups), key=lambda g: (-two[g], g))[:kept]
+        ids.append(sorted((e for e in range(len(row)) if e // size in best), key=lambda e: (-row[e], e))[:k])
+    return np.array(ids)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("experts,groups,kept,k", [(64, 4, 2, 8), (256, 8, 4, 8), (30, 5, 2, 6), (1024, 16, 3, 20)])
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_without_a_bias_the_order_is_that_of_the_logits(lib, sigmoid, experts, groups, kept, k, dtype):
+    """Logits whose 64-bit scores coincide (sigmoids from 37 on, what lies 700
+    and more under a softmax's largest), in groups ranked by their two best."""
+    say("route_scores by logits", sigmoid, experts, groups, dtype)
+    rng = np.random.default_rng(experts)
+    z = 100 + 100 * rng.random((7, experts)) if sigmoid else rng.normal(size=(7, experts))
+    if not sigmoid:  # two large logits per group decide its rank, the rest are far under them
+        z = z - 1500
+        for g in range(groups):
+            z[:, g * (experts // groups):g * (experts // groups) + 2] = rng.normal(size=(7, 2))
+    zb, z = stored(z, dtype)
+    p = lib.Routing(experts=experts, k=k, score=int(sigmoid), groups=groups, groups_kept=kept, group_rank=1, renormalize=1, scale=1.0)
+    ids, weights = Guarded(lib, 7 * k * 4), Guarded(lib, 7 * k * 4)
+    lib.route_scores(dev(lib, zb), 7, p, ids.ptr, weights.ptr, CODE[dtype])
+    lib.synchronize()
+    want = by_logits(z, k, sigmoid, groups, kept)
+    np.testing.assert_array_equal(ids.read(np.uint32).reshape(7, k), want)
+    w = np.ones((7, k)) if sigmoid else np.exp(np.take_along_axis(z, want, 1) - z.max(1, keepdims=True))  # sigmoids: all 1
+    np.testing.assert_allclose(weights.read(np.float32).reshape(7, k), w / w.sum(1, keepdims=True), rtol=12 * U, atol=2.0 ** -140)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_extreme_logits_in_groups(lib, sigmoid):
+    z = np.array([[500.0, 400, 300, -300, -500, 0, 1, 2], [-1000, -999, -1001, -2000, -1500, -1200, -998, -3000], [39, 40, 41, 38, 45, 44, 46, 43]])
+    say("route_scores extremes in groups", sigmoid)
+    for kept in (1, 2, 3):
+        k = 2 * kept
+        p = lib.Routing(experts=8, k=k, score=int(sigmoid), groups=4, groups_kept=kept, group_rank=1, renormalize=0, scale=1.0)
+        ids, weights = Guarded(lib, 3 * k * 4), Guarded(lib, 3 * k * 4)
+        lib.route_scores(dev(lib, stored(z, "f32")[0]), 3, p, ids.ptr, weights.ptr, 0)
+        lib.synchronize()
+        got = ids.read(np.uint32).reshape(3, k).astype(int)
+        for row, chosen in zip(z, got):  # whole groups, in the order of their logits
+            assert len({e // 2 for e in chosen}) == kept and list(chosen) == sorted(chosen, key=lambda e: (-row[e], e))
