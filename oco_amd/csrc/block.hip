@@ -9,9 +9,10 @@
 //
 // x' is rounded to the residual's type and the second norm reads the rounded
 // values, as oco_add_norm does.  Everything between is f32; with 8-bit rows
-// the values between and the sums over the threads are 64-bit, since one value
-// in a million lies within the f32 roundings of a border between two codes
-// (512 x 2880 with a gate per row: 10.2 us, 9.3 in f32).
+// the squares, their sums and the values between are 64-bit (the gate's value
+// f32), since one value in a million lies within the f32 roundings of a border
+// between two codes (512 x 2880 with a gate per row: 10.3 us, 9.3 in f32; 8192
+// x 4096 bf16: 95 us, 91 with f32 squares).
 //
 // Bound by memory: x, y and the gate are read once, x' and out written once.
 // A row stays in its threads' registers (runs of eight columns per thread,
@@ -36,11 +37,11 @@ struct BlockArgs {
 
 // 1 / sqrt(mean + epsilon) from the T threads' sums of squares of a row, in every one of them (fixed order).
 template <int T, class V>
-__device__ __forceinline__ V row_inverse(const BlockArgs &a, float mine, V *part) {
+__device__ __forceinline__ V row_inverse(const BlockArgs &a, V mine, V *part) {
     // one lane's of it: the order of the additions differs between lanes
     V s;
     if constexpr (sizeof(V) == 8)
-        s = wave_sum_f64((double)mine);
+        s = wave_sum_f64(mine);
     else
         s = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_sum(mine))));
     if constexpr (T > 64) {
@@ -124,6 +125,12 @@ __device__ __forceinline__ void block_out(const BlockArgs &a, const float *v, co
     }
 }
 
+// s + v^2 (64-bit: the square is exact).
+template <class V>
+__device__ __forceinline__ V block_square(float v, V s) {
+    return __builtin_elementwise_fma((V)v, (V)v, s);
+}
+
 // T threads per row (64: four rows per workgroup), P runs of eight columns
 // per thread; P == 0: any n, a row read again for each of its three passes.
 // A thread of one run requests its weights and gate with the rows, so that
@@ -142,8 +149,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
     XT *x_out = (XT *)a.x_out + row * a.x_stride;
     if constexpr (P > 0) {
         constexpr bool EARLY = P == 1;
-        float xv[P][8], v[P][8], s = 0.f;
-        V inv = 1;
+        float xv[P][8], v[P][8];
+        V s = 0, inv = 1;
         BlockRun w[EARLY ? P : 1];
 #pragma unroll
         for (int p = 0; p < P; p++) load_run(y, 8 * (t + T * p), a.n, v[p]);
@@ -159,10 +166,10 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
 #pragma unroll
             for (int p = 0; p < P; p++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) s = fmaf(v[p][j], v[p][j], s);
+                for (int j = 0; j < 8; j++) s = block_square<V>(v[p][j], s);
             inv = row_inverse<T, V>(a, s, part[0]);
         }
-        s = 0.f;
+        s = 0;
 #pragma unroll
         for (int p = 0; p < P; p++) {
             const uint32_t c0 = 8 * (t + T * p);
@@ -171,7 +178,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
             store_run(x_out, c0, a.n, v[p]);
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (c0 + j < a.n) s = fmaf(v[p][j], v[p][j], s);
+                if (c0 + j < a.n) s = block_square<V>(v[p][j], s);
         }
         if (!a.pre_w) return;
         inv = row_inverse<T, V>(a, s, part[1]);
@@ -181,18 +188,18 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
             block_out<YT, V>(a, v[p], w[EARLY ? p : 0], row, 8 * (t + T * p), inv);
         }
     } else {
-        float xv[8], v[8], s = 0.f;
-        V inv = 1;
+        float xv[8], v[8];
+        V s = 0, inv = 1;
         BlockRun w;
         if (a.post_w) {
             for (uint32_t c0 = 8 * t; c0 < a.n; c0 += 8 * T) {
                 load_run(y, c0, a.n, v);
 #pragma unroll
-                for (int j = 0; j < 8; j++) s = fmaf(v[j], v[j], s);
+                for (int j = 0; j < 8; j++) s = block_square<V>(v[j], s);
             }
             inv = row_inverse<T, V>(a, s, part[0]);
         }
-        s = 0.f;
+        s = 0;
         for (uint32_t c0 = 8 * t; c0 < a.n; c0 += 8 * T) {
             load_run(y, c0, a.n, v);
             load_run(x, c0, a.n, xv);
@@ -201,7 +208,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
             store_run(x_out, c0, a.n, v);
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (c0 + j < a.n) s = fmaf(v[j], v[j], s);
+                if (c0 + j < a.n) s = block_square<V>(v[j], s);
         }
         if (!a.pre_w) return;
         inv = row_inverse<T, V>(a, s, part[1]);

@@ -195,3 +195,46 @@ def test_8_bit_rows_at_every_width(lib, rows, n):
 def test_threads_that_fit_the_row(lib, n):
     check(lib, 5, n, "bf16", "bf16", kind=3)
     check(lib, 3, n // 16 * 16, "f32", "f16", kind=2, gate_rows=2, codes=True)
+
+
+def rounded_e4m3(q):
+    step = 2.0 ** (np.maximum(np.floor(np.log2(np.maximum(np.abs(q), 2.0 ** -30))), -6) - 3)
+    return np.rint(q / step) * step
+
+
+@pytest.mark.parametrize("rows,n", [(3, 144), (33, 512), (1030, 1024), (70, 2880), (9, 8192), (5, 16384), (3, 32768), (3, 40000)])
+@pytest.mark.parametrize("x_dtype,dtype,kind", [("f32", "bf16", 2), ("bf16", "bf16", 1), ("f32", "f32", 0), ("f16", "f16", 3)])
+def test_codes_and_scales_are_those_of_the_64_bit_rows(lib, rows, n, x_dtype, dtype, kind):
+    """Codes and scales from the x_out that the call returned, to the last bit
+    but where the 64-bit roundings reach a border: at most 62 additions of squares
+    (40 in a thread, 6 and 16 over the threads) and the oracle's 28, halved by the
+    root, and 18 for roots, reciprocals and products: under 64 * 2^-53 together."""
+    say("block codes", rows, n, x_dtype, dtype, kind)
+    near = 64 * 2.0 ** -53
+    rng = np.random.default_rng(rows + n)
+    xb, yb = (stored(rng.normal(size=(rows, n)) * s, t)[0] for s, t in ((4, x_dtype), (1, dtype)))
+    gb = stored(rng.normal(size=(rows, n)), dtype)[0]
+    post_w, pre_w = (1 + 0.3 * rng.normal(size=n)).astype(np.float32), (1 + 0.3 * rng.normal(size=n)).astype(np.float32)
+    x_out, codes, scales = Guarded(lib, rows * n * SIZE[x_dtype]), Guarded(lib, rows * n), Guarded(lib, -(-n // 128) * rows * 4)
+    p = lib.Block(rows=rows, n=n, x_dtype=CODE[x_dtype], dtype=CODE[dtype], gate=kind, gate_rows=1, scale=0.5, epsilon=EPS, weight_offset=0.25)
+    lib.block_norm(dev(lib, xb), dev(lib, yb), p, x_out=x_out.ptr, gate=dev(lib, gb), post_w=dev(lib, post_w), pre_w=dev(lib, pre_w),
+                   codes=codes.ptr, scales=scales.ptr)
+    lib.synchronize()
+    kept = values(x_out.read(np.uint8), x_dtype, (rows, n))
+    exact = kept / np.sqrt((kept * kept).mean(1, keepdims=True) + np.float64(np.float32(EPS))) * (pre_w.astype(np.float64) + 0.25)
+    got, s = e4m3(codes.read(np.uint8), (rows, n)), scales.read(np.float32).reshape(-1, rows)
+    for b in range(len(s)):
+        part = exact[:, 128 * b:128 * b + 128]
+        top = np.maximum(np.abs(part).max(1), 448 * 2.0 ** -126)
+        lo, hi = ((top * (1 + e) / 448).astype(np.float32) for e in (-near, near))
+        assert np.all((s[b] == lo) | (s[b] == hi))
+        q, c = 448 * part / top[:, None], got[:, 128 * b:128 * b + 128]
+        assert np.all((c == rounded_e4m3(q * (1 - near))) | (c == rounded_e4m3(q * (1 + near))))
+
+
+@pytest.mark.parametrize("spread", [2.0 ** 80, 2.0 ** -90])
+@pytest.mark.parametrize("n", [704, 40000])
+def test_8_bit_rows_of_values_whose_squares_f32_cannot_hold(lib, spread, n):
+    """With 8-bit rows the values between are 64-bit, the squares and their sums among them."""
+    check(lib, 3, n, "bf16", "bf16", spread=spread, codes=True)
+    check(lib, 3, n, "f32", "f32", kind=0, spread=spread, codes=True)
