@@ -28,7 +28,8 @@ __device__ __forceinline__ uint32_t row16_max(uint32_t v) {
 // rounded to f32 once: reciprocal, product, and one residual step, which
 // returns the rounded quotient where the reciprocal is itself rounded
 // correctly (Markstein).  A quotient on the border between two codes thus
-// stays on it.  A block that holds a NaN or an infinity has a NaN scale (its
+// stays on it.  Blocks under 2^-64 enter 2^64 times larger, as the residual of
+// those near the least normal number would be subnormal.  A block that holds a NaN or an infinity has a NaN scale (its
 // row's products are NaN) and NaN codes.
 // |v| orders by its bits: finite values, then infinity, then NaN.
 __device__ __forceinline__ uint2 fp8_block(const float *v, float &scale) {
@@ -36,17 +37,24 @@ __device__ __forceinline__ uint2 fp8_block(const float *v, float &scale) {
 #pragma unroll
     for (int j = 0; j < 8; j++) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
     m = row16_max(m);
-    const float top = fmaxf(__uint_as_float(m), FP8_FLOOR);
+    float top = fmaxf(__uint_as_float(m), FP8_FLOOR);
     if (m >= 0x7f800000u) {
         scale = __uint_as_float(0x7fc00000u);
         return make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
     }
     scale = top / 448.0f;
+    float rate = 0.875f;
+    if (__builtin_expect(__ballot(top < 0x1p-64f) != 0, 0)) {  // a branch: as selects 11.1 us for 4096 x 4096 bf16, 10.7 without
+        asm volatile("" ::: "memory");
+        const bool tiny = top < 0x1p-64f;
+        top = tiny ? top * 0x1p64f : top;
+        rate = tiny ? 0.875f * 0x1p64f : 0.875f;
+    }
     const float den = top * 0x1p-9f, inv = 1.0f / den;
     float q[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        const float num = v[j] * 0.875f, first = num * inv;
+        const float num = v[j] * rate, first = num * inv;
         q[j] = copysignf(fmaf(fmaf(-first, den, num), inv, first), first);  // -0 stays -0
     }
     int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);

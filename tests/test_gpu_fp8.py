@@ -302,3 +302,24 @@ def test_f16_outputs_keep_every_bit_of_the_products(lib, m, n, k, plan):
     assert fits.mean() > 0.9
     bound = (2 * 128 + len(xs) + 12) * U * mag + HALF["f16"] * 1.01 * np.abs(want) + LEAST["f16"]  # as check()'s
     assert np.all((np.abs(got - want) <= bound)[fits]), float(np.max(np.abs(got - want)[fits] / bound[fits]))
+
+
+@pytest.mark.parametrize("exponent", [-100, -108, -110, -115, -118, -121, -124])
+def test_blocks_of_tiny_values_are_exact_too(lib, exponent):
+    """bf16 rows whose largest value is near the least normal one, with quotients on borders between codes."""
+    say("quantize tiny", exponent)
+    rng = np.random.default_rng(-exponent)
+    rows, k = 64, 256
+    x = rng.normal(size=(rows, k)) * 2.0 ** exponent
+    top = np.abs(stored(x, "bf16")[1]).reshape(rows, 2, 128).max(2)
+    borders = np.concatenate([(2 * np.arange(8, 16) + 1) / 2 * 2.0 ** e for e in range(-9, 5)] + [(2 * np.arange(8) + 1) / 2 * 2.0 ** -9])
+    for b in range(2):  # the largest stays the largest
+        x[:, 128 * b + 1:128 * b + 100] = top[:, b:b + 1] * rng.choice(borders, (rows, 99)) / 448
+        x[:, 128 * b] = top[:, b]
+    xb, x = stored(x, "bf16")
+    codes, scales = Guarded(lib, rows * k), Guarded(lib, 2 * rows * 4)
+    lib.fp8_quantize(dev(lib, xb), rows, k, codes.ptr, scales.ptr, CODE["bf16"])
+    lib.synchronize()
+    want_codes, want_scales = quantized(x, True)
+    np.testing.assert_array_equal(scales.read(np.float32).reshape(2, rows), want_scales)
+    np.testing.assert_array_equal(codes.read(np.uint8).reshape(rows, k), want_codes)
