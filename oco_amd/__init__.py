@@ -320,6 +320,21 @@ class overridden:
         plan_override(self.knob, ())
 
 
+class Scratch:
+    """Device memory that the calls on one stream take in turn.  A buffer that
+    is too small gets a successor of at least twice its size and stays, as a
+    captured call may use it: together under four times the largest need."""
+
+    def __init__(self):
+        self.buffers = []
+
+    def at_least(self, nbytes: int) -> "DeviceBuffer":
+        last = self.buffers[-1].nbytes if self.buffers else 0
+        if last < nbytes:
+            self.buffers.append(DeviceBuffer(max(nbytes, 2 * last)))
+        return self.buffers[-1]
+
+
 class Stream:
     """One HIP stream (the reference's per-session queue, compute.rs:36-55)."""
 
@@ -328,6 +343,7 @@ class Stream:
         h = ctypes.c_void_p()
         _check(load_library().oco_stream_create(ctypes.byref(h)))
         self.handle = h
+        self.scratch = Scratch()  # lives as long as the object, which its graphs hold
 
     def sync(self):
         _check(load_library().oco_stream_sync(self.handle))
@@ -818,24 +834,33 @@ class Fp8Matrix:
         if input % 16:
             raise ValueError(f"input={input} is not whole groups of 16")
         self.values, self.scales, self.input, self.output = values, scales, input, output
-        self._workspaces = {}  # by stream, the largest last; none is freed while a captured graph may use it
+        self._scratches = {}  # of streams that are given by their handle
 
     def apply(self, codes, scales, y, rows: int, y_dtype=DType.F32, bias=None, workspace=None, stream=None):
         """Y = X W^T for rows of oco_fp8_quantize or oco_block_norm.  Without a
-        `workspace` (a DeviceBuffer of fp8_matmul_workspace bytes) the matrix
-        keeps one per stream; a first call that needs one is made outside a
-        capture, and graphs that run on other streams than they were captured
-        on bring their own."""
+        `workspace` (a DeviceBuffer of fp8_matmul_workspace bytes) a Stream
+        keeps one for all its matrices, and the matrix one for each stream that
+        is given by its handle and for the default one.  Before a capture
+        reserve() draws it, and graphs that run on other streams than they were
+        captured on bring their own."""
         p = Matrix(self.input, self.output, rows, 0, 1, 1, 1 if bias is not None else 0)
         need = fp8_matmul_workspace(p)
         if need and workspace is None:
-            handle = _stream(stream)
-            kept = self._workspaces.setdefault(getattr(handle, "value", handle), [])
-            if not kept or kept[-1].nbytes < need:
-                kept.append(DeviceBuffer(need))
-            workspace = kept[-1]
+            workspace = self._scratch(stream).at_least(need)
         fp8_matmul(self.values, self.scales, codes, scales, y, p, y_dtype, bias, workspace if need else None,
                    workspace.nbytes if need else 0, stream)
+
+    def reserve(self, rows: int, stream=None):
+        """The workspace of calls of 1 to `rows` rows on a stream (the need
+        does not rise with the rows throughout), which then draw no memory."""
+        need = max((fp8_matmul_workspace(Matrix(self.input, self.output, m, 0, 1, 1, 0)) for m in range(1, rows + 1)), default=0)
+        if need:
+            self._scratch(stream).at_least(need)
+
+    def _scratch(self, stream) -> Scratch:
+        if isinstance(stream, Stream):
+            return stream.scratch
+        return self._scratches.setdefault(getattr(stream, "value", stream), Scratch())
 
 
 class ExpertBank:
