@@ -315,3 +315,46 @@ def test_values_under_zero_count_as_zero(lib, monkeypatch, S, t_dtype, d_dtype):
     d[:, :, 17] = 1.0  # nothing left but what negative values would add
     got = run(lib, t, d, np.zeros_like(ids), None, u, False, False, t_dtype=t_dtype, d_dtype=d_dtype)
     assert np.all(got[1][:, 0] == 17)
+
+
+BATCH = dict(S=130, D=2, V=17001)  # 650 chunks of 4096: past the number that decide for themselves
+
+
+@pytest.mark.parametrize("t_dtype,d_dtype,draft,temperature,ragged", [
+    ("f32", "f32", "logits", 1.0, False), ("bf16", "f32", "logits", 0.7, True), ("bf16", "f32", None, 0.8, True), ("f16", "bf16", "probabilities", 1.0, True),
+    ("f32", "f16", "logits", 1.3, True), ("f32", "f32", None, 0.0, True)])
+def test_large_batches(lib, t_dtype, d_dtype, draft, temperature, ragged):
+    """Decisions in a launch of their own: vocabularies of several chunks and
+    of steps that are not whole, masked, absent and NaN rows."""
+    rng = np.random.default_rng(17)
+    t, d, ids, u = sample(rng, **BATCH)
+    lengths = rng.integers(0, 4, BATCH["S"]) if ragged else None
+    t[5, :, :4096] = -np.inf
+    t[6, 1, 17000] = np.nan
+    t[7, 0] = -np.inf
+    t[8, :, 17000] = 60.0  # all of it in the last, partial step
+    ids[9, 0] = 17001
+    d = None if draft is None else softmax(d) if draft == "probabilities" else d
+    run(lib, t, d, ids, lengths, u, True, draft != "probabilities", temperature, t_dtype, d_dtype, pad=(3, 0))
+
+
+@pytest.mark.parametrize("t_logits,draft", [(True, "logits"), (True, None), (False, "probabilities")])
+def test_a_batch_equals_its_sequences_in_small_calls(lib, t_logits, draft):
+    rng = np.random.default_rng(18)
+    t, d, ids, u = sample(rng, **BATCH)
+    t = t if t_logits else softmax(t)
+    d = None if draft is None else softmax(d) if draft == "probabilities" else d
+    whole = run(lib, t, d, ids, None, u, t_logits, draft == "logits")
+    for s in range(0, BATCH["S"], 13):
+        part = run(lib, t[s:s + 13], None if d is None else d[s:s + 13], ids[s:s + 13], None, u[s:s + 13], t_logits, draft == "logits")
+        for a, b in zip(whole, part):
+            np.testing.assert_array_equal(a[s:s + 13], b)
+
+
+@pytest.mark.parametrize("S", [1, 3])
+def test_more_chunks_than_lanes_in_few_sequences(lib, S):
+    """Decisions in every workgroup, on rows of more than 64 chunks."""
+    rng = np.random.default_rng(19)
+    t, d, ids, u = sample(rng, S, 2, 300001, sharp=1.0)
+    run(lib, t, d, ids, None, u)
+    run(lib, t, None, t[:, :2].argmax(2), None, u, temperature=0.2)
