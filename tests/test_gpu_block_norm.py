@@ -238,3 +238,10 @@ def test_8_bit_rows_of_values_whose_squares_f32_cannot_hold(lib, spread, n):
     """With 8-bit rows the values between are 64-bit, the squares and their sums among them."""
     check(lib, 3, n, "bf16", "bf16", spread=spread, codes=True)
     check(lib, 3, n, "f32", "f32", kind=0, spread=spread, codes=True)
+
+
+@pytest.mark.parametrize("n", [513, 600, 1023, 1024])
+@pytest.mark.parametrize("x_dtype,dtype,kind,gate_rows", [("f32", "f32", 0, 0), ("f32", "bf16", 3, 7), ("bf16", "bf16", 1, 0), ("f16", "f16", 2, 1)])
+def test_a_wavefront_per_row(lib, n, x_dtype, dtype, kind, gate_rows):
+    """More than 1024 rows of 513 to 1024 columns, four to a workgroup, the last one's not whole."""
+    check(lib, 1030, n, x_dtype, dtype, kind=kind, gate_rows=gate_rows)
