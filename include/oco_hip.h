@@ -593,7 +593,7 @@ int oco_argmax_f32_ws(const float *logits, uint32_t n, uint32_t *out, void *work
  * counts as 0).  The temperature is 2^-126 to 2^64, or 0 for greedy: p_i is 1
  * at the row's first largest value, draft and uniforms are not read.
  * Decisions are made in 64 bits, on rows' sums of f32 exponentials (relative
- * error about 1e-8).  A row without a distribution (a NaN or +Inf, or nothing
+ * error up to about 1e-7).  A row without a distribution (a NaN or +Inf, or nothing
  * above zero) ends its sequence there: the token is 0xffffffff and its
  * probability NaN; rows of probabilities are read, and so seen, at the drafted
  * ids and in the rows that the last token is drawn from.  A drafted id past

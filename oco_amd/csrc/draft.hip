@@ -13,8 +13,9 @@
 // A decision must follow from the inputs and not from the order of sums or
 // the rounding of exp: the two rows that a token is drawn from are 64-bit
 // exponentials (7e-12) and 64-bit running sums.  The rows' normalising sums
-// are f32 exponentials added in 64 bits: their error, some 1e-8, shifts a
-// whole row alike, and so a decision only where u is within that of its border.
+// are f32 exponentials, sixteen added in f32 and the rest in 64 bits: their
+// error, 1e-8 to 1e-7, shifts a whole row alike, and so a decision only where u
+// is within that of its border.
 //
 // Bound by reading the rows once where they are logits: each chunk of each
 // row gives its maximum and its sum of exponentials; the decisions follow
