@@ -323,3 +323,29 @@ def test_blocks_of_tiny_values_are_exact_too(lib, exponent):
     want_codes, want_scales = quantized(x, True)
     np.testing.assert_array_equal(scales.read(np.float32).reshape(2, rows), want_scales)
     np.testing.assert_array_equal(codes.read(np.uint8).reshape(rows, k), want_codes)
+
+
+@pytest.mark.parametrize("y_dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("m,plan", [(9, ()), (150, (128, 1)), (150, (128, 2)), (300, (256, 1))])
+def test_rows_that_are_not_finite_to_16_bit_outputs(lib, m, plan, y_dtype):
+    """A NaN scale, and NaN codes of a row and of a weight row, on the matrix
+    instructions of 16-bit outputs; K ends inside a block whose rest is NaN codes."""
+    say("fp8 not finite", m, plan, y_dtype)
+    rng = np.random.default_rng(m)
+    n, k = 144, 400
+    x, w, xs, ws = operands(rng, m, n, k)
+    xs, ws = xs * np.float32(2.0 ** -8), ws * np.float32(2.0 ** -4)
+    xs[1, 3] = np.nan
+    x[5, 399], w[143, 0] = 0x7F, 0xFF
+    pad = np.full(4096, 0x7F, np.uint8)
+    with lib.overridden(lib.Knob.FP8, plan):
+        p = lib.Matrix(k, n, m, 0, 1, 1, 0)
+        need = lib.fp8_matmul_workspace(p)
+        out = Guarded(lib, m * n * 2)
+        lib.fp8_matmul(dev(lib, np.concatenate([w.ravel(), pad])), dev(lib, ws), dev(lib, np.concatenate([x.ravel(), pad])), dev(lib, xs), out.ptr, p,
+                       CODE[y_dtype], workspace=lib.DeviceBuffer(max(need, 16)), workspace_bytes=need)
+        lib.synchronize()
+    got = values(out.read(np.uint8), y_dtype, (m, n))
+    bad = np.zeros((m, n), bool)
+    bad[[3, 5]], bad[:, 143] = True, True
+    np.testing.assert_array_equal(np.isnan(got), bad)
