@@ -17,8 +17,8 @@
 // Bound by memory: x, y and the gate are read once, x' and out written once.
 // A row stays in its threads' registers (runs of eight columns per thread,
 // 16-byte accesses for 16-bit types) from its only read to its last write:
-// 8192 x 4096 bf16 in 56.7 us (268 MB, 4.73 TB/s: the rate of a large copy);
-// one row of 4096 in 3.5 us, two memory latencies and two sums over the row.
+// 8192 x 4096 bf16 in 57 to 59 us (268 MB, 4.5 to 4.7 TB/s: the rate of a large
+// copy); one row of 4096 in 3.7 us, two memory latencies and two sums over the row.
 #include "fp8.h"
 #include "rows.h"
 
@@ -64,7 +64,7 @@ __device__ __forceinline__ float recip_f32(float d) {
 }
 // tanh: its Taylor series to g^21 up to 0.625 (relative remainder 0.16^11), 1 - 2 / (exp(2 |g|) + 1) beyond, within
 // 3 x 2^-24.  A gate row that all rows share is formed again for each row, so its instructions count: 8192 x 4096
-// bf16 70.9 us with tanh and 66.6 with the sigmoid, 73.1 and 72.1 by tanhf and a division, 52.5 without a gate.
+// bf16 70.5 us with tanh and 67.3 with the sigmoid, 73.1 and 72.1 by tanhf and a division, 54 without a gate.
 __device__ __forceinline__ float gate_value(float g, uint32_t kind) {
     if (kind == OCO_GATE_SIGMOID) return recip_f32(1.0f + expf(-g));
     if (kind == OCO_GATE_TANH) {
@@ -134,9 +134,10 @@ __device__ __forceinline__ V block_square(float v, V s) {
 // T threads per row (64: four rows per workgroup), P runs of eight columns
 // per thread; P == 0: any n, a row read again for each of its three passes.
 // A thread of one run requests its weights and gate with the rows, so that
-// one memory latency stands before the first sum and none behind it (8192 x
-// 4096: 56.7 us with one run of 512 threads, 59.9 with two of 256); with two
-// runs the registers cost more than that gives (66 us).
+// one memory latency stands before the first sum and none behind it (calls on
+// 4096 columns with one run of 512 threads and with two of 256: one row 5.2 and
+// 5.6 us, 256 rows 5.2 and 6.3, 1024 rows 11.4 and 11.0, 8192 rows 59 both);
+// with two runs the registers cost more than that gives (66 us).
 template <class XT, class YT, class V, int T, int P>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
     __shared__ V part[2][T / 64];
@@ -224,12 +225,12 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void block_kernel(BlockArgs a) {
 typedef void (*BlockFn)(BlockArgs);
 
 // Threads per row and runs per thread: one run up to 8192 columns, the row in
-// registers up to 32768.  The threads fit the row, as those without columns
-// take places on the compute unit (5339 x 2502 bf16: 36 us with 320, 43 with
-// 512; 3855 x 4352: 44 with 640, 49 with 1024).  Rows of up to 1024 columns,
-// many of them: a wavefront per row with two runs and no barrier (1024 bf16
-// columns, 4096 rows: 11.3 us, 13.1 with a workgroup per row; 512 rows: 5.7
-// against 4.2).
+// registers up to 32768.  The threads are the least of the steps that hold
+// the row, as those without columns take places on the compute unit (5339 x
+// 2502 bf16: 45 us with 320, 53.5 with 512; 3855 x 4352: 51 with 640, 56 with
+// 1024).  Rows of up to 1024 columns, many of them: a wavefront per row with
+// two runs and no barrier (1024 bf16 columns, 4096 rows: 11.0 us, 13.0 with a
+// workgroup per row; 512 rows: 5.9 against 5.1).
 template <class XT, class YT, class V>
 static BlockFn block_pick(uint32_t n, uint32_t rows, int &threads) {
 #define PICK(T, P) (threads = T, block_kernel<XT, YT, V, T, P>)

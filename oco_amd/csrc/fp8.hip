@@ -42,7 +42,7 @@ struct QuantArgs {
 };
 
 // 16 threads per block of 128 columns, four consecutive blocks of a row per
-// wavefront.  Bound by memory: 2048 x 4096 bf16 in 6.8 us (25 MB, 3.7 TB/s);
+// wavefront.  Bound by memory: 2048 x 4096 bf16 in 6.6 us (25 MB, 3.8 TB/s);
 // two or four such sets per wavefront with their loads ahead take 7.7 and 8.5.
 template <class T>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs a) {
@@ -212,9 +212,9 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_rows_kernel(Fp8Args a) {
 
 typedef void (*Fp8RowsFn)(Fp8Args);
 // Up to 512 tiles of 16 weight rows, eight wavefronts on one tile, so that the
-// loads in flight fill the card (2880 x 4096, one row: 5.4 us; two tiles and
-// four wavefronts 6.3); beyond, four wavefronts on two tiles, which read the
-// activations half as often (12288 x 4096, 32 rows: 19.8 us against 21.9).
+// loads in flight fill the card (2880 x 4096, one row: 5.6 us; two tiles and
+// four wavefronts 8.2); beyond, four wavefronts on two tiles, which read the
+// activations half as often (12288 x 4096, 32 rows: 18.6 us against 21.8).
 static Fp8RowsFn fp8_rows_pick(uint32_t m, uint32_t n, uint32_t &cols, uint32_t &waves) {
     const bool small = n <= 512 * 16;
     cols = small ? 16 : 32;
@@ -250,7 +250,7 @@ static Fp8RowsFn fp8_rows_pick(uint32_t m, uint32_t n, uint32_t &cols, uint32_t 
 // Workgroups stay and take tile after tile: the next tile's first stage is
 // requested before this one's results are written.
 //
-// 4096 x 12288 x 4096 to bf16 on 256-tiles: 196 us, 2.1 PFLOP/s; the matrix
+// 4096 x 12288 x 4096 to bf16 on 256-tiles: 200 us, 2.1 PFLOP/s; the matrix
 // cores are busy for 46% of the clocks, the four FMAs behind each product and
 // the waits at the barrier take the rest.  1999 x 4096 x 12288 to f32 on
 // 128-tiles: 190 us, 1.06 PFLOP/s, with the conversions to f16 beside the products.
@@ -351,7 +351,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8TileArgs t
         for (int i = 0; i < LOADS; i++) fetch_one(b, s, i);
     };
     // Requests between the products, where registers allow: ahead of them they hold the wavefront up before its
-    // first LDS read (1024 x 4096 x 12288: 88 us against 96).
+    // first LDS read.  Gains where workgroups take several tiles (1999 x 4096 x 12288 to f32 191 us against 196, to
+    // bf16 114 against 117) and costs where the card holds all of them (1024 x 4096 x 12288 to bf16 79 against 73,
+    // 300 x 4096 x 4096 24.7 against 23.6).
     constexpr bool BETWEEN = BM * BN <= 128 * 128;
     // fragment addresses: chunks q and 4 + q of the lane's rows
     const uint32_t xlo = (wm + r) * FP8_BLOCK + (q ^ (r & 7)) * 16, wrow = wn + OUT * (r >> 2) + (r & 3);
