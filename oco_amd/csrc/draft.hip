@@ -502,9 +502,10 @@ static int draft_launch(const DraftArgs &a, bool greedy, hipStream_t stream) {
         return launch_check("oco_draft_verify (greedy)");
     }
     // Decisions in every workgroup while they all run at once (one of 1024 threads per compute unit: its registers
-    // leave six of the eight wavefronts per SIMD that two would need), in a launch of their own beyond.  The whole call,
-    // logits on both sides, 7 drafts, 151936 tokens: 6 sequences (228 workgroups) 25.6 us against 27.4, 7 (266) 30.9 against 29.3, 10 (380)
-    // 35.2 against 33.5; 8 and 11 lookups of 100003 bf16 logits (200, 275) 17.6 against 20.8 and 22.3 against 21.6.
+    // leave six of the eight wavefronts per SIMD that two would need), in a launch of their own beyond.  The whole
+    // call, logits on both sides, 7 drafts, 151936 tokens: 6 sequences (228 workgroups) 25.6 us against 27.4, 7 (266)
+    // 30.9 against 29.3, 10 (380) 35.2 against 33.5; 8 and 11 lookups of 100003 bf16 logits (200, 275) 17.6 against
+    // 20.8 and 22.3 against 21.6.
     if ((uint64_t)a.sequences * a.chunks <= 256) {
         hipLaunchKernelGGL((draft_rest_kernel<TT, TD, true>), dim3(a.sequences * a.chunks), dim3(1024), 0, stream, a);
     } else {

@@ -29,8 +29,8 @@ __device__ __forceinline__ uint32_t row16_max(uint32_t v) {
 // returns the rounded quotient where the reciprocal is itself rounded
 // correctly (Markstein).  A quotient on the border between two codes thus
 // stays on it.  Blocks under 2^-64 enter 2^64 times larger, as the residual of
-// those near the least normal number would be subnormal.  A block that holds a NaN or an infinity has a NaN scale (its
-// row's products are NaN) and NaN codes.
+// those near the least normal number would be subnormal.  A block that holds a
+// NaN or an infinity has a NaN scale (its row's products are NaN) and NaN codes.
 // |v| orders by its bits: finite values, then infinity, then NaN.
 __device__ __forceinline__ uint2 fp8_block(const float *v, float &scale) {
     uint32_t m = 0;
@@ -44,7 +44,7 @@ __device__ __forceinline__ uint2 fp8_block(const float *v, float &scale) {
     }
     scale = top / 448.0f;
     float rate = 0.875f;
-    if (__builtin_expect(__ballot(top < 0x1p-64f) != 0, 0)) {  // a branch: as selects 11.1 us for 4096 x 4096 bf16, 10.7 without
+    if (__ballot(top < 0x1p-64f)) {  // a branch, which the asm keeps: 4096 x 4096 bf16 in 10.7 us, 11.1 as selects
         asm volatile("" ::: "memory");
         const bool tiny = top < 0x1p-64f;
         top = tiny ? top * 0x1p64f : top;
