@@ -621,6 +621,144 @@ int oco_draft_verify(const void *target, const void *draft, const uint32_t *draf
                      const float *uniforms, uint32_t *accepted, uint32_t *tokens, float *probabilities, const oco_draft *p,
                      void *workspace, uint64_t workspace_bytes, oco_stream stream);
 
+/* ---- positions, a paged cache in 4 bits, attention over it ---------------- */
+
+/* Rotary positions (the reference turns its queries and keys inside its
+ * attention shaders, shaders/attention*.metal).  Pair j of a head's first
+ * `dim` values (dim even) is (j, j + dim / 2) in halves or (2j, 2j + 1)
+ * interleaved, and turns by position * frequencies[j] radians:
+ *   a' = a cos - b sin,  b' = b cos + a sin,  both times magnitude,
+ * angles, functions and products in 64 bits, rounded to the type once.  Values
+ * from dim on stay.
+ *   frequencies: f64 [dim / 2] on the device (oco_rotation_frequencies) */
+typedef enum oco_rotation_layout { OCO_ROTATION_HALF = 0, OCO_ROTATION_INTERLEAVED = 1 } oco_rotation_layout;
+#define OCO_ROTATION_DIM 1024u
+typedef struct oco_rotation {
+    uint32_t dim;    /* at most OCO_ROTATION_DIM */
+    uint32_t layout; /* oco_rotation_layout */
+    double magnitude;
+    const double *frequencies;
+} oco_rotation;
+
+/* Frequencies on the host, out[j] = base^(-2j / dim) / factors[j] (factors
+ * f32 [dim / 2] or NULL), scaled for contexts longer than `original`:
+ *   LINEAR: all divided by `factor`
+ *   YARN:   pairs that turn more than `fast` times over `original` positions
+ *           stay, those that turn less than `slow` times are divided by
+ *           factor, in between by their place between the two pairs;
+ *           *magnitude = 0.1 ln(factor) + 1
+ *   BANDS:  the same in between by the number of turns itself, and
+ *           *magnitude = 1
+ * magnitude may be NULL.  fast > slow > 0 and factor >= 1. */
+typedef enum oco_scaling { OCO_SCALING_NONE = 0, OCO_SCALING_LINEAR = 1, OCO_SCALING_YARN = 2, OCO_SCALING_BANDS = 3 } oco_scaling;
+typedef struct oco_frequencies {
+    uint32_t dim, scaling; /* oco_scaling */
+    double base, factor, original, fast, slow;
+    const float *factors;
+} oco_frequencies;
+int oco_rotation_frequencies(const oco_frequencies *p, double *out, double *magnitude);
+
+/* Rows of `heads` heads of head_dim values, turned: out[r][h] = x[r][h] at
+ * positions[r] (u32).  Row strides in elements, 0: heads * head_dim.  out may
+ * be x where their strides agree. */
+int oco_rotate(const void *x, oco_dtype dtype, uint32_t rows, uint32_t heads, uint32_t head_dim, uint64_t x_stride,
+               const uint32_t *positions, void *out, uint64_t out_stride, const oco_rotation *rotation, oco_stream stream);
+
+/* A pool of pages that hold keys and values in 4 bits, and a batch of rows on
+ * it.  Page i starts at pages + i * oco_cache_page_bytes(p), 16-byte aligned,
+ * and holds page_size tokens of each key-value head after the other:
+ *   keys' codes    [page_size][head_dim / 2]: E2M1, the value of lower index in the lower four bits
+ *   values' codes  [page_size / 4][16][4][head_dim / 32]: token t's bytes of values
+ *                  w head_dim / 16 on at [t / 4][w][t % 4]
+ *   keys' scales   [page_size][head_dim / 32]: E8M0 per 32 values
+ *   values' scales [page_size / 4][head_dim / 32][4]: block b of token t at [t / 4][b][t % 4]
+ * A block's scale is 2^floor(log2(max |x|)) / 4, at least 2^-126; its codes
+ * are x / scale rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4 and 6 (ties
+ * to the even code, beyond 6 to 6).  A block with a NaN or an infinity has
+ * scale 255 and reads as NaN.
+ *
+ * Sequence s has rows starts[s] .. starts[s + 1] - 1 of the batch (starts
+ * NULL: rows / sequences each), at most max_rows, and lengths[s] tokens (more
+ * than max_length count as max_length), those rows as the last ones among
+ * them: its row i of n is at position lengths[s] - n + i.  A row whose
+ * position is under 0 has no token.  The token at position t is in page
+ * table[s][t / page_size].  Rows from starts[sequences] on, and rows of a
+ * sequence past max_rows, are left as they were.
+ *   table: u32 [sequences][table_stride]; starts: u32 [sequences + 1]; lengths: u32 [sequences] */
+typedef struct oco_cache {
+    uint32_t head_dim;                  /* 64, 128 or 256 */
+    uint32_t heads, kv_heads;           /* of the queries (a multiple of kv_heads), of the cache */
+    uint32_t page_size, pages;          /* tokens per page, a multiple of 16 */
+    uint32_t sequences, rows;           /* of the batch */
+    uint32_t max_rows, max_length;      /* per sequence; max_length <= table_stride * page_size */
+    uint32_t table_stride;
+    uint32_t dtype;                     /* oco_dtype of the rows */
+    uint32_t window;                    /* 0, or how many tokens a query sees, its own among them */
+    float scale;                        /* of the scores; 0: 1 / sqrt(head_dim) */
+    uint64_t q_stride, k_stride, v_stride, out_stride; /* between rows, in elements; 0: heads (kv_heads) * head_dim */
+} oco_cache;
+uint64_t oco_cache_page_bytes(const oco_cache *p);  /* of head_dim, kv_heads and page_size; 0 where they are refused */
+
+/* Appends the batch's rows to the pages: keys turned by their position
+ * (rotation NULL: as they are), rounded to the rows' type and quantised, values
+ * quantised; with q, the queries turned into q_out (out_stride apart; q_out
+ * may be q where their strides agree).  positions: u32 [rows] to turn by in
+ * the place of the cache's own, or NULL.  A row without a token is not
+ * appended (its query turns by position 0), nor is a row whose page is not
+ * in the pool.  A place must not be appended to twice in one call. */
+int oco_cache_append(void *pages, const uint32_t *table, const uint32_t *starts, const uint32_t *lengths,
+                     const uint32_t *positions, const void *q, const void *k, const void *v, void *q_out,
+                     const oco_rotation *rotation, const oco_cache *p, oco_stream stream);
+
+/* Reads the batch's rows back into k and v ([rows][kv_heads][head_dim]) as the
+ * values they stand for; NaN where the page is not in the pool, 0 for a row without a token. */
+int oco_cache_read(const void *pages, const uint32_t *table, const uint32_t *starts, const uint32_t *lengths,
+                   void *k, void *v, const oco_cache *p, oco_stream stream);
+
+/* Causal attention of the batch's rows over their sequences' cached tokens:
+ * out[r][h] = sum_t p_t value_t, p = softmax over the tokens t that row r sees
+ * (its own position and before, within the window) of scale * q[r][h] . key_t,
+ * of head h / (heads / kv_heads).  sinks: f32 [heads], one more score per head
+ * that takes part in the sum and has no value, or NULL.  A row that sees
+ * nothing is 0; what it does not see (a NaN among it) has no effect on it; a
+ * page that is not in the pool reads as NaN.  q and out are bf16 or f16; the
+ * probabilities are rounded to that type, sums are f32.
+ *   workspace: oco_cache_attention_workspace bytes (0 for a description that is
+ *   refused, and where none is needed), 16-byte aligned; calls sharing one must be ordered */
+uint64_t oco_cache_attention_workspace(const oco_cache *p);
+int oco_cache_attention(const void *q, const void *pages, const uint32_t *table, const uint32_t *starts,
+                        const uint32_t *lengths, const float *sinks, void *out, const oco_cache *p, void *workspace,
+                        uint64_t workspace_bytes, oco_stream stream);
+
+/* ---- logits before a token is chosen ---------------------------------------- */
+
+/* What stands between the head's rows and oco_argmax_f32 or oco_draft_verify
+ * (no counterpart in the reference).  Per row, in f32, rounded once:
+ *   v in the row's history n > 0 times:
+ *     x = x / repetition if x > 0, else x * repetition;  x = x - (frequency * n + presence)
+ *   v in the row's biases:  x = x + its bias (of several the last one's)
+ *   v not in the row's mask:  x = -Inf, whatever it was
+ * `group` consecutive rows share a history, penalties and biases, mask_group
+ * rows a mask (0: 1).  Ids past the vocabulary are passed over.
+ *   history: u32 [groups][history_stride], history_lengths: u32 [groups] (NULL or more: history_stride)
+ *   penalties: f32 [groups][3]: repetition (> 0), frequency, presence; with history
+ *   bias_ids: u32 [groups][bias_stride], biases: f32 alike, bias_lengths as history_lengths
+ *   mask: u32 [mask groups][mask_stride], bit v % 32 of word v / 32: v may be chosen
+ * Each of history, bias_ids and mask may be NULL.  out may be logits where
+ * their strides agree. */
+#define OCO_LOGITS_HISTORY 0xfffffu
+#define OCO_LOGITS_BIASES 4095u
+typedef struct oco_logits {
+    uint32_t rows, vocabulary, dtype;         /* oco_dtype */
+    uint32_t history_stride, bias_stride;     /* at most OCO_LOGITS_HISTORY, OCO_LOGITS_BIASES */
+    uint32_t mask_stride;                     /* words, 0: (vocabulary + 31) / 32 */
+    uint32_t group, mask_group;
+    uint64_t stride, out_stride;              /* between rows, in elements; 0: vocabulary */
+} oco_logits;
+int oco_logits_adjust(const void *logits, void *out, const uint32_t *history, const uint32_t *history_lengths,
+                      const float *penalties, const uint32_t *bias_ids, const float *biases, const uint32_t *bias_lengths,
+                      const uint32_t *mask, const oco_logits *p, oco_stream stream);
+
 /* ---- GGUF checkpoints and residency (src/gguf.rs) ------------------------- */
 
 /* An open GGUF v3 file: memory-mapped, metadata structurally validated,

@@ -94,6 +94,20 @@ class DraftValues(enum.IntEnum):
     PROBABILITIES = 1
 
 
+class RotationLayout(enum.IntEnum):
+    """oco_rotation_layout."""
+    HALF = 0
+    INTERLEAVED = 1
+
+
+class Scaling(enum.IntEnum):
+    """oco_scaling."""
+    NONE = 0
+    LINEAR = 1
+    YARN = 2
+    BANDS = 3
+
+
 NO_TOKEN = 0xFFFFFFFF  # oco_draft_verify's places without a token
 
 _BLOCKS = {0: (1, 4), 1: (1, 2), 30: (1, 2), 2: (32, 18), 3: (32, 20), 8: (32, 34),
@@ -163,6 +177,33 @@ class Draft(ctypes.Structure):
                 [("temperature", ctypes.c_float), ("target_stride", ctypes.c_uint64), ("draft_stride", ctypes.c_uint64)])
 
 
+class Rotation(ctypes.Structure):
+    """oco_rotation: how the pairs of a head turn; frequencies: address of f64 [dim / 2] on the device."""
+    _fields_ = [("dim", ctypes.c_uint32), ("layout", ctypes.c_uint32), ("magnitude", ctypes.c_double),
+                ("frequencies", ctypes.c_void_p)]
+
+
+class Frequencies(ctypes.Structure):
+    """oco_frequencies."""
+    _fields_ = ([(n, ctypes.c_uint32) for n in ("dim", "scaling")] +
+                [(n, ctypes.c_double) for n in ("base", "factor", "original", "fast", "slow")] + [("factors", ctypes.c_void_p)])
+
+
+class Cache(ctypes.Structure):
+    """oco_cache: a pool of pages in 4 bits and a batch of rows on it."""
+    _fields_ = ([(n, ctypes.c_uint32) for n in ("head_dim", "heads", "kv_heads", "page_size", "pages", "sequences", "rows",
+                                                "max_rows", "max_length", "table_stride", "dtype", "window")] +
+                [("scale", ctypes.c_float)] +
+                [(n, ctypes.c_uint64) for n in ("q_stride", "k_stride", "v_stride", "out_stride")])
+
+
+class Logits(ctypes.Structure):
+    """oco_logits: rows of logits that are adjusted before a token is chosen."""
+    _fields_ = ([(n, ctypes.c_uint32) for n in ("rows", "vocabulary", "dtype", "history_stride", "bias_stride", "mask_stride",
+                                                "group", "mask_group")] +
+                [("stride", ctypes.c_uint64), ("out_stride", ctypes.c_uint64)])
+
+
 class GgufEntry(ctypes.Structure):
     """oco_gguf_entry (Entry, gguf.rs:24-33)."""
     _fields_ = [("shape", ctypes.c_uint64 * 4), ("rank", ctypes.c_uint32), ("code", ctypes.c_uint32),
@@ -222,6 +263,14 @@ SIGNATURES = {
     "oco_block_norm": (_i32, [_vp] * 9 + [ctypes.POINTER(Block), _vp]),
     "oco_draft_verify_workspace": (_u64, [ctypes.POINTER(Draft)]),
     "oco_draft_verify": (_i32, [_vp] * 8 + [ctypes.POINTER(Draft), _vp, _u64, _vp]),
+    "oco_rotation_frequencies": (_i32, [ctypes.POINTER(Frequencies), _vp, _vp]),
+    "oco_rotate": (_i32, [_vp, _i32, _u32, _u32, _u32, _u64, _vp, _vp, _u64, ctypes.POINTER(Rotation), _vp]),
+    "oco_cache_page_bytes": (_u64, [ctypes.POINTER(Cache)]),
+    "oco_cache_append": (_i32, [_vp] * 9 + [ctypes.POINTER(Rotation), ctypes.POINTER(Cache), _vp]),
+    "oco_cache_read": (_i32, [_vp] * 6 + [ctypes.POINTER(Cache), _vp]),
+    "oco_cache_attention_workspace": (_u64, [ctypes.POINTER(Cache)]),
+    "oco_cache_attention": (_i32, [_vp] * 7 + [ctypes.POINTER(Cache), _vp, _u64, _vp]),
+    "oco_logits_adjust": (_i32, [_vp] * 9 + [ctypes.POINTER(Logits), _vp]),
     "oco_route_select": (_i32, [_vp, _u32, _u32, _u32, _vp, _vp, _vp]),
     "oco_router": (_i32, [_vp, _i32, _vp, _vp, _u32, _u32, _u32, _u32, _vp, _vp, _vp, _vp]),
     "oco_route_plan_words": (_u64, [_u32, _u32]),
@@ -615,6 +664,63 @@ def draft_verify(target, draft, draft_ids, uniforms, accepted, tokens, p: Draft,
     _check(load_library().oco_draft_verify(_addr(target), _addr(draft), _addr(draft_ids), _addr(lengths), _addr(uniforms),
                                            _addr(accepted), _addr(tokens), _addr(probabilities), ctypes.byref(p),
                                            _addr(workspace), int(workspace_bytes), _stream(stream)))
+
+
+def rotation_frequencies(dim: int, base: float = 10000.0, scaling=Scaling.NONE, factor: float = 1.0, original: float = 0.0,
+                         fast: float = 32.0, slow: float = 1.0, factors=None):
+    """oco_rotation_frequencies: (f64 [dim / 2] radians per position, magnitude), on the host."""
+    extra = None if factors is None else np.ascontiguousarray(factors, np.float32)
+    if extra is not None and extra.shape != (dim // 2,):
+        raise ValueError(f"factors of {extra.shape} for {dim // 2} pairs")
+    out, magnitude = np.empty(dim // 2), ctypes.c_double()
+    p = Frequencies(dim, int(scaling), base, factor, original, fast, slow, None if extra is None else extra.ctypes.data)
+    _check(load_library().oco_rotation_frequencies(ctypes.byref(p), out.ctypes.data, ctypes.byref(magnitude)))
+    return out, magnitude.value
+
+
+def rotate(x, rows: int, heads: int, head_dim: int, out, rotation: Rotation, positions, dtype=DType.BF16, x_stride: int = 0,
+           out_stride: int = 0, stream=None):
+    """oco_rotate: rows of heads, turned by their positions (out may be x)."""
+    _check(load_library().oco_rotate(_addr(x), int(dtype), rows, heads, head_dim, x_stride, _addr(positions), _addr(out),
+                                     out_stride, ctypes.byref(rotation), _stream(stream)))
+
+
+def cache_page_bytes(p: Cache) -> int:
+    return int(load_library().oco_cache_page_bytes(ctypes.byref(p)))
+
+
+def cache_append(pages, table, lengths, k, v, p: Cache, starts=None, q=None, q_out=None, positions=None, rotation=None,
+                 stream=None):
+    """oco_cache_append: a batch's keys (turned) and values into the pages, its queries turned into q_out (q by default)."""
+    _check(load_library().oco_cache_append(_addr(pages), _addr(table), _addr(starts), _addr(lengths), _addr(positions), _addr(q),
+                                           _addr(k), _addr(v), _addr(q if q_out is None else q_out),
+                                           None if rotation is None else ctypes.byref(rotation), ctypes.byref(p), _stream(stream)))
+
+
+def cache_read(pages, table, lengths, k, v, p: Cache, starts=None, stream=None):
+    """oco_cache_read: a batch's rows out of the pages, as the values they stand for."""
+    _check(load_library().oco_cache_read(_addr(pages), _addr(table), _addr(starts), _addr(lengths), _addr(k), _addr(v),
+                                         ctypes.byref(p), _stream(stream)))
+
+
+def cache_attention_workspace(p: Cache) -> int:
+    return int(load_library().oco_cache_attention_workspace(ctypes.byref(p)))
+
+
+def cache_attention(q, pages, table, lengths, out, p: Cache, starts=None, sinks=None, workspace=None, workspace_bytes: int = 0,
+                    stream=None):
+    """oco_cache_attention: causal attention of a batch's rows over their sequences' pages."""
+    _check(load_library().oco_cache_attention(_addr(q), _addr(pages), _addr(table), _addr(starts), _addr(lengths), _addr(sinks),
+                                              _addr(out), ctypes.byref(p), _addr(workspace), int(workspace_bytes),
+                                              _stream(stream)))
+
+
+def logits_adjust(logits, out, p: Logits, history=None, history_lengths=None, penalties=None, bias_ids=None, biases=None,
+                  bias_lengths=None, mask=None, stream=None):
+    """oco_logits_adjust: penalties for repeated tokens, biases and masks (out may be logits)."""
+    _check(load_library().oco_logits_adjust(_addr(logits), _addr(out), _addr(history), _addr(history_lengths), _addr(penalties),
+                                            _addr(bias_ids), _addr(biases), _addr(bias_lengths), _addr(mask), ctypes.byref(p),
+                                            _stream(stream)))
 
 
 def route_select(logits, tokens: int, experts: int, k: int, ids, probs, stream=None):

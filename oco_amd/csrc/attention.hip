@@ -1,0 +1,489 @@
+// Causal attention over the paged cache in 4 bits.
+//
+// out = sum_t p_t v_t with p = softmax(c q . k_t), one pass over the tokens
+// with a running maximum m and sum l per row: a step of 32 tokens adds
+// exp2(s - m) and its products, and rescales what is there when a row's maximum
+// rises.  Rows are the query heads of one key-value head and their tokens, so
+// the cache is read once for all of them.
+//
+// Everything is computed transposed, S^T = K Q^T and O^T = V^T P^T: a row is
+// then a lane (of four) from the scores to the output, its statistics need no
+// broadcast, and the scores leave the first product in the very lanes that
+// feed the second.  The matrix instruction takes its 32 inner indexes in any
+// order that both operands share, so a lane's probabilities of tokens 4g ..
+// 4g + 3 of two halves stay where they are, and the values' pages hold four
+// tokens together to match.
+//
+// E2M1 times a power of two is exact in bf16 and f16 (an f16 model's cache
+// stays in range), so codes go to the matrix instruction through the hardware's
+// conversion, two values per instruction, with their scale.
+#include "cache.h"
+
+namespace oco {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+struct AttentionArgs {
+    CacheBatch b;
+    const uint8_t *cache;
+    const void *q;
+    void *out;
+    const float *sinks;
+    float *parts;  // [rows][heads][chunks][D], then m and l [rows][heads][chunks][2]
+    uint64_t q_stride, out_stride;
+    uint32_t heads, group, window;
+    uint32_t chunks, chunk;  // parts of the tokens, each of `chunk` tokens
+    float c;                 // scale * log2(e)
+};
+
+template <bool BF>
+struct Half;  // the 16-bit type of the rows
+template <>
+struct Half<true> {
+    template <int I>
+    static __device__ __forceinline__ uint32_t pair(uint32_t w, float s) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, I));
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+    }
+    static __device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static constexpr uint32_t ONE = 0x3f80;
+};
+template <>
+struct Half<false> {
+    template <int I>
+    static __device__ __forceinline__ uint32_t pair(uint32_t w, float s) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, I));
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+    }
+    static __device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static constexpr uint32_t ONE = 0x3c00;
+};
+template <bool BF>
+using half_t = std::conditional_t<BF, bf16_t, f16_t>;
+
+// Maximum and sum over the lanes l, l ^ 16, l ^ 32, l ^ 48, which hold one row.
+__device__ __forceinline__ float row_max(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float row_sum(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// The tokens that any row of a sequence sees: from .. length, from a multiple of 32.
+__device__ __forceinline__ uint32_t first_seen(const CacheSpan &s, uint32_t window) {
+    const uint32_t p = s.length > s.rows ? s.length - s.rows : 0;
+    return window && p + 1 > window ? (p + 1 - window) / 32 * 32 : 0;
+}
+
+// exp2 of m - to, 0 for m = -Inf whatever `to` is.
+__device__ __forceinline__ float carry(float m, float to) { return m > -INFINITY ? __builtin_amdgcn_exp2f(m - to) : 0.f; }
+
+// ---- few rows: a wavefront holds 16 R rows and reads its tokens itself ----------------
+
+// One half-step's 16 tokens as a lane holds them: lane m + 16 g has a quarter
+// of token m's key, and of tokens 4g .. 4g + 3 one sixteenth of the value.
+template <uint32_t D>
+struct Tokens {
+    static constexpr int KW = D / 32, VW = D / 32;  // words
+    uint32_t k[KW], v[VW], ks, vs;
+};
+
+template <uint32_t D>
+__device__ __forceinline__ void load_tokens(Tokens<D> &x, const uint8_t *head, uint32_t page_size, uint32_t t) {
+    const uint32_t m = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+    const uint8_t *const k = head + (t + m) * (D / 2) + g * (D / 8);
+    const uint8_t *const v = head + page_size * (D / 2) + (t / 4 + g) * (2 * D) + m * (D / 8);
+    const uint8_t *const ks = head + page_size * D + (t + m) * (D / 32) + g * (D / 128);
+    const uint8_t *const vs = head + page_size * D + page_size * (D / 32) + (t / 4 + g) * (D / 8) + m * D / 512 * 4;
+    if constexpr (D == 64) {
+        const uint2 a = *(const uint2 *)k, b = *(const uint2 *)v;
+        x.k[0] = a.x;
+        x.k[1] = a.y;
+        x.v[0] = b.x;
+        x.v[1] = b.y;
+        x.ks = head[page_size * D + (t + m) * 2 + g / 2];
+    } else {
+#pragma unroll
+        for (int i = 0; i < (int)D / 128; i++) {
+            const u32x4 a = ((const u32x4 *)k)[i], b = ((const u32x4 *)v)[i];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                x.k[4 * i + j] = a[j];
+                x.v[4 * i + j] = b[j];
+            }
+        }
+        x.ks = D == 256 ? *(const uint16_t *)ks : *ks;
+    }
+    x.vs = *(const uint32_t *)vs;
+}
+
+template <uint32_t D, bool BF, int R>
+__global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, uint32_t tiles) {
+    constexpr int KW = D / 32, NT = D / 16;  // key words per lane and token; tiles of 16 columns
+    using H = Half<BF>;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    const uint32_t chunk = blockIdx.x % a.chunks, tile = blockIdx.x / a.chunks % tiles, sh = blockIdx.x / a.chunks / tiles;
+    const uint32_t s = sh / a.b.kv_heads, h = sh % a.b.kv_heads;
+    const CacheSpan span = cache_span(a.b, s);
+    const uint32_t row0 = tile * (16 * R), rows = span.rows * a.group;
+    if (row0 >= rows) return;
+    // the rows' positions (-1: no token, and no row)
+    int32_t at[R];
+    const uint16_t *qrow[R];
+    u32x4 q[R][KW];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const uint32_t i = row0 + 16 * r + n;
+        const bool live = i < rows;
+        const uint32_t token = live ? i / a.group : 0, head = h * a.group + (live ? i % a.group : 0);
+        at[r] = live ? (int32_t)(span.length + token) - (int32_t)span.rows : -1;
+        qrow[r] = (const uint16_t *)a.q + (uint64_t)(span.first + token) * a.q_stride + (uint64_t)head * D + g * (D / 4);
+#pragma unroll
+        for (int w = 0; w < KW; w++) q[r][w] = *(const u32x4_u *)(qrow[r] + 8 * w);
+    }
+    const uint32_t last_row = min(row0 + 16 * R, rows) - 1;
+    const int32_t least = (int32_t)(span.length + row0 / a.group) - (int32_t)span.rows;
+    const int32_t most = (int32_t)(span.length + last_row / a.group) - (int32_t)span.rows;
+    // this chunk's tokens
+    const uint32_t base = first_seen(span, a.window) + chunk * a.chunk;
+    const uint32_t end = most < 0 ? 0 : min(min(base + a.chunk, span.length), (uint32_t)most + 1);
+
+    float m[R], l[R];
+    f32x4 o[R][NT];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NT; j++) o[r][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const uint32_t head_bytes = cache_head_bytes(a.b.page_size, D);
+    const uint32_t *const table = a.b.table + (uint64_t)s * a.b.table_stride;
+    for (uint32_t t0 = base + 32 * wave; t0 < end; t0 += 128) {
+        Tokens<D> x[2];
+        bool lost[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const uint32_t t = t0 + 16 * e;
+            uint32_t page = t < end ? table[t / a.b.page_size] : 0;
+            lost[e] = page >= a.b.pages;
+            page = lost[e] ? 0 : page;
+            load_tokens(x[e], a.cache + ((uint64_t)page * a.b.kv_heads + h) * head_bytes, a.b.page_size, t % a.b.page_size);
+        }
+        // scores: lane (n, g) has row n's tokens 16 e + 4 g + i
+        f32x4 sc[R][2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            if (lost[e]) {
+                x[e].ks = 0xffff;
+                x[e].vs = 0xffffffffu;
+            }
+#pragma unroll
+            for (int r = 0; r < R; r++) sc[r][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < KW; w++) {
+                const float scale = cache_scale(D == 256 ? (w < 4 ? x[e].ks & 0xff : x[e].ks >> 8) : x[e].ks & 0xff);
+                const u32x4 k = {H::template pair<0>(x[e].k[w], scale), H::template pair<1>(x[e].k[w], scale),
+                                 H::template pair<2>(x[e].k[w], scale), H::template pair<3>(x[e].k[w], scale)};
+#pragma unroll
+                for (int r = 0; r < R; r++) sc[r][e] = H::product(k, q[r][w], sc[r][e]);
+            }
+        }
+        const bool edge = (int32_t)t0 + 31 > least || (a.window && (int32_t)t0 + (int32_t)a.window <= most);
+        u32x4 p[R];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                v[i] = sc[r][i / 4][i % 4] * a.c;
+                const int32_t t = (int32_t)t0 + 16 * (i / 4) + 4 * (int32_t)g + i % 4;
+                if (edge) v[i] = t <= at[r] && (!a.window || t + (int32_t)a.window > at[r]) ? v[i] : -INFINITY;
+            }
+            float top = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+            top = fmaxf(row_max(top), m[r]);
+            if (__any(top > m[r])) {
+                const float f = carry(m[r], top);
+                m[r] = top;
+                l[r] *= f;
+#pragma unroll
+                for (int j = 0; j < NT; j++) o[r][j] *= f;
+            }
+            const float ref = m[r] > -INFINITY ? m[r] : 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                v[i] = __builtin_amdgcn_exp2f(v[i] - ref);
+                l[r] += v[i];
+            }
+            p[r] = u32x4{H::pack(v[0], v[1]), H::pack(v[2], v[3]), H::pack(v[4], v[5]), H::pack(v[6], v[7])};
+        }
+        // values: a scale for each token of the lane's column block
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < 8; i++) bad |= byte_of(x[i / 4].vs, i % 4) == 255;
+        if (__any(bad)) {
+            // 0 * NaN is NaN: a NaN block enters the product as numbers, and the rows that see
+            // it (counted by a product of their own) become NaN in its columns
+            u32x4 lost_at;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t lo = byte_of(x[i / 2].vs, 2 * i % 4) == 255, hi = byte_of(x[i / 2].vs, 2 * i % 4 + 1) == 255;
+                lost_at[i] = lo * H::ONE | hi * (H::ONE << 16);
+            }
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                u32x4 sees;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int32_t t = (int32_t)t0 + 16 * (i / 4) + 4 * (int32_t)g + i % 4;
+                    const uint32_t one = t <= at[r] && (!a.window || t + (int32_t)a.window > at[r]) ? H::ONE : 0;
+                    sees[i / 2] = i % 2 ? sees[i / 2] | one << 16 : one;
+                }
+                const f32x4 count = H::product(lost_at, sees, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+#pragma unroll
+                    for (int j = 0; j < NT; j++) o[r][j][k] = count[k] > 0.f ? __uint_as_float(0x7fc00000u) : o[r][j][k];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (byte_of(x[i / 4].vs, i % 4) == 255) x[i / 4].vs ^= 128u << (8 * (i % 4));
+        }
+        float scale[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) scale[i] = __uint_as_float(byte_of(x[i / 4].vs, i % 4) << 23);
+        // byte b of a token's piece: columns 2b and 2b + 1 of the piece
+#pragma unroll
+        for (int b = 0; b < NT / 2; b++) {
+            uint32_t c[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                constexpr int W = D / 128;  // words per token, 0: two tokens share one
+                const int byte = D == 64 ? 2 * (i % 2) + b : b % 4;
+                const uint32_t w = D == 64 ? x[i / 4].v[i % 4 / 2] : x[i / 4].v[i % 4 * W + b / 4];
+                c[i] = byte == 0 ? H::template pair<0>(w, scale[i]) : byte == 1 ? H::template pair<1>(w, scale[i])
+                     : byte == 2 ? H::template pair<2>(w, scale[i]) : H::template pair<3>(w, scale[i]);
+            }
+            u32x4 lo, hi;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                lo[i] = __builtin_amdgcn_perm(c[2 * i + 1], c[2 * i], 0x05040100);
+                hi[i] = __builtin_amdgcn_perm(c[2 * i + 1], c[2 * i], 0x07060302);
+            }
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                o[r][2 * b] = H::product(lo, p[r], o[r][2 * b]);
+                o[r][2 * b + 1] = H::product(hi, p[r], o[r][2 * b + 1]);
+            }
+        }
+    }
+    // the four wavefronts' parts, in pairs
+    __shared__ __attribute__((aligned(16))) f32x4 so[2][NT][64];
+    __shared__ float sm[2][64], sl[2][64];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        l[r] = row_sum(l[r]);
+#pragma unroll
+        for (int half = 2; half; half /= 2) {
+            __syncthreads();
+            if (wave >= (uint32_t)half && wave < 2u * half) {
+                sm[wave - half][lane] = m[r];
+                sl[wave - half][lane] = l[r];
+#pragma unroll
+                for (int j = 0; j < NT; j++) so[wave - half][j][lane] = o[r][j];
+            }
+            __syncthreads();
+            if (wave < (uint32_t)half) {
+                const float m2 = sm[wave][lane], top = fmaxf(m[r], m2), f1 = carry(m[r], top), f2 = carry(m2, top);
+                m[r] = top;
+                l[r] = l[r] * f1 + sl[wave][lane] * f2;
+#pragma unroll
+                for (int j = 0; j < NT; j++) o[r][j] = o[r][j] * f1 + so[wave][j][lane] * f2;
+            }
+        }
+    }
+    if (wave) return;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const uint32_t i = row0 + 16 * r + n;
+        if (i >= rows) continue;
+        const uint32_t row = span.first + i / a.group, head = h * a.group + i % a.group;
+        float *part = nullptr;
+        float f = 1.f;
+        if (a.chunks > 1) {
+            const uint64_t index = ((uint64_t)row * a.heads + head) * a.chunks + chunk;
+            part = a.parts + index * D;
+            if (g == 0) {
+                float *const ml = a.parts + (uint64_t)a.b.rows * a.heads * a.chunks * D + index * 2;
+                ml[0] = m[r];
+                ml[1] = l[r];
+            }
+        } else {
+            float top = m[r], total = l[r];
+            if (a.sinks) {
+                const float sink = a.sinks[head] * 1.44269504088896341f;
+                top = fmaxf(m[r], sink);
+                total = l[r] * carry(m[r], top) + carry(sink, top);
+            }
+            f = total > 0.f || total != total ? carry(m[r], top) / total : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t column = (4 * g + k) * NT;
+#pragma unroll
+            for (int j = 0; j < NT; j += 4) {
+                const f32x4 v = {o[r][j][k], o[r][j + 1][k], o[r][j + 2][k], o[r][j + 3][k]};
+                if (part) {
+                    *(f32x4 *)(part + column + j) = v;
+                } else {
+                    uint16_t *const out = (uint16_t *)a.out + (uint64_t)row * a.out_stride + (uint64_t)head * D + column + j;
+                    *(u32x2_u *)out = u32x2_u{H::pack(v[0] * f, v[1] * f), H::pack(v[2] * f, v[3] * f)};
+                }
+            }
+        }
+    }
+}
+
+// ---- chunks joined: a wavefront per row and head ----------------------------------------
+
+template <uint32_t D, bool BF>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
+    const uint32_t lane = threadIdx.x & 63, i = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint32_t row = i / a.heads, head = i % a.heads;
+    if (row >= a.b.rows) return;
+    const uint32_t s = cache_sequence(a.b, row);
+    if (s >= a.b.sequences) return;
+    const CacheSpan span = cache_span(a.b, s);
+    if (row - span.first >= span.rows) return;
+    const uint32_t from = first_seen(span, a.window), used = span.length > from ? (span.length - from + a.chunk - 1) / a.chunk : 0;
+    const uint64_t index = (uint64_t)i * a.chunks;
+    const float *const ml = a.parts + (uint64_t)a.b.rows * a.heads * a.chunks * D + index * 2;
+    const float sink = a.sinks ? a.sinks[head] * 1.44269504088896341f : -INFINITY;
+    float top = sink;
+    for (uint32_t c = 0; c < used; c++) top = fmaxf(top, ml[2 * c]);
+    float total = carry(sink, top), o[D / 64];
+#pragma unroll
+    for (int j = 0; j < (int)D / 64; j++) o[j] = 0.f;
+    for (uint32_t c = 0; c < used; c++) {
+        const float f = carry(ml[2 * c], top);
+        const float *const p = a.parts + (index + c) * D + lane * (D / 64);
+        total += ml[2 * c + 1] * f;
+#pragma unroll
+        for (int j = 0; j < (int)D / 64; j++) o[j] += p[j] * f;
+    }
+    const float f = total > 0.f || total != total ? 1.f / total : 0.f;
+    half_t<BF> *const out = (half_t<BF> *)a.out + (uint64_t)row * a.out_stride + (uint64_t)head * D + lane * (D / 64);
+#pragma unroll
+    for (int j = 0; j < (int)D / 64; j++) RowIO<half_t<BF>>::put(out + j, o[j] * f);
+}
+
+// ---- choices and launches -------------------------------------------------------------------
+
+struct AttentionPlan {
+    uint32_t tiles, chunks, chunk;
+    uint64_t bytes;
+};
+static AttentionPlan attention_plan(const oco_cache *p) {
+    AttentionPlan l;
+    const uint64_t rows = (uint64_t)p->max_rows * (p->heads / p->kv_heads);
+    l.tiles = (uint32_t)((rows + 15) / 16);
+    uint64_t seen = p->max_length;
+    if (p->window && (uint64_t)p->window + p->max_rows + 31 < seen) seen = (uint64_t)p->window + p->max_rows + 31;
+    const uint64_t blocks = (uint64_t)p->sequences * p->kv_heads * l.tiles;
+    uint64_t chunks = blocks ? (1024 + blocks - 1) / blocks : 1;
+    const uint64_t most = (seen + 127) / 128;
+    if (chunks > most) chunks = most;
+    if (chunks < 1) chunks = 1;
+    l.chunk = (uint32_t)(((seen + chunks - 1) / chunks + 127) / 128 * 128);
+    if (l.chunk == 0) l.chunk = 128;
+    l.chunks = (uint32_t)((seen + l.chunk - 1) / l.chunk);
+    if (l.chunks < 1) l.chunks = 1;
+    l.bytes = l.chunks > 1 ? (uint64_t)p->rows * p->heads * l.chunks * (p->head_dim + 2) * 4 : 0;
+    return l;
+}
+
+template <uint32_t D, bool BF>
+static int attention_launch(const AttentionArgs &a, const AttentionPlan &l, hipStream_t stream) {
+    const uint64_t grid = (uint64_t)a.b.sequences * a.b.kv_heads * l.tiles * l.chunks;
+    if (grid > 0x7fffffffull) return fail(OCO_ERR_INVALID, "oco_cache_attention: too many rows for one call");
+    hipLaunchKernelGGL((attention_few_kernel<D, BF, 1>), dim3((uint32_t)grid), dim3(256), 0, stream, a, l.tiles);
+    OCO_TRY(launch_check("oco_cache_attention"));
+    if (l.chunks > 1) {
+        const uint64_t heads = (uint64_t)a.b.rows * a.heads;
+        hipLaunchKernelGGL((attention_join_kernel<D, BF>), dim3((uint32_t)((heads + 3) / 4)), dim3(256), 0, stream, a);
+        OCO_TRY(launch_check("oco_cache_attention (join)"));
+    }
+    return OCO_OK;
+}
+
+static const char *attention_problem(const oco_cache *p) {
+    if (const char *why = cache_problem(p)) return why;
+    if (p->heads == 0) return "no heads";
+    if ((uint64_t)p->rows * p->heads > 0x7fffffffull) return "too many rows for one call";
+    return nullptr;
+}
+
+}  // namespace oco
+
+using namespace oco;
+
+extern "C" uint64_t oco_cache_attention_workspace(const oco_cache *p) {
+    return p && !attention_problem(p) ? attention_plan(p).bytes : 0;
+}
+
+extern "C" int oco_cache_attention(const void *q, const void *pages, const uint32_t *table, const uint32_t *starts,
+                                   const uint32_t *lengths, const float *sinks, void *out, const oco_cache *p, void *workspace,
+                                   uint64_t workspace_bytes, oco_stream stream) {
+    if (!p) return fail(OCO_ERR_INVALID, "oco_cache_attention: null description");
+    if (const char *why = attention_problem(p)) return fail(OCO_ERR_INVALID, "oco_cache_attention: %s", why);
+    if (p->dtype != OCO_DT_BF16 && p->dtype != OCO_DT_F16) return fail(OCO_ERR_UNSUPPORTED, "oco_cache_attention: type %u", p->dtype);
+    if (p->rows == 0 || p->sequences == 0 || p->max_rows == 0) return OCO_OK;
+    if (!q || !pages || !table || !lengths || !out) return fail(OCO_ERR_INVALID, "oco_cache_attention: null pointer");
+    if ((uintptr_t)pages & 15u) return fail(OCO_ERR_INVALID, "oco_cache_attention: pages must be 16-byte aligned");
+    if (!starts && p->rows % p->sequences)
+        return fail(OCO_ERR_INVALID, "oco_cache_attention: %u rows of %u sequences without starts", p->rows, p->sequences);
+    const AttentionPlan l = attention_plan(p);
+    if (l.bytes && (!workspace || ((uintptr_t)workspace & 15u) || workspace_bytes < l.bytes))
+        return fail(OCO_ERR_INVALID, "oco_cache_attention: workspace of %llu bytes, need %llu, 16-byte aligned",
+                    (unsigned long long)workspace_bytes, (unsigned long long)l.bytes);
+    AttentionArgs a;
+    a.b = cache_batch(p, table, starts, lengths);
+    a.cache = (const uint8_t *)pages;
+    a.q = q;
+    a.out = out;
+    a.sinks = sinks;
+    a.parts = (float *)workspace;
+    a.q_stride = p->q_stride ? p->q_stride : (uint64_t)p->heads * p->head_dim;
+    a.out_stride = p->out_stride ? p->out_stride : (uint64_t)p->heads * p->head_dim;
+    a.heads = p->heads;
+    a.group = p->heads / p->kv_heads;
+    a.window = p->window >= p->max_length ? 0 : p->window;
+    a.chunks = l.chunks;
+    a.chunk = l.chunk;
+    a.c = (p->scale != 0.f ? p->scale : 1.f / sqrtf((float)p->head_dim)) * 1.44269504088896341f;
+    hipStream_t st = (hipStream_t)stream;
+    const bool bf = p->dtype == OCO_DT_BF16;
+    switch (p->head_dim) {
+    case 64: return bf ? attention_launch<64, true>(a, l, st) : attention_launch<64, false>(a, l, st);
+    case 128: return bf ? attention_launch<128, true>(a, l, st) : attention_launch<128, false>(a, l, st);
+    default: return bf ? attention_launch<256, true>(a, l, st) : attention_launch<256, false>(a, l, st);
+    }
+}

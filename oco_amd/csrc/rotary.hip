@@ -1,0 +1,462 @@
+// Rotary positions, and the pages of a cache in 4 bits: appending rows with
+// their rotation on the way, and reading them back.
+//
+// Angles are position * frequency in 64 bits, at most 2^-53 of themselves off
+// (1e-10 at a million radians, where f32 would be off by 0.06), their cosines
+// and sines by Taylor series on a quarter turn, and the products are 64-bit
+// too: a key next to a border between two codes falls where the exact one
+// does.  One token's pairs are the same for all its heads, so a workgroup
+// takes one token (or a slice of its heads) and keeps them in LDS.
+#include "cache.h"
+
+namespace oco {
+
+// cos and sin of a: a - k pi/2 with pi/2 in two parts, then Taylor series for
+// |r| <= pi/4, whose first terms left out are r^19 / 19! and r^20 / 20! (1e-19).
+__device__ __forceinline__ double2 cos_sin(double a) {
+    const double k = __builtin_rint(a * 0.63661977236758134308);
+    double r = __builtin_fma(-k, 1.57079632679489655800, a);
+    r = __builtin_fma(-k, 6.12323399573676603587e-17, r);
+    const double q = r * r;
+    constexpr double S[8] = {1.0 / 355687428096000.0, -1.0 / 1307674368000.0, 1.0 / 6227020800.0, -1.0 / 39916800.0,
+                             1.0 / 362880.0, -1.0 / 5040.0, 1.0 / 120.0, -1.0 / 6.0};
+    constexpr double C[9] = {-1.0 / 6402373705728000.0, 1.0 / 20922789888000.0, -1.0 / 87178291200.0, 1.0 / 479001600.0, -1.0 / 3628800.0,
+                             1.0 / 40320.0, -1.0 / 720.0, 1.0 / 24.0, -0.5};
+    double s = S[0], c = C[0];
+#pragma unroll
+    for (int i = 1; i < 9; i++) {
+        if (i < 8) s = __builtin_fma(s, q, S[i]);
+        c = __builtin_fma(c, q, C[i]);
+    }
+    s = __builtin_fma(s * q, r, r);
+    c = __builtin_fma(c, q, 1.0);
+    const uint32_t quarter = (uint32_t)(long long)k & 3;
+    const double x = quarter & 1 ? s : c, y = quarter & 1 ? c : s;
+    return make_double2(quarter == 1 || quarter == 2 ? -x : x, quarter & 2 ? -y : y);
+}
+
+struct Rotation {
+    const double *frequencies;
+    double magnitude;
+    uint32_t dim, interleaved;
+};
+
+// The pairs' cosines and sines of one position, for the whole workgroup.
+__device__ __forceinline__ void rotation_table(const Rotation &r, uint32_t position, double2 *table) {
+    for (uint32_t i = threadIdx.x; i < r.dim / 2; i += blockDim.x) {
+        const double2 t = cos_sin((double)position * r.frequencies[i]);
+        table[i] = make_double2(t.x * r.magnitude, t.y * r.magnitude);
+    }
+    __syncthreads();
+}
+
+// A head as units of work: eight pairs (four interleaved), then runs of eight
+// values that stay.  A unit reads what it writes and nothing else, so the
+// result may take the place of the row.
+struct HeadUnits {
+    uint32_t turns, all;
+};
+__device__ __forceinline__ HeadUnits head_units(const Rotation &r, uint32_t head_dim) {
+    HeadUnits u;
+    u.turns = r.interleaved ? (r.dim + 7) / 8 : (r.dim / 2 + 7) / 8;
+    u.all = u.turns + (head_dim - r.dim + 7) / 8;
+    return u;
+}
+
+// Unit u of a head.  put(column, count limit, values): eight values from a column on, those under the limit.
+template <class T, class Put>
+__device__ __forceinline__ void turn_unit(const T *x, uint32_t u, uint32_t turns, uint32_t head_dim, const Rotation &r, const double2 *table, Put put) {
+    float a[8], b[8];
+    if (u >= turns) {
+        const uint32_t c = r.dim + 8 * (u - turns);
+        load_run(x, c, head_dim, a);
+        put(c, head_dim, a);
+        return;
+    }
+    if (r.interleaved) {
+        load_run(x, 8 * u, r.dim, a);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const double2 t = table[min(4 * u + j, r.dim / 2 - 1)];
+            const double v = a[2 * j], w = a[2 * j + 1];
+            a[2 * j] = (float)__builtin_fma(v, t.x, -(w * t.y));
+            a[2 * j + 1] = (float)__builtin_fma(w, t.x, v * t.y);
+        }
+        put(8 * u, r.dim, a);
+        return;
+    }
+    const uint32_t half = r.dim / 2;
+    load_run(x, 8 * u, half, a);
+    load_run(x + half, 8 * u, half, b);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const double2 t = table[min(8 * u + j, half - 1)];
+        const double v = a[j], w = b[j];
+        a[j] = (float)__builtin_fma(v, t.x, -(w * t.y));
+        b[j] = (float)__builtin_fma(w, t.x, v * t.y);
+    }
+    put(8 * u, half, a);
+#pragma unroll
+    for (int j = 0; j < 8; j++) a[j] = b[j];
+    put(half + 8 * u, r.dim, a);
+}
+
+// ---- rotation alone ----------------------------------------------------------------
+
+struct RotateArgs {
+    const void *x;
+    void *out;
+    const uint32_t *positions;
+    uint64_t x_stride, out_stride;
+    uint32_t heads, head_dim, parts;
+    Rotation r;
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
+    extern __shared__ double2 table[];
+    const uint32_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    rotation_table(a.r, a.positions[row], table);
+    const HeadUnits n = head_units(a.r, a.head_dim);
+    const T *x = (const T *)a.x + row * a.x_stride;
+    T *out = (T *)a.out + row * a.out_stride;
+    const uint32_t total = a.heads * n.all;
+    for (uint32_t i = part * 256 + threadIdx.x; i < total; i += a.parts * 256) {
+        const uint32_t h = i / n.all, u = i % n.all;
+        T *const o = out + (uint64_t)h * a.head_dim;
+        turn_unit(x + (uint64_t)h * a.head_dim, u, n.turns, a.head_dim, a.r, table,
+                  [&](uint32_t c, uint32_t limit, const float *v) { store_run(o, c, limit, v); });
+    }
+}
+
+// ---- appending -----------------------------------------------------------------------
+
+struct AppendArgs {
+    CacheBatch b;
+    uint8_t *cache;
+    const uint32_t *positions;
+    const void *q, *k, *v;
+    void *q_out;
+    uint64_t q_stride, k_stride, v_stride, out_stride;
+    uint32_t heads, parts, part_heads;  // part_heads: of the cache
+    Rotation r;
+};
+
+constexpr uint32_t APPEND_VALUES = 2048;  // of keys in LDS per workgroup, at most
+
+template <class T, uint32_t D>
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
+    __shared__ double2 table[D / 2];
+    __shared__ __attribute__((aligned(16))) float keys[APPEND_VALUES];
+    const uint32_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    const uint32_t s = cache_sequence(a.b, row);
+    if (s >= a.b.sequences) return;
+    const CacheSpan span = cache_span(a.b, s);
+    if (row - span.first >= span.rows) return;
+    const uint32_t back = span.rows - (row - span.first);  // the row's place from the end
+    const bool token = span.length >= back;
+    const uint32_t at = token ? span.length - back : 0;
+    rotation_table(a.r, a.positions ? a.positions[row] : at, table);
+    const HeadUnits n = head_units(a.r, D);
+    const uint32_t h0 = part * a.part_heads, heads = min(a.part_heads, a.b.kv_heads - h0), group = a.heads / a.b.kv_heads;
+    if (token)
+        for (uint32_t i = threadIdx.x; i < heads * n.all; i += 256) {
+            const uint32_t h = i / n.all, u = i % n.all;
+            float *const o = keys + h * D;
+            turn_unit((const T *)a.k + row * a.k_stride + (h0 + h) * D, u, n.turns, D, a.r, table, [&](uint32_t c, uint32_t limit, const float *v) {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (c + j < limit) o[c + j] = RowIO<T>::round(v[j]);
+            });
+        }
+    if (a.q)
+        for (uint32_t i = threadIdx.x; i < heads * group * n.all; i += 256) {
+            const uint32_t h = h0 * group + i / n.all, u = i % n.all;
+            T *const o = (T *)a.q_out + row * a.out_stride + h * D;
+            turn_unit((const T *)a.q + row * a.q_stride + h * D, u, n.turns, D, a.r, table,
+                      [&](uint32_t c, uint32_t limit, const float *v) { store_run(o, c, limit, v); });
+        }
+    if (!token) return;
+    const uint32_t page = a.b.table[(uint64_t)s * a.b.table_stride + at / a.b.page_size], t = at % a.b.page_size;
+    if (page >= a.b.pages) return;
+    __syncthreads();
+    const uint32_t head_bytes = cache_head_bytes(a.b.page_size, D);
+    constexpr uint32_t WORDS = D / 8;
+    // keys' words, then values'; blocks of four words stay in four adjacent threads
+    for (uint32_t i = threadIdx.x; i < 2 * heads * WORDS; i += 256) {
+        const bool value = i >= heads * WORDS;
+        const uint32_t j = value ? i - heads * WORDS : i, h = j / WORDS, w = j % WORDS;
+        float x[8];
+        if (value)
+            RowIO<T>::load8((const T *)a.v + row * a.v_stride + (h0 + h) * D + 8 * w, x);
+        else
+            RowIO<float>::load8(keys + h * D + 8 * w, x);
+        uint32_t scale;
+        const uint32_t codes = cache_quantize(x, scale);
+        uint8_t *const head = a.cache + ((uint64_t)page * a.b.kv_heads + h0 + h) * head_bytes;
+        if (!value) {
+            *(uint32_t *)(head + cache_key_at(t, w, D)) = codes;
+        } else if constexpr (D == 64) {  // a word is two pieces
+            *(uint16_t *)(head + cache_value_at(a.b.page_size, t, 4 * w, D)) = (uint16_t)codes;
+            *(uint16_t *)(head + cache_value_at(a.b.page_size, t, 4 * w + 2, D)) = (uint16_t)(codes >> 16);
+        } else {
+            *(uint32_t *)(head + cache_value_at(a.b.page_size, t, 4 * w, D)) = codes;
+        }
+        if (w % 4 == 0)
+            head[value ? cache_value_scale_at(a.b.page_size, t, w / 4, D) : cache_key_scale_at(a.b.page_size, t, w / 4, D)] = (uint8_t)scale;
+    }
+}
+
+// ---- reading back ----------------------------------------------------------------------
+
+struct ReadArgs {
+    CacheBatch b;
+    const uint8_t *cache;
+    void *k, *v;
+    uint64_t k_stride, v_stride;
+};
+
+template <class T, uint32_t D>
+__global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
+    const uint32_t row = blockIdx.x, s = cache_sequence(a.b, row);
+    if (s >= a.b.sequences) return;
+    const CacheSpan span = cache_span(a.b, s);
+    if (row - span.first >= span.rows) return;
+    const uint32_t back = span.rows - (row - span.first);
+    const bool token = span.length >= back;
+    const uint32_t at = token ? span.length - back : 0, t = at % a.b.page_size;
+    const uint32_t page = token ? a.b.table[(uint64_t)s * a.b.table_stride + at / a.b.page_size] : 0;
+    const bool known = page < a.b.pages;
+    const uint32_t head_bytes = cache_head_bytes(a.b.page_size, D);
+    constexpr uint32_t WORDS = D / 8;
+    for (uint32_t i = threadIdx.x; i < 2 * a.b.kv_heads * WORDS; i += 256) {
+        const bool value = i >= a.b.kv_heads * WORDS;
+        const uint32_t j = value ? i - a.b.kv_heads * WORDS : i, h = j / WORDS, w = j % WORDS;
+        float x[8];
+#pragma unroll
+        for (int c = 0; c < 8; c++) x[c] = token ? __uint_as_float(0x7fc00000u) : 0.f;
+        if (token && known) {
+            const uint8_t *const head = a.cache + ((uint64_t)page * a.b.kv_heads + h) * head_bytes;
+            uint32_t codes;
+            if (!value) {
+                codes = *(const uint32_t *)(head + cache_key_at(t, w, D));
+            } else if constexpr (D == 64) {
+                codes = *(const uint16_t *)(head + cache_value_at(a.b.page_size, t, 4 * w, D));
+                codes |= (uint32_t)*(const uint16_t *)(head + cache_value_at(a.b.page_size, t, 4 * w + 2, D)) << 16;
+            } else {
+                codes = *(const uint32_t *)(head + cache_value_at(a.b.page_size, t, 4 * w, D));
+            }
+            cache_dequantize(codes, head[value ? cache_value_scale_at(a.b.page_size, t, w / 4, D) : cache_key_scale_at(a.b.page_size, t, w / 4, D)], x);
+        }
+        T *const out = value ? (T *)a.v + row * a.v_stride : (T *)a.k + row * a.k_stride;
+        RowIO<T>::store8(out + h * D + 8 * w, x);
+    }
+}
+
+// ---- checks ------------------------------------------------------------------------------
+
+static const char *pool_problem(const oco_cache *p) {
+    if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256) return "head_dim is not 64, 128 or 256";
+    if (p->kv_heads == 0 || p->kv_heads > 65535) return "kv_heads is not in 1 .. 65535";
+    if (p->page_size == 0 || p->page_size % 16 || p->page_size > 65536) return "page_size is not a multiple of 16 up to 65536";
+    return nullptr;
+}
+const char *cache_problem(const oco_cache *p) {
+    if (const char *why = pool_problem(p)) return why;
+    if (p->heads > 65535 || p->heads % p->kv_heads) return "heads is not a multiple of kv_heads under 65536";
+    if (p->pages == 0) return "no pages";
+    if ((uint64_t)p->max_length > (uint64_t)p->table_stride * p->page_size || p->max_length > 0x3fffffffu) return "max_length is past the table's pages";
+    if (!(p->scale >= 0.f && p->scale < INFINITY)) return "the scale is not in 0 .. Inf";
+    const uint64_t q = (uint64_t)p->heads * p->head_dim, kv = (uint64_t)p->kv_heads * p->head_dim;
+    if ((p->q_stride && p->q_stride < q) || (p->out_stride && p->out_stride < q) || (p->k_stride && p->k_stride < kv) || (p->v_stride && p->v_stride < kv))
+        return "a row stride under the row";
+    return nullptr;
+}
+
+CacheBatch cache_batch(const oco_cache *p, const uint32_t *table, const uint32_t *starts, const uint32_t *lengths) {
+    return CacheBatch{table, starts, lengths, p->sequences, p->rows, p->max_rows, p->max_length, p->table_stride, p->page_size, p->pages, p->kv_heads};
+}
+
+static const char *rotation_problem(const oco_rotation *r, uint32_t head_dim) {
+    if (r->dim % 2 || r->dim > head_dim || r->dim > OCO_ROTATION_DIM) return "dim is odd or past the head";
+    if (r->layout > OCO_ROTATION_INTERLEAVED) return "unknown layout";
+    if (r->dim && !r->frequencies) return "no frequencies";
+    return nullptr;
+}
+static Rotation rotation_of(const oco_rotation *r) {
+    if (!r) return Rotation{nullptr, 1.0, 0, 0};
+    return Rotation{r->frequencies, r->magnitude, r->dim, r->layout == OCO_ROTATION_INTERLEAVED};
+}
+
+// What append and read share: 0 rows or a refusal end the call (done).
+static int cache_call(const char *name, const oco_cache *p, const void *pages, const uint32_t *table, const uint32_t *starts,
+                      const uint32_t *lengths, bool rest, bool *done) {
+    *done = true;
+    if (!p) return fail(OCO_ERR_INVALID, "%s: null description", name);
+    if (const char *why = cache_problem(p)) return fail(OCO_ERR_INVALID, "%s: %s", name, why);
+    if (p->dtype > OCO_DT_F16) return fail(OCO_ERR_UNSUPPORTED, "%s: type %u", name, p->dtype);
+    if (p->rows == 0 || p->sequences == 0 || p->max_rows == 0) return OCO_OK;
+    if (!pages || !table || !lengths || !rest) return fail(OCO_ERR_INVALID, "%s: null pointer", name);
+    if ((uintptr_t)pages & 15u) return fail(OCO_ERR_INVALID, "%s: pages must be 16-byte aligned", name);
+    if (!starts && p->rows % p->sequences)
+        return fail(OCO_ERR_INVALID, "%s: %u rows of %u sequences without starts", name, p->rows, p->sequences);
+    *done = false;
+    return OCO_OK;
+}
+
+}  // namespace oco
+
+using namespace oco;
+
+extern "C" int oco_rotation_frequencies(const oco_frequencies *p, double *out, double *magnitude) {
+    if (!p || !out) return fail(OCO_ERR_INVALID, "oco_rotation_frequencies: null pointer");
+    if (p->dim % 2 || p->dim > OCO_ROTATION_DIM) return fail(OCO_ERR_INVALID, "oco_rotation_frequencies: dim %u is odd or past %u", p->dim, OCO_ROTATION_DIM);
+    if (p->scaling > OCO_SCALING_BANDS) return fail(OCO_ERR_INVALID, "oco_rotation_frequencies: scaling %u", p->scaling);
+    if (!(p->base > 1.0 && p->base < INFINITY)) return fail(OCO_ERR_INVALID, "oco_rotation_frequencies: the base is not past 1");
+    const bool bands = p->scaling >= OCO_SCALING_YARN;
+    if (p->scaling != OCO_SCALING_NONE && !(p->factor >= 1.0 && p->factor < INFINITY))
+        return fail(OCO_ERR_INVALID, "oco_rotation_frequencies: the factor is under 1");
+    if (bands && !(p->original >= 1.0 && p->original < INFINITY && p->slow > 0.0 && p->fast > p->slow && p->fast < INFINITY))
+        return fail(OCO_ERR_INVALID, "oco_rotation_frequencies: original, fast and slow");
+    const uint32_t n = p->dim / 2;
+    const double pi = 3.14159265358979323846;
+    // the pair that turns `turns` times over the original context, as a real number
+    auto pair_of = [&](double turns) { return p->dim * log(p->original / (turns * 2.0 * pi)) / (2.0 * log(p->base)); };
+    double low = 0.0, high = 0.0;
+    if (p->scaling == OCO_SCALING_YARN) {
+        low = fmax(floor(pair_of(p->fast)), 0.0);
+        high = fmin(ceil(pair_of(p->slow)), p->dim - 1.0);
+    }
+    for (uint32_t j = 0; j < n; j++) {
+        double f = pow(p->base, -2.0 * j / p->dim);
+        if (p->factors) {
+            if (!(p->factors[j] > 0.f && p->factors[j] < INFINITY)) return fail(OCO_ERR_INVALID, "oco_rotation_frequencies: factor of pair %u", j);
+            f /= (double)p->factors[j];
+        }
+        if (p->scaling == OCO_SCALING_LINEAR) {
+            f /= p->factor;
+        } else if (bands) {
+            // how far the pair is from `stays` (0) to `divided` (1)
+            const double ramp = p->scaling == OCO_SCALING_YARN ? (j - low) / fmax(high - low, 0.001)
+                                                               : (p->fast - p->original * f / (2.0 * pi)) / (p->fast - p->slow);
+            const double r = fmin(fmax(ramp, 0.0), 1.0);
+            f = f / p->factor * r + f * (1.0 - r);
+        }
+        out[j] = f;
+    }
+    if (magnitude) *magnitude = p->scaling == OCO_SCALING_YARN ? 0.1 * log(p->factor) + 1.0 : 1.0;
+    return OCO_OK;
+}
+
+extern "C" int oco_rotate(const void *x, oco_dtype dtype, uint32_t rows, uint32_t heads, uint32_t head_dim, uint64_t x_stride,
+                          const uint32_t *positions, void *out, uint64_t out_stride, const oco_rotation *rotation, oco_stream stream) {
+    if (!rotation) return fail(OCO_ERR_INVALID, "oco_rotate: null rotation");
+    if (const char *why = rotation_problem(rotation, head_dim)) return fail(OCO_ERR_INVALID, "oco_rotate: %s", why);
+    if ((uint32_t)dtype > OCO_DT_F16) return fail(OCO_ERR_UNSUPPORTED, "oco_rotate: type %u", (uint32_t)dtype);
+    const uint64_t width = (uint64_t)heads * head_dim;
+    if ((x_stride && x_stride < width) || (out_stride && out_stride < width)) return fail(OCO_ERR_INVALID, "oco_rotate: a row stride under the row");
+    if (width > 0x7fffffffull) return fail(OCO_ERR_INVALID, "oco_rotate: rows of %llu values", (unsigned long long)width);
+    if (rows == 0 || width == 0) return OCO_OK;
+    if (!x || !out || !positions) return fail(OCO_ERR_INVALID, "oco_rotate: null pointer");
+    RotateArgs a;
+    a.x = x;
+    a.out = out;
+    a.positions = positions;
+    a.x_stride = x_stride ? x_stride : width;
+    a.out_stride = out_stride ? out_stride : width;
+    if (x == out && a.x_stride != a.out_stride) return fail(OCO_ERR_INVALID, "oco_rotate: in place with another stride");
+    a.heads = heads;
+    a.head_dim = head_dim;
+    a.r = rotation_of(rotation);
+    a.parts = rows < 128 ? (uint32_t)((width + 2047) / 2048) : 1;
+    if (a.parts > 16) a.parts = 16;
+    if ((uint64_t)rows * a.parts > 0x7fffffffull) return fail(OCO_ERR_INVALID, "oco_rotate: %u rows", rows);
+    const dim3 grid(rows * a.parts);
+    const uint32_t lds = (rotation->dim / 2) * sizeof(double2);
+    hipStream_t st = (hipStream_t)stream;
+    switch (dtype) {
+    case OCO_DT_F32: hipLaunchKernelGGL((rotate_kernel<float>), grid, dim3(256), lds, st, a); break;
+    case OCO_DT_BF16: hipLaunchKernelGGL((rotate_kernel<bf16_t>), grid, dim3(256), lds, st, a); break;
+    default: hipLaunchKernelGGL((rotate_kernel<f16_t>), grid, dim3(256), lds, st, a);
+    }
+    return launch_check("oco_rotate");
+}
+
+extern "C" uint64_t oco_cache_page_bytes(const oco_cache *p) {
+    return p && !pool_problem(p) ? (uint64_t)cache_head_bytes(p->page_size, p->head_dim) * p->kv_heads : 0;
+}
+
+extern "C" int oco_cache_append(void *pages, const uint32_t *table, const uint32_t *starts, const uint32_t *lengths,
+                                const uint32_t *positions, const void *q, const void *k, const void *v, void *q_out,
+                                const oco_rotation *rotation, const oco_cache *p, oco_stream stream) {
+    bool done;
+    const int rc = cache_call("oco_cache_append", p, pages, table, starts, lengths, k && v && (!q || q_out), &done);
+    if (done) return rc;
+    if (rotation)
+        if (const char *why = rotation_problem(rotation, p->head_dim)) return fail(OCO_ERR_INVALID, "oco_cache_append: %s", why);
+    AppendArgs a;
+    a.b = cache_batch(p, table, starts, lengths);
+    a.cache = (uint8_t *)pages;
+    a.positions = positions;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q_out = q_out;
+    a.q_stride = p->q_stride ? p->q_stride : (uint64_t)p->heads * p->head_dim;
+    a.out_stride = p->out_stride ? p->out_stride : (uint64_t)p->heads * p->head_dim;
+    a.k_stride = p->k_stride ? p->k_stride : (uint64_t)p->kv_heads * p->head_dim;
+    a.v_stride = p->v_stride ? p->v_stride : (uint64_t)p->kv_heads * p->head_dim;
+    if (q && q == q_out && a.q_stride != a.out_stride) return fail(OCO_ERR_INVALID, "oco_cache_append: queries in place with another stride");
+    a.heads = p->heads;
+    a.r = rotation_of(rotation);
+    a.part_heads = APPEND_VALUES / p->head_dim;
+    a.parts = (p->kv_heads + a.part_heads - 1) / a.part_heads;
+    if ((uint64_t)p->rows * a.parts > 0x7fffffffull) return fail(OCO_ERR_INVALID, "oco_cache_append: %u rows", p->rows);
+    const dim3 grid(p->rows * a.parts);
+    hipStream_t st = (hipStream_t)stream;
+#define GO(T)                                                                                               \
+    switch (p->head_dim) {                                                                                  \
+    case 64: hipLaunchKernelGGL((append_kernel<T, 64>), grid, dim3(256), 0, st, a); break;                  \
+    case 128: hipLaunchKernelGGL((append_kernel<T, 128>), grid, dim3(256), 0, st, a); break;                \
+    default: hipLaunchKernelGGL((append_kernel<T, 256>), grid, dim3(256), 0, st, a);                        \
+    }                                                                                                       \
+    break;
+    switch (p->dtype) {
+    case OCO_DT_F32: GO(float)
+    case OCO_DT_BF16: GO(bf16_t)
+    default: GO(f16_t)
+    }
+#undef GO
+    return launch_check("oco_cache_append");
+}
+
+extern "C" int oco_cache_read(const void *pages, const uint32_t *table, const uint32_t *starts, const uint32_t *lengths, void *k,
+                              void *v, const oco_cache *p, oco_stream stream) {
+    bool done;
+    const int rc = cache_call("oco_cache_read", p, pages, table, starts, lengths, k && v, &done);
+    if (done) return rc;
+    ReadArgs a;
+    a.b = cache_batch(p, table, starts, lengths);
+    a.cache = (const uint8_t *)pages;
+    a.k = k;
+    a.v = v;
+    a.k_stride = p->k_stride ? p->k_stride : (uint64_t)p->kv_heads * p->head_dim;
+    a.v_stride = p->v_stride ? p->v_stride : (uint64_t)p->kv_heads * p->head_dim;
+    const dim3 grid(p->rows);
+    if (p->rows > 0x7fffffffu) return fail(OCO_ERR_INVALID, "oco_cache_read: %u rows", p->rows);
+    hipStream_t st = (hipStream_t)stream;
+#define GO(T)                                                                                               \
+    switch (p->head_dim) {                                                                                  \
+    case 64: hipLaunchKernelGGL((read_kernel<T, 64>), grid, dim3(256), 0, st, a); break;                    \
+    case 128: hipLaunchKernelGGL((read_kernel<T, 128>), grid, dim3(256), 0, st, a); break;                  \
+    default: hipLaunchKernelGGL((read_kernel<T, 256>), grid, dim3(256), 0, st, a);                          \
+    }                                                                                                       \
+    break;
+    switch (p->dtype) {
+    case OCO_DT_F32: GO(float)
+    case OCO_DT_BF16: GO(bf16_t)
+    default: GO(f16_t)
+    }
+#undef GO
+    return launch_check("oco_cache_read");
+}

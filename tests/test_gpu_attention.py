@@ -1,0 +1,318 @@
+"""oco_cache_attention against softmax attention in 64 bits over the values that the pages stand for."""
+import numpy as np
+import pytest
+
+from _cache import Batch, Pool, dequantize, quantize
+from _ops import CODE, HALF, LEAST, SIZE, dev, stored, values
+from _util import Guarded, say
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+class Case:
+    def __init__(self, lib, rng, rows, lengths, heads, kv, d, P, dtype, window=0, sinks=False, extra_rows=0, pad=(0, 0), q_scale=2.0, scale=0.0,
+                 holes=0, max_rows=None, v_scale=1.0):
+        self.lib, self.dtype, self.heads, self.kv, self.d, self.window = lib, dtype, heads, kv, d, window
+        b = self.b = Batch(rng, rows, lengths, P, extra_rows=extra_rows)
+        self.scale = scale or 1 / np.sqrt(d)
+        self.k, self.v, pool = [], [], Pool(b.pages, kv, P, d)
+        for s, n in enumerate(lengths):
+            k, v = rng.normal(size=(n, kv, d)), rng.normal(size=(n, kv, d)) * v_scale + 0.3
+            for _ in range(holes if n else 0):  # blocks of NaN among the tokens
+                (k if rng.random() < 0.5 else v)[rng.integers(0, n), rng.integers(0, kv), rng.integers(0, d)] = np.nan
+            ck, cv = quantize(k), quantize(v)
+            for t in range(n):
+                page, slot = b.place(s, t)
+                for j in range(kv):
+                    pool.put(page, slot, j, (ck[0][t, j], ck[1][t, j]), (cv[0][t, j], cv[1][t, j]))
+            self.k.append(dequantize(*ck))
+            self.v.append(dequantize(*cv))
+        self.pool = pool
+        self.q_stride, self.out_stride = heads * d + pad[0], heads * d + pad[1]
+        raw, q = stored(rng.normal(size=(b.total, self.q_stride)) * q_scale, dtype)
+        self.q = q[:, :heads * d].reshape(b.total, heads, d)
+        self.sinks = (rng.normal(size=heads) * 2).astype(np.float32) if sinks else None
+        self.p = b.describe(lib, heads, kv, d, CODE[dtype], window=window, scale=scale, q_stride=self.q_stride if pad[0] else 0,
+                            out_stride=self.out_stride if pad[1] else 0, **({} if max_rows is None else {"max_rows": max_rows}))
+        self.dev = [dev(lib, raw), dev(lib, pool.bytes), dev(lib, b.table), dev(lib, np.array(lengths, np.uint32)), dev(lib, b.starts),
+                    dev(lib, self.sinks) if sinks else None]
+        self.out = Guarded(lib, b.total * self.out_stride * SIZE[dtype])
+        self.need = lib.cache_attention_workspace(self.p)
+        self.work = Guarded(lib, self.need)
+
+    def call(self, stream=None, starts=True):
+        q, cache, table, lengths, st, sinks = self.dev
+        self.lib.cache_attention(q, cache, table, lengths, self.out.ptr, self.p, starts=st if starts else None, sinks=sinks,
+                                 workspace=self.work.ptr if self.need else None, workspace_bytes=self.need, stream=stream)
+
+    def want(self, b=None):
+        """The rows, and how far off they may be."""
+        b = b or self.b
+        out, tol = np.zeros(self.q.shape), np.zeros(self.q.shape)
+        g = self.heads // self.kv
+        for s, (n, length) in enumerate(zip(b.rows, b.lengths)):
+            for i in range(n):
+                r, at = int(b.starts[s]) + i, length - n + i
+                lo = max(0, at + 1 - self.window) if self.window else 0
+                for h in range(self.heads):
+                    if at < 0:
+                        continue
+                    q, k, v = self.q[r, h], self.k[s][lo:at + 1, h // g], self.v[s][lo:at + 1, h // g]
+                    with np.errstate(all="ignore"):
+                        score, mag = k @ q * self.scale, np.abs(k) @ np.abs(q) * self.scale
+                        top = score.max() if self.sinks is None else max(score.max(), float(self.sinks[h]))
+                        e = np.exp(score - top)
+                        total = e.sum() + (0.0 if self.sinks is None else np.exp(float(self.sinks[h]) - top))
+                        out[r, h], a = e @ v / total, e @ np.abs(v) / total
+                        # scores: products are exact, d sums in f32, then the factor, the maximum's subtraction and the exponential
+                        # (a step each, of numbers up to |score| log2 e and |top| log2 e): a relative error of each e of
+                        d = ((self.d + 2) * mag.max() + 4 * (np.abs(score).max() + abs(top)) + 4) * U
+                        # of the products' sum and of the total: d each, a step per f32 sum; e rounds to the 16-bit type (its
+                        # subnormal numbers in f16: half of 2^-24 each, where the largest e is 1 or more); the result rounds
+                        m = len(score) + 16
+                        tol[r, h] = a * (HALF[self.dtype] + 2 * d + 2 * m * U) + HALF[self.dtype] * np.abs(out[r, h]) * (1 + U) + LEAST[self.dtype]
+                        if self.dtype == "f16":
+                            tol[r, h] += 2.0 ** -25 * np.abs(v).sum(0) / total
+        return out, tol
+
+    def check(self, b=None):
+        want, tol = self.want(b)
+        z = SIZE[self.dtype]
+        raw = self.out.read(np.uint8)[:self.b.total * self.out_stride * z]
+        self.work.read(np.uint8)
+        n = int(self.b.starts[-1])
+        got = values(raw, self.dtype, (self.b.total, self.out_stride))[:n, :self.heads * self.d].reshape(n, self.heads, self.d)
+        want, tol = want[:n], tol[:n]
+        np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+        fine = ~np.isnan(want)
+        bad = np.abs(got - want)[fine] > tol[fine]
+        assert not bad.any(), (int(bad.sum()), got[fine][bad][:4], want[fine][bad][:4])
+        return got
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows,lengths", [([1], [1]), ([1], [2]), ([1, 1, 1, 1], [15, 16, 17, 33]), ([1, 1], [500, 1300]), ([3, 0, 5], [40, 7, 300]),
+                                          ([4], [4]), ([40, 1], [90, 260])])
+def test_lengths(lib, dtype, d, rows, lengths):
+    rng = np.random.default_rng(d + sum(lengths))
+    say("attention", dtype, d, rows, lengths)
+    c = Case(lib, rng, rows, lengths, 4, 2, d, 16, dtype)
+    c.call()
+    lib.synchronize()
+    c.check()
+
+
+@pytest.mark.parametrize("heads,kv", [(1, 1), (3, 3), (5, 1), (14, 2), (16, 1), (17, 1), (32, 1), (40, 8), (72, 2)])
+@pytest.mark.parametrize("rows", [1, 3])
+def test_heads(lib, heads, kv, rows):
+    """Groups of one head to more than a tile of rows."""
+    rng = np.random.default_rng(heads * 10 + rows)
+    say("attention", heads, kv, rows)
+    c = Case(lib, rng, [rows, rows], [70, 133], heads, kv, 64, 48, "bf16")
+    c.call()
+    lib.synchronize()
+    c.check()
+
+
+@pytest.mark.parametrize("P", [16, 32, 48, 64, 256])
+@pytest.mark.parametrize("window", [0, 1, 16, 31, 100, 5000])
+def test_windows_and_pages(lib, P, window):
+    rng = np.random.default_rng(P + window)
+    say("attention", P, window)
+    for rows, lengths in (([1, 4, 2], [333, 64, 1]), ([65, 20], [200, 20])):
+        c = Case(lib, rng, rows, lengths, 8, 2, 64, P, "bf16", window=window)
+        c.call()
+        lib.synchronize()
+        c.check()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,lengths", [([1, 1], [50, 2100]), ([6, 3], [6, 700]), ([80], [160])])
+def test_sinks(lib, dtype, rows, lengths):
+    rng = np.random.default_rng(7)
+    say("sinks", dtype, rows)
+    c = Case(lib, rng, rows, lengths, 6, 2, 128, 64, dtype, sinks=True, q_scale=0.5)
+    c.sinks[0], c.sinks[1] = -np.inf, 60.0
+    c.dev[5].upload(c.sinks)
+    c.call()
+    lib.synchronize()
+    c.check()
+
+
+@pytest.mark.parametrize("sinks", [False, True])
+def test_rows_that_see_nothing(lib, sinks):
+    """Sequences without tokens, and with fewer tokens than rows: zeros; rows behind the last sequence stay."""
+    rng = np.random.default_rng(2)
+    for rows, lengths in (([1, 2, 5], [0, 0, 3]), ([90, 40], [30, 0])):
+        c = Case(lib, rng, rows, lengths, 4, 2, 128, 16, "bf16", sinks=sinks, extra_rows=4)
+        say("nothing seen", rows, lengths)
+        c.call()
+        lib.synchronize()
+        got = c.check()
+        assert not got[0].any()
+        tail = c.out.read(np.uint8).reshape(c.b.total, -1)[sum(rows):]
+        assert np.all(np.ascontiguousarray(tail).reshape(-1).view(np.uint32) == 0x7FC12345)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows,lengths,window", [([1, 8], [300, 40], 0), ([4, 3], [60, 200], 24), ([70, 33], [140, 33], 0), ([100], [150], 40)])
+def test_blocks_of_nan(lib, dtype, d, rows, lengths, window):
+    """A NaN reaches the rows that see it, a value's in its own 32 columns, and no other row: not those before it, not those
+    whose window has passed it."""
+    rng = np.random.default_rng(d + sum(rows))
+    say("nan", dtype, d, rows, lengths, window)
+    c = Case(lib, rng, rows, lengths, 4, 2, d, 32, dtype, window=window, holes=3)
+    c.call()
+    lib.synchronize()
+    c.check()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [5, 60])
+def test_nan_in_the_last_token(lib, d, rows):
+    """Only the last row sees it: a value's NaN its block of columns, a key's all of them."""
+    rng = np.random.default_rng(d)
+    for in_key in (False, True):
+        c = Case(lib, rng, [rows], [200], 4, 2, d, 16, "bf16")
+        page, slot = c.b.place(0, 199)
+        at = 16 * d + (slot * (d // 32) + 1 if in_key else 16 * (d // 32) + slot // 4 * (d // 8) + 4 + slot % 4)
+        c.pool.bytes[page, 1, at] = 255  # block 1 of the second head
+        (c.k if in_key else c.v)[0][199, 1, 32:64] = np.nan
+        c.dev[1].upload(c.pool.bytes)
+        say("last token", d, rows, in_key)
+        c.call()
+        lib.synchronize()
+        got = np.isnan(c.check())
+        want = np.zeros(got.shape, bool)
+        want[-1, 2:, slice(None) if in_key else slice(32, 64)] = True
+        np.testing.assert_array_equal(got, want)
+
+
+def test_pages_outside_the_pool(lib):
+    """They read as NaN where a row sees them, and nothing is read there."""
+    rng = np.random.default_rng(12)
+    for rows, lengths in (([1, 1], [100, 60]), ([40, 3], [100, 60])):
+        c = Case(lib, rng, rows, lengths, 4, 2, 128, 16, "bf16", window=30)
+        c.b.table[0, 1], c.b.table[0, 5], c.b.table[1, 3] = 0xFFFFFFFF, c.b.pages, 0x7FFFFFFF
+        c.dev[2].upload(c.b.table)
+        for s, page in ((0, 1), (0, 5), (1, 3)):
+            c.k[s][page * 16:page * 16 + 16] = np.nan
+        say("bad pages", rows)
+        c.call()
+        lib.synchronize()
+        c.check()
+
+
+@pytest.mark.parametrize("rows,lengths", [([2, 2, 2], [90, 5, 400]), ([30, 30], [30, 77])])
+def test_strides_and_no_starts(lib, rows, lengths):
+    rng = np.random.default_rng(5)
+    c = Case(lib, rng, rows, lengths, 6, 2, 64, 32, "f16", pad=(6, 10), scale=0.2)
+    say("strides", rows)
+    c.call(starts=False)
+    lib.synchronize()
+    c.check()
+    raw = c.out.read(np.uint8)[:c.b.total * c.out_stride * 2].view(np.uint16).reshape(c.b.total, c.out_stride)
+    guard = np.tile(np.array([0x2345, 0x7FC1], np.uint16), c.out_stride * c.b.total // 2 + 1)[:raw.size].reshape(raw.shape)
+    np.testing.assert_array_equal(raw[:, 6 * 64:], guard[:, 6 * 64:])
+
+
+@pytest.mark.parametrize("rows", [[1], [130]])
+def test_scores_that_rise_and_fall(lib, rows):
+    """Maxima that come early, late and in between, scores over a range of hundreds."""
+    rng = np.random.default_rng(6)
+    for order in (1, -1, 0):
+        c = Case(lib, rng, rows, [2000], 4, 1, 128, 64, "bf16", q_scale=30.0)
+        pool = Pool(c.b.pages, 1, 64, 128)
+        ramp = np.linspace(0.01, 1, 2000)[::order] if order else rng.random(2000)
+        k = rng.normal(size=(1, 128)) * 0.1 + ramp[:, None] * np.sign(c.q[0, 0])[None]
+        k, v = quantize(k), quantize(rng.normal(size=(2000, 128)))
+        for t in range(2000):
+            page, slot = c.b.place(0, t)
+            pool.put(page, slot, 0, (k[0][t], k[1][t]), (v[0][t], v[1][t]))
+        c.k[0], c.v[0] = dequantize(*k)[:, None], dequantize(*v)[:, None]
+        c.dev[1].upload(pool.bytes)
+        say("ramp", rows, order)
+        c.call()
+        lib.synchronize()
+        c.check()
+
+
+def test_infinite_queries(lib):
+    """An infinity or a NaN in a query makes its own row NaN and no other."""
+    rng = np.random.default_rng(15)
+    for rows in ([3], [50]):
+        c = Case(lib, rng, rows, [120], 4, 2, 64, 16, "bf16")
+        raw = c.dev[0].download(np.uint16).reshape(c.b.total, 4, 64)
+        raw[0, 1, 5], raw[1, 3, 2] = 0x7F80, 0x7FC0
+        c.dev[0].upload(raw)
+        c.q[0, 1, 5], c.q[1, 3, 2] = np.inf, np.nan
+        say("infinite", rows)
+        c.call()
+        lib.synchronize()
+        got = c.check()
+        bad = np.isnan(got).any(-1)
+        assert bad.sum() == 2 and bad[0, 1] and bad[1, 3]
+
+
+@pytest.mark.parametrize("dtype,v_scale", [("bf16", 2.0 ** 100), ("bf16", 2.0 ** -100), ("f16", 2.0 ** 11), ("f16", 2.0 ** -11)])
+def test_large_and_small_values(lib, dtype, v_scale):
+    rng = np.random.default_rng(16)
+    for rows in ([2], [40]):
+        c = Case(lib, rng, rows, [150], 4, 2, 128, 32, dtype, v_scale=v_scale)
+        say("range", dtype, v_scale, rows)
+        c.call()
+        lib.synchronize()
+        c.check()
+
+
+def test_shorter_bounds(lib):
+    """Lengths past max_length count as max_length; rows past max_rows stay."""
+    rng = np.random.default_rng(17)
+    c = Case(lib, rng, [3, 6], [50, 80], 4, 2, 64, 16, "bf16", max_rows=4)
+    c.p.max_length = 64
+    c.need = lib.cache_attention_workspace(c.p)
+    say("bounds")
+    c.call()
+    lib.synchronize()
+    raw = c.out.read(np.uint8).reshape(c.b.total, -1)
+    assert np.all(np.ascontiguousarray(raw[7:]).reshape(-1).view(np.uint32) == 0x7FC12345)
+    c.b.rows[1], c.b.lengths[1] = 4, 64
+    want, tol = c.want()
+    got = values(raw[:7], "bf16", (7, 4, 64))
+    assert np.all(np.abs(got - want[:7]) <= tol[:7])
+
+
+def test_same_result_every_time(lib):
+    rng = np.random.default_rng(18)
+    for rows, lengths in (([1, 1], [3000, 10]), ([200], [700])):
+        c = Case(lib, rng, rows, lengths, 8, 2, 128, 64, "bf16")
+        first = None
+        for _ in range(3):
+            c.call()
+            lib.synchronize()
+            raw = c.out.read(np.uint8).copy()
+            first = raw if first is None else first
+            np.testing.assert_array_equal(raw, first)
+
+
+def test_a_cache_past_32_bits(lib):
+    """Pages whose byte offsets pass 2^32."""
+    rng = np.random.default_rng(19)
+    for rows in ([1], [40]):
+        c = Case(lib, rng, rows, [100], 4, 2, 128, 16, "bf16")
+        page = int(lib.cache_page_bytes(c.p))
+        far = (1 << 32) // page + 5
+        big = lib.DeviceBuffer((far + c.b.pages) * page)
+        big.upload(c.pool.bytes, far * page)
+        c.p.pages = far + c.b.pages
+        c.b.table[0, :7] += far
+        c.dev[1] = big
+        c.dev[2].upload(c.b.table)
+        say("far pages", rows, far)
+        c.call()
+        lib.synchronize()
+        c.check()
+        big.free()
