@@ -80,6 +80,13 @@ __device__ __forceinline__ float row_max(float v) {
     auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, dpp_f32<0xB1>(v));
+    v = fmaxf(v, dpp_f32<0x4E>(v));
+    v = fmaxf(v, dpp_f32<0x124>(v));
+    v = fmaxf(v, dpp_f32<0x128>(v));
+    return row_max(v);
+}
 __device__ __forceinline__ float row_sum(float v) {
     auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
@@ -101,53 +108,82 @@ __device__ __forceinline__ float carry(float m, float to) { return m > -INFINITY
 // One half-step's 16 tokens as a lane holds them: lane m + 16 g has a quarter
 // of token m's key, and of tokens 4g .. 4g + 3 one sixteenth of the value.
 template <uint32_t D>
-struct Tokens {
-    static constexpr int KW = D / 32, VW = D / 32;  // words
-    uint32_t k[KW], v[VW], ks, vs;
+struct Keys {
+    uint32_t w[D / 32], scale;
+};
+template <uint32_t D>
+struct Values {
+    uint32_t w[D / 32], scale;  // the scale bytes of four tokens
 };
 
 template <uint32_t D>
-__device__ __forceinline__ void load_tokens(Tokens<D> &x, const uint8_t *head, uint32_t page_size, uint32_t t) {
-    const uint32_t m = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
-    const uint8_t *const k = head + (t + m) * (D / 2) + g * (D / 8);
-    const uint8_t *const v = head + page_size * (D / 2) + (t / 4 + g) * (2 * D) + m * (D / 8);
-    const uint8_t *const ks = head + page_size * D + (t + m) * (D / 32) + g * (D / 128);
-    const uint8_t *const vs = head + page_size * D + page_size * (D / 32) + (t / 4 + g) * (D / 8) + m * D / 512 * 4;
+__device__ __forceinline__ void load_words(uint32_t *w, const uint8_t *p) {
     if constexpr (D == 64) {
-        const uint2 a = *(const uint2 *)k, b = *(const uint2 *)v;
-        x.k[0] = a.x;
-        x.k[1] = a.y;
-        x.v[0] = b.x;
-        x.v[1] = b.y;
-        x.ks = head[page_size * D + (t + m) * 2 + g / 2];
+        const u32x2 a = *(const GLOBAL u32x2 *)gp(p);
+        w[0] = a[0];
+        w[1] = a[1];
     } else {
 #pragma unroll
         for (int i = 0; i < (int)D / 128; i++) {
-            const u32x4 a = ((const u32x4 *)k)[i], b = ((const u32x4 *)v)[i];
+            const u32x4 a = ((const GLOBAL u32x4 *)gp(p))[i];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                x.k[4 * i + j] = a[j];
-                x.v[4 * i + j] = b[j];
-            }
+            for (int j = 0; j < 4; j++) w[4 * i + j] = a[j];
         }
-        x.ks = D == 256 ? *(const uint16_t *)ks : *ks;
     }
-    x.vs = *(const uint32_t *)vs;
+}
+template <uint32_t D>
+__device__ __forceinline__ void load_keys(Keys<D> &x, const uint8_t *head, uint32_t page_size, uint32_t t) {
+    const uint32_t m = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+    load_words<D>(x.w, head + (t + m) * (D / 2) + g * (D / 8));
+    const uint8_t *const s = head + page_size * D + (t + m) * (D / 32) + (D == 64 ? g / 2 : g * (D / 128));
+    x.scale = D == 256 ? *(const GLOBAL uint16_t *)gp(s) : *gp(s);
+}
+template <uint32_t D>
+__device__ __forceinline__ void load_values(Values<D> &x, const uint8_t *head, uint32_t page_size, uint32_t t) {
+    const uint32_t m = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+    load_words<D>(x.w, head + page_size * (D / 2) + (t / 4 + g) * (2 * D) + m * (D / 8));
+    x.scale = *(const GLOBAL uint32_t *)gp(head + page_size * D + page_size * (D / 32) + (t / 4 + g) * (D / 8) + m * D / 512 * 4);
+}
+// Whether a byte of a word is 255.
+__device__ __forceinline__ bool holds_255(uint32_t x) { return ((~x - 0x01010101u) & x & 0x80808080u) != 0; }
+
+// The halves of a wavefront's steps, their pages and their places in them: a
+// lane per half, read once for 32 steps, so that a step's loads do not wait
+// for the table.
+struct Halves {
+    uint32_t page, slot;
+};
+__device__ __forceinline__ Halves load_halves(const uint32_t *table, uint32_t t0, uint32_t stride, uint32_t end, uint32_t page_size) {
+    const uint32_t lane = threadIdx.x & 63, t = t0 + lane / 2 * stride + lane % 2 * 16;
+    Halves h;
+    h.page = t < end ? table[t / page_size] : 0;
+    h.slot = t % page_size;
+    return h;
 }
 
 template <uint32_t D, bool BF, int R>
-__global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, uint32_t tiles) {
+__global__ __launch_bounds__(256, (D / 64) * R == 1 ? 4 : (D / 64) * R == 2 ? 3 : 2) void attention_few_kernel(AttentionArgs a, uint32_t tiles) {
     constexpr int KW = D / 32, NT = D / 16;  // key words per lane and token; tiles of 16 columns
     using H = Half<BF>;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const uint32_t chunk = blockIdx.x % a.chunks, tile = blockIdx.x / a.chunks % tiles, sh = blockIdx.x / a.chunks / tiles;
     const uint32_t s = sh / a.b.kv_heads, h = sh % a.b.kv_heads;
     const CacheSpan span = cache_span(a.b, s);
     const uint32_t row0 = tile * (16 * R), rows = span.rows * a.group;
     if (row0 >= rows) return;
+    const uint32_t last_row = min(row0 + 16 * R, rows) - 1;
+    const int32_t least = (int32_t)(span.length + row0 / a.group) - (int32_t)span.rows;
+    const int32_t most = (int32_t)(span.length + last_row / a.group) - (int32_t)span.rows;
+    // this chunk's tokens
+    const uint32_t base = first_seen(span, a.window) + chunk * a.chunk;
+    if (chunk && base >= span.length) return;  // the sequence has fewer chunks
+    const uint32_t end = most < 0 ? 0 : min(min(base + a.chunk, span.length), (uint32_t)most + 1);
+    const uint32_t head_bytes = cache_head_bytes(a.b.page_size, D);
+    const uint32_t *const table = a.b.table + (uint64_t)s * a.b.table_stride;
+    uint32_t t0 = base + 32 * wave, step = 0;
+    Halves halves = load_halves(table, t0, 128, end, a.b.page_size);
     // the rows' positions (-1: no token, and no row)
     int32_t at[R];
-    const uint16_t *qrow[R];
     u32x4 q[R][KW];
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -155,17 +191,10 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, uin
         const bool live = i < rows;
         const uint32_t token = live ? i / a.group : 0, head = h * a.group + (live ? i % a.group : 0);
         at[r] = live ? (int32_t)(span.length + token) - (int32_t)span.rows : -1;
-        qrow[r] = (const uint16_t *)a.q + (uint64_t)(span.first + token) * a.q_stride + (uint64_t)head * D + g * (D / 4);
+        const uint16_t *const row = (const uint16_t *)a.q + (uint64_t)(span.first + token) * a.q_stride + (uint64_t)head * D + g * (D / 4);
 #pragma unroll
-        for (int w = 0; w < KW; w++) q[r][w] = *(const u32x4_u *)(qrow[r] + 8 * w);
+        for (int w = 0; w < KW; w++) q[r][w] = *(const GLOBAL u32x4_u *)gp(row + 8 * w);
     }
-    const uint32_t last_row = min(row0 + 16 * R, rows) - 1;
-    const int32_t least = (int32_t)(span.length + row0 / a.group) - (int32_t)span.rows;
-    const int32_t most = (int32_t)(span.length + last_row / a.group) - (int32_t)span.rows;
-    // this chunk's tokens
-    const uint32_t base = first_seen(span, a.window) + chunk * a.chunk;
-    const uint32_t end = most < 0 ? 0 : min(min(base + a.chunk, span.length), (uint32_t)most + 1);
-
     float m[R], l[R];
     f32x4 o[R][NT];
 #pragma unroll
@@ -175,52 +204,74 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, uin
 #pragma unroll
         for (int j = 0; j < NT; j++) o[r][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const uint32_t head_bytes = cache_head_bytes(a.b.page_size, D);
-    const uint32_t *const table = a.b.table + (uint64_t)s * a.b.table_stride;
-    for (uint32_t t0 = base + 32 * wave; t0 < end; t0 += 128) {
-        Tokens<D> x[2];
-        bool lost[2];
+    // the next step's keys are requested when this step's are used up, its values likewise: the
+    // registers of one step, and always half a step's loads on their way
+    Keys<D> k[2];
+    Values<D> v[2];
+    const uint8_t *head[2];
+    uint32_t slot[2];
+    bool lost[2] = {false, false}, lost_next[2];
+    auto find = [&](uint32_t i) {
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            const uint32_t t = t0 + 16 * e;
-            uint32_t page = t < end ? table[t / a.b.page_size] : 0;
-            lost[e] = page >= a.b.pages;
-            page = lost[e] ? 0 : page;
-            load_tokens(x[e], a.cache + ((uint64_t)page * a.b.kv_heads + h) * head_bytes, a.b.page_size, t % a.b.page_size);
+            uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)halves.page, 2 * (i % 32) + e);
+            slot[e] = (uint32_t)__builtin_amdgcn_readlane((int)halves.slot, 2 * (i % 32) + e);
+            lost_next[e] = page >= a.b.pages;
+            page = lost_next[e] ? 0 : page;
+            head[e] = a.cache + ((uint64_t)page * a.b.kv_heads + h) * head_bytes;
         }
+    };
+    if (t0 < end) {
+        find(0);
+#pragma unroll
+        for (int e = 0; e < 2; e++) load_keys(k[e], head[e], a.b.page_size, slot[e]);
+#pragma unroll
+        for (int e = 0; e < 2; e++) load_values(v[e], head[e], a.b.page_size, slot[e]);
+    }
+    for (; t0 < end; t0 += 128) {
+        lost[0] = lost_next[0];
+        lost[1] = lost_next[1];
         // scores: lane (n, g) has row n's tokens 16 e + 4 g + i
         f32x4 sc[R][2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            if (lost[e]) {
-                x[e].ks = 0xffff;
-                x[e].vs = 0xffffffffu;
-            }
+            if (lost[e]) k[e].scale = 0xffff;
 #pragma unroll
             for (int r = 0; r < R; r++) sc[r][e] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < KW; w++) {
-                const float scale = cache_scale(D == 256 ? (w < 4 ? x[e].ks & 0xff : x[e].ks >> 8) : x[e].ks & 0xff);
-                const u32x4 k = {H::template pair<0>(x[e].k[w], scale), H::template pair<1>(x[e].k[w], scale),
-                                 H::template pair<2>(x[e].k[w], scale), H::template pair<3>(x[e].k[w], scale)};
+                const float scale = cache_scale(D == 256 ? (w < 4 ? k[e].scale & 0xff : k[e].scale >> 8) : k[e].scale & 0xff);
+                const u32x4 x = {H::template pair<0>(k[e].w[w], scale), H::template pair<1>(k[e].w[w], scale),
+                                 H::template pair<2>(k[e].w[w], scale), H::template pair<3>(k[e].w[w], scale)};
 #pragma unroll
-                for (int r = 0; r < R; r++) sc[r][e] = H::product(k, q[r][w], sc[r][e]);
+                for (int r = 0; r < R; r++) sc[r][e] = H::product(x, q[r][w], sc[r][e]);
             }
+        }
+        step++;
+        const bool more = t0 + 128 < end;
+        if (more) {
+            if (step % 32 == 0) halves = load_halves(table, t0 + 128, 128, end, a.b.page_size);
+            find(step);
+#pragma unroll
+            for (int e = 0; e < 2; e++) load_keys(k[e], head[e], a.b.page_size, slot[e]);
         }
         const bool edge = (int32_t)t0 + 31 > least || (a.window && (int32_t)t0 + (int32_t)a.window <= most);
         u32x4 p[R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            float v[8];
+            if (edge) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                v[i] = sc[r][i / 4][i % 4] * a.c;
-                const int32_t t = (int32_t)t0 + 16 * (i / 4) + 4 * (int32_t)g + i % 4;
-                if (edge) v[i] = t <= at[r] && (!a.window || t + (int32_t)a.window > at[r]) ? v[i] : -INFINITY;
+                for (int i = 0; i < 8; i++) {
+                    const int32_t t = (int32_t)t0 + 16 * (i / 4) + 4 * (int32_t)g + i % 4;
+                    if (!(t <= at[r] && (!a.window || t + (int32_t)a.window > at[r]))) sc[r][i / 4][i % 4] = -INFINITY;
+                }
             }
-            float top = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
-            top = fmaxf(row_max(top), m[r]);
-            if (__any(top > m[r])) {
+            const f32x4 x = sc[r][0], y = sc[r][1];
+            float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+            top = row_max(top) * a.c;
+            // A maximum may lag by 8 (probabilities up to 256) before the sums are rescaled
+            if (__any(top > m[r] + 8.f)) {
+                top = fmaxf(top, m[r]);
                 const float f = carry(m[r], top);
                 m[r] = top;
                 l[r] *= f;
@@ -228,24 +279,22 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, uin
                 for (int j = 0; j < NT; j++) o[r][j] *= f;
             }
             const float ref = m[r] > -INFINITY ? m[r] : 0.f;
+            float u[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                v[i] = __builtin_amdgcn_exp2f(v[i] - ref);
-                l[r] += v[i];
-            }
-            p[r] = u32x4{H::pack(v[0], v[1]), H::pack(v[2], v[3]), H::pack(v[4], v[5]), H::pack(v[6], v[7])};
+            for (int i = 0; i < 8; i++) u[i] = __builtin_amdgcn_exp2f(fmaf(sc[r][i / 4][i % 4], a.c, -ref));
+            l[r] += ((u[0] + u[1]) + (u[2] + u[3])) + ((u[4] + u[5]) + (u[6] + u[7]));
+            p[r] = u32x4{H::pack(u[0], u[1]), H::pack(u[2], u[3]), H::pack(u[4], u[5]), H::pack(u[6], u[7])};
         }
-        // values: a scale for each token of the lane's column block
-        bool bad = false;
 #pragma unroll
-        for (int i = 0; i < 8; i++) bad |= byte_of(x[i / 4].vs, i % 4) == 255;
-        if (__any(bad)) {
+        for (int e = 0; e < 2; e++)
+            if (lost[e]) v[e].scale = 0xffffffffu;
+        if (__any(holds_255(v[0].scale) || holds_255(v[1].scale))) {
             // 0 * NaN is NaN: a NaN block enters the product as numbers, and the rows that see
             // it (counted by a product of their own) become NaN in its columns
             u32x4 lost_at;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const uint32_t lo = byte_of(x[i / 2].vs, 2 * i % 4) == 255, hi = byte_of(x[i / 2].vs, 2 * i % 4 + 1) == 255;
+                const uint32_t lo = byte_of(v[i / 2].scale, 2 * i % 4) == 255, hi = byte_of(v[i / 2].scale, 2 * i % 4 + 1) == 255;
                 lost_at[i] = lo * H::ONE | hi * (H::ONE << 16);
             }
 #pragma unroll
@@ -259,17 +308,17 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, uin
                 }
                 const f32x4 count = H::product(lost_at, sees, f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-                for (int k = 0; k < 4; k++)
+                for (int i = 0; i < 4; i++)
 #pragma unroll
-                    for (int j = 0; j < NT; j++) o[r][j][k] = count[k] > 0.f ? __uint_as_float(0x7fc00000u) : o[r][j][k];
+                    for (int j = 0; j < NT; j++) o[r][j][i] = count[i] > 0.f ? __uint_as_float(0x7fc00000u) : o[r][j][i];
             }
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                if (byte_of(x[i / 4].vs, i % 4) == 255) x[i / 4].vs ^= 128u << (8 * (i % 4));
+                if (byte_of(v[i / 4].scale, i % 4) == 255) v[i / 4].scale ^= 128u << (8 * (i % 4));
         }
-        float scale[8];
+        float scale[8];  // of the tokens' column block
 #pragma unroll
-        for (int i = 0; i < 8; i++) scale[i] = __uint_as_float(byte_of(x[i / 4].vs, i % 4) << 23);
+        for (int i = 0; i < 8; i++) scale[i] = __uint_as_float(byte_of(v[i / 4].scale, i % 4) << 23);
         // byte b of a token's piece: columns 2b and 2b + 1 of the piece
 #pragma unroll
         for (int b = 0; b < NT / 2; b++) {
@@ -278,7 +327,7 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, uin
             for (int i = 0; i < 8; i++) {
                 constexpr int W = D / 128;  // words per token, 0: two tokens share one
                 const int byte = D == 64 ? 2 * (i % 2) + b : b % 4;
-                const uint32_t w = D == 64 ? x[i / 4].v[i % 4 / 2] : x[i / 4].v[i % 4 * W + b / 4];
+                const uint32_t w = D == 64 ? v[i / 4].w[i % 4 / 2] : v[i / 4].w[i % 4 * W + b / 4];
                 c[i] = byte == 0 ? H::template pair<0>(w, scale[i]) : byte == 1 ? H::template pair<1>(w, scale[i])
                      : byte == 2 ? H::template pair<2>(w, scale[i]) : H::template pair<3>(w, scale[i]);
             }
@@ -293,6 +342,10 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, uin
                 o[r][2 * b] = H::product(lo, p[r], o[r][2 * b]);
                 o[r][2 * b + 1] = H::product(hi, p[r], o[r][2 * b + 1]);
             }
+        }
+        if (more) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) load_values(v[e], head[e], a.b.page_size, slot[e]);
         }
     }
     // the four wavefronts' parts, in pairs
@@ -362,37 +415,54 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, uin
     }
 }
 
-// ---- chunks joined: a wavefront per row and head ----------------------------------------
+// ---- chunks joined: a workgroup per row and head ------------------------------------------
 
+// Eight groups of 32 lanes (D = 64: 16 of 16) take the chunks in turn.
 template <uint32_t D, bool BF>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
-    const uint32_t lane = threadIdx.x & 63, i = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const uint32_t row = i / a.heads, head = i % a.heads;
-    if (row >= a.b.rows) return;
+    constexpr uint32_t N = D / 64, LANES = D / (4 * (N > 1 ? N / 2 : 1)), GROUPS = 256 / LANES;  // 16, 32 and 32 lanes
+    constexpr uint32_t V = D / LANES / 4;                                                            // of 4, 4 and 8 values
+    __shared__ __attribute__((aligned(16))) f32x4 so[GROUPS][LANES * V];
+    __shared__ float st[GROUPS];
+    const uint32_t row = blockIdx.x / a.heads, head = blockIdx.x % a.heads, group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
     const uint32_t s = cache_sequence(a.b, row);
     if (s >= a.b.sequences) return;
     const CacheSpan span = cache_span(a.b, s);
     if (row - span.first >= span.rows) return;
     const uint32_t from = first_seen(span, a.window), used = span.length > from ? (span.length - from + a.chunk - 1) / a.chunk : 0;
-    const uint64_t index = (uint64_t)i * a.chunks;
+    const uint64_t index = (uint64_t)blockIdx.x * a.chunks;
     const float *const ml = a.parts + (uint64_t)a.b.rows * a.heads * a.chunks * D + index * 2;
+    const f32x4 *const parts = (const f32x4 *)(a.parts + index * D) + lane * V;
     const float sink = a.sinks ? a.sinks[head] * 1.44269504088896341f : -INFINITY;
     float top = sink;
-    for (uint32_t c = 0; c < used; c++) top = fmaxf(top, ml[2 * c]);
-    float total = carry(sink, top), o[D / 64];
+    for (uint32_t c = threadIdx.x & 63; c < used; c += 64) top = fmaxf(top, ml[2 * c]);
+    top = wave_max(top);
+    float total = 0.f;
+    f32x4 o[V];
 #pragma unroll
-    for (int j = 0; j < (int)D / 64; j++) o[j] = 0.f;
-    for (uint32_t c = 0; c < used; c++) {
+    for (uint32_t j = 0; j < V; j++) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (uint32_t c = group; c < used; c += GROUPS) {
         const float f = carry(ml[2 * c], top);
-        const float *const p = a.parts + (index + c) * D + lane * (D / 64);
         total += ml[2 * c + 1] * f;
 #pragma unroll
-        for (int j = 0; j < (int)D / 64; j++) o[j] += p[j] * f;
+        for (uint32_t j = 0; j < V; j++) o[j] += parts[(uint64_t)c * (D / 4) + j] * f;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < V; j++) so[group][lane * V + j] = o[j];
+    if (lane == 0) st[group] = total;
+    __syncthreads();
+    if (threadIdx.x >= D / 4) return;
+    f32x4 sum = so[0][threadIdx.x];
+    total = carry(sink, top) + st[0];
+#pragma unroll
+    for (uint32_t i = 1; i < GROUPS; i++) {
+        sum += so[i][threadIdx.x];
+        total += st[i];
     }
     const float f = total > 0.f || total != total ? 1.f / total : 0.f;
-    half_t<BF> *const out = (half_t<BF> *)a.out + (uint64_t)row * a.out_stride + (uint64_t)head * D + lane * (D / 64);
-#pragma unroll
-    for (int j = 0; j < (int)D / 64; j++) RowIO<half_t<BF>>::put(out + j, o[j] * f);
+    uint16_t *const out = (uint16_t *)a.out + (uint64_t)row * a.out_stride + (uint64_t)head * D + 4 * threadIdx.x;
+    *(GLOBAL u32x2_u *)gp(out) = u32x2_u{Half<BF>::pack(sum[0] * f, sum[1] * f), Half<BF>::pack(sum[2] * f, sum[3] * f)};
 }
 
 // ---- choices and launches -------------------------------------------------------------------
@@ -427,8 +497,7 @@ static int attention_launch(const AttentionArgs &a, const AttentionPlan &l, hipS
     hipLaunchKernelGGL((attention_few_kernel<D, BF, 1>), dim3((uint32_t)grid), dim3(256), 0, stream, a, l.tiles);
     OCO_TRY(launch_check("oco_cache_attention"));
     if (l.chunks > 1) {
-        const uint64_t heads = (uint64_t)a.b.rows * a.heads;
-        hipLaunchKernelGGL((attention_join_kernel<D, BF>), dim3((uint32_t)((heads + 3) / 4)), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((attention_join_kernel<D, BF>), dim3(a.b.rows * a.heads), dim3(256), 0, stream, a);
         OCO_TRY(launch_check("oco_cache_attention (join)"));
     }
     return OCO_OK;
