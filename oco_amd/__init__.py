@@ -55,6 +55,7 @@ class Knob(enum.IntEnum):
     STREAM_DIRECT = 11
     MATMUL_VENDOR = 12
     FP8 = 13
+    ATTENTION = 14
 
 
 class DType(enum.IntEnum):

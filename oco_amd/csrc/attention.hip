@@ -103,13 +103,13 @@ __device__ __forceinline__ uint32_t first_seen(const CacheSpan &s, uint32_t wind
 // exp2 of m - to, 0 for m = -Inf whatever `to` is.
 __device__ __forceinline__ float carry(float m, float to) { return m > -INFINITY ? __builtin_amdgcn_exp2f(m - to) : 0.f; }
 
-// ---- few rows: a wavefront holds 16 R rows and reads its tokens itself ----------------
+// ---- a workgroup's four wavefronts hold the same 16 R rows and take steps of 32 tokens in turn ----
 
 // One half-step's 16 tokens as a lane holds them: lane m + 16 g has a quarter
 // of token m's key, and of tokens 4g .. 4g + 3 one sixteenth of the value.
 template <uint32_t D>
 struct Keys {
-    uint32_t w[D / 32], scale;
+    uint32_t w[D / 32], scale;  // one or two scale bytes
 };
 template <uint32_t D>
 struct Values {
@@ -117,33 +117,40 @@ struct Values {
 };
 
 template <uint32_t D>
-__device__ __forceinline__ void load_words(uint32_t *w, const uint8_t *p) {
+__device__ __forceinline__ void load_words(uint32_t *w, gbytes p, uint32_t at) {
     if constexpr (D == 64) {
-        const u32x2 a = *(const GLOBAL u32x2 *)gp(p);
+        const u32x2 a = *(const GLOBAL u32x2 *)(p + at);
         w[0] = a[0];
         w[1] = a[1];
     } else {
 #pragma unroll
         for (int i = 0; i < (int)D / 128; i++) {
-            const u32x4 a = ((const GLOBAL u32x4 *)gp(p))[i];
+            const u32x4 a = *(const GLOBAL u32x4 *)(p + at + 16 * i);
 #pragma unroll
             for (int j = 0; j < 4; j++) w[4 * i + j] = a[j];
         }
     }
 }
+// A half-step's tokens and a lane's places among them: the head's bytes and
+// the slot are the same for all lanes, the places the same for all steps.
 template <uint32_t D>
-__device__ __forceinline__ void load_keys(Keys<D> &x, const uint8_t *head, uint32_t page_size, uint32_t t) {
-    const uint32_t m = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
-    load_words<D>(x.w, head + (t + m) * (D / 2) + g * (D / 8));
-    const uint8_t *const s = head + page_size * D + (t + m) * (D / 32) + (D == 64 ? g / 2 : g * (D / 128));
-    x.scale = D == 256 ? *(const GLOBAL uint16_t *)gp(s) : *gp(s);
-}
-template <uint32_t D>
-__device__ __forceinline__ void load_values(Values<D> &x, const uint8_t *head, uint32_t page_size, uint32_t t) {
-    const uint32_t m = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
-    load_words<D>(x.w, head + page_size * (D / 2) + (t / 4 + g) * (2 * D) + m * (D / 8));
-    x.scale = *(const GLOBAL uint32_t *)gp(head + page_size * D + page_size * (D / 32) + (t / 4 + g) * (D / 8) + m * D / 512 * 4);
-}
+struct Places {
+    uint32_t key, key_scale, value, value_scale;
+    __device__ __forceinline__ Places(uint32_t page_size) {
+        const uint32_t m = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+        key = m * (D / 2) + g * (D / 8);
+        key_scale = page_size * D + m * (D / 32) + (D == 64 ? g / 2 : g * (D / 128));
+        value = page_size * (D / 2) + g * (2 * D) + m * (D / 8);
+        value_scale = page_size * D + page_size * (D / 32) + g * (D / 8) + m * D / 512 * 4;
+    }
+    __device__ __forceinline__ void load(Keys<D> &k, Values<D> &v, gbytes head, uint32_t slot) const {
+        load_words<D>(k.w, head + slot * (D / 2), key);
+        const gbytes s = head + slot * (D / 32);
+        k.scale = D == 256 ? *(const GLOBAL uint16_t *)(s + key_scale) : s[key_scale];
+        load_words<D>(v.w, head + slot * (D / 2), value);
+        v.scale = *(const GLOBAL uint32_t *)(s + value_scale);
+    }
+};
 // Whether a byte of a word is 255.
 __device__ __forceinline__ bool holds_255(uint32_t x) { return ((~x - 0x01010101u) & x & 0x80808080u) != 0; }
 
@@ -162,12 +169,17 @@ __device__ __forceinline__ Halves load_halves(const uint32_t *table, uint32_t t0
 }
 
 template <uint32_t D, bool BF, int R>
-__global__ __launch_bounds__(256, (D / 64) * R == 1 ? 4 : (D / 64) * R == 2 ? 3 : 2) void attention_few_kernel(AttentionArgs a, uint32_t tiles) {
+__global__ __launch_bounds__(256, (D / 64) * R == 1 ? 4 : (D / 64) * R == 2 ? 3 : 2) void attention_kernel(AttentionArgs a, uint32_t tiles) {
     constexpr int KW = D / 32, NT = D / 16;  // key words per lane and token; tiles of 16 columns
     using H = Half<BF>;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-    const uint32_t chunk = blockIdx.x % a.chunks, tile = blockIdx.x / a.chunks % tiles, sh = blockIdx.x / a.chunks / tiles;
-    const uint32_t s = sh / a.b.kv_heads, h = sh % a.b.kv_heads;
+    // Workgroups of a head in a row of 8 kv_heads apart share an XCD's L2 (heads come first); the tiles with most to do start first.
+    uint32_t id = blockIdx.x;
+    const uint32_t h = id % a.b.kv_heads;
+    id /= a.b.kv_heads;
+    const uint32_t chunk = id % a.chunks;
+    id /= a.chunks;
+    const uint32_t s = id % a.b.sequences, tile = tiles - 1 - id / a.b.sequences;
     const CacheSpan span = cache_span(a.b, s);
     const uint32_t row0 = tile * (16 * R), rows = span.rows * a.group;
     if (row0 >= rows) return;
@@ -180,11 +192,15 @@ __global__ __launch_bounds__(256, (D / 64) * R == 1 ? 4 : (D / 64) * R == 2 ? 3 
     const uint32_t end = most < 0 ? 0 : min(min(base + a.chunk, span.length), (uint32_t)most + 1);
     const uint32_t head_bytes = cache_head_bytes(a.b.page_size, D);
     const uint32_t *const table = a.b.table + (uint64_t)s * a.b.table_stride;
-    uint32_t t0 = base + 32 * wave, step = 0;
+    const uint32_t low = a.window && least >= (int32_t)a.window ? ((uint32_t)least + 1 - a.window) / 32 * 32 : 0;  // the tile's first token
+    uint32_t t0 = max(base, low) + 32 * wave, step = 0;
     Halves halves = load_halves(table, t0, 128, end, a.b.page_size);
     // the rows' positions (-1: no token, and no row)
     int32_t at[R];
-    u32x4 q[R][KW];
+    constexpr bool SHARED = R > 1;  // the queries in LDS, by fragment
+    constexpr int QF = SHARED ? R * KW * 64 : 1, OF = 4 * NT * 64;
+    __shared__ __attribute__((aligned(16))) u32x4 lds[QF > OF ? QF : OF];
+    u32x4 q[R][SHARED ? 1 : KW];
 #pragma unroll
     for (int r = 0; r < R; r++) {
         const uint32_t i = row0 + 16 * r + n;
@@ -192,9 +208,16 @@ __global__ __launch_bounds__(256, (D / 64) * R == 1 ? 4 : (D / 64) * R == 2 ? 3 
         const uint32_t token = live ? i / a.group : 0, head = h * a.group + (live ? i % a.group : 0);
         at[r] = live ? (int32_t)(span.length + token) - (int32_t)span.rows : -1;
         const uint16_t *const row = (const uint16_t *)a.q + (uint64_t)(span.first + token) * a.q_stride + (uint64_t)head * D + g * (D / 4);
+        if constexpr (SHARED) {
+            if (r == (int)wave)
 #pragma unroll
-        for (int w = 0; w < KW; w++) q[r][w] = *(const GLOBAL u32x4_u *)gp(row + 8 * w);
+                for (int w = 0; w < KW; w++) lds[(r * KW + w) * 64 + lane] = *(const GLOBAL u32x4_u *)gp(row + 8 * w);
+        } else {
+#pragma unroll
+            for (int w = 0; w < KW; w++) q[r][w] = *(const GLOBAL u32x4_u *)gp(row + 8 * w);
+        }
     }
+    if constexpr (SHARED) __syncthreads();
     float m[R], l[R];
     f32x4 o[R][NT];
 #pragma unroll
@@ -204,33 +227,30 @@ __global__ __launch_bounds__(256, (D / 64) * R == 1 ? 4 : (D / 64) * R == 2 ? 3 
 #pragma unroll
         for (int j = 0; j < NT; j++) o[r][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    // the next step's keys are requested when this step's are used up, its values likewise: the
-    // registers of one step, and always half a step's loads on their way
-    Keys<D> k[2];
-    Values<D> v[2];
-    const uint8_t *head[2];
-    uint32_t slot[2];
-    bool lost[2] = {false, false}, lost_next[2];
-    auto find = [&](uint32_t i) {
+    // a step's tokens are requested before the step before it is computed
+    struct Step {
+        Keys<D> k[2];
+        Values<D> v[2];
+        bool lost[2];  // not in the pool
+    };
+    const Places<D> places(a.b.page_size);
+    auto request = [&](Step &x) {  // of step `step`
+        if (step && step % 32 == 0) halves = load_halves(table, t0, 128, end, a.b.page_size);
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)halves.page, 2 * (i % 32) + e);
-            slot[e] = (uint32_t)__builtin_amdgcn_readlane((int)halves.slot, 2 * (i % 32) + e);
-            lost_next[e] = page >= a.b.pages;
-            page = lost_next[e] ? 0 : page;
-            head[e] = a.cache + ((uint64_t)page * a.b.kv_heads + h) * head_bytes;
+            uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)halves.page, 2 * (step % 32) + e);
+            const uint32_t slot = (uint32_t)__builtin_amdgcn_readlane((int)halves.slot, 2 * (step % 32) + e);
+            x.lost[e] = page >= a.b.pages;
+            page = x.lost[e] ? 0 : page;
+            places.load(x.k[e], x.v[e], (gbytes)gp(a.cache) + ((uint64_t)page * a.b.kv_heads + h) * head_bytes, slot);
         }
+        step++;
+        t0 += 128;
     };
-    if (t0 < end) {
-        find(0);
-#pragma unroll
-        for (int e = 0; e < 2; e++) load_keys(k[e], head[e], a.b.page_size, slot[e]);
-#pragma unroll
-        for (int e = 0; e < 2; e++) load_values(v[e], head[e], a.b.page_size, slot[e]);
-    }
-    for (; t0 < end; t0 += 128) {
-        lost[0] = lost_next[0];
-        lost[1] = lost_next[1];
+    auto compute = [&](Step &x, const uint32_t t0) {
+        Keys<D>(&k)[2] = x.k;
+        Values<D>(&v)[2] = x.v;
+        const bool(&lost)[2] = x.lost;
         // scores: lane (n, g) has row n's tokens 16 e + 4 g + i
         f32x4 sc[R][2];
 #pragma unroll
@@ -238,22 +258,22 @@ __global__ __launch_bounds__(256, (D / 64) * R == 1 ? 4 : (D / 64) * R == 2 ? 3 
             if (lost[e]) k[e].scale = 0xffff;
 #pragma unroll
             for (int r = 0; r < R; r++) sc[r][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w = 0; w < KW; w++) {
-                const float scale = cache_scale(D == 256 ? (w < 4 ? k[e].scale & 0xff : k[e].scale >> 8) : k[e].scale & 0xff);
-                const u32x4 x = {H::template pair<0>(k[e].w[w], scale), H::template pair<1>(k[e].w[w], scale),
-                                 H::template pair<2>(k[e].w[w], scale), H::template pair<3>(k[e].w[w], scale)};
-#pragma unroll
-                for (int r = 0; r < R; r++) sc[r][e] = H::product(x, q[r][w], sc[r][e]);
-            }
         }
-        step++;
-        const bool more = t0 + 128 < end;
-        if (more) {
-            if (step % 32 == 0) halves = load_halves(table, t0 + 128, 128, end, a.b.page_size);
-            find(step);
 #pragma unroll
-            for (int e = 0; e < 2; e++) load_keys(k[e], head[e], a.b.page_size, slot[e]);
+        for (int w = 0; w < KW; w++) {
+            u32x4 x[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const float scale = cache_scale(D == 256 ? (w < 4 ? k[e].scale & 0xff : k[e].scale >> 8) : k[e].scale & 0xff);
+                x[e] = u32x4{H::template pair<0>(k[e].w[w], scale), H::template pair<1>(k[e].w[w], scale),
+                             H::template pair<2>(k[e].w[w], scale), H::template pair<3>(k[e].w[w], scale)};
+            }
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const u32x4 f = SHARED ? lds[(r * KW + w) * 64 + lane] : q[r][SHARED ? 0 : w];
+#pragma unroll
+                for (int e = 0; e < 2; e++) sc[r][e] = H::product(x[e], f, sc[r][e]);
+            }
         }
         const bool edge = (int32_t)t0 + 31 > least || (a.window && (int32_t)t0 + (int32_t)a.window <= most);
         u32x4 p[R];
@@ -343,74 +363,64 @@ __global__ __launch_bounds__(256, (D / 64) * R == 1 ? 4 : (D / 64) * R == 2 ? 3 
                 o[r][2 * b + 1] = H::product(hi, p[r], o[r][2 * b + 1]);
             }
         }
-        if (more) {
-#pragma unroll
-            for (int e = 0; e < 2; e++) load_values(v[e], head[e], a.b.page_size, slot[e]);
-        }
+    };
+    Step x, y;
+    if (t0 < end) request(x);
+    for (uint32_t now = max(base, low) + 32 * wave; now < end; now += 256) {
+        if (t0 < end) request(y);
+        compute(x, now);
+        if (now + 128 >= end) break;
+        if (t0 < end) request(x);
+        compute(y, now + 128);
     }
-    // the four wavefronts' parts, in pairs
-    __shared__ __attribute__((aligned(16))) f32x4 so[2][NT][64];
-    __shared__ float sm[2][64], sl[2][64];
+    // The four wavefronts' parts: each writes all of its own and joins a quarter, NT consecutive
+    // columns of every lane's row.
+    f32x4(*const so)[4][NT / 4][64] = (f32x4(*)[4][NT / 4][64])lds;
+    __shared__ float sm[4][64], sl[4][64];
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        l[r] = row_sum(l[r]);
+        if (r || SHARED) __syncthreads();
+        sm[wave][lane] = m[r];
+        sl[wave][lane] = row_sum(l[r]);
 #pragma unroll
-        for (int half = 2; half; half /= 2) {
-            __syncthreads();
-            if (wave >= (uint32_t)half && wave < 2u * half) {
-                sm[wave - half][lane] = m[r];
-                sl[wave - half][lane] = l[r];
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int j = 0; j < NT; j++) so[wave - half][j][lane] = o[r][j];
-            }
-            __syncthreads();
-            if (wave < (uint32_t)half) {
-                const float m2 = sm[wave][lane], top = fmaxf(m[r], m2), f1 = carry(m[r], top), f2 = carry(m2, top);
-                m[r] = top;
-                l[r] = l[r] * f1 + sl[wave][lane] * f2;
-#pragma unroll
-                for (int j = 0; j < NT; j++) o[r][j] = o[r][j] * f1 + so[wave][j][lane] * f2;
-            }
-        }
-    }
-    if (wave) return;
-#pragma unroll
-    for (int r = 0; r < R; r++) {
+            for (int j = 0; j < NT / 4; j++) so[wave][i][j][lane] = f32x4{o[r][4 * j][i], o[r][4 * j + 1][i], o[r][4 * j + 2][i], o[r][4 * j + 3][i]};
+        __syncthreads();
         const uint32_t i = row0 + 16 * r + n;
         if (i >= rows) continue;
-        const uint32_t row = span.first + i / a.group, head = h * a.group + i % a.group;
-        float *part = nullptr;
-        float f = 1.f;
+        const float top = fmaxf(fmaxf(sm[0][lane], sm[1][lane]), fmaxf(sm[2][lane], sm[3][lane]));
+        float total = 0.f, f[4];
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            f[w] = carry(sm[w][lane], top);
+            total += sl[w][lane] * f[w];
+        }
+        f32x4 sum[NT / 4];
+#pragma unroll
+        for (int j = 0; j < NT / 4; j++) {
+            sum[j] = so[0][wave][j][lane] * f[0];
+#pragma unroll
+            for (int w = 1; w < 4; w++) sum[j] += so[w][wave][j][lane] * f[w];
+        }
+        const uint32_t row = span.first + i / a.group, head = h * a.group + i % a.group, column = (4 * g + wave) * NT;
         if (a.chunks > 1) {
             const uint64_t index = ((uint64_t)row * a.heads + head) * a.chunks + chunk;
-            part = a.parts + index * D;
-            if (g == 0) {
-                float *const ml = a.parts + (uint64_t)a.b.rows * a.heads * a.chunks * D + index * 2;
-                ml[0] = m[r];
-                ml[1] = l[r];
-            }
+#pragma unroll
+            for (int j = 0; j < NT / 4; j++) *(GLOBAL f32x4 *)gp(a.parts + index * D + column + 4 * j) = sum[j];
+            if (g == 0 && wave == 0) *(GLOBAL f32x2 *)gp(a.parts + (uint64_t)a.b.rows * a.heads * a.chunks * D + index * 2) = f32x2{top, total};
         } else {
-            float top = m[r], total = l[r];
+            float end_top = top;
             if (a.sinks) {
                 const float sink = a.sinks[head] * 1.44269504088896341f;
-                top = fmaxf(m[r], sink);
-                total = l[r] * carry(m[r], top) + carry(sink, top);
+                end_top = fmaxf(top, sink);
+                total = total * carry(top, end_top) + carry(sink, end_top);
             }
-            f = total > 0.f || total != total ? carry(m[r], top) / total : 0.f;
-        }
+            const float by = total > 0.f || total != total ? carry(top, end_top) / total : 0.f;
+            uint16_t *const out = (uint16_t *)a.out + (uint64_t)row * a.out_stride + (uint64_t)head * D + column;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const uint32_t column = (4 * g + k) * NT;
-#pragma unroll
-            for (int j = 0; j < NT; j += 4) {
-                const f32x4 v = {o[r][j][k], o[r][j + 1][k], o[r][j + 2][k], o[r][j + 3][k]};
-                if (part) {
-                    *(f32x4 *)(part + column + j) = v;
-                } else {
-                    uint16_t *const out = (uint16_t *)a.out + (uint64_t)row * a.out_stride + (uint64_t)head * D + column + j;
-                    *(u32x2_u *)out = u32x2_u{H::pack(v[0] * f, v[1] * f), H::pack(v[2] * f, v[3] * f)};
-                }
-            }
+            for (int j = 0; j < NT / 4; j++)
+                *(GLOBAL u32x2_u *)gp(out + 4 * j) = u32x2_u{H::pack(sum[j][0] * by, sum[j][1] * by), H::pack(sum[j][2] * by, sum[j][3] * by)};
         }
     }
 }
@@ -468,21 +478,26 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
 // ---- choices and launches -------------------------------------------------------------------
 
 struct AttentionPlan {
-    uint32_t tiles, chunks, chunk;
+    uint32_t tile, tiles, chunks, chunk;  // tile: of 16 rows
     uint64_t bytes;
 };
 static AttentionPlan attention_plan(const oco_cache *p) {
     AttentionPlan l;
     const uint64_t rows = (uint64_t)p->max_rows * (p->heads / p->kv_heads);
-    l.tiles = (uint32_t)((rows + 15) / 16);
+    int32_t knob[4];
+    const int set = plan_override(OCO_KNOB_ATTENTION, knob);
+    l.tile = rows <= 16 ? 1 : p->head_dim == 256 || rows <= 64 ? 1 : 2;
+    if (set && (knob[0] == 1 || knob[0] == 2 || (knob[0] == 4 && p->head_dim < 256))) l.tile = (uint32_t)knob[0];
+    l.tiles = (uint32_t)((rows + 16 * l.tile - 1) / (16 * l.tile));
     uint64_t seen = p->max_length;
     if (p->window && (uint64_t)p->window + p->max_rows + 31 < seen) seen = (uint64_t)p->window + p->max_rows + 31;
     const uint64_t blocks = (uint64_t)p->sequences * p->kv_heads * l.tiles;
-    uint64_t chunks = blocks ? (1024 + blocks - 1) / blocks : 1;
-    const uint64_t most = (seen + 127) / 128;
+    uint64_t chunks = blocks ? (2048 + blocks - 1) / blocks : 1;
+    const uint64_t most = (seen + 255) / 256;
     if (chunks > most) chunks = most;
     if (chunks < 1) chunks = 1;
     l.chunk = (uint32_t)(((seen + chunks - 1) / chunks + 127) / 128 * 128);
+    if (set > 1 && knob[1] > 0 && knob[1] % 128 == 0) l.chunk = (uint32_t)knob[1];
     if (l.chunk == 0) l.chunk = 128;
     l.chunks = (uint32_t)((seen + l.chunk - 1) / l.chunk);
     if (l.chunks < 1) l.chunks = 1;
@@ -494,7 +509,12 @@ template <uint32_t D, bool BF>
 static int attention_launch(const AttentionArgs &a, const AttentionPlan &l, hipStream_t stream) {
     const uint64_t grid = (uint64_t)a.b.sequences * a.b.kv_heads * l.tiles * l.chunks;
     if (grid > 0x7fffffffull) return fail(OCO_ERR_INVALID, "oco_cache_attention: too many rows for one call");
-    hipLaunchKernelGGL((attention_few_kernel<D, BF, 1>), dim3((uint32_t)grid), dim3(256), 0, stream, a, l.tiles);
+    if (l.tile == 1)
+        hipLaunchKernelGGL((attention_kernel<D, BF, 1>), dim3((uint32_t)grid), dim3(256), 0, stream, a, l.tiles);
+    else if (l.tile == 2)
+        hipLaunchKernelGGL((attention_kernel<D, BF, 2>), dim3((uint32_t)grid), dim3(256), 0, stream, a, l.tiles);
+    else if constexpr (D < 256)
+        hipLaunchKernelGGL((attention_kernel<D, BF, 4>), dim3((uint32_t)grid), dim3(256), 0, stream, a, l.tiles);
     OCO_TRY(launch_check("oco_cache_attention"));
     if (l.chunks > 1) {
         hipLaunchKernelGGL((attention_join_kernel<D, BF>), dim3(a.b.rows * a.heads), dim3(256), 0, stream, a);
