@@ -1,0 +1,109 @@
+// Attention over the paged cache: what its kernels share.
+#pragma once
+#include "cache.h"
+
+namespace oco {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+struct AttentionArgs {
+    CacheBatch b;
+    const uint8_t *cache;
+    const void *q;
+    void *out;
+    const float *sinks;
+    float *parts;  // [rows][heads][chunks][D], then m and l [rows][heads][chunks][2]
+    uint64_t q_stride, out_stride;
+    uint32_t heads, group, window;
+    uint32_t chunks, chunk;  // parts of the tokens, each of `chunk` tokens
+    float c;                 // scale * log2(e)
+};
+
+template <bool BF>
+struct Half;  // the 16-bit type of the rows
+template <>
+struct Half<true> {
+    template <int I>
+    static __device__ __forceinline__ uint32_t pair(uint32_t w, float s) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, I));
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+    }
+    static __device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 product32(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static constexpr uint32_t ONE = 0x3f80;
+};
+template <>
+struct Half<false> {
+    template <int I>
+    static __device__ __forceinline__ uint32_t pair(uint32_t w, float s) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, I));
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+    }
+    static __device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 product32(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static constexpr uint32_t ONE = 0x3c00;
+};
+// Four tokens' pairs of columns -> the two columns' four tokens.
+__device__ __forceinline__ u32x2 low_halves(const uint32_t *c) {
+    return u32x2{__builtin_amdgcn_perm(c[1], c[0], 0x05040100), __builtin_amdgcn_perm(c[3], c[2], 0x05040100)};
+}
+__device__ __forceinline__ u32x2 high_halves(const uint32_t *c) {
+    return u32x2{__builtin_amdgcn_perm(c[1], c[0], 0x07060302), __builtin_amdgcn_perm(c[3], c[2], 0x07060302)};
+}
+
+// Maximum and sum over the lanes l, l ^ 16, l ^ 32, l ^ 48, which hold one row.
+__device__ __forceinline__ float row_max(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, dpp_f32<0xB1>(v));
+    v = fmaxf(v, dpp_f32<0x4E>(v));
+    v = fmaxf(v, dpp_f32<0x124>(v));
+    v = fmaxf(v, dpp_f32<0x128>(v));
+    return row_max(v);
+}
+__device__ __forceinline__ float row_sum(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// The tokens that any row of a sequence sees: from .. length, from a multiple of 32.
+__device__ __forceinline__ uint32_t first_seen(const CacheSpan &s, uint32_t window) {
+    const uint32_t p = s.length > s.rows ? s.length - s.rows : 0;
+    return window && p + 1 > window ? (p + 1 - window) / 32 * 32 : 0;
+}
+
+// exp2 of m - to, 0 for m = -Inf whatever `to` is.
+__device__ __forceinline__ float carry(float m, float to) { return m > -INFINITY ? __builtin_amdgcn_exp2f(m - to) : 0.f; }
+
+// Whether a byte of a word is 255.
+__device__ __forceinline__ bool holds_255(uint32_t x) { return ((~x - 0x01010101u) & x & 0x80808080u) != 0; }
+
+// Prompt chunks (attention_prompt.hip): rows of a tile, tokens of a step.
+constexpr uint32_t PROMPT_ROWS = 128;
+constexpr uint32_t prompt_step(uint32_t d) { return d == 256 ? 32 : 64; }
+int attention_prompt_launch(const AttentionArgs &a, uint32_t head_dim, bool bf, uint32_t tiles, uint32_t grid, hipStream_t stream);
+
+}  // namespace oco

@@ -17,91 +17,9 @@
 // E2M1 times a power of two is exact in bf16 and f16 (an f16 model's cache
 // stays in range), so codes go to the matrix instruction through the hardware's
 // conversion, two values per instruction, with their scale.
-#include "cache.h"
+#include "attention.h"
 
 namespace oco {
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-struct AttentionArgs {
-    CacheBatch b;
-    const uint8_t *cache;
-    const void *q;
-    void *out;
-    const float *sinks;
-    float *parts;  // [rows][heads][chunks][D], then m and l [rows][heads][chunks][2]
-    uint64_t q_stride, out_stride;
-    uint32_t heads, group, window;
-    uint32_t chunks, chunk;  // parts of the tokens, each of `chunk` tokens
-    float c;                 // scale * log2(e)
-};
-
-template <bool BF>
-struct Half;  // the 16-bit type of the rows
-template <>
-struct Half<true> {
-    template <int I>
-    static __device__ __forceinline__ uint32_t pair(uint32_t w, float s) {
-        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, I));
-    }
-    static __device__ __forceinline__ uint32_t pack(float a, float b) {
-        return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
-    }
-    static __device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    }
-    static constexpr uint32_t ONE = 0x3f80;
-};
-template <>
-struct Half<false> {
-    template <int I>
-    static __device__ __forceinline__ uint32_t pair(uint32_t w, float s) {
-        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, I));
-    }
-    static __device__ __forceinline__ uint32_t pack(float a, float b) {
-        return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
-    }
-    static __device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    }
-    static constexpr uint32_t ONE = 0x3c00;
-};
-template <bool BF>
-using half_t = std::conditional_t<BF, bf16_t, f16_t>;
-
-// Maximum and sum over the lanes l, l ^ 16, l ^ 32, l ^ 48, which hold one row.
-__device__ __forceinline__ float row_max(float v) {
-    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float wave_max(float v) {
-    v = fmaxf(v, dpp_f32<0xB1>(v));
-    v = fmaxf(v, dpp_f32<0x4E>(v));
-    v = fmaxf(v, dpp_f32<0x124>(v));
-    v = fmaxf(v, dpp_f32<0x128>(v));
-    return row_max(v);
-}
-__device__ __forceinline__ float row_sum(float v) {
-    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
-// The tokens that any row of a sequence sees: from .. length, from a multiple of 32.
-__device__ __forceinline__ uint32_t first_seen(const CacheSpan &s, uint32_t window) {
-    const uint32_t p = s.length > s.rows ? s.length - s.rows : 0;
-    return window && p + 1 > window ? (p + 1 - window) / 32 * 32 : 0;
-}
-
-// exp2 of m - to, 0 for m = -Inf whatever `to` is.
-__device__ __forceinline__ float carry(float m, float to) { return m > -INFINITY ? __builtin_amdgcn_exp2f(m - to) : 0.f; }
 
 // ---- a workgroup's four wavefronts hold the same 16 R rows and take steps of 32 tokens in turn ----
 
@@ -151,9 +69,6 @@ struct Places {
         v.scale = *(const GLOBAL uint32_t *)(s + value_scale);
     }
 };
-// Whether a byte of a word is 255.
-__device__ __forceinline__ bool holds_255(uint32_t x) { return ((~x - 0x01010101u) & x & 0x80808080u) != 0; }
-
 // The halves of a wavefront's steps, their pages and their places in them: a
 // lane per half, read once for 32 steps, so that a step's loads do not wait
 // for the table.
@@ -351,12 +266,8 @@ __global__ __launch_bounds__(256, (D / 64) * R == 1 ? 4 : (D / 64) * R == 2 ? 3 
                 c[i] = byte == 0 ? H::template pair<0>(w, scale[i]) : byte == 1 ? H::template pair<1>(w, scale[i])
                      : byte == 2 ? H::template pair<2>(w, scale[i]) : H::template pair<3>(w, scale[i]);
             }
-            u32x4 lo, hi;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                lo[i] = __builtin_amdgcn_perm(c[2 * i + 1], c[2 * i], 0x05040100);
-                hi[i] = __builtin_amdgcn_perm(c[2 * i + 1], c[2 * i], 0x07060302);
-            }
+            const u32x2 l0 = low_halves(c), l1 = low_halves(c + 4), h0 = high_halves(c), h1 = high_halves(c + 4);
+            const u32x4 lo = {l0.x, l0.y, l1.x, l1.y}, hi = {h0.x, h0.y, h1.x, h1.y};
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 o[r][2 * b] = H::product(lo, p[r], o[r][2 * b]);
@@ -486,13 +397,13 @@ static AttentionPlan attention_plan(const oco_cache *p) {
     const uint64_t rows = (uint64_t)p->max_rows * (p->heads / p->kv_heads);
     int32_t knob[4];
     const int set = plan_override(OCO_KNOB_ATTENTION, knob);
-    l.tile = rows <= 16 ? 1 : p->head_dim == 256 || rows <= 64 ? 1 : 2;
-    if (set && (knob[0] == 1 || knob[0] == 2 || (knob[0] == 4 && p->head_dim < 256))) l.tile = (uint32_t)knob[0];
+    l.tile = rows <= 16 ? 1 : rows <= 64 ? 1 : PROMPT_ROWS / 16;
+    if (set && (knob[0] == 1 || knob[0] == 2 || (knob[0] == 4 && p->head_dim < 256) || knob[0] == (int)PROMPT_ROWS / 16)) l.tile = (uint32_t)knob[0];
     l.tiles = (uint32_t)((rows + 16 * l.tile - 1) / (16 * l.tile));
     uint64_t seen = p->max_length;
     if (p->window && (uint64_t)p->window + p->max_rows + 31 < seen) seen = (uint64_t)p->window + p->max_rows + 31;
     const uint64_t blocks = (uint64_t)p->sequences * p->kv_heads * l.tiles;
-    uint64_t chunks = blocks ? (2048 + blocks - 1) / blocks : 1;
+    uint64_t chunks = blocks ? (3072 + blocks - 1) / blocks : 1;
     const uint64_t most = (seen + 255) / 256;
     if (chunks > most) chunks = most;
     if (chunks < 1) chunks = 1;
@@ -505,11 +416,16 @@ static AttentionPlan attention_plan(const oco_cache *p) {
     return l;
 }
 
+// Which kernel: by the rows of a sequence and key-value head.
+static bool attention_is_prompt(const AttentionPlan &l) { return l.tile == PROMPT_ROWS / 16; }
+
 template <uint32_t D, bool BF>
 static int attention_launch(const AttentionArgs &a, const AttentionPlan &l, hipStream_t stream) {
     const uint64_t grid = (uint64_t)a.b.sequences * a.b.kv_heads * l.tiles * l.chunks;
     if (grid > 0x7fffffffull) return fail(OCO_ERR_INVALID, "oco_cache_attention: too many rows for one call");
-    if (l.tile == 1)
+    if (attention_is_prompt(l)) {
+        OCO_TRY(attention_prompt_launch(a, D, BF, l.tiles, (uint32_t)grid, stream));
+    } else if (l.tile == 1)
         hipLaunchKernelGGL((attention_kernel<D, BF, 1>), dim3((uint32_t)grid), dim3(256), 0, stream, a, l.tiles);
     else if (l.tile == 2)
         hipLaunchKernelGGL((attention_kernel<D, BF, 2>), dim3((uint32_t)grid), dim3(256), 0, stream, a, l.tiles);

@@ -1,0 +1,292 @@
+// Attention over the paged cache for many rows: the matrix cores' side.
+//
+// A workgroup's four wavefronts hold 32 rows each and share steps of 64 tokens
+// (32 of wide heads), whose codes are converted once for all of them into LDS:
+// keys as rows, values transposed, so that both products read 16 bytes per
+// lane.  Two buffers, one barrier per step: the next step's codes are on their
+// way while this one is computed.  As in the kernel for few rows a lane is a
+// row throughout (here of two), and the products' inner indexes are in the order
+// in which the scores leave the first product.
+//
+// A wavefront converts 16 tokens of a step, which lie in one page.
+#include "attention.h"
+
+namespace oco {
+
+template <uint32_t D, bool BF>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel(AttentionArgs a, uint32_t tiles) {
+    using H = Half<BF>;
+    constexpr uint32_t KT = prompt_step(D), HALVES = KT / 16;  // tokens of a step; wavefronts per 16 tokens: 4 / HALVES
+    constexpr int KN = KT / 32, NS = D / 16, NO = D / 32;       // key tiles, key steps, column tiles
+    constexpr uint32_t PIECE = D / 16;                          // columns of a value's piece
+    // rows of 16-byte pieces, one piece of padding: eight consecutive rows fall into different banks
+    constexpr uint32_t KROW = D / 8 + 1, VROW = KT / 8 + 1;
+    __shared__ __attribute__((aligned(16))) u32x4 keys[2][KT * KROW], values[2][D * VROW];
+    __shared__ uint32_t flags[2];  // the step, from 1, whose values hold a block of NaN
+
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, g = lane >> 5;
+    uint32_t id = blockIdx.x;
+    const uint32_t h = id % a.b.kv_heads;
+    id /= a.b.kv_heads;
+    const uint32_t chunk = id % a.chunks;
+    id /= a.chunks;
+    const uint32_t s = id % a.b.sequences, tile = tiles - 1 - id / a.b.sequences;
+    const CacheSpan span = cache_span(a.b, s);
+    const uint32_t tile0 = tile * PROMPT_ROWS, rows = span.rows * a.group;
+    if (tile0 >= rows) return;
+    const int32_t before = (int32_t)span.length - (int32_t)span.rows;
+    const int32_t tile_least = before + (int32_t)(tile0 / a.group), tile_most = before + (int32_t)((min(tile0 + PROMPT_ROWS, rows) - 1) / a.group);
+    const uint32_t base = first_seen(span, a.window) + chunk * a.chunk;
+    if (chunk && base >= span.length) return;
+    const uint32_t low = a.window && tile_least >= (int32_t)a.window ? ((uint32_t)tile_least + 1 - a.window) / 32 * 32 : 0;
+    const uint32_t first = max(base, low), end = tile_most < 0 ? 0 : min(min(base + a.chunk, span.length), (uint32_t)tile_most + 1);
+    const uint32_t head_bytes = cache_head_bytes(a.b.page_size, D);
+    const uint32_t *const table = a.b.table + (uint64_t)s * a.b.table_stride;
+
+    // this lane's row
+    const uint32_t row0 = tile0 + 32 * wave, i0 = row0 + n;
+    const bool live = i0 < rows;
+    const uint32_t token = live ? i0 / a.group : 0, head = h * a.group + (live ? i0 % a.group : 0);
+    const int32_t at = live ? before + (int32_t)token : -1;
+    const int32_t least = before + (int32_t)(row0 / a.group), most = before + (int32_t)((min(row0 + 32, rows) - 1) / a.group);
+    u32x4 q[NS];
+    {
+        const uint16_t *const row = (const uint16_t *)a.q + (uint64_t)(span.first + token) * a.q_stride + (uint64_t)head * D + 8 * g;
+#pragma unroll
+        for (int i = 0; i < NS; i++) q[i] = *(const GLOBAL u32x4_u *)gp(row + 16 * i);
+    }
+    float m = -INFINITY, l = 0.f;
+    f32x16 o[NO];
+#pragma unroll
+    for (int j = 0; j < NO; j++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[j][i] = 0.f;
+    if (threadIdx.x < 2) flags[threadIdx.x] = 0;
+
+    // ---- converting: a thread's share of a step
+    const uint32_t half = wave * HALVES / 4;
+    constexpr uint32_t KB = D == 64 ? 8 : 16, KPIECES = D / 2 / KB;  // bytes of a key per thread, threads per key
+    const uint32_t kt = threadIdx.x / KPIECES, kp = threadIdx.x % KPIECES;
+    const uint32_t vu = D == 256 ? threadIdx.x / 2 : threadIdx.x, vg = vu / 16, vm = vu % 16;  // four tokens, a piece (D = 256: half of it)
+    struct Raw {
+        uint32_t k[4], v[4], ks, vs;
+        bool lost;
+    };
+    const uint32_t k_at = kt % 16 * (D / 2) + kp * KB, ks_at = a.b.page_size * D + kt % 16 * (D / 32) + kp * KB / 16;
+    const uint32_t v_at = a.b.page_size * (D / 2) + vg % 4 * (2 * D) + vm * (D / 8) + (D == 256 ? threadIdx.x % 2 * 4 : 0);
+    const uint32_t vs_at = a.b.page_size * D + a.b.page_size * (D / 32) + vg % 4 * (D / 8) + vm * D / 512 * 4;
+    uint32_t page_of = 0, slot_of = 0, step = 0;  // lane i: of step 64 k + i
+    auto request = [&](Raw &x) {
+        if (step % 64 == 0) {
+            const uint32_t t = first + (step + lane) * KT + 16 * half;
+            page_of = t < end ? table[t / a.b.page_size] : 0;
+            slot_of = t % a.b.page_size;
+        }
+        uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)page_of, step % 64);
+        const uint32_t slot = (uint32_t)__builtin_amdgcn_readlane((int)slot_of, step % 64);
+        step++;
+        x.lost = page >= a.b.pages;
+        page = x.lost ? 0 : page;
+        const gbytes p = (gbytes)gp(a.cache) + ((uint64_t)page * a.b.kv_heads + h) * head_bytes;
+        const gbytes words = p + slot * (D / 2), scales = p + slot * (D / 32);
+        if constexpr (D == 64) {
+            const u32x2 k = *(const GLOBAL u32x2 *)(words + k_at), v = *(const GLOBAL u32x2 *)(words + v_at);
+            x.k[0] = k.x;
+            x.k[1] = k.y;
+            x.v[0] = v.x;
+            x.v[1] = v.y;
+        } else {
+            const u32x4 k = *(const GLOBAL u32x4 *)(words + k_at);
+#pragma unroll
+            for (int i = 0; i < 4; i++) x.k[i] = k[i];
+            if constexpr (D == 128) {
+                const u32x4 v = *(const GLOBAL u32x4 *)(words + v_at);
+#pragma unroll
+                for (int i = 0; i < 4; i++) x.v[i] = v[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) x.v[i] = *(const GLOBAL uint32_t *)(words + v_at + 8 * i);
+            }
+        }
+        x.ks = scales[ks_at];
+        x.vs = *(const GLOBAL uint32_t *)(scales + vs_at);
+    };
+    auto convert = [&](Raw &x, uint32_t into, uint32_t number) {
+        const float ks = cache_scale(x.lost ? 255 : x.ks);
+#pragma unroll
+        for (int i = 0; i < (int)KB / 4; i++)
+            keys[into][kt * KROW + kp * (KB / 4) + i] = u32x4{H::template pair<0>(x.k[i], ks), H::template pair<1>(x.k[i], ks),
+                                                            H::template pair<2>(x.k[i], ks), H::template pair<3>(x.k[i], ks)};
+        uint32_t vs = x.lost ? 0xffffffffu : x.vs;
+        if (__any(holds_255(vs))) {  // numbers in their place: 0 * NaN is NaN
+            if (lane == 0) flags[into] = number;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (byte_of(vs, i) == 255) vs ^= 128u << (8 * i);
+        }
+        float scale[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) scale[i] = __uint_as_float(byte_of(vs, i) << 23);
+        // column PIECE m + c is in row 16 c + m; groups of four tokens of 16 in the order 0, 2, 1, 3
+        u32x2 *const out = (u32x2 *)&values[into][0] + (vg / 4 * 4 + vg % 2 * 2 + vg % 4 / 2);
+        const uint32_t c0 = D == 256 ? threadIdx.x % 2 * 8 : 0;
+#pragma unroll
+        for (int b = 0; b < (D == 64 ? 2 : 4); b++) {
+            uint32_t c[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int byte = D == 64 ? 2 * (i % 2) + b : b;
+                const uint32_t w = D == 64 ? x.v[i / 2] : x.v[i];
+                c[i] = byte == 0 ? H::template pair<0>(w, scale[i]) : byte == 1 ? H::template pair<1>(w, scale[i])
+                     : byte == 2 ? H::template pair<2>(w, scale[i]) : H::template pair<3>(w, scale[i]);
+            }
+            out[((c0 + 2 * b) * 16 + vm) * (2 * VROW)] = low_halves(c);
+            out[((c0 + 2 * b + 1) * 16 + vm) * (2 * VROW)] = high_halves(c);
+        }
+    };
+
+    Raw x;
+    __syncthreads();
+    if (first < end) {
+        request(x);
+        convert(x, 0, 1);
+    }
+    if (first + KT < end) request(x);
+    __syncthreads();
+    uint32_t number = 1;
+    for (uint32_t t0 = first; t0 < end; t0 += KT, number++) {
+        const uint32_t buffer = (number - 1) & 1;
+        if ((int32_t)t0 <= most) {
+            f32x16 sc[KN];
+#pragma unroll
+            for (int k = 0; k < KN; k++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) sc[k][i] = 0.f;
+#pragma unroll
+            for (int i = 0; i < NS; i++)
+#pragma unroll
+                for (int k = 0; k < KN; k++) sc[k] = H::product32(keys[buffer][(32 * k + n) * KROW + 2 * i + g], q[i], sc[k]);
+            if ((int32_t)(t0 + KT) - 1 > least || (a.window && (int32_t)t0 + (int32_t)a.window <= most)) {
+#pragma unroll
+                for (int k = 0; k < KN; k++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int32_t t = (int32_t)t0 + 32 * k + 8 * (i / 4) + 4 * (int32_t)g + i % 4;
+                        if (!(t <= at && (!a.window || t + (int32_t)a.window > at))) sc[k][i] = -INFINITY;
+                    }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < KN; k++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) top = fmaxf(top, sc[k][i]);
+            {
+                auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                top = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])) * a.c;
+            }
+            if (__any(top > m + 8.f)) {
+                top = fmaxf(top, m);
+                const float f = carry(m, top);
+                m = top;
+                l *= f;
+#pragma unroll
+                for (int j = 0; j < NO; j++) o[j] *= f;
+            }
+            const float ref = m > -INFINITY ? m : 0.f;
+            u32x4 p[2 * KN];
+#pragma unroll
+            for (int k = 0; k < KN; k++) {
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    sc[k][i] = __builtin_amdgcn_exp2f(fmaf(sc[k][i], a.c, -ref));
+                    sum += sc[k][i];
+                }
+                l += sum;
+#pragma unroll
+                for (int i = 0; i < 8; i++) p[2 * k + i / 4][i % 4] = H::pack(sc[k][2 * i], sc[k][2 * i + 1]);
+            }
+            if (flags[buffer] == number) {
+                // rows that see a block of NaN: every lane looks at the step's tokens itself
+                uint32_t bad = 0;
+                for (uint32_t t = t0; t < min(t0 + KT, end); t++) {
+                    if (!((int32_t)t <= at && (!a.window || (int32_t)(t + a.window) > at))) continue;
+                    const uint32_t page = table[t / a.b.page_size];
+                    for (uint32_t b = 0; b < D / 32; b++)
+                        if (page >= a.b.pages ||
+                            a.cache[((uint64_t)page * a.b.kv_heads + h) * head_bytes + cache_value_scale_at(a.b.page_size, t % a.b.page_size, b, D)] == 255)
+                            bad |= 1u << b;
+                }
+#pragma unroll
+                for (int j = 0; j < NO; j++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const uint32_t r = 32 * j + 8 * (i / 4) + 4 * g + i % 4;
+                        if (bad >> ((PIECE * (r % 16) + r / 16) / 32) & 1) o[j][i] = __uint_as_float(0x7fc00000u);
+                    }
+            }
+#pragma unroll
+            for (int t = 0; t < 2 * KN; t++)
+#pragma unroll
+                for (int j = 0; j < NO; j++) o[j] = H::product32(values[buffer][(32 * j + n) * VROW + 2 * t + g], p[t], o[j]);
+        }
+        if (t0 + KT < end) {
+            convert(x, buffer ^ 1, number + 1);
+            if (t0 + 2 * KT < end) request(x);
+        }
+        __syncthreads();
+    }
+    if (!live) return;
+    {
+        auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        l = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+    }
+    const uint32_t row = span.first + token;
+    float by = 1.f;
+    const uint64_t index = ((uint64_t)row * a.heads + head) * a.chunks + chunk;
+    if (a.chunks > 1) {
+        if (g == 0) *(GLOBAL f32x2 *)gp(a.parts + (uint64_t)a.b.rows * a.heads * a.chunks * D + index * 2) = f32x2{m, l};
+    } else {
+        float top = m, total = l;
+        if (a.sinks) {
+            const float sink = a.sinks[head] * 1.44269504088896341f;
+            top = fmaxf(m, sink);
+            total = l * carry(m, top) + carry(sink, top);
+        }
+        by = total > 0.f || total != total ? carry(m, top) / total : 0.f;
+    }
+    // accumulator row 16 c + m is column PIECE m + c: a lane has all columns of a piece
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t column = PIECE * (8 * (i / 4) + 4 * g + i % 4);
+        float v[PIECE];
+#pragma unroll
+        for (uint32_t c = 0; c < PIECE; c++) v[c] = o[c / 2][i + 8 * (c % 2)] * by;
+        if (a.chunks > 1) {
+            float *const out = a.parts + index * D + column;
+#pragma unroll
+            for (uint32_t c = 0; c < PIECE; c += 4) *(GLOBAL f32x4 *)gp(out + c) = f32x4{v[c], v[c + 1], v[c + 2], v[c + 3]};
+        } else {
+            uint16_t *const out = (uint16_t *)a.out + (uint64_t)row * a.out_stride + (uint64_t)head * D + column;
+#pragma unroll
+            for (uint32_t c = 0; c < PIECE; c += 4) *(GLOBAL u32x2_u *)gp(out + c) = u32x2_u{H::pack(v[c], v[c + 1]), H::pack(v[c + 2], v[c + 3])};
+        }
+    }
+}
+
+int attention_prompt_launch(const AttentionArgs &a, uint32_t head_dim, bool bf, uint32_t tiles, uint32_t grid, hipStream_t stream) {
+#define GO(D)                                                                                                             \
+    if (bf)                                                                                                               \
+        hipLaunchKernelGGL((attention_prompt_kernel<D, true>), dim3(grid), dim3(256), 0, stream, a, tiles);               \
+    else                                                                                                                  \
+        hipLaunchKernelGGL((attention_prompt_kernel<D, false>), dim3(grid), dim3(256), 0, stream, a, tiles);
+    switch (head_dim) {
+    case 64: GO(64) break;
+    case 128: GO(128) break;
+    default: GO(256)
+    }
+#undef GO
+    return launch_check("oco_cache_attention (prompt)");
+}
+
+}  // namespace oco
