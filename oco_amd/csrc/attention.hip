@@ -403,8 +403,10 @@ static AttentionPlan attention_plan(const oco_cache *p) {
     uint64_t seen = p->max_length;
     if (p->window && (uint64_t)p->window + p->max_rows + 31 < seen) seen = (uint64_t)p->window + p->max_rows + 31;
     const uint64_t blocks = (uint64_t)p->sequences * p->kv_heads * l.tiles;
-    uint64_t chunks = blocks ? (3072 + blocks - 1) / blocks : 1;
-    const uint64_t most = (seen + 255) / 256;
+    const bool prompt = l.tile == PROMPT_ROWS / 16;
+    const uint64_t wanted = prompt ? 512 : 3072;
+    uint64_t chunks = blocks ? (wanted + blocks - 1) / blocks : 1;
+    const uint64_t least = prompt ? 512 : 256, most = (seen + least - 1) / least;
     if (chunks > most) chunks = most;
     if (chunks < 1) chunks = 1;
     l.chunk = (uint32_t)(((seen + chunks - 1) / chunks + 127) / 128 * 128);
