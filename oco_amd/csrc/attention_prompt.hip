@@ -61,7 +61,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
     for (int j = 0; j < NO; j++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[j][i] = 0.f;
-    if (threadIdx.x < 2) flags[threadIdx.x] = 0;
 
     // ---- converting: a thread's share of a step
     const uint32_t half = wave * HALVES / 4;
@@ -69,55 +68,73 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
     const uint32_t kt = threadIdx.x / KPIECES, kp = threadIdx.x % KPIECES;
     const uint32_t vu = D == 256 ? threadIdx.x / 2 : threadIdx.x, vg = vu / 16, vm = vu % 16;  // four tokens, a piece (D = 256: half of it)
     struct Raw {
-        uint32_t k[4], v[4], ks, vs;
+        uint32_t w[4], scale;
         bool lost;
     };
     const uint32_t k_at = kt % 16 * (D / 2) + kp * KB, ks_at = a.b.page_size * D + kt % 16 * (D / 32) + kp * KB / 16;
     const uint32_t v_at = a.b.page_size * (D / 2) + vg % 4 * (2 * D) + vm * (D / 8) + (D == 256 ? threadIdx.x % 2 * 4 : 0);
     const uint32_t vs_at = a.b.page_size * D + a.b.page_size * (D / 32) + vg % 4 * (D / 8) + vm * D / 512 * 4;
-    uint32_t page_of = 0, slot_of = 0, step = 0;  // lane i: of step 64 k + i
-    auto request = [&](Raw &x) {
-        if (step % 64 == 0) {
-            const uint32_t t = first + (step + lane) * KT + 16 * half;
-            page_of = t < end ? table[t / a.b.page_size] : 0;
-            slot_of = t % a.b.page_size;
-        }
+    uint32_t page_of = 0, slot_of = 0;  // lane i: of step 64 c + i
+    auto read_table = [&](uint32_t step) {
+        const uint32_t t = first + (step + lane) * KT + 16 * half;
+        page_of = t < end ? table[t / a.b.page_size] : 0;
+        slot_of = t % a.b.page_size;
+    };
+    // the head's bytes in a step's page, and the step's place there
+    struct Place {
+        gbytes head;
+        uint32_t slot;
+        bool lost;
+    };
+    auto find = [&](uint32_t step) {
+        Place x;
         uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)page_of, step % 64);
-        const uint32_t slot = (uint32_t)__builtin_amdgcn_readlane((int)slot_of, step % 64);
-        step++;
+        x.slot = (uint32_t)__builtin_amdgcn_readlane((int)slot_of, step % 64);
         x.lost = page >= a.b.pages;
         page = x.lost ? 0 : page;
-        const gbytes p = (gbytes)gp(a.cache) + ((uint64_t)page * a.b.kv_heads + h) * head_bytes;
-        const gbytes words = p + slot * (D / 2), scales = p + slot * (D / 32);
+        x.head = (gbytes)gp(a.cache) + ((uint64_t)page * a.b.kv_heads + h) * head_bytes;
+        return x;
+    };
+    auto request_keys = [&](Raw &x, const Place &p) {
+        const gbytes words = p.head + p.slot * (D / 2);
         if constexpr (D == 64) {
-            const u32x2 k = *(const GLOBAL u32x2 *)(words + k_at), v = *(const GLOBAL u32x2 *)(words + v_at);
-            x.k[0] = k.x;
-            x.k[1] = k.y;
-            x.v[0] = v.x;
-            x.v[1] = v.y;
+            const u32x2 k = *(const GLOBAL u32x2 *)(words + k_at);
+            x.w[0] = k.x;
+            x.w[1] = k.y;
         } else {
             const u32x4 k = *(const GLOBAL u32x4 *)(words + k_at);
 #pragma unroll
-            for (int i = 0; i < 4; i++) x.k[i] = k[i];
-            if constexpr (D == 128) {
-                const u32x4 v = *(const GLOBAL u32x4 *)(words + v_at);
-#pragma unroll
-                for (int i = 0; i < 4; i++) x.v[i] = v[i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) x.v[i] = *(const GLOBAL uint32_t *)(words + v_at + 8 * i);
-            }
+            for (int i = 0; i < 4; i++) x.w[i] = k[i];
         }
-        x.ks = scales[ks_at];
-        x.vs = *(const GLOBAL uint32_t *)(scales + vs_at);
+        x.scale = (p.head + p.slot * (D / 32))[ks_at];
+        x.lost = p.lost;
     };
-    auto convert = [&](Raw &x, uint32_t into, uint32_t number) {
-        const float ks = cache_scale(x.lost ? 255 : x.ks);
+    auto request_values = [&](Raw &x, const Place &p) {
+        const gbytes words = p.head + p.slot * (D / 2);
+        if constexpr (D == 64) {
+            const u32x2 v = *(const GLOBAL u32x2 *)(words + v_at);
+            x.w[0] = v.x;
+            x.w[1] = v.y;
+        } else if constexpr (D == 128) {
+            const u32x4 v = *(const GLOBAL u32x4 *)(words + v_at);
+#pragma unroll
+            for (int i = 0; i < 4; i++) x.w[i] = v[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) x.w[i] = *(const GLOBAL uint32_t *)(words + v_at + 8 * i);
+        }
+        x.scale = *(const GLOBAL uint32_t *)(p.head + p.slot * (D / 32) + vs_at);
+        x.lost = p.lost;
+    };
+    auto convert_keys = [&](const Raw &x, uint32_t into) {
+        const float ks = cache_scale(x.lost ? 255 : x.scale);
 #pragma unroll
         for (int i = 0; i < (int)KB / 4; i++)
-            keys[into][kt * KROW + kp * (KB / 4) + i] = u32x4{H::template pair<0>(x.k[i], ks), H::template pair<1>(x.k[i], ks),
-                                                            H::template pair<2>(x.k[i], ks), H::template pair<3>(x.k[i], ks)};
-        uint32_t vs = x.lost ? 0xffffffffu : x.vs;
+            keys[into][kt * KROW + kp * (KB / 4) + i] = u32x4{H::template pair<0>(x.w[i], ks), H::template pair<1>(x.w[i], ks),
+                                                            H::template pair<2>(x.w[i], ks), H::template pair<3>(x.w[i], ks)};
+    };
+    auto convert_values = [&](const Raw &x, uint32_t into, uint32_t number) {
+        uint32_t vs = x.lost ? 0xffffffffu : x.scale;
         if (__any(holds_255(vs))) {  // numbers in their place: 0 * NaN is NaN
             if (lane == 0) flags[into] = number;
 #pragma unroll
@@ -136,7 +153,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int byte = D == 64 ? 2 * (i % 2) + b : b;
-                const uint32_t w = D == 64 ? x.v[i / 2] : x.v[i];
+                const uint32_t w = D == 64 ? x.w[i / 2] : x.w[i];
                 c[i] = byte == 0 ? H::template pair<0>(w, scale[i]) : byte == 1 ? H::template pair<1>(w, scale[i])
                      : byte == 2 ? H::template pair<2>(w, scale[i]) : H::template pair<3>(w, scale[i]);
             }
@@ -144,96 +161,115 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
             out[((c0 + 2 * b + 1) * 16 + vm) * (2 * VROW)] = high_halves(c);
         }
     };
+    auto scores = [&](f32x16 *sc, uint32_t from) {
+#pragma unroll
+        for (int k = 0; k < KN; k++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) sc[k][i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NS; i++)
+#pragma unroll
+            for (int k = 0; k < KN; k++) sc[k] = H::product32(keys[from][(32 * k + n) * KROW + 2 * i + g], q[i], sc[k]);
+    };
 
-    Raw x;
-    __syncthreads();
-    if (first < end) {
-        request(x);
-        convert(x, 0, 1);
+    // Step i computes the scores of step i + 1 beside the probabilities of its own, and converts the
+    // keys of step i + 2 and the values of step i + 1; the ones after those are on their way.  Past
+    // the last step the first one's page is read again.
+    const uint32_t steps = end > first ? (end - first + KT - 1) / KT : 0;
+    Raw rk, rv;
+    f32x16 sc[KN];
+    if (steps) {
+        read_table(0);
+        Place p = find(0);
+        request_keys(rk, p);
+        request_values(rv, p);
+        p = find(1);
+        Raw second;
+        request_keys(second, p);
+        convert_keys(rk, 0);
+        if (threadIdx.x < 2) flags[threadIdx.x] = 0;
+        __syncthreads();
+        convert_values(rv, 0, 1);
+        request_values(rv, p);
+        request_keys(rk, find(2));
+        convert_keys(second, 1);
+        __syncthreads();
+        scores(sc, 0);
     }
-    if (first + KT < end) request(x);
-    __syncthreads();
-    uint32_t number = 1;
-    for (uint32_t t0 = first; t0 < end; t0 += KT, number++) {
-        const uint32_t buffer = (number - 1) & 1;
-        if ((int32_t)t0 <= most) {
-            f32x16 sc[KN];
+    for (uint32_t step = 0; step < steps; step++) {
+        const uint32_t buffer = step & 1, t0 = first + step * KT;
+        if ((int32_t)(t0 + KT) - 1 > least || t0 + KT > end || (a.window && (int32_t)t0 + (int32_t)a.window <= most)) {
 #pragma unroll
             for (int k = 0; k < KN; k++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) sc[k][i] = 0.f;
-#pragma unroll
-            for (int i = 0; i < NS; i++)
-#pragma unroll
-                for (int k = 0; k < KN; k++) sc[k] = H::product32(keys[buffer][(32 * k + n) * KROW + 2 * i + g], q[i], sc[k]);
-            if ((int32_t)(t0 + KT) - 1 > least || (a.window && (int32_t)t0 + (int32_t)a.window <= most)) {
-#pragma unroll
-                for (int k = 0; k < KN; k++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int32_t t = (int32_t)t0 + 32 * k + 8 * (i / 4) + 4 * (int32_t)g + i % 4;
-                        if (!(t <= at && (!a.window || t + (int32_t)a.window > at))) sc[k][i] = -INFINITY;
-                    }
-            }
-            float top = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < KN; k++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) top = fmaxf(top, sc[k][i]);
-            {
-                auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-                top = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])) * a.c;
-            }
-            if (__any(top > m + 8.f)) {
-                top = fmaxf(top, m);
-                const float f = carry(m, top);
-                m = top;
-                l *= f;
-#pragma unroll
-                for (int j = 0; j < NO; j++) o[j] *= f;
-            }
-            const float ref = m > -INFINITY ? m : 0.f;
-            u32x4 p[2 * KN];
-#pragma unroll
-            for (int k = 0; k < KN; k++) {
-                float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    sc[k][i] = __builtin_amdgcn_exp2f(fmaf(sc[k][i], a.c, -ref));
-                    sum += sc[k][i];
+                    const int32_t t = (int32_t)t0 + 32 * k + 8 * (i / 4) + 4 * (int32_t)g + i % 4;
+                    if (!(t <= at && (uint32_t)t < end && (!a.window || t + (int32_t)a.window > at))) sc[k][i] = -INFINITY;
                 }
-                l += sum;
+        }
+        float top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 8; i++) p[2 * k + i / 4][i % 4] = H::pack(sc[k][2 * i], sc[k][2 * i + 1]);
+        for (int k = 0; k < KN; k++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, sc[k][i]);
+        {
+            auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            top = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])) * a.c;
+        }
+        if (__any(top > m + 8.f)) {
+            top = fmaxf(top, m);
+            const float f = carry(m, top);
+            m = top;
+            l *= f;
+#pragma unroll
+            for (int j = 0; j < NO; j++) o[j] *= f;
+        }
+        if (flags[buffer] == step + 1) {
+            // rows that see a block of NaN: every lane looks at the step's tokens itself
+            uint32_t bad = 0;
+            for (uint32_t t = t0; t < min(t0 + KT, end); t++) {
+                if (!((int32_t)t <= at && (!a.window || (int32_t)(t + a.window) > at))) continue;
+                const uint32_t page = table[t / a.b.page_size];
+                for (uint32_t b = 0; b < D / 32; b++)
+                    if (page >= a.b.pages ||
+                        a.cache[((uint64_t)page * a.b.kv_heads + h) * head_bytes + cache_value_scale_at(a.b.page_size, t % a.b.page_size, b, D)] == 255)
+                        bad |= 1u << b;
             }
-            if (flags[buffer] == number) {
-                // rows that see a block of NaN: every lane looks at the step's tokens itself
-                uint32_t bad = 0;
-                for (uint32_t t = t0; t < min(t0 + KT, end); t++) {
-                    if (!((int32_t)t <= at && (!a.window || (int32_t)(t + a.window) > at))) continue;
-                    const uint32_t page = table[t / a.b.page_size];
-                    for (uint32_t b = 0; b < D / 32; b++)
-                        if (page >= a.b.pages ||
-                            a.cache[((uint64_t)page * a.b.kv_heads + h) * head_bytes + cache_value_scale_at(a.b.page_size, t % a.b.page_size, b, D)] == 255)
-                            bad |= 1u << b;
+#pragma unroll
+            for (int j = 0; j < NO; j++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const uint32_t r = 32 * j + 8 * (i / 4) + 4 * g + i % 4;
+                    if (bad >> ((PIECE * (r % 16) + r / 16) / 32) & 1) o[j][i] = __uint_as_float(0x7fc00000u);
                 }
+        }
+        f32x16 next[KN];
+        scores(next, buffer ^ 1);
+        const float ref = m > -INFINITY ? m : 0.f;
+        u32x4 p[2 * KN];
 #pragma unroll
-                for (int j = 0; j < NO; j++)
+        for (int k = 0; k < KN; k++) {
+            float sum = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const uint32_t r = 32 * j + 8 * (i / 4) + 4 * g + i % 4;
-                        if (bad >> ((PIECE * (r % 16) + r / 16) / 32) & 1) o[j][i] = __uint_as_float(0x7fc00000u);
-                    }
+            for (int i = 0; i < 16; i++) {
+                sc[k][i] = __builtin_amdgcn_exp2f(fmaf(sc[k][i], a.c, -ref));
+                sum += sc[k][i];
             }
+            l += sum;
 #pragma unroll
-            for (int t = 0; t < 2 * KN; t++)
+            for (int i = 0; i < 8; i++) p[2 * k + i / 4][i % 4] = H::pack(sc[k][2 * i], sc[k][2 * i + 1]);
+        }
 #pragma unroll
-                for (int j = 0; j < NO; j++) o[j] = H::product32(values[buffer][(32 * j + n) * VROW + 2 * t + g], p[t], o[j]);
-        }
-        if (t0 + KT < end) {
-            convert(x, buffer ^ 1, number + 1);
-            if (t0 + 2 * KT < end) request(x);
-        }
+        for (int t = 0; t < 2 * KN; t++)
+#pragma unroll
+            for (int j = 0; j < NO; j++) o[j] = H::product32(values[buffer][(32 * j + n) * VROW + 2 * t + g], p[t], o[j]);
+        convert_keys(rk, buffer);
+        convert_values(rv, buffer ^ 1, step + 2);
+        request_values(rv, find(step + 2));
+        if ((step + 3) % 64 == 0) read_table(step + 3);
+        request_keys(rk, find(step + 3));
+#pragma unroll
+        for (int k = 0; k < KN; k++) sc[k] = next[k];
         __syncthreads();
     }
     if (!live) return;

@@ -285,6 +285,21 @@ def test_shorter_bounds(lib):
     assert np.all(np.abs(got - want[:7]) <= tol[:7])
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("tile", [1, 2, 4, 8])
+@pytest.mark.parametrize("chunk", [0, 128, 384])
+def test_every_kernel_and_chunk(lib, d, tile, chunk):
+    """Each kernel on few and many rows, whole and in chunks, with windows that begin inside a step."""
+    rng = np.random.default_rng(d + tile + chunk)
+    with lib.overridden(lib.Knob.ATTENTION, (tile, chunk)):
+        for rows, lengths, window in (([1, 3], [5, 700], 0), ([45, 7], [900, 450], 0), ([45, 70], [900, 450], 333), ([30], [30], 0)):
+            say("kernel", d, tile, chunk, rows, lengths, window)
+            c = Case(lib, rng, rows, lengths, 8, 2, d, 48, "bf16", window=window, sinks=True, holes=1)
+            c.call()
+            lib.synchronize()
+            c.check()
+
+
 def test_same_result_every_time(lib):
     rng = np.random.default_rng(18)
     for rows, lengths in (([1, 1], [3000, 10]), ([200], [700])):
