@@ -98,8 +98,9 @@ __device__ __forceinline__ uint32_t first_seen(const CacheSpan &s, uint32_t wind
 // exp2 of m - to, 0 for m = -Inf whatever `to` is.
 __device__ __forceinline__ float carry(float m, float to) { return m > -INFINITY ? __builtin_amdgcn_exp2f(m - to) : 0.f; }
 
-// Whether a byte of a word is 255.
-__device__ __forceinline__ bool holds_255(uint32_t x) { return ((~x - 0x01010101u) & x & 0x80808080u) != 0; }
+// 0x80 in the bytes of a word of scales that are 255 (and in a 254 above one,
+// which no block has).
+__device__ __forceinline__ uint32_t bytes_255(uint32_t x) { return (~x - 0x01010101u) & x & 0x80808080u; }
 
 // Prompt chunks (attention_prompt.hip): rows of a tile, tokens of a step.
 constexpr uint32_t PROMPT_ROWS = 128;

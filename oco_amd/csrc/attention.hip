@@ -223,7 +223,7 @@ __global__ __launch_bounds__(256, (D / 64) * R == 1 ? 4 : (D / 64) * R == 2 ? 3 
 #pragma unroll
         for (int e = 0; e < 2; e++)
             if (lost[e]) v[e].scale = 0xffffffffu;
-        if (__any(holds_255(v[0].scale) || holds_255(v[1].scale))) {
+        if (__any((bytes_255(v[0].scale) | bytes_255(v[1].scale)) != 0)) {
             // 0 * NaN is NaN: a NaN block enters the product as numbers, and the rows that see
             // it (counted by a product of their own) become NaN in its columns
             u32x4 lost_at;
@@ -248,8 +248,7 @@ __global__ __launch_bounds__(256, (D / 64) * R == 1 ? 4 : (D / 64) * R == 2 ? 3 
                     for (int j = 0; j < NT; j++) o[r][j][i] = count[i] > 0.f ? __uint_as_float(0x7fc00000u) : o[r][j][i];
             }
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (byte_of(v[i / 4].scale, i % 4) == 255) v[i / 4].scale ^= 128u << (8 * (i % 4));
+            for (int e = 0; e < 2; e++) v[e].scale ^= bytes_255(v[e].scale);
         }
         float scale[8];  // of the tokens' column block
 #pragma unroll

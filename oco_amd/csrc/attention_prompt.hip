@@ -22,7 +22,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
     // rows of 16-byte pieces, one piece of padding: eight consecutive rows fall into different banks
     constexpr uint32_t KROW = D / 8 + 1, VROW = KT / 8 + 1;
     __shared__ __attribute__((aligned(16))) u32x4 keys[2][KT * KROW], values[2][D * VROW];
-    __shared__ uint32_t flags[2];  // the step, from 1, whose values hold a block of NaN
+    __shared__ uint32_t flags[3];  // the step, from 1, whose values hold a block of NaN; the last one is not read
 
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, g = lane >> 5;
     uint32_t id = blockIdx.x;
@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
     const uint32_t vs_at = a.b.page_size * D + a.b.page_size * (D / 32) + vg % 4 * (D / 8) + vm * D / 512 * 4;
     uint32_t page_of = 0, slot_of = 0;  // lane i: of step 64 c + i
     auto read_table = [&](uint32_t step) {
-        const uint32_t t = first + (step + lane) * KT + 16 * half;
+        const uint32_t t = first + (step + lane) * KT + 16 * half;  // step: the first of 64
         page_of = t < end ? table[t / a.b.page_size] : 0;
         slot_of = t % a.b.page_size;
     };
@@ -135,12 +135,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
     };
     auto convert_values = [&](const Raw &x, uint32_t into, uint32_t number) {
         uint32_t vs = x.lost ? 0xffffffffu : x.scale;
-        if (__any(holds_255(vs))) {  // numbers in their place: 0 * NaN is NaN
-            if (lane == 0) flags[into] = number;
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (byte_of(vs, i) == 255) vs ^= 128u << (8 * i);
-        }
+        // a NaN block enters as numbers, for 0 * NaN is NaN; without a branch, which would keep the
+        // products before it from running beside
+        const uint32_t bad = bytes_255(vs);
+        vs ^= bad;
+        flags[__any(bad != 0) ? into : 2] = number;
         float scale[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) scale[i] = __uint_as_float(byte_of(vs, i) << 23);
@@ -177,6 +176,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
     // the last step the first one's page is read again.
     const uint32_t steps = end > first ? (end - first + KT - 1) / KT : 0;
     Raw rk, rv;
+    Place ahead;
     f32x16 sc[KN];
     if (steps) {
         read_table(0);
@@ -191,13 +191,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
         __syncthreads();
         convert_values(rv, 0, 1);
         request_values(rv, p);
-        request_keys(rk, find(2));
+        ahead = find(2);
+        request_keys(rk, ahead);
         convert_keys(second, 1);
         __syncthreads();
         scores(sc, 0);
     }
-    for (uint32_t step = 0; step < steps; step++) {
-        const uint32_t buffer = step & 1, t0 = first + step * KT;
+    // step, its scores, where the next step's go, the buffer of its values
+    auto compute = [&](const uint32_t step, f32x16 *sc, f32x16 *next, const uint32_t buffer) {
+        const uint32_t t0 = first + step * KT;
+        if ((step + 3) % 64 == 0) read_table(step + 3);
         if ((int32_t)(t0 + KT) - 1 > least || t0 + KT > end || (a.window && (int32_t)t0 + (int32_t)a.window <= most)) {
 #pragma unroll
             for (int k = 0; k < KN; k++)
@@ -243,34 +246,64 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
                     if (bad >> ((PIECE * (r % 16) + r / 16) / 32) & 1) o[j][i] = __uint_as_float(0x7fc00000u);
                 }
         }
-        f32x16 next[KN];
-        scores(next, buffer ^ 1);
+        // Scores of the next step between the exponentials of this one, then the second product between
+        // the conversions.  Each group requests the next one's fragments, and nothing moves across groups.
         const float ref = m > -INFINITY ? m : 0.f;
-        u32x4 p[2 * KN];
+        u32x4 p[2 * KN], kf[2][KN], vf[2][NO];
+        float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < KN; k++) {
-            float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                sc[k][i] = __builtin_amdgcn_exp2f(fmaf(sc[k][i], a.c, -ref));
-                sum += sc[k][i];
-            }
-            l += sum;
-#pragma unroll
-            for (int i = 0; i < 8; i++) p[2 * k + i / 4][i % 4] = H::pack(sc[k][2 * i], sc[k][2 * i + 1]);
+            for (int i = 0; i < 16; i++) next[k][i] = 0.f;
+            kf[0][k] = keys[buffer ^ 1][(32 * k + n) * KROW + g];
         }
 #pragma unroll
-        for (int t = 0; t < 2 * KN; t++)
+        for (int i = 0; i < NS; i++) {
+            if (i + 1 < NS) {
 #pragma unroll
-            for (int j = 0; j < NO; j++) o[j] = H::product32(values[buffer][(32 * j + n) * VROW + 2 * t + g], p[t], o[j]);
-        convert_keys(rk, buffer);
-        convert_values(rv, buffer ^ 1, step + 2);
-        request_values(rv, find(step + 2));
-        if ((step + 3) % 64 == 0) read_table(step + 3);
-        request_keys(rk, find(step + 3));
+                for (int k = 0; k < KN; k++) kf[(i + 1) % 2][k] = keys[buffer ^ 1][(32 * k + n) * KROW + 2 * (i + 1) + g];
+            } else {
 #pragma unroll
-        for (int k = 0; k < KN; k++) sc[k] = next[k];
+                for (int j = 0; j < NO; j++) vf[0][j] = values[buffer][(32 * j + n) * VROW + g];
+            }
+#pragma unroll
+            for (int k = 0; k < KN; k++) next[k] = H::product32(kf[i % 2][k], q[i], next[k]);
+            constexpr int E = KN * 16 / NS;  // a group's exponentials
+#pragma unroll
+            for (int e = E * i; e < E * i + E; e++) {
+                const float u = __builtin_amdgcn_exp2f(fmaf(sc[e / 16][e % 16], a.c, -ref));
+                sc[e / 16][e % 16] = u;
+                sum += u;
+                if (e % 2) p[e / 8][e % 8 / 2] = H::pack(sc[e / 16][e % 16 - 1], u);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        l += sum;
+#pragma unroll
+        for (int t = 0; t < 2 * KN; t++) {
+            if (t + 1 < 2 * KN) {
+#pragma unroll
+                for (int j = 0; j < NO; j++) vf[(t + 1) % 2][j] = values[buffer][(32 * j + n) * VROW + 2 * (t + 1) + g];
+            }
+#pragma unroll
+            for (int j = 0; j < NO; j++) o[j] = H::product32(vf[t % 2][j], p[t], o[j]);
+            if (t == 0) {
+                convert_keys(rk, buffer);
+            } else if (t == KN) {
+                convert_values(rv, buffer ^ 1, step + 2);
+                request_values(rv, ahead);
+                ahead = find(step + 3);
+                request_keys(rk, ahead);
+            }
+            if (t + 1 < 2 * KN && (t == 0 || t + 1 == KN)) __builtin_amdgcn_sched_barrier(0);
+        }
         __syncthreads();
+    };
+    f32x16 other[KN];
+    for (uint32_t step = 0; step < steps; step += 2) {
+        compute(step, sc, other, 0);
+        if (step + 1 == steps) break;
+        compute(step + 1, other, sc, 1);
     }
     if (!live) return;
     {
