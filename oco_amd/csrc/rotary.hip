@@ -50,55 +50,154 @@ __device__ __forceinline__ void rotation_table(const Rotation &r, uint32_t posit
     __syncthreads();
 }
 
+// The same by one wavefront for itself: what it writes to LDS it reads in order.
+__device__ __forceinline__ void rotation_table_wave(const Rotation &r, uint32_t position, double2 *table) {
+    for (uint32_t i = threadIdx.x & 63; i < r.dim / 2; i += 64) {
+        const double2 t = cos_sin((double)position * r.frequencies[i]);
+        table[i] = make_double2(t.x * r.magnitude, t.y * r.magnitude);
+    }
+}
+
 // A head as units of work: eight pairs (four interleaved), then runs of eight
 // values that stay.  A unit reads what it writes and nothing else, so the
 // result may take the place of the row.
 struct HeadUnits {
     uint32_t turns, all;
+    bool whole;  // every unit has all its values
 };
 __device__ __forceinline__ HeadUnits head_units(const Rotation &r, uint32_t head_dim) {
     HeadUnits u;
     u.turns = r.interleaved ? (r.dim + 7) / 8 : (r.dim / 2 + 7) / 8;
     u.all = u.turns + (head_dim - r.dim + 7) / 8;
+    u.whole = r.dim % (r.interleaved ? 8 : 16) == 0 && head_dim % 8 == 0;
     return u;
 }
 
-// Unit u of a head.  put(column, count limit, values): eight values from a column on, those under the limit.
-template <class T, class Put>
-__device__ __forceinline__ void turn_unit(const T *x, uint32_t u, uint32_t turns, uint32_t head_dim, const Rotation &r, const double2 *table, Put put) {
+// A unit's values: a from column `first` on, and b (of a turning unit in halves) half further.
+struct Unit {
     float a[8], b[8];
-    if (u >= turns) {
-        const uint32_t c = r.dim + 8 * (u - turns);
-        load_run(x, c, head_dim, a);
-        put(c, head_dim, a);
-        return;
-    }
-    if (r.interleaved) {
-        load_run(x, 8 * u, r.dim, a);
+};
+// The same as they are loaded.
+template <class T>
+struct Eight {
+    u32x4_u w[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T *p) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const double2 t = table[min(4 * u + j, r.dim / 2 - 1)];
-            const double v = a[2 * j], w = a[2 * j + 1];
-            a[2 * j] = (float)__builtin_fma(v, t.x, -(w * t.y));
-            a[2 * j + 1] = (float)__builtin_fma(w, t.x, v * t.y);
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) w[i] = ((const GLOBAL u32x4_u *)gp((const u32x4_u *)p))[i];
+    }
+    __device__ __forceinline__ void values(float *v) const { RowIO<T>::load8((const T *)w, v); }
+};
+template <class T>
+struct RawUnit {
+    Eight<T> a, b;
+    __device__ __forceinline__ void values(Unit &x, const Rotation &r) const {
+        a.values(x.a);
+        if (!r.interleaved) b.values(x.b);
+    }
+};
+struct UnitPlace {
+    uint32_t first;
+    bool turns, pairs;  // pairs: b is there
+};
+__device__ __forceinline__ UnitPlace unit_place(uint32_t u, const HeadUnits &n, const Rotation &r) {
+    UnitPlace p;
+    p.turns = u < n.turns;
+    p.pairs = p.turns && !r.interleaved;
+    p.first = p.turns ? 8 * u : r.dim + 8 * (u - n.turns);
+    return p;
+}
+template <class T>
+__device__ __forceinline__ void load_unit(RawUnit<T> &x, const T *head, const UnitPlace &p, const Rotation &r) {
+    x.a.load(head + p.first);
+    if (!r.interleaved) x.b.load(head + p.first + (p.pairs ? r.dim / 2 : 0));
+}
+template <class T>
+__device__ __forceinline__ void load_unit_tail(Unit &x, const T *head, const UnitPlace &p, const Rotation &r, uint32_t head_dim) {
+    load_run(head, p.first, p.pairs ? r.dim / 2 : p.turns ? r.dim : head_dim, x.a);
+    if (p.pairs) load_run(head + r.dim / 2, p.first, r.dim / 2, x.b);
+}
+__device__ __forceinline__ void turn_pair(float &x, float &y, const double2 &t) {
+    const double v = x, w = y;
+    x = (float)__builtin_fma(v, t.x, -(w * t.y));
+    y = (float)__builtin_fma(w, t.x, v * t.y);
+}
+__device__ __forceinline__ void turn_unit(Unit &x, const UnitPlace &p, const Rotation &r, const double2 *table) {
+    const uint32_t last = r.dim / 2 - 1;  // pairs past it are not stored
+    if (p.pairs) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) turn_pair(x.a[j], x.b[j], table[min(p.first + j, last)]);
+    } else if (p.turns) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) turn_pair(x.a[2 * j], x.a[2 * j + 1], table[min(p.first / 2 + j, last)]);
+    }
+}
+template <class T>
+__device__ __forceinline__ void store_unit(T *head, const Unit &x, const UnitPlace &p, const Rotation &r) {
+    RowIO<T>::store8(head + p.first, x.a);
+    if (p.pairs) RowIO<T>::store8(head + p.first + r.dim / 2, x.b);
+}
+template <class T>
+__device__ __forceinline__ void store_unit_tail(T *head, const Unit &x, const UnitPlace &p, const Rotation &r, uint32_t head_dim) {
+    store_run(head, p.first, p.pairs ? r.dim / 2 : p.turns ? r.dim : head_dim, x.a);
+    if (p.pairs) store_run(head + r.dim / 2, p.first, r.dim / 2, x.b);
+}
+
+// A unit among those of `heads` consecutive heads, and the one `step` on.
+struct Cursor {
+    uint32_t head, unit;
+    __device__ __forceinline__ Cursor(uint32_t i, const HeadUnits &n) : head(i / n.all), unit(i % n.all) {}
+    __device__ __forceinline__ void advance(uint32_t dh, uint32_t du, const HeadUnits &n) {
+        unit += du;
+        const bool over = unit >= n.all;
+        head += dh + over;
+        unit -= over ? n.all : 0;
+    }
+};
+
+// Turns the units first, first + step, ... of `heads` heads.  Whole units go N
+// at a time, and the loads of the first ones are out before the table of
+// angles is made.
+template <class T, class In, class Out, class Table>
+__device__ __forceinline__ void turn_heads(uint32_t first, uint32_t step, uint32_t heads, uint32_t head_dim, const HeadUnits &n, const Rotation &r,
+                                           const double2 *table, In in, Out out, Table make_table) {
+    constexpr int N = sizeof(T) == 4 ? 2 : 4;
+    Cursor now(first, n);
+    const uint32_t dh = step / n.all, du = step % n.all;
+    if (n.whole) {
+        RawUnit<T> x[N];
+        bool first_time = true;
+        do {
+            Cursor ahead = now;
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                const bool live = ahead.head < heads;
+                if (heads) load_unit<T>(x[k], in(live ? ahead.head : 0), unit_place(live ? ahead.unit : 0, n, r), r);
+                ahead.advance(dh, du, n);
+            }
+            if (first_time) make_table();
+            first_time = false;
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                if (now.head < heads) {
+                    const UnitPlace p = unit_place(now.unit, n, r);
+                    Unit y;
+                    x[k].values(y, r);
+                    turn_unit(y, p, r, table);
+                    store_unit<T>(out(now.head), y, p, r);
+                }
+                now.advance(dh, du, n);
+            }
+        } while (__any(now.head < heads));
+    } else {
+        make_table();
+        for (; now.head < heads; now.advance(dh, du, n)) {
+            const UnitPlace p = unit_place(now.unit, n, r);
+            Unit x;
+            load_unit_tail<T>(x, in(now.head), p, r, head_dim);
+            turn_unit(x, p, r, table);
+            store_unit_tail<T>(out(now.head), x, p, r, head_dim);
         }
-        put(8 * u, r.dim, a);
-        return;
     }
-    const uint32_t half = r.dim / 2;
-    load_run(x, 8 * u, half, a);
-    load_run(x + half, 8 * u, half, b);
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const double2 t = table[min(8 * u + j, half - 1)];
-        const double v = a[j], w = b[j];
-        a[j] = (float)__builtin_fma(v, t.x, -(w * t.y));
-        b[j] = (float)__builtin_fma(w, t.x, v * t.y);
-    }
-    put(8 * u, half, a);
-#pragma unroll
-    for (int j = 0; j < 8; j++) a[j] = b[j];
-    put(half + 8 * u, r.dim, a);
 }
 
 // ---- rotation alone ----------------------------------------------------------------
@@ -116,17 +215,12 @@ template <class T>
 __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
     extern __shared__ double2 table[];
     const uint32_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
-    rotation_table(a.r, a.positions[row], table);
     const HeadUnits n = head_units(a.r, a.head_dim);
-    const T *x = (const T *)a.x + row * a.x_stride;
-    T *out = (T *)a.out + row * a.out_stride;
-    const uint32_t total = a.heads * n.all;
-    for (uint32_t i = part * 256 + threadIdx.x; i < total; i += a.parts * 256) {
-        const uint32_t h = i / n.all, u = i % n.all;
-        T *const o = out + (uint64_t)h * a.head_dim;
-        turn_unit(x + (uint64_t)h * a.head_dim, u, n.turns, a.head_dim, a.r, table,
-                  [&](uint32_t c, uint32_t limit, const float *v) { store_run(o, c, limit, v); });
-    }
+    const T *const x = (const T *)a.x + row * a.x_stride;
+    T *const out = (T *)a.out + row * a.out_stride;
+    turn_heads<T>(part * 256 + threadIdx.x, a.parts * 256, a.heads, a.head_dim, n, a.r, table,
+                  [&](uint32_t h) { return x + (uint64_t)h * a.head_dim; }, [&](uint32_t h) { return out + (uint64_t)h * a.head_dim; },
+                  [&] { rotation_table(a.r, a.positions[row], table); });
 }
 
 // ---- appending -----------------------------------------------------------------------
@@ -142,68 +236,91 @@ struct AppendArgs {
     Rotation r;
 };
 
-constexpr uint32_t APPEND_VALUES = 2048;  // of keys in LDS per workgroup, at most
+// Eight values of a value's or key's word, quantised into their page.
+template <uint32_t D>
+__device__ __forceinline__ void append_word(uint8_t *head, uint32_t page_size, uint32_t t, uint32_t w, bool value, const float *x) {
+    uint32_t scale;
+    const uint32_t codes = cache_quantize(x, scale);
+    if (!value) {
+        *(GLOBAL uint32_t *)gp(head + cache_key_at(t, w, D)) = codes;
+    } else if constexpr (D == 64) {  // a word is two pieces
+        *(GLOBAL uint16_t *)gp(head + cache_value_at(page_size, t, 4 * w, D)) = (uint16_t)codes;
+        *(GLOBAL uint16_t *)gp(head + cache_value_at(page_size, t, 4 * w + 2, D)) = (uint16_t)(codes >> 16);
+    } else {
+        *(GLOBAL uint32_t *)gp(head + cache_value_at(page_size, t, 4 * w, D)) = codes;
+    }
+    if (w % 4 == 0) *gp(head + (value ? cache_value_scale_at(page_size, t, w / 4, D) : cache_key_scale_at(page_size, t, w / 4, D))) = (uint8_t)scale;
+}
+
+// A wavefront takes a token, or some of its heads, and waits for no other.
+constexpr uint32_t APPEND_VALUES = 1024;  // of keys in LDS per wavefront, at most
 
 template <class T, uint32_t D>
-__global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
-    __shared__ double2 table[D / 2];
-    __shared__ __attribute__((aligned(16))) float keys[APPEND_VALUES];
-    const uint32_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) void append_kernel(AppendArgs a) {
+    __shared__ double2 tables[4][D / 2];
+    __shared__ __attribute__((aligned(16))) float all_keys[4][APPEND_VALUES];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), id = blockIdx.x * 4 + wave;
+    double2 *const table = tables[wave];
+    float *const keys = all_keys[wave];
+    const uint32_t row = id / a.parts, part = id % a.parts;
+    if (row >= a.b.rows) return;
     const uint32_t s = cache_sequence(a.b, row);
     if (s >= a.b.sequences) return;
     const CacheSpan span = cache_span(a.b, s);
     if (row - span.first >= span.rows) return;
     const uint32_t back = span.rows - (row - span.first);  // the row's place from the end
     const bool token = span.length >= back;
-    const uint32_t at = token ? span.length - back : 0;
-    rotation_table(a.r, a.positions ? a.positions[row] : at, table);
+    const uint32_t at = token ? span.length - back : 0, position = a.positions ? a.positions[row] : at;
     const HeadUnits n = head_units(a.r, D);
-    const uint32_t h0 = part * a.part_heads, heads = min(a.part_heads, a.b.kv_heads - h0), group = a.heads / a.b.kv_heads;
-    if (token)
-        for (uint32_t i = threadIdx.x; i < heads * n.all; i += 256) {
-            const uint32_t h = i / n.all, u = i % n.all;
-            float *const o = keys + h * D;
-            turn_unit((const T *)a.k + row * a.k_stride + (h0 + h) * D, u, n.turns, D, a.r, table, [&](uint32_t c, uint32_t limit, const float *v) {
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (c + j < limit) o[c + j] = RowIO<T>::round(v[j]);
-            });
-        }
-    if (a.q)
-        for (uint32_t i = threadIdx.x; i < heads * group * n.all; i += 256) {
-            const uint32_t h = h0 * group + i / n.all, u = i % n.all;
-            T *const o = (T *)a.q_out + row * a.out_stride + h * D;
-            turn_unit((const T *)a.q + row * a.q_stride + h * D, u, n.turns, D, a.r, table,
-                      [&](uint32_t c, uint32_t limit, const float *v) { store_run(o, c, limit, v); });
-        }
-    if (!token) return;
-    const uint32_t page = a.b.table[(uint64_t)s * a.b.table_stride + at / a.b.page_size], t = at % a.b.page_size;
-    if (page >= a.b.pages) return;
-    __syncthreads();
-    const uint32_t head_bytes = cache_head_bytes(a.b.page_size, D);
+    const uint32_t h0 = part * a.part_heads, heads = min(a.part_heads, a.b.kv_heads - h0), group = a.q ? a.heads / a.b.kv_heads : 0;
+    const T *const k = (const T *)a.k + row * a.k_stride + h0 * D, *const v = (const T *)a.v + row * a.v_stride + h0 * D;
+    const T *const q = (const T *)a.q + row * a.q_stride + (uint64_t)h0 * group * D;
+    T *const q_out = (T *)a.q_out + row * a.out_stride + (uint64_t)h0 * group * D;
+    const uint32_t page = token ? a.b.table[(uint64_t)s * a.b.table_stride + at / a.b.page_size] : 0, t = at % a.b.page_size;
+    // A lane's first unit of a key and first two words of values go out with its queries' units, before
+    // the angles are computed: a token waits for memory once.
     constexpr uint32_t WORDS = D / 8;
-    // keys' words, then values'; blocks of four words stay in four adjacent threads
-    for (uint32_t i = threadIdx.x; i < 2 * heads * WORDS; i += 256) {
-        const bool value = i >= heads * WORDS;
-        const uint32_t j = value ? i - heads * WORDS : i, h = j / WORDS, w = j % WORDS;
-        float x[8];
-        if (value)
-            RowIO<T>::load8((const T *)a.v + row * a.v_stride + (h0 + h) * D + 8 * w, x);
+    Cursor c(lane, n);
+    RawUnit<T> first_key;
+    Eight<T> first_values[2];
+    if (token) {
+        if (n.whole) load_unit<T>(first_key, k + (c.head < heads ? c.head : 0) * D, unit_place(c.head < heads ? c.unit : 0, n, a.r), a.r);
+#pragma unroll
+        for (int i = 0; i < 2; i++) first_values[i].load(v + 8 * min(lane + 64 * i, heads * WORDS - 1));
+    }
+    turn_heads<T>(lane, 64, heads * group, D, n, a.r, table, [&](uint32_t h) { return q + h * D; }, [&](uint32_t h) { return q_out + h * D; },
+                  [&] { rotation_table_wave(a.r, position, table); });
+    if (!token || page >= a.b.pages) return;
+    for (bool first = n.whole; c.head < heads; c.advance(64 / n.all, 64 % n.all, n), first = false) {
+        const UnitPlace p = unit_place(c.unit, n, a.r);
+        Unit x;
+        if (first)
+            first_key.values(x, a.r);
         else
-            RowIO<float>::load8(keys + h * D + 8 * w, x);
-        uint32_t scale;
-        const uint32_t codes = cache_quantize(x, scale);
-        uint8_t *const head = a.cache + ((uint64_t)page * a.b.kv_heads + h0 + h) * head_bytes;
-        if (!value) {
-            *(uint32_t *)(head + cache_key_at(t, w, D)) = codes;
-        } else if constexpr (D == 64) {  // a word is two pieces
-            *(uint16_t *)(head + cache_value_at(a.b.page_size, t, 4 * w, D)) = (uint16_t)codes;
-            *(uint16_t *)(head + cache_value_at(a.b.page_size, t, 4 * w + 2, D)) = (uint16_t)(codes >> 16);
-        } else {
-            *(uint32_t *)(head + cache_value_at(a.b.page_size, t, 4 * w, D)) = codes;
+            load_unit_tail<T>(x, k + c.head * D, p, a.r, D);
+        turn_unit(x, p, a.r, table);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            x.a[j] = RowIO<T>::round(x.a[j]);
+            x.b[j] = RowIO<T>::round(x.b[j]);
         }
-        if (w % 4 == 0)
-            head[value ? cache_value_scale_at(a.b.page_size, t, w / 4, D) : cache_key_scale_at(a.b.page_size, t, w / 4, D)] = (uint8_t)scale;
+        store_unit_tail<float>(keys + c.head * D, x, p, a.r, D);
+    }
+    const uint32_t head_bytes = cache_head_bytes(a.b.page_size, D);
+    uint8_t *const head = a.cache + ((uint64_t)page * a.b.kv_heads + h0) * head_bytes;
+    // blocks of four words stay in four adjacent lanes
+    for (uint32_t j = lane, i = 0; j < heads * WORDS; j += 64, i++) {
+        float x[8];
+        if (i < 2)
+            first_values[i].values(x);
+        else
+            RowIO<T>::load8(v + 8 * j, x);
+        append_word<D>(head + j / WORDS * head_bytes, a.b.page_size, t, j % WORDS, true, x);
+    }
+    for (uint32_t j = lane; j < heads * WORDS; j += 64) {
+        float x[8];
+        RowIO<float>::load8(keys + 8 * j, x);
+        append_word<D>(head + j / WORDS * head_bytes, a.b.page_size, t, j % WORDS, false, x);
     }
 }
 
@@ -218,7 +335,9 @@ struct ReadArgs {
 
 template <class T, uint32_t D>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
-    const uint32_t row = blockIdx.x, s = cache_sequence(a.b, row);
+    const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (row >= a.b.rows) return;
+    const uint32_t s = cache_sequence(a.b, row);
     if (s >= a.b.sequences) return;
     const CacheSpan span = cache_span(a.b, s);
     if (row - span.first >= span.rows) return;
@@ -229,27 +348,35 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
     const bool known = page < a.b.pages;
     const uint32_t head_bytes = cache_head_bytes(a.b.page_size, D);
     constexpr uint32_t WORDS = D / 8;
-    for (uint32_t i = threadIdx.x; i < 2 * a.b.kv_heads * WORDS; i += 256) {
-        const bool value = i >= a.b.kv_heads * WORDS;
-        const uint32_t j = value ? i - a.b.kv_heads * WORDS : i, h = j / WORDS, w = j % WORDS;
+    T *const k = (T *)a.k + row * a.k_stride, *const v = (T *)a.v + row * a.v_stride;
+    if (!token || !known) {  // no token: 0
         float x[8];
 #pragma unroll
         for (int c = 0; c < 8; c++) x[c] = token ? __uint_as_float(0x7fc00000u) : 0.f;
-        if (token && known) {
-            const uint8_t *const head = a.cache + ((uint64_t)page * a.b.kv_heads + h) * head_bytes;
-            uint32_t codes;
-            if (!value) {
-                codes = *(const uint32_t *)(head + cache_key_at(t, w, D));
-            } else if constexpr (D == 64) {
-                codes = *(const uint16_t *)(head + cache_value_at(a.b.page_size, t, 4 * w, D));
-                codes |= (uint32_t)*(const uint16_t *)(head + cache_value_at(a.b.page_size, t, 4 * w + 2, D)) << 16;
-            } else {
-                codes = *(const uint32_t *)(head + cache_value_at(a.b.page_size, t, 4 * w, D));
-            }
-            cache_dequantize(codes, head[value ? cache_value_scale_at(a.b.page_size, t, w / 4, D) : cache_key_scale_at(a.b.page_size, t, w / 4, D)], x);
+        for (uint32_t i = lane; i < a.b.kv_heads * WORDS; i += 64) {
+            RowIO<T>::store8(k + 8 * i, x);
+            RowIO<T>::store8(v + 8 * i, x);
         }
-        T *const out = value ? (T *)a.v + row * a.v_stride : (T *)a.k + row * a.k_stride;
-        RowIO<T>::store8(out + h * D + 8 * w, x);
+        return;
+    }
+#pragma unroll 2
+    for (uint32_t i = lane; i < a.b.kv_heads * WORDS; i += 64) {
+        const uint32_t h = i / WORDS, w = i % WORDS;
+        const gbytes head = (gbytes)gp(a.cache) + ((uint64_t)page * a.b.kv_heads + h) * head_bytes;
+        const uint32_t key = *(const GLOBAL uint32_t *)(head + cache_key_at(t, w, D)), key_scale = head[cache_key_scale_at(a.b.page_size, t, w / 4, D)];
+        uint32_t value;
+        if constexpr (D == 64) {
+            value = *(const GLOBAL uint16_t *)(head + cache_value_at(a.b.page_size, t, 4 * w, D));
+            value |= (uint32_t)*(const GLOBAL uint16_t *)(head + cache_value_at(a.b.page_size, t, 4 * w + 2, D)) << 16;
+        } else {
+            value = *(const GLOBAL uint32_t *)(head + cache_value_at(a.b.page_size, t, 4 * w, D));
+        }
+        const uint32_t value_scale = head[cache_value_scale_at(a.b.page_size, t, w / 4, D)];
+        float x[8];
+        cache_dequantize(key, key_scale, x);
+        RowIO<T>::store8(k + 8 * i, x);
+        cache_dequantize(value, value_scale, x);
+        RowIO<T>::store8(v + 8 * i, x);
     }
 }
 
@@ -409,10 +536,12 @@ extern "C" int oco_cache_append(void *pages, const uint32_t *table, const uint32
     if (q && q == q_out && a.q_stride != a.out_stride) return fail(OCO_ERR_INVALID, "oco_cache_append: queries in place with another stride");
     a.heads = p->heads;
     a.r = rotation_of(rotation);
+    // few tokens: their heads over as many wavefronts as there are, down to one each
     a.part_heads = APPEND_VALUES / p->head_dim;
+    while (a.part_heads > 1 && (uint64_t)p->rows * ((p->kv_heads + a.part_heads - 1) / a.part_heads) < 1024) a.part_heads /= 2;
     a.parts = (p->kv_heads + a.part_heads - 1) / a.part_heads;
     if ((uint64_t)p->rows * a.parts > 0x7fffffffull) return fail(OCO_ERR_INVALID, "oco_cache_append: %u rows", p->rows);
-    const dim3 grid(p->rows * a.parts);
+    const dim3 grid((uint32_t)(((uint64_t)p->rows * a.parts + 3) / 4));
     hipStream_t st = (hipStream_t)stream;
 #define GO(T)                                                                                               \
     switch (p->head_dim) {                                                                                  \
@@ -442,8 +571,7 @@ extern "C" int oco_cache_read(const void *pages, const uint32_t *table, const ui
     a.v = v;
     a.k_stride = p->k_stride ? p->k_stride : (uint64_t)p->kv_heads * p->head_dim;
     a.v_stride = p->v_stride ? p->v_stride : (uint64_t)p->kv_heads * p->head_dim;
-    const dim3 grid(p->rows);
-    if (p->rows > 0x7fffffffu) return fail(OCO_ERR_INVALID, "oco_cache_read: %u rows", p->rows);
+    const dim3 grid((uint32_t)(((uint64_t)p->rows + 3) / 4));
     hipStream_t st = (hipStream_t)stream;
 #define GO(T)                                                                                               \
     switch (p->head_dim) {                                                                                  \
