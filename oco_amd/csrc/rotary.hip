@@ -41,22 +41,20 @@ struct Rotation {
     uint32_t dim, interleaved;
 };
 
-// The pairs' cosines and sines of one position, for the whole workgroup.
-__device__ __forceinline__ void rotation_table(const Rotation &r, uint32_t position, double2 *table) {
-    for (uint32_t i = threadIdx.x; i < r.dim / 2; i += blockDim.x) {
-        const double2 t = cos_sin((double)position * r.frequencies[i]);
-        table[i] = make_double2(t.x * r.magnitude, t.y * r.magnitude);
+// The pairs' cosines and sines of one position, by one wavefront for itself: what it writes to LDS it reads in order.
+struct Angles {
+    double first;  // a lane's first frequency, which can be read before the position is known
+    __device__ __forceinline__ Angles(const Rotation &r) {
+        const uint32_t lane = threadIdx.x & 63;
+        first = lane < r.dim / 2 ? r.frequencies[lane] : 0.0;
     }
-    __syncthreads();
-}
-
-// The same by one wavefront for itself: what it writes to LDS it reads in order.
-__device__ __forceinline__ void rotation_table_wave(const Rotation &r, uint32_t position, double2 *table) {
-    for (uint32_t i = threadIdx.x & 63; i < r.dim / 2; i += 64) {
-        const double2 t = cos_sin((double)position * r.frequencies[i]);
-        table[i] = make_double2(t.x * r.magnitude, t.y * r.magnitude);
+    __device__ __forceinline__ void table(const Rotation &r, uint32_t position, double2 *out) const {
+        for (uint32_t i = threadIdx.x & 63; i < r.dim / 2; i += 64) {
+            const double2 t = cos_sin((double)position * (i < 64 ? first : r.frequencies[i]));
+            out[i] = make_double2(t.x * r.magnitude, t.y * r.magnitude);
+        }
     }
-}
+};
 
 // A head as units of work: eight pairs (four interleaved), then runs of eight
 // values that stay.  A unit reads what it writes and nothing else, so the
@@ -156,9 +154,9 @@ struct Cursor {
 
 // Turns the units first, first + step, ... of `heads` heads.  Whole units go N
 // at a time, and the loads of the first ones are out before the table of
-// angles is made.
+// angles is made (false: there is nothing to turn).
 template <class T, class In, class Out, class Table>
-__device__ __forceinline__ void turn_heads(uint32_t first, uint32_t step, uint32_t heads, uint32_t head_dim, const HeadUnits &n, const Rotation &r,
+__device__ __forceinline__ bool turn_heads(uint32_t first, uint32_t step, uint32_t heads, uint32_t head_dim, const HeadUnits &n, const Rotation &r,
                                            const double2 *table, In in, Out out, Table make_table) {
     constexpr int N = sizeof(T) == 4 ? 2 : 4;
     Cursor now(first, n);
@@ -174,7 +172,7 @@ __device__ __forceinline__ void turn_heads(uint32_t first, uint32_t step, uint32
                 if (heads) load_unit<T>(x[k], in(live ? ahead.head : 0), unit_place(live ? ahead.unit : 0, n, r), r);
                 ahead.advance(dh, du, n);
             }
-            if (first_time) make_table();
+            if (first_time && !make_table()) return false;
             first_time = false;
 #pragma unroll
             for (int k = 0; k < N; k++) {
@@ -189,7 +187,7 @@ __device__ __forceinline__ void turn_heads(uint32_t first, uint32_t step, uint32
             }
         } while (__any(now.head < heads));
     } else {
-        make_table();
+        if (!make_table()) return false;
         for (; now.head < heads; now.advance(dh, du, n)) {
             const UnitPlace p = unit_place(now.unit, n, r);
             Unit x;
@@ -198,6 +196,7 @@ __device__ __forceinline__ void turn_heads(uint32_t first, uint32_t step, uint32
             store_unit_tail<T>(out(now.head), x, p, r, head_dim);
         }
     }
+    return true;
 }
 
 // ---- rotation alone ----------------------------------------------------------------
@@ -211,16 +210,23 @@ struct RotateArgs {
     Rotation r;
 };
 
+// A wavefront takes a row, or some of its units.
 template <class T>
-__global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
-    extern __shared__ double2 table[];
-    const uint32_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+__global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a, uint32_t rows) {
+    extern __shared__ double2 tables[];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), id = blockIdx.x * 4 + wave;
+    const uint32_t row = id / a.parts, part = id % a.parts;
+    if (row >= rows) return;
+    double2 *const table = tables + wave * (a.r.dim / 2);
+    const Angles angles(a.r);
     const HeadUnits n = head_units(a.r, a.head_dim);
     const T *const x = (const T *)a.x + row * a.x_stride;
     T *const out = (T *)a.out + row * a.out_stride;
-    turn_heads<T>(part * 256 + threadIdx.x, a.parts * 256, a.heads, a.head_dim, n, a.r, table,
-                  [&](uint32_t h) { return x + (uint64_t)h * a.head_dim; }, [&](uint32_t h) { return out + (uint64_t)h * a.head_dim; },
-                  [&] { rotation_table(a.r, a.positions[row], table); });
+    turn_heads<T>(part * 64 + lane, a.parts * 64, a.heads, a.head_dim, n, a.r, table, [&](uint32_t h) { return x + (uint64_t)h * a.head_dim; },
+                  [&](uint32_t h) { return out + (uint64_t)h * a.head_dim; }, [&] {
+                      angles.table(a.r, a.positions[row], table);
+                      return true;
+                  });
 }
 
 // ---- appending -----------------------------------------------------------------------
@@ -264,33 +270,36 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) void append_kernel(App
     float *const keys = all_keys[wave];
     const uint32_t row = id / a.parts, part = id % a.parts;
     if (row >= a.b.rows) return;
-    const uint32_t s = cache_sequence(a.b, row);
-    if (s >= a.b.sequences) return;
-    const CacheSpan span = cache_span(a.b, s);
-    if (row - span.first >= span.rows) return;
-    const uint32_t back = span.rows - (row - span.first);  // the row's place from the end
-    const bool token = span.length >= back;
-    const uint32_t at = token ? span.length - back : 0, position = a.positions ? a.positions[row] : at;
     const HeadUnits n = head_units(a.r, D);
     const uint32_t h0 = part * a.part_heads, heads = min(a.part_heads, a.b.kv_heads - h0), group = a.q ? a.heads / a.b.kv_heads : 0;
     const T *const k = (const T *)a.k + row * a.k_stride + h0 * D, *const v = (const T *)a.v + row * a.v_stride + h0 * D;
     const T *const q = (const T *)a.q + row * a.q_stride + (uint64_t)h0 * group * D;
     T *const q_out = (T *)a.q_out + row * a.out_stride + (uint64_t)h0 * group * D;
-    const uint32_t page = token ? a.b.table[(uint64_t)s * a.b.table_stride + at / a.b.page_size] : 0, t = at % a.b.page_size;
-    // A lane's first unit of a key and first two words of values go out with its queries' units, before
-    // the angles are computed: a token waits for memory once.
+    // A lane's first unit of a key and first two words of values go out with its queries' units, before the
+    // row's place is looked up and the angles are computed.
     constexpr uint32_t WORDS = D / 8;
     Cursor c(lane, n);
+    const Angles angles(a.r);
     RawUnit<T> first_key;
     Eight<T> first_values[2];
-    if (token) {
-        if (n.whole) load_unit<T>(first_key, k + (c.head < heads ? c.head : 0) * D, unit_place(c.head < heads ? c.unit : 0, n, a.r), a.r);
+    if (n.whole) load_unit<T>(first_key, k + (c.head < heads ? c.head : 0) * D, unit_place(c.head < heads ? c.unit : 0, n, a.r), a.r);
 #pragma unroll
-        for (int i = 0; i < 2; i++) first_values[i].load(v + 8 * min(lane + 64 * i, heads * WORDS - 1));
-    }
-    turn_heads<T>(lane, 64, heads * group, D, n, a.r, table, [&](uint32_t h) { return q + h * D; }, [&](uint32_t h) { return q_out + h * D; },
-                  [&] { rotation_table_wave(a.r, position, table); });
-    if (!token || page >= a.b.pages) return;
+    for (int i = 0; i < 2; i++) first_values[i].load(v + 8 * min(lane + 64 * i, heads * WORDS - 1));
+    uint32_t page = 0xffffffffu, t = 0;
+    const bool mine = turn_heads<T>(lane, 64, heads * group, D, n, a.r, table, [&](uint32_t h) { return q + h * D; }, [&](uint32_t h) { return q_out + h * D; }, [&] {
+        const uint32_t s = cache_sequence(a.b, row);
+        if (s >= a.b.sequences) return false;
+        const CacheSpan span = cache_span(a.b, s);
+        if (row - span.first >= span.rows) return false;
+        const uint32_t back = span.rows - (row - span.first);  // the row's place from the end
+        const bool token = span.length >= back;
+        const uint32_t at = token ? span.length - back : 0;
+        if (token) page = a.b.table[(uint64_t)s * a.b.table_stride + at / a.b.page_size];
+        t = at % a.b.page_size;
+        angles.table(a.r, a.positions ? a.positions[row] : at, table);
+        return true;
+    });
+    if (!mine || page >= a.b.pages) return;
     for (bool first = n.whole; c.head < heads; c.advance(64 / n.all, 64 % n.all, n), first = false) {
         const UnitPlace p = unit_place(c.unit, n, a.r);
         Unit x;
@@ -331,11 +340,14 @@ struct ReadArgs {
     const uint8_t *cache;
     void *k, *v;
     uint64_t k_stride, v_stride;
+    uint32_t parts;
 };
 
+// A wavefront takes a token, or some of its heads.
 template <class T, uint32_t D>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
-    const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = id / a.parts;
+    const uint32_t lane = id % a.parts * 64 + (threadIdx.x & 63), step = 64 * a.parts;
     if (row >= a.b.rows) return;
     const uint32_t s = cache_sequence(a.b, row);
     if (s >= a.b.sequences) return;
@@ -353,14 +365,14 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
         float x[8];
 #pragma unroll
         for (int c = 0; c < 8; c++) x[c] = token ? __uint_as_float(0x7fc00000u) : 0.f;
-        for (uint32_t i = lane; i < a.b.kv_heads * WORDS; i += 64) {
+        for (uint32_t i = lane; i < a.b.kv_heads * WORDS; i += step) {
             RowIO<T>::store8(k + 8 * i, x);
             RowIO<T>::store8(v + 8 * i, x);
         }
         return;
     }
 #pragma unroll 2
-    for (uint32_t i = lane; i < a.b.kv_heads * WORDS; i += 64) {
+    for (uint32_t i = lane; i < a.b.kv_heads * WORDS; i += step) {
         const uint32_t h = i / WORDS, w = i % WORDS;
         const gbytes head = (gbytes)gp(a.cache) + ((uint64_t)page * a.b.kv_heads + h) * head_bytes;
         const uint32_t key = *(const GLOBAL uint32_t *)(head + cache_key_at(t, w, D)), key_scale = head[cache_key_scale_at(a.b.page_size, t, w / 4, D)];
@@ -495,16 +507,17 @@ extern "C" int oco_rotate(const void *x, oco_dtype dtype, uint32_t rows, uint32_
     a.heads = heads;
     a.head_dim = head_dim;
     a.r = rotation_of(rotation);
-    a.parts = rows < 128 ? (uint32_t)((width + 2047) / 2048) : 1;
-    if (a.parts > 16) a.parts = 16;
+    // few rows: their units over as many wavefronts as there are
+    a.parts = 1;
+    while ((uint64_t)a.parts * 512 < width && (uint64_t)rows * a.parts < 1024) a.parts *= 2;
     if ((uint64_t)rows * a.parts > 0x7fffffffull) return fail(OCO_ERR_INVALID, "oco_rotate: %u rows", rows);
-    const dim3 grid(rows * a.parts);
-    const uint32_t lds = (rotation->dim / 2) * sizeof(double2);
+    const dim3 grid((rows * a.parts + 3) / 4);
+    const uint32_t lds = 4 * (rotation->dim / 2) * sizeof(double2);
     hipStream_t st = (hipStream_t)stream;
     switch (dtype) {
-    case OCO_DT_F32: hipLaunchKernelGGL((rotate_kernel<float>), grid, dim3(256), lds, st, a); break;
-    case OCO_DT_BF16: hipLaunchKernelGGL((rotate_kernel<bf16_t>), grid, dim3(256), lds, st, a); break;
-    default: hipLaunchKernelGGL((rotate_kernel<f16_t>), grid, dim3(256), lds, st, a);
+    case OCO_DT_F32: hipLaunchKernelGGL((rotate_kernel<float>), grid, dim3(256), lds, st, a, rows); break;
+    case OCO_DT_BF16: hipLaunchKernelGGL((rotate_kernel<bf16_t>), grid, dim3(256), lds, st, a, rows); break;
+    default: hipLaunchKernelGGL((rotate_kernel<f16_t>), grid, dim3(256), lds, st, a, rows);
     }
     return launch_check("oco_rotate");
 }
@@ -571,7 +584,9 @@ extern "C" int oco_cache_read(const void *pages, const uint32_t *table, const ui
     a.v = v;
     a.k_stride = p->k_stride ? p->k_stride : (uint64_t)p->kv_heads * p->head_dim;
     a.v_stride = p->v_stride ? p->v_stride : (uint64_t)p->kv_heads * p->head_dim;
-    const dim3 grid((uint32_t)(((uint64_t)p->rows + 3) / 4));
+    a.parts = 1;
+    while (a.parts * 64 < p->kv_heads * (p->head_dim / 8) && (uint64_t)p->rows * a.parts < 1024) a.parts *= 2;
+    const dim3 grid((uint32_t)(((uint64_t)p->rows * a.parts + 3) / 4));
     hipStream_t st = (hipStream_t)stream;
 #define GO(T)                                                                                               \
     switch (p->head_dim) {                                                                                  \
