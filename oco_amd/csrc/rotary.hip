@@ -11,6 +11,9 @@
 
 namespace oco {
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
 // cos and sin of a: a - k pi/2 with pi/2 in two parts, then Taylor series for
 // |r| <= pi/4, whose first terms left out are r^19 / 19! and r^20 / 20! (1e-19).
 __device__ __forceinline__ double2 cos_sin(double a) {
@@ -38,7 +41,7 @@ __device__ __forceinline__ double2 cos_sin(double a) {
 struct Rotation {
     const double *frequencies;
     double magnitude;
-    uint32_t dim, interleaved;
+    uint32_t dim;
 };
 
 // The pairs' cosines and sines of one position, by one wavefront for itself: what it writes to LDS it reads in order.
@@ -63,11 +66,12 @@ struct HeadUnits {
     uint32_t turns, all;
     bool whole;  // every unit has all its values
 };
+template <bool INTERLEAVED>
 __device__ __forceinline__ HeadUnits head_units(const Rotation &r, uint32_t head_dim) {
     HeadUnits u;
-    u.turns = r.interleaved ? (r.dim + 7) / 8 : (r.dim / 2 + 7) / 8;
+    u.turns = INTERLEAVED ? (r.dim + 7) / 8 : (r.dim / 2 + 7) / 8;
     u.all = u.turns + (head_dim - r.dim + 7) / 8;
-    u.whole = r.dim % (r.interleaved ? 8 : 16) == 0 && head_dim % 8 == 0;
+    u.whole = r.dim % (INTERLEAVED ? 8 : 16) == 0 && head_dim % 8 == 0;
     return u;
 }
 
@@ -78,36 +82,77 @@ struct Unit {
 // The same as they are loaded.
 template <class T>
 struct Eight {
-    u32x4_u w[sizeof(T) / 2];
+    u32x4 w[sizeof(T) / 2];
     __device__ __forceinline__ void load(const T *p) {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; i++) w[i] = ((const GLOBAL u32x4_u *)gp((const u32x4_u *)p))[i];
     }
-    __device__ __forceinline__ void values(float *v) const { RowIO<T>::load8((const T *)w, v); }
+    __device__ __forceinline__ void values(float *v) const {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint32_t u = sizeof(T) == 4 ? w[j / 4 % (sizeof(T) / 2)][j % 4] : w[0][j / 2];
+            if constexpr (sizeof(T) == 4)
+                v[j] = __uint_as_float(u);
+            else if constexpr (std::is_same_v<T, bf16_t>)
+                v[j] = __uint_as_float(j % 2 ? u & 0xffff0000u : u << 16);
+            else
+                v[j] = half_bits_to_f32(j % 2 ? u >> 16 : u & 0xffff);
+        }
+    }
+    // rounded by the hardware's conversions
+    __device__ __forceinline__ void round(const float *v) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if constexpr (sizeof(T) == 4) {
+                w[j / 4][j % 4] = __float_as_uint(v[j]);
+            } else if (j % 2 == 0) {
+                if constexpr (std::is_same_v<T, bf16_t>)
+                    w[0][j / 2] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)v[j], (__bf16)v[j + 1]});
+                else
+                    w[0][j / 2] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)v[j], (_Float16)v[j + 1]});
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T *p) const {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) ((GLOBAL u32x4_u *)gp((u32x4_u *)p))[i] = w[i];
+    }
+    // the first n of them (LDS or memory)
+    __device__ __forceinline__ void store_some(T *p, uint32_t n) const {
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j++) {
+            if (j >= n) break;
+            if constexpr (sizeof(T) == 4)
+                p[j] = __uint_as_float(w[j / 4][j % 4]);
+            else
+                p[j].bits = (uint16_t)(w[0][j / 2] >> (16 * (j % 2)));
+        }
+    }
 };
-template <class T>
+template <class T, bool INTERLEAVED>
 struct RawUnit {
     Eight<T> a, b;
-    __device__ __forceinline__ void values(Unit &x, const Rotation &r) const {
+    __device__ __forceinline__ void values(Unit &x) const {
         a.values(x.a);
-        if (!r.interleaved) b.values(x.b);
+        if constexpr (!INTERLEAVED) b.values(x.b);
     }
 };
 struct UnitPlace {
     uint32_t first;
     bool turns, pairs;  // pairs: b is there
 };
+template <bool INTERLEAVED>
 __device__ __forceinline__ UnitPlace unit_place(uint32_t u, const HeadUnits &n, const Rotation &r) {
     UnitPlace p;
     p.turns = u < n.turns;
-    p.pairs = p.turns && !r.interleaved;
+    p.pairs = p.turns && !INTERLEAVED;
     p.first = p.turns ? 8 * u : r.dim + 8 * (u - n.turns);
     return p;
 }
-template <class T>
-__device__ __forceinline__ void load_unit(RawUnit<T> &x, const T *head, const UnitPlace &p, const Rotation &r) {
+template <class T, bool INTERLEAVED>
+__device__ __forceinline__ void load_unit(RawUnit<T, INTERLEAVED> &x, const T *head, const UnitPlace &p, const Rotation &r) {
     x.a.load(head + p.first);
-    if (!r.interleaved) x.b.load(head + p.first + (p.pairs ? r.dim / 2 : 0));
+    if constexpr (!INTERLEAVED) x.b.load(head + p.first + (p.pairs ? r.dim / 2 : 0));
 }
 template <class T>
 __device__ __forceinline__ void load_unit_tail(Unit &x, const T *head, const UnitPlace &p, const Rotation &r, uint32_t head_dim) {
@@ -119,25 +164,38 @@ __device__ __forceinline__ void turn_pair(float &x, float &y, const double2 &t) 
     x = (float)__builtin_fma(v, t.x, -(w * t.y));
     y = (float)__builtin_fma(w, t.x, v * t.y);
 }
+template <bool INTERLEAVED, bool WHOLE>
 __device__ __forceinline__ void turn_unit(Unit &x, const UnitPlace &p, const Rotation &r, const double2 *table) {
-    const uint32_t last = r.dim / 2 - 1;  // pairs past it are not stored
-    if (p.pairs) {
+    if (!p.turns) return;
+    const uint32_t first = INTERLEAVED ? p.first / 2 : p.first, last = r.dim / 2 - 1;  // pairs past it are not stored
+    if constexpr (!INTERLEAVED) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) turn_pair(x.a[j], x.b[j], table[min(p.first + j, last)]);
-    } else if (p.turns) {
+        for (int j = 0; j < 8; j++) turn_pair(x.a[j], x.b[j], table[WHOLE ? first + j : min(first + j, last)]);
+    } else {
 #pragma unroll
-        for (int j = 0; j < 4; j++) turn_pair(x.a[2 * j], x.a[2 * j + 1], table[min(p.first / 2 + j, last)]);
+        for (int j = 0; j < 4; j++) turn_pair(x.a[2 * j], x.a[2 * j + 1], table[WHOLE ? first + j : min(first + j, last)]);
     }
 }
 template <class T>
 __device__ __forceinline__ void store_unit(T *head, const Unit &x, const UnitPlace &p, const Rotation &r) {
-    RowIO<T>::store8(head + p.first, x.a);
-    if (p.pairs) RowIO<T>::store8(head + p.first + r.dim / 2, x.b);
+    Eight<T> y;
+    y.round(x.a);
+    y.store(head + p.first);
+    if (p.pairs) {
+        y.round(x.b);
+        y.store(head + p.first + r.dim / 2);
+    }
 }
 template <class T>
 __device__ __forceinline__ void store_unit_tail(T *head, const Unit &x, const UnitPlace &p, const Rotation &r, uint32_t head_dim) {
-    store_run(head, p.first, p.pairs ? r.dim / 2 : p.turns ? r.dim : head_dim, x.a);
-    if (p.pairs) store_run(head + r.dim / 2, p.first, r.dim / 2, x.b);
+    const uint32_t n = (p.pairs ? r.dim / 2 : p.turns ? r.dim : head_dim) - p.first;
+    Eight<T> y;
+    y.round(x.a);
+    y.store_some(head + p.first, n);
+    if (p.pairs) {
+        y.round(x.b);
+        y.store_some(head + p.first + r.dim / 2, n);
+    }
 }
 
 // A unit among those of `heads` consecutive heads, and the one `step` on.
@@ -155,21 +213,21 @@ struct Cursor {
 // Turns the units first, first + step, ... of `heads` heads.  Whole units go N
 // at a time, and the loads of the first ones are out before the table of
 // angles is made (false: there is nothing to turn).
-template <class T, class In, class Out, class Table>
+template <class T, bool INTERLEAVED, class In, class Out, class Table>
 __device__ __forceinline__ bool turn_heads(uint32_t first, uint32_t step, uint32_t heads, uint32_t head_dim, const HeadUnits &n, const Rotation &r,
                                            const double2 *table, In in, Out out, Table make_table) {
     constexpr int N = sizeof(T) == 4 ? 2 : 4;
     Cursor now(first, n);
     const uint32_t dh = step / n.all, du = step % n.all;
     if (n.whole) {
-        RawUnit<T> x[N];
+        RawUnit<T, INTERLEAVED> x[N];
         bool first_time = true;
         do {
             Cursor ahead = now;
 #pragma unroll
             for (int k = 0; k < N; k++) {
                 const bool live = ahead.head < heads;
-                if (heads) load_unit<T>(x[k], in(live ? ahead.head : 0), unit_place(live ? ahead.unit : 0, n, r), r);
+                if (heads) load_unit<T, INTERLEAVED>(x[k], in(live ? ahead.head : 0), unit_place<INTERLEAVED>(live ? ahead.unit : 0, n, r), r);
                 ahead.advance(dh, du, n);
             }
             if (first_time && !make_table()) return false;
@@ -177,22 +235,23 @@ __device__ __forceinline__ bool turn_heads(uint32_t first, uint32_t step, uint32
 #pragma unroll
             for (int k = 0; k < N; k++) {
                 if (now.head < heads) {
-                    const UnitPlace p = unit_place(now.unit, n, r);
+                    const UnitPlace p = unit_place<INTERLEAVED>(now.unit, n, r);
                     Unit y;
-                    x[k].values(y, r);
-                    turn_unit(y, p, r, table);
+                    x[k].values(y);
+                    turn_unit<INTERLEAVED, true>(y, p, r, table);
                     store_unit<T>(out(now.head), y, p, r);
                 }
                 now.advance(dh, du, n);
+                __builtin_amdgcn_sched_barrier(0);  // one unit's angles and 64-bit values at a time
             }
         } while (__any(now.head < heads));
     } else {
         if (!make_table()) return false;
         for (; now.head < heads; now.advance(dh, du, n)) {
-            const UnitPlace p = unit_place(now.unit, n, r);
+            const UnitPlace p = unit_place<INTERLEAVED>(now.unit, n, r);
             Unit x;
             load_unit_tail<T>(x, in(now.head), p, r, head_dim);
-            turn_unit(x, p, r, table);
+            turn_unit<INTERLEAVED, false>(x, p, r, table);
             store_unit_tail<T>(out(now.head), x, p, r, head_dim);
         }
     }
@@ -211,7 +270,7 @@ struct RotateArgs {
 };
 
 // A wavefront takes a row, or some of its units.
-template <class T>
+template <class T, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a, uint32_t rows) {
     extern __shared__ double2 tables[];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), id = blockIdx.x * 4 + wave;
@@ -219,10 +278,10 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a, uint32_t rows
     if (row >= rows) return;
     double2 *const table = tables + wave * (a.r.dim / 2);
     const Angles angles(a.r);
-    const HeadUnits n = head_units(a.r, a.head_dim);
+    const HeadUnits n = head_units<INTERLEAVED>(a.r, a.head_dim);
     const T *const x = (const T *)a.x + row * a.x_stride;
     T *const out = (T *)a.out + row * a.out_stride;
-    turn_heads<T>(part * 64 + lane, a.parts * 64, a.heads, a.head_dim, n, a.r, table, [&](uint32_t h) { return x + (uint64_t)h * a.head_dim; },
+    turn_heads<T, INTERLEAVED>(part * 64 + lane, a.parts * 64, a.heads, a.head_dim, n, a.r, table, [&](uint32_t h) { return x + (uint64_t)h * a.head_dim; },
                   [&](uint32_t h) { return out + (uint64_t)h * a.head_dim; }, [&] {
                       angles.table(a.r, a.positions[row], table);
                       return true;
@@ -261,16 +320,16 @@ __device__ __forceinline__ void append_word(uint8_t *head, uint32_t page_size, u
 // A wavefront takes a token, or some of its heads, and waits for no other.
 constexpr uint32_t APPEND_VALUES = 1024;  // of keys in LDS per wavefront, at most
 
-template <class T, uint32_t D>
+template <class T, uint32_t D, bool INTERLEAVED>
 __global__ __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) void append_kernel(AppendArgs a) {
     __shared__ double2 tables[4][D / 2];
-    __shared__ __attribute__((aligned(16))) float all_keys[4][APPEND_VALUES];
+    __shared__ __attribute__((aligned(16))) T all_keys[4][APPEND_VALUES];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), id = blockIdx.x * 4 + wave;
     double2 *const table = tables[wave];
-    float *const keys = all_keys[wave];
+    T *const keys = all_keys[wave];
     const uint32_t row = id / a.parts, part = id % a.parts;
     if (row >= a.b.rows) return;
-    const HeadUnits n = head_units(a.r, D);
+    const HeadUnits n = head_units<INTERLEAVED>(a.r, D);
     const uint32_t h0 = part * a.part_heads, heads = min(a.part_heads, a.b.kv_heads - h0), group = a.q ? a.heads / a.b.kv_heads : 0;
     const T *const k = (const T *)a.k + row * a.k_stride + h0 * D, *const v = (const T *)a.v + row * a.v_stride + h0 * D;
     const T *const q = (const T *)a.q + row * a.q_stride + (uint64_t)h0 * group * D;
@@ -280,13 +339,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) void append_kernel(App
     constexpr uint32_t WORDS = D / 8;
     Cursor c(lane, n);
     const Angles angles(a.r);
-    RawUnit<T> first_key;
+    RawUnit<T, INTERLEAVED> first_key;
     Eight<T> first_values[2];
-    if (n.whole) load_unit<T>(first_key, k + (c.head < heads ? c.head : 0) * D, unit_place(c.head < heads ? c.unit : 0, n, a.r), a.r);
+    if (n.whole) load_unit<T, INTERLEAVED>(first_key, k + (c.head < heads ? c.head : 0) * D, unit_place<INTERLEAVED>(c.head < heads ? c.unit : 0, n, a.r), a.r);
 #pragma unroll
     for (int i = 0; i < 2; i++) first_values[i].load(v + 8 * min(lane + 64 * i, heads * WORDS - 1));
     uint32_t page = 0xffffffffu, t = 0;
-    const bool mine = turn_heads<T>(lane, 64, heads * group, D, n, a.r, table, [&](uint32_t h) { return q + h * D; }, [&](uint32_t h) { return q_out + h * D; }, [&] {
+    const bool mine = turn_heads<T, INTERLEAVED>(lane, 64, heads * group, D, n, a.r, table, [&](uint32_t h) { return q + h * D; }, [&](uint32_t h) { return q_out + h * D; }, [&] {
         const uint32_t s = cache_sequence(a.b, row);
         if (s >= a.b.sequences) return false;
         const CacheSpan span = cache_span(a.b, s);
@@ -300,20 +359,26 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) void append_kernel(App
         return true;
     });
     if (!mine || page >= a.b.pages) return;
-    for (bool first = n.whole; c.head < heads; c.advance(64 / n.all, 64 % n.all, n), first = false) {
-        const UnitPlace p = unit_place(c.unit, n, a.r);
+    for (bool first = true; c.head < heads; c.advance(64 / n.all, 64 % n.all, n), first = false) {
+        const UnitPlace p = unit_place<INTERLEAVED>(c.unit, n, a.r);
         Unit x;
-        if (first)
-            first_key.values(x, a.r);
-        else
+        if (n.whole) {
+            if (!first) load_unit<T, INTERLEAVED>(first_key, k + c.head * D, p, a.r);
+            first_key.values(x);
+            turn_unit<INTERLEAVED, true>(x, p, a.r, table);
+            Eight<T> y;
+            y.round(x.a);
+            T *const out = keys + c.head * D + p.first;
+            *(Eight<T> *)out = y;
+            if (p.pairs) {
+                y.round(x.b);
+                *(Eight<T> *)(out + a.r.dim / 2) = y;
+            }
+        } else {
             load_unit_tail<T>(x, k + c.head * D, p, a.r, D);
-        turn_unit(x, p, a.r, table);
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            x.a[j] = RowIO<T>::round(x.a[j]);
-            x.b[j] = RowIO<T>::round(x.b[j]);
+            turn_unit<INTERLEAVED, false>(x, p, a.r, table);
+            store_unit_tail<T>(keys + c.head * D, x, p, a.r, D);
         }
-        store_unit_tail<float>(keys + c.head * D, x, p, a.r, D);
     }
     const uint32_t head_bytes = cache_head_bytes(a.b.page_size, D);
     uint8_t *const head = a.cache + ((uint64_t)page * a.b.kv_heads + h0) * head_bytes;
@@ -328,7 +393,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) void append_kernel(App
     }
     for (uint32_t j = lane; j < heads * WORDS; j += 64) {
         float x[8];
-        RowIO<float>::load8(keys + 8 * j, x);
+        ((const Eight<T> *)(keys + 8 * j))->values(x);
         append_word<D>(head + j / WORDS * head_bytes, a.b.page_size, t, j % WORDS, false, x);
     }
 }
@@ -423,8 +488,7 @@ static const char *rotation_problem(const oco_rotation *r, uint32_t head_dim) {
     return nullptr;
 }
 static Rotation rotation_of(const oco_rotation *r) {
-    if (!r) return Rotation{nullptr, 1.0, 0, 0};
-    return Rotation{r->frequencies, r->magnitude, r->dim, r->layout == OCO_ROTATION_INTERLEAVED};
+    return r ? Rotation{r->frequencies, r->magnitude, r->dim} : Rotation{nullptr, 1.0, 0};
 }
 
 // What append and read share: 0 rows or a refusal end the call (done).
@@ -514,11 +578,18 @@ extern "C" int oco_rotate(const void *x, oco_dtype dtype, uint32_t rows, uint32_
     const dim3 grid((rows * a.parts + 3) / 4);
     const uint32_t lds = 4 * (rotation->dim / 2) * sizeof(double2);
     hipStream_t st = (hipStream_t)stream;
+#define GO(T)                                                                                                   \
+    if (rotation->layout == OCO_ROTATION_INTERLEAVED)                                                           \
+        hipLaunchKernelGGL((rotate_kernel<T, true>), grid, dim3(256), lds, st, a, rows);                        \
+    else                                                                                                        \
+        hipLaunchKernelGGL((rotate_kernel<T, false>), grid, dim3(256), lds, st, a, rows);                       \
+    break;
     switch (dtype) {
-    case OCO_DT_F32: hipLaunchKernelGGL((rotate_kernel<float>), grid, dim3(256), lds, st, a, rows); break;
-    case OCO_DT_BF16: hipLaunchKernelGGL((rotate_kernel<bf16_t>), grid, dim3(256), lds, st, a, rows); break;
-    default: hipLaunchKernelGGL((rotate_kernel<f16_t>), grid, dim3(256), lds, st, a, rows);
+    case OCO_DT_F32: GO(float)
+    case OCO_DT_BF16: GO(bf16_t)
+    default: GO(f16_t)
     }
+#undef GO
     return launch_check("oco_rotate");
 }
 
@@ -556,12 +627,19 @@ extern "C" int oco_cache_append(void *pages, const uint32_t *table, const uint32
     if ((uint64_t)p->rows * a.parts > 0x7fffffffull) return fail(OCO_ERR_INVALID, "oco_cache_append: %u rows", p->rows);
     const dim3 grid((uint32_t)(((uint64_t)p->rows * a.parts + 3) / 4));
     hipStream_t st = (hipStream_t)stream;
-#define GO(T)                                                                                               \
-    switch (p->head_dim) {                                                                                  \
-    case 64: hipLaunchKernelGGL((append_kernel<T, 64>), grid, dim3(256), 0, st, a); break;                  \
-    case 128: hipLaunchKernelGGL((append_kernel<T, 128>), grid, dim3(256), 0, st, a); break;                \
-    default: hipLaunchKernelGGL((append_kernel<T, 256>), grid, dim3(256), 0, st, a);                        \
-    }                                                                                                       \
+    const bool interleaved = rotation && rotation->layout == OCO_ROTATION_INTERLEAVED;
+#define GO2(T, D)                                                                                               \
+    if (interleaved)                                                                                            \
+        hipLaunchKernelGGL((append_kernel<T, D, true>), grid, dim3(256), 0, st, a);                             \
+    else                                                                                                        \
+        hipLaunchKernelGGL((append_kernel<T, D, false>), grid, dim3(256), 0, st, a);                            \
+    break;
+#define GO(T)                                                                                                   \
+    switch (p->head_dim) {                                                                                      \
+    case 64: GO2(T, 64)                                                                                         \
+    case 128: GO2(T, 128)                                                                                       \
+    default: GO2(T, 256)                                                                                        \
+    }                                                                                                           \
     break;
     switch (p->dtype) {
     case OCO_DT_F32: GO(float)
@@ -569,6 +647,7 @@ extern "C" int oco_cache_append(void *pages, const uint32_t *table, const uint32
     default: GO(f16_t)
     }
 #undef GO
+#undef GO2
     return launch_check("oco_cache_append");
 }
 
