@@ -28,8 +28,11 @@ __device__ __forceinline__ double2 cos_sin(double a) {
     double s = S[0], c = C[0];
 #pragma unroll
     for (int i = 1; i < 9; i++) {
-        if (i < 8) s = __builtin_fma(s, q, S[i]);
-        c = __builtin_fma(c, q, C[i]);
+        // constants in scalar registers: as vector ones they cost the callers 30, and spills
+        double si = S[i < 8 ? i : 7], ci = C[i];
+        asm("" : "+s"(si), "+s"(ci));
+        if (i < 8) s = __builtin_fma(s, q, si);
+        c = __builtin_fma(c, q, ci);
     }
     s = __builtin_fma(s * q, r, r);
     c = __builtin_fma(c, q, 1.0);
@@ -216,7 +219,7 @@ struct Cursor {
 template <class T, bool INTERLEAVED, class In, class Out, class Table>
 __device__ __forceinline__ bool turn_heads(uint32_t first, uint32_t step, uint32_t heads, uint32_t head_dim, const HeadUnits &n, const Rotation &r,
                                            const double2 *table, In in, Out out, Table make_table) {
-    constexpr int N = sizeof(T) == 4 ? 2 : 4;
+    constexpr int N = sizeof(T) == 4 ? 1 : 2;
     Cursor now(first, n);
     const uint32_t dh = step / n.all, du = step % n.all;
     if (n.whole) {
@@ -321,7 +324,7 @@ __device__ __forceinline__ void append_word(uint8_t *head, uint32_t page_size, u
 constexpr uint32_t APPEND_VALUES = 1024;  // of keys in LDS per wavefront, at most
 
 template <class T, uint32_t D, bool INTERLEAVED>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) void append_kernel(AppendArgs a) {
+__global__ __launch_bounds__(256, 4) void append_kernel(AppendArgs a) {
     __shared__ double2 tables[4][D / 2];
     __shared__ __attribute__((aligned(16))) T all_keys[4][APPEND_VALUES];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), id = blockIdx.x * 4 + wave;
