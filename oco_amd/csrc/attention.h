@@ -20,7 +20,8 @@ struct AttentionArgs {
     float *parts;  // [rows][heads][chunks][D], then m and l [rows][heads][chunks][2]
     uint64_t q_stride, out_stride;
     uint32_t heads, group, window;
-    uint32_t chunks, chunk;  // parts of the tokens, each of `chunk` tokens
+    uint32_t tile_rows;      // rows of a tile
+    uint32_t chunks, chunk;  // parts of a tile's tokens, each of `chunk` tokens
     float c;                 // scale * log2(e)
 };
 
@@ -89,10 +90,24 @@ __device__ __forceinline__ float row_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// The tokens that any row of a sequence sees: from .. length, from a multiple of 32.
-__device__ __forceinline__ uint32_t first_seen(const CacheSpan &s, uint32_t window) {
-    const uint32_t p = s.length > s.rows ? s.length - s.rows : 0;
-    return window && p + 1 > window ? (p + 1 - window) / 32 * 32 : 0;
+// A tile of a sequence's rows (a token's query heads of one key-value head
+// after the other): its rows, their first and last positions and the tokens
+// that any of them sees, from a multiple of 32 on.
+struct AttentionTile {
+    uint32_t first_row, rows;  // rows: of the sequence
+    int32_t least, most;
+    uint32_t first, end;
+};
+__device__ __forceinline__ AttentionTile attention_tile(const CacheSpan &s, uint32_t tile, uint32_t tile_rows, uint32_t group, uint32_t window) {
+    AttentionTile t;
+    t.first_row = tile * tile_rows;
+    t.rows = s.rows * group;
+    const int32_t before = (int32_t)s.length - (int32_t)s.rows;
+    t.least = before + (int32_t)(t.first_row / group);
+    t.most = before + (int32_t)((min(t.first_row + tile_rows, max(t.rows, 1u)) - 1) / group);
+    t.first = window && t.least >= (int32_t)window ? ((uint32_t)t.least + 1 - window) / 32 * 32 : 0;
+    t.end = t.most < 0 ? 0 : (uint32_t)t.most + 1;
+    return t;
 }
 
 // exp2 of m - to, 0 for m = -Inf whatever `to` is.
@@ -102,9 +117,9 @@ __device__ __forceinline__ float carry(float m, float to) { return m > -INFINITY
 // which no block has).
 __device__ __forceinline__ uint32_t bytes_255(uint32_t x) { return (~x - 0x01010101u) & x & 0x80808080u; }
 
-// Prompt chunks (attention_prompt.hip): rows of a tile, tokens of a step.
+// Prompts (attention_prompt.hip; heads of 64 and 128): rows of a tile, tokens of a step.
 constexpr uint32_t PROMPT_ROWS = 128;
-constexpr uint32_t prompt_step(uint32_t d) { return d == 256 ? 32 : 64; }
+constexpr uint32_t PROMPT_STEP = 64;
 int attention_prompt_launch(const AttentionArgs &a, uint32_t head_dim, bool bf, uint32_t tiles, uint32_t grid, hipStream_t stream);
 
 }  // namespace oco

@@ -61,14 +61,17 @@ struct Places {
         value = page_size * (D / 2) + g * (2 * D) + m * (D / 8);
         value_scale = page_size * D + page_size * (D / 32) + g * (D / 8) + m * D / 512 * 4;
     }
-    __device__ __forceinline__ void load(Keys<D> &k, Values<D> &v, gbytes head, uint32_t slot) const {
+    __device__ __forceinline__ void load(Keys<D> &k, gbytes head, uint32_t slot) const {
         load_words<D>(k.w, head + slot * (D / 2), key);
         const gbytes s = head + slot * (D / 32);
         k.scale = D == 256 ? *(const GLOBAL uint16_t *)(s + key_scale) : s[key_scale];
+    }
+    __device__ __forceinline__ void load(Values<D> &v, gbytes head, uint32_t slot) const {
         load_words<D>(v.w, head + slot * (D / 2), value);
-        v.scale = *(const GLOBAL uint32_t *)(s + value_scale);
+        v.scale = *(const GLOBAL uint32_t *)(head + slot * (D / 32) + value_scale);
     }
 };
+
 // The halves of a wavefront's steps, their pages and their places in them: a
 // lane per half, read once for 32 steps, so that a step's loads do not wait
 // for the table.
@@ -84,7 +87,7 @@ __device__ __forceinline__ Halves load_halves(const uint32_t *table, uint32_t t0
 }
 
 template <uint32_t D, bool BF, int R>
-__global__ __launch_bounds__(256, (D / 64) * R == 1 ? 4 : (D / 64) * R == 2 ? 3 : 2) void attention_kernel(AttentionArgs a, uint32_t tiles) {
+__global__ __launch_bounds__(256, D * R == 64 ? 4 : D * R == 128 ? 3 : 2) void attention_kernel(AttentionArgs a, uint32_t tiles) {
     constexpr int KW = D / 32, NT = D / 16;  // key words per lane and token; tiles of 16 columns
     using H = Half<BF>;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
@@ -96,19 +99,15 @@ __global__ __launch_bounds__(256, (D / 64) * R == 1 ? 4 : (D / 64) * R == 2 ? 3 
     id /= a.chunks;
     const uint32_t s = id % a.b.sequences, tile = tiles - 1 - id / a.b.sequences;
     const CacheSpan span = cache_span(a.b, s);
-    const uint32_t row0 = tile * (16 * R), rows = span.rows * a.group;
+    const AttentionTile range = attention_tile(span, tile, 16 * R, a.group, a.window);
+    const uint32_t row0 = range.first_row, rows = range.rows;
     if (row0 >= rows) return;
-    const uint32_t last_row = min(row0 + 16 * R, rows) - 1;
-    const int32_t least = (int32_t)(span.length + row0 / a.group) - (int32_t)span.rows;
-    const int32_t most = (int32_t)(span.length + last_row / a.group) - (int32_t)span.rows;
-    // this chunk's tokens
-    const uint32_t base = first_seen(span, a.window) + chunk * a.chunk;
-    if (chunk && base >= span.length) return;  // the sequence has fewer chunks
-    const uint32_t end = most < 0 ? 0 : min(min(base + a.chunk, span.length), (uint32_t)most + 1);
+    const int32_t least = range.least, most = range.most;
+    const uint32_t first = range.first + chunk * a.chunk, end = min(first + a.chunk, range.end);  // this chunk's tokens
+    if (chunk && first >= range.end) return;  // the tile has fewer chunks
     const uint32_t head_bytes = cache_head_bytes(a.b.page_size, D);
     const uint32_t *const table = a.b.table + (uint64_t)s * a.b.table_stride;
-    const uint32_t low = a.window && least >= (int32_t)a.window ? ((uint32_t)least + 1 - a.window) / 32 * 32 : 0;  // the tile's first token
-    uint32_t t0 = max(base, low) + 32 * wave, step = 0;
+    uint32_t t0 = first + 32 * wave, step = 0;
     Halves halves = load_halves(table, t0, 128, end, a.b.page_size);
     // the rows' positions (-1: no token, and no row)
     int32_t at[R];
@@ -142,30 +141,43 @@ __global__ __launch_bounds__(256, (D / 64) * R == 1 ? 4 : (D / 64) * R == 2 ? 3 
 #pragma unroll
         for (int j = 0; j < NT; j++) o[r][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    // a step's tokens are requested before the step before it is computed
+    // A step's tokens are requested before the step before it is computed; where that does not leave the
+    // registers for it (STAGED), the keys once that step's are used up, and its values likewise.
+    constexpr bool STAGED = D * R >= 512;  // 256 wide, 32 rows
     struct Step {
         Keys<D> k[2];
         Values<D> v[2];
+        gbytes head[2];
+        uint32_t slot[2];
         bool lost[2];  // not in the pool
     };
     const Places<D> places(a.b.page_size);
-    auto request = [&](Step &x) {  // of step `step`
+    auto request_keys = [&](Step &x) {  // of step `step`
         if (step && step % 32 == 0) halves = load_halves(table, t0, 128, end, a.b.page_size);
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)halves.page, 2 * (step % 32) + e);
-            const uint32_t slot = (uint32_t)__builtin_amdgcn_readlane((int)halves.slot, 2 * (step % 32) + e);
+            x.slot[e] = (uint32_t)__builtin_amdgcn_readlane((int)halves.slot, 2 * (step % 32) + e);
             x.lost[e] = page >= a.b.pages;
             page = x.lost[e] ? 0 : page;
-            places.load(x.k[e], x.v[e], (gbytes)gp(a.cache) + ((uint64_t)page * a.b.kv_heads + h) * head_bytes, slot);
+            x.head[e] = (gbytes)gp(a.cache) + ((uint64_t)page * a.b.kv_heads + h) * head_bytes;
+            places.load(x.k[e], x.head[e], x.slot[e]);
         }
         step++;
         t0 += 128;
     };
-    auto compute = [&](Step &x, const uint32_t t0) {
+    auto request_values = [&](Step &x) {
+#pragma unroll
+        for (int e = 0; e < 2; e++) places.load(x.v[e], x.head[e], x.slot[e]);
+    };
+    auto request = [&](Step &x) {
+        request_keys(x);
+        request_values(x);
+    };
+    auto compute = [&](Step &x, const uint32_t now) {
         Keys<D>(&k)[2] = x.k;
         Values<D>(&v)[2] = x.v;
-        const bool(&lost)[2] = x.lost;
+        const bool lost[2] = {x.lost[0], x.lost[1]}, more = now + 128 < end;
         // scores: lane (n, g) has row n's tokens 16 e + 4 g + i
         f32x4 sc[R][2];
 #pragma unroll
@@ -189,15 +201,19 @@ __global__ __launch_bounds__(256, (D / 64) * R == 1 ? 4 : (D / 64) * R == 2 ? 3 
 #pragma unroll
                 for (int e = 0; e < 2; e++) sc[r][e] = H::product(x[e], f, sc[r][e]);
             }
+            if constexpr (STAGED)
+                if (w % 2) __builtin_amdgcn_sched_barrier(0);
         }
-        const bool edge = (int32_t)t0 + 31 > least || (a.window && (int32_t)t0 + (int32_t)a.window <= most);
+        if constexpr (STAGED)
+            if (more) request_keys(x);
+        const bool edge = (int32_t)now + 31 > least || (a.window && (int32_t)now + (int32_t)a.window <= most);
         u32x4 p[R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
             if (edge) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const int32_t t = (int32_t)t0 + 16 * (i / 4) + 4 * (int32_t)g + i % 4;
+                    const int32_t t = (int32_t)now + 16 * (i / 4) + 4 * (int32_t)g + i % 4;
                     if (!(t <= at[r] && (!a.window || t + (int32_t)a.window > at[r]))) sc[r][i / 4][i % 4] = -INFINITY;
                 }
             }
@@ -237,7 +253,7 @@ __global__ __launch_bounds__(256, (D / 64) * R == 1 ? 4 : (D / 64) * R == 2 ? 3 
                 u32x4 sees;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const int32_t t = (int32_t)t0 + 16 * (i / 4) + 4 * (int32_t)g + i % 4;
+                    const int32_t t = (int32_t)now + 16 * (i / 4) + 4 * (int32_t)g + i % 4;
                     const uint32_t one = t <= at[r] && (!a.window || t + (int32_t)a.window > at[r]) ? H::ONE : 0;
                     sees[i / 2] = i % 2 ? sees[i / 2] | one << 16 : one;
                 }
@@ -272,16 +288,24 @@ __global__ __launch_bounds__(256, (D / 64) * R == 1 ? 4 : (D / 64) * R == 2 ? 3 
                 o[r][2 * b] = H::product(lo, p[r], o[r][2 * b]);
                 o[r][2 * b + 1] = H::product(hi, p[r], o[r][2 * b + 1]);
             }
+            if constexpr (STAGED) __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (STAGED)
+            if (more) request_values(x);
     };
     Step x, y;
     if (t0 < end) request(x);
-    for (uint32_t now = max(base, low) + 32 * wave; now < end; now += 256) {
-        if (t0 < end) request(y);
+    for (uint32_t now = first + 32 * wave; now < end; now += 256) {
+        if constexpr (!STAGED)
+            if (t0 < end) request(y);
         compute(x, now);
         if (now + 128 >= end) break;
-        if (t0 < end) request(x);
-        compute(y, now + 128);
+        if constexpr (!STAGED) {
+            if (t0 < end) request(x);
+            compute(y, now + 128);
+        } else {
+            compute(x, now + 128);
+        }
     }
     // The four wavefronts' parts: each writes all of its own and joins a quarter, NT consecutive
     // columns of every lane's row.
@@ -349,7 +373,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
     if (s >= a.b.sequences) return;
     const CacheSpan span = cache_span(a.b, s);
     if (row - span.first >= span.rows) return;
-    const uint32_t from = first_seen(span, a.window), used = span.length > from ? (span.length - from + a.chunk - 1) / a.chunk : 0;
+    const AttentionTile range = attention_tile(span, ((row - span.first) * a.group + head % a.group) / a.tile_rows, a.tile_rows, a.group, a.window);
+    const uint32_t used = range.end > range.first ? (range.end - range.first + a.chunk - 1) / a.chunk : 0;
     const uint64_t index = (uint64_t)blockIdx.x * a.chunks;
     const float *const ml = a.parts + (uint64_t)a.b.rows * a.heads * a.chunks * D + index * 2;
     const f32x4 *const parts = (const f32x4 *)(a.parts + index * D) + lane * V;
@@ -394,18 +419,36 @@ struct AttentionPlan {
 static AttentionPlan attention_plan(const oco_cache *p) {
     AttentionPlan l;
     const uint64_t rows = (uint64_t)p->max_rows * (p->heads / p->kv_heads);
+    // Tiles of 16 rows while that is all, of 32 beyond (of 16 where the second one would be half empty).  With narrow heads
+    // tiles of 128 of the prompts' kernel from 256 of them on, one per compute unit.  us, tiles of 16 / 32 / 128:
+    // 32 sequences of 5 x 4 rows over 8000 tokens, 128 wide 115 / 84 / 141; 8 of 5 x 8 rows, 64 wide 20.7 / 22.1 / 33;
+    // 4 of 128 x 4 rows over 2000 (128 tiles) 41 / 33 / 49, 16 of 64 x 4 over 4000 (256 tiles) 142 / 108 / 86, 64 of 32 x 4
+    // over 1000 (512) 92 / 75 / 49; 1000 x 4 rows from the start on (256) 26 / 24 / 28; 4096 x 4 rows over 8192 722 / 569 /
+    // 392, 256 wide (16 heads) 623 / 443 / 715.
     int32_t knob[4];
     const int set = plan_override(OCO_KNOB_ATTENTION, knob);
-    l.tile = rows <= 16 ? 1 : rows <= 64 ? 1 : PROMPT_ROWS / 16;
-    if (set && (knob[0] == 1 || knob[0] == 2 || (knob[0] == 4 && p->head_dim < 256) || knob[0] == (int)PROMPT_ROWS / 16)) l.tile = (uint32_t)knob[0];
+    const bool narrow = p->head_dim <= 128;
+    const uint64_t wide_tiles = (rows + PROMPT_ROWS - 1) / PROMPT_ROWS * p->kv_heads * p->sequences;
+    l.tile = rows <= 16 || (rows > 32 && rows <= 48) ? 1 : 2;
+    if (narrow && rows >= PROMPT_ROWS && wide_tiles >= 256) l.tile = PROMPT_ROWS / 16;
+    if (set && (knob[0] == 1 || knob[0] == 2 || (knob[0] == (int)PROMPT_ROWS / 16 && narrow))) l.tile = (uint32_t)knob[0];
     l.tiles = (uint32_t)((rows + 16 * l.tile - 1) / (16 * l.tile));
+    // the most tokens that a tile sees
+    const uint64_t tile_tokens = (16 * l.tile + p->heads / p->kv_heads - 1) / (p->heads / p->kv_heads);
     uint64_t seen = p->max_length;
-    if (p->window && (uint64_t)p->window + p->max_rows + 31 < seen) seen = (uint64_t)p->window + p->max_rows + 31;
+    if (p->window && p->window + tile_tokens + 31 < seen) seen = p->window + tile_tokens + 31;
     const uint64_t blocks = (uint64_t)p->sequences * p->kv_heads * l.tiles;
     const bool prompt = l.tile == PROMPT_ROWS / 16;
+    // Chunks until the card is full: 3072 workgroups of few rows, of at least two steps per wavefront (32 sequences of up to
+    // 16384 tokens: 1152 to 2048 tokens a chunk 75 to 78 us, 4096 74 to 95 by how they divide, 256 104; one of 4101: 256
+    // tokens 9.2, 512 10.9), 512 of a prompt's tiles.
     const uint64_t wanted = prompt ? 512 : 3072;
     uint64_t chunks = blocks ? (wanted + blocks - 1) / blocks : 1;
-    const uint64_t least = prompt ? 512 : 256, most = (seen + least - 1) / least;
+    const uint64_t least = prompt ? 512 : 256;
+    uint64_t most = (seen + least - 1) / least;
+    // what the chunks write and the join reads, in proportion to the rows: 16 MB at most
+    const uint64_t part = (uint64_t)p->rows * p->heads * (p->head_dim + 2) * 4;
+    if (part && (16ull << 20) / part < most) most = (16ull << 20) / part;
     if (chunks > most) chunks = most;
     if (chunks < 1) chunks = 1;
     l.chunk = (uint32_t)(((seen + chunks - 1) / chunks + 127) / 128 * 128);
@@ -417,21 +460,16 @@ static AttentionPlan attention_plan(const oco_cache *p) {
     return l;
 }
 
-// Which kernel: by the rows of a sequence and key-value head.
-static bool attention_is_prompt(const AttentionPlan &l) { return l.tile == PROMPT_ROWS / 16; }
-
 template <uint32_t D, bool BF>
 static int attention_launch(const AttentionArgs &a, const AttentionPlan &l, hipStream_t stream) {
     const uint64_t grid = (uint64_t)a.b.sequences * a.b.kv_heads * l.tiles * l.chunks;
     if (grid > 0x7fffffffull) return fail(OCO_ERR_INVALID, "oco_cache_attention: too many rows for one call");
-    if (attention_is_prompt(l)) {
-        OCO_TRY(attention_prompt_launch(a, D, BF, l.tiles, (uint32_t)grid, stream));
-    } else if (l.tile == 1)
+    if (l.tile == 1)
         hipLaunchKernelGGL((attention_kernel<D, BF, 1>), dim3((uint32_t)grid), dim3(256), 0, stream, a, l.tiles);
     else if (l.tile == 2)
         hipLaunchKernelGGL((attention_kernel<D, BF, 2>), dim3((uint32_t)grid), dim3(256), 0, stream, a, l.tiles);
-    else if constexpr (D < 256)
-        hipLaunchKernelGGL((attention_kernel<D, BF, 4>), dim3((uint32_t)grid), dim3(256), 0, stream, a, l.tiles);
+    else
+        OCO_TRY(attention_prompt_launch(a, D, BF, l.tiles, (uint32_t)grid, stream));
     OCO_TRY(launch_check("oco_cache_attention"));
     if (l.chunks > 1) {
         hipLaunchKernelGGL((attention_join_kernel<D, BF>), dim3(a.b.rows * a.heads), dim3(256), 0, stream, a);
@@ -482,6 +520,7 @@ extern "C" int oco_cache_attention(const void *q, const void *pages, const uint3
     a.heads = p->heads;
     a.group = p->heads / p->kv_heads;
     a.window = p->window >= p->max_length ? 0 : p->window;
+    a.tile_rows = 16 * l.tile;
     a.chunks = l.chunks;
     a.chunk = l.chunk;
     a.c = (p->scale != 0.f ? p->scale : 1.f / sqrtf((float)p->head_dim)) * 1.44269504088896341f;

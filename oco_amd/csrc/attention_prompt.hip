@@ -1,7 +1,7 @@
 // Attention over the paged cache for many rows: the matrix cores' side.
 //
 // A workgroup's four wavefronts hold 32 rows each and share steps of 64 tokens
-// (32 of wide heads), whose codes are converted once for all of them into LDS:
+// whose codes are converted once for all of them into LDS:
 // keys as rows, values transposed, so that both products read 16 bytes per
 // lane.  Two buffers, one barrier per step: the next step's codes are on their
 // way while this one is computed.  As in the kernel for few rows a lane is a
@@ -14,9 +14,9 @@
 namespace oco {
 
 template <uint32_t D, bool BF>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel(AttentionArgs a, uint32_t tiles) {
+__global__ __launch_bounds__(256, 2) void attention_prompt_kernel(AttentionArgs a, uint32_t tiles) {
     using H = Half<BF>;
-    constexpr uint32_t KT = prompt_step(D), HALVES = KT / 16;  // tokens of a step; wavefronts per 16 tokens: 4 / HALVES
+    constexpr uint32_t KT = PROMPT_STEP;
     constexpr int KN = KT / 32, NS = D / 16, NO = D / 32;       // key tiles, key steps, column tiles
     constexpr uint32_t PIECE = D / 16;                          // columns of a value's piece
     // rows of 16-byte pieces, one piece of padding: eight consecutive rows fall into different banks
@@ -32,19 +32,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
     id /= a.chunks;
     const uint32_t s = id % a.b.sequences, tile = tiles - 1 - id / a.b.sequences;
     const CacheSpan span = cache_span(a.b, s);
-    const uint32_t tile0 = tile * PROMPT_ROWS, rows = span.rows * a.group;
-    if (tile0 >= rows) return;
+    const AttentionTile range = attention_tile(span, tile, PROMPT_ROWS, a.group, a.window);
+    const uint32_t rows = range.rows;
+    if (range.first_row >= rows) return;
     const int32_t before = (int32_t)span.length - (int32_t)span.rows;
-    const int32_t tile_least = before + (int32_t)(tile0 / a.group), tile_most = before + (int32_t)((min(tile0 + PROMPT_ROWS, rows) - 1) / a.group);
-    const uint32_t base = first_seen(span, a.window) + chunk * a.chunk;
-    if (chunk && base >= span.length) return;
-    const uint32_t low = a.window && tile_least >= (int32_t)a.window ? ((uint32_t)tile_least + 1 - a.window) / 32 * 32 : 0;
-    const uint32_t first = max(base, low), end = tile_most < 0 ? 0 : min(min(base + a.chunk, span.length), (uint32_t)tile_most + 1);
+    const uint32_t first = range.first + chunk * a.chunk, end = min(first + a.chunk, range.end);
+    if (chunk && first >= range.end) return;
     const uint32_t head_bytes = cache_head_bytes(a.b.page_size, D);
     const uint32_t *const table = a.b.table + (uint64_t)s * a.b.table_stride;
 
     // this lane's row
-    const uint32_t row0 = tile0 + 32 * wave, i0 = row0 + n;
+    const uint32_t row0 = range.first_row + 32 * wave, i0 = row0 + n;
     const bool live = i0 < rows;
     const uint32_t token = live ? i0 / a.group : 0, head = h * a.group + (live ? i0 % a.group : 0);
     const int32_t at = live ? before + (int32_t)token : -1;
@@ -63,16 +61,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
         for (int i = 0; i < 16; i++) o[j][i] = 0.f;
 
     // ---- converting: a thread's share of a step
-    const uint32_t half = wave * HALVES / 4;
+    const uint32_t half = wave;  // the 16 tokens that this wavefront converts
     constexpr uint32_t KB = D == 64 ? 8 : 16, KPIECES = D / 2 / KB;  // bytes of a key per thread, threads per key
     const uint32_t kt = threadIdx.x / KPIECES, kp = threadIdx.x % KPIECES;
-    const uint32_t vu = D == 256 ? threadIdx.x / 2 : threadIdx.x, vg = vu / 16, vm = vu % 16;  // four tokens, a piece (D = 256: half of it)
+    const uint32_t vg = threadIdx.x / 16, vm = threadIdx.x % 16;  // four tokens, a piece
     struct Raw {
         uint32_t w[4], scale;
         bool lost;
     };
     const uint32_t k_at = kt % 16 * (D / 2) + kp * KB, ks_at = a.b.page_size * D + kt % 16 * (D / 32) + kp * KB / 16;
-    const uint32_t v_at = a.b.page_size * (D / 2) + vg % 4 * (2 * D) + vm * (D / 8) + (D == 256 ? threadIdx.x % 2 * 4 : 0);
+    const uint32_t v_at = a.b.page_size * (D / 2) + vg % 4 * (2 * D) + vm * (D / 8);
     const uint32_t vs_at = a.b.page_size * D + a.b.page_size * (D / 32) + vg % 4 * (D / 8) + vm * D / 512 * 4;
     uint32_t page_of = 0, slot_of = 0;  // lane i: of step 64 c + i
     auto read_table = [&](uint32_t step) {
@@ -115,13 +113,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
             const u32x2 v = *(const GLOBAL u32x2 *)(words + v_at);
             x.w[0] = v.x;
             x.w[1] = v.y;
-        } else if constexpr (D == 128) {
+        } else {
             const u32x4 v = *(const GLOBAL u32x4 *)(words + v_at);
 #pragma unroll
             for (int i = 0; i < 4; i++) x.w[i] = v[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++) x.w[i] = *(const GLOBAL uint32_t *)(words + v_at + 8 * i);
         }
         x.scale = *(const GLOBAL uint32_t *)(p.head + p.slot * (D / 32) + vs_at);
         x.lost = p.lost;
@@ -145,7 +140,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
         for (int i = 0; i < 4; i++) scale[i] = __uint_as_float(byte_of(vs, i) << 23);
         // column PIECE m + c is in row 16 c + m; groups of four tokens of 16 in the order 0, 2, 1, 3
         u32x2 *const out = (u32x2 *)&values[into][0] + (vg / 4 * 4 + vg % 2 * 2 + vg % 4 / 2);
-        const uint32_t c0 = D == 256 ? threadIdx.x % 2 * 8 : 0;
 #pragma unroll
         for (int b = 0; b < (D == 64 ? 2 : 4); b++) {
             uint32_t c[4];
@@ -156,8 +150,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_prompt_kernel
                 c[i] = byte == 0 ? H::template pair<0>(w, scale[i]) : byte == 1 ? H::template pair<1>(w, scale[i])
                      : byte == 2 ? H::template pair<2>(w, scale[i]) : H::template pair<3>(w, scale[i]);
             }
-            out[((c0 + 2 * b) * 16 + vm) * (2 * VROW)] = low_halves(c);
-            out[((c0 + 2 * b + 1) * 16 + vm) * (2 * VROW)] = high_halves(c);
+            out[(2 * b * 16 + vm) * (2 * VROW)] = low_halves(c);
+            out[((2 * b + 1) * 16 + vm) * (2 * VROW)] = high_halves(c);
         }
     };
     auto scores = [&](f32x16 *sc, uint32_t from) {
@@ -349,10 +343,10 @@ int attention_prompt_launch(const AttentionArgs &a, uint32_t head_dim, bool bf, 
         hipLaunchKernelGGL((attention_prompt_kernel<D, true>), dim3(grid), dim3(256), 0, stream, a, tiles);               \
     else                                                                                                                  \
         hipLaunchKernelGGL((attention_prompt_kernel<D, false>), dim3(grid), dim3(256), 0, stream, a, tiles);
-    switch (head_dim) {
-    case 64: GO(64) break;
-    case 128: GO(128) break;
-    default: GO(256)
+    if (head_dim == 64) {
+        GO(64)
+    } else {
+        GO(128)
     }
 #undef GO
     return launch_check("oco_cache_attention (prompt)");

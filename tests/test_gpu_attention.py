@@ -286,7 +286,7 @@ def test_shorter_bounds(lib):
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
-@pytest.mark.parametrize("tile", [1, 2, 4, 8])
+@pytest.mark.parametrize("tile", [1, 2, 8])
 @pytest.mark.parametrize("chunk", [0, 128, 384])
 def test_every_kernel_and_chunk(lib, d, tile, chunk):
     """Each kernel on few and many rows, whole and in chunks, with windows that begin inside a step."""
