@@ -9,6 +9,7 @@ the reference's operator seam so callers and tests read like oco's own:
 - ``DenseMatrix`` (apply_row / apply)   -> src/weights/operands.rs:4-9, compute/matrix.rs:63,130
 - ``Output``                            -> compute/matrix.rs:519-548 (f32 logits)
 - ``ExpertBank`` / ``Router``           -> operands.rs ExpertWeight/Router, feed_forward.rs:107
+- ``PagedCache`` / ``CacheBatch``       -> keys and values in 4-bit pages, and the attention over them
 
 There is no CPU fallback: every compute call goes through the HIP library,
 and loading fails loudly when the library is missing.
@@ -961,6 +962,74 @@ class Fp8Matrix:
         """The workspace of calls of 1 to `rows` rows on a stream (the need
         does not rise with the rows throughout), which then draw no memory."""
         need = max((fp8_matmul_workspace(Matrix(self.input, self.output, m, 0, 1, 1, 0)) for m in range(1, rows + 1)), default=0)
+        if need:
+            self._scratch(stream).at_least(need)
+
+    def _scratch(self, stream) -> Scratch:
+        if isinstance(stream, Stream):
+            return stream.scratch
+        return self._scratches.setdefault(getattr(stream, "value", stream), Scratch())
+
+
+class PagedCache:
+    """A pool of pages with keys and values in 4 bits (oco_cache), and the calls on it.
+
+    A batch is described once and kept: ``batch(table, lengths, ...)`` binds the
+    sequences' pages and lengths to the pool, and append, read and attention
+    take their rows from it."""
+
+    def __init__(self, pages: int, head_dim: int, kv_heads: int, page_size: int = 64, buffer=None):
+        self.pages, self.head_dim, self.kv_heads, self.page_size = pages, head_dim, kv_heads, page_size
+        page = cache_page_bytes(Cache(head_dim=head_dim, kv_heads=kv_heads, page_size=page_size))
+        if page == 0:
+            raise ValueError(f"no cache of {kv_heads} heads of {head_dim} in pages of {page_size} tokens")
+        self.buffer = DeviceBuffer(pages * page) if buffer is None else buffer
+
+    def batch(self, table, lengths, sequences: int, rows: int, max_rows: int, max_length: int, table_stride: int, heads: int,
+              starts=None, dtype=DType.BF16, window: int = 0, scale: float = 0.0) -> "CacheBatch":
+        p = Cache(head_dim=self.head_dim, heads=heads, kv_heads=self.kv_heads, page_size=self.page_size, pages=self.pages,
+                  sequences=sequences, rows=rows, max_rows=max_rows, max_length=max_length, table_stride=table_stride,
+                  dtype=int(dtype), window=window, scale=scale)
+        return CacheBatch(self, p, table, starts, lengths)
+
+
+class CacheBatch:
+    """The rows of a step on a PagedCache."""
+
+    def __init__(self, cache: PagedCache, p: Cache, table, starts, lengths):
+        self.cache, self.p, self.table, self.starts, self.lengths = cache, p, table, starts, lengths
+        self._scratches = {}  # of streams that are given by their handle
+
+    def append(self, k, v, q=None, q_out=None, positions=None, rotation=None, stride: int = 0, stream=None):
+        """Keys (turned) and values into the pages, queries turned into q_out (q
+        by default).  stride: between the rows of q, k and v where they lie
+        together, as one product writes them (q_out's stay head after head)."""
+        p = self.p
+        if stride:
+            p = Cache.from_buffer_copy(p)
+            p.q_stride = p.k_stride = p.v_stride = stride
+        cache_append(self.cache.buffer, self.table, self.lengths, k, v, p, self.starts, q, q_out, positions, rotation, stream)
+
+    def read(self, k, v, stream=None):
+        """The rows' keys and values as the pages hold them."""
+        cache_read(self.cache.buffer, self.table, self.lengths, k, v, self.p, self.starts, stream)
+
+    def attention(self, q, out, sinks=None, workspace=None, stream=None):
+        """Causal attention of the rows.  Without a `workspace` (a DeviceBuffer
+        of workspace_bytes()) a Stream keeps one, and the batch one for each
+        stream that is given by its handle and for the default one; reserve()
+        draws it before a capture."""
+        need = self.workspace_bytes()
+        if need and workspace is None:
+            workspace = self._scratch(stream).at_least(need)
+        cache_attention(q, self.cache.buffer, self.table, self.lengths, out, self.p, self.starts, sinks, workspace if need else None,
+                        workspace.nbytes if need else 0, stream)
+
+    def workspace_bytes(self) -> int:
+        return cache_attention_workspace(self.p)
+
+    def reserve(self, stream=None):
+        need = self.workspace_bytes()
         if need:
             self._scratch(stream).at_least(need)
 

@@ -10,6 +10,13 @@ pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 
 
+@pytest.fixture(params=[0, 8], ids=["", "prompt"])
+def kernel(request, lib):
+    """The kernel that the rule takes, and the one of long prompts (which heads of 256 do not have)."""
+    with lib.overridden(lib.Knob.ATTENTION, (request.param,)):
+        yield request.param
+
+
 class Case:
     def __init__(self, lib, rng, rows, lengths, heads, kv, d, P, dtype, window=0, sinks=False, extra_rows=0, pad=(0, 0), q_scale=2.0, scale=0.0,
                  holes=0, max_rows=None, v_scale=1.0):
@@ -95,7 +102,7 @@ class Case:
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("rows,lengths", [([1], [1]), ([1], [2]), ([1, 1, 1, 1], [15, 16, 17, 33]), ([1, 1], [500, 1300]), ([3, 0, 5], [40, 7, 300]),
                                           ([4], [4]), ([40, 1], [90, 260])])
-def test_lengths(lib, dtype, d, rows, lengths):
+def test_lengths(kernel, lib, dtype, d, rows, lengths):
     rng = np.random.default_rng(d + sum(lengths))
     say("attention", dtype, d, rows, lengths)
     c = Case(lib, rng, rows, lengths, 4, 2, d, 16, dtype)
@@ -106,7 +113,7 @@ def test_lengths(lib, dtype, d, rows, lengths):
 
 @pytest.mark.parametrize("heads,kv", [(1, 1), (3, 3), (5, 1), (14, 2), (16, 1), (17, 1), (32, 1), (40, 8), (72, 2)])
 @pytest.mark.parametrize("rows", [1, 3])
-def test_heads(lib, heads, kv, rows):
+def test_heads(kernel, lib, heads, kv, rows):
     """Groups of one head to more than a tile of rows."""
     rng = np.random.default_rng(heads * 10 + rows)
     say("attention", heads, kv, rows)
@@ -118,7 +125,7 @@ def test_heads(lib, heads, kv, rows):
 
 @pytest.mark.parametrize("P", [16, 32, 48, 64, 256])
 @pytest.mark.parametrize("window", [0, 1, 16, 31, 100, 5000])
-def test_windows_and_pages(lib, P, window):
+def test_windows_and_pages(kernel, lib, P, window):
     rng = np.random.default_rng(P + window)
     say("attention", P, window)
     for rows, lengths in (([1, 4, 2], [333, 64, 1]), ([65, 20], [200, 20])):
@@ -130,7 +137,7 @@ def test_windows_and_pages(lib, P, window):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("rows,lengths", [([1, 1], [50, 2100]), ([6, 3], [6, 700]), ([80], [160])])
-def test_sinks(lib, dtype, rows, lengths):
+def test_sinks(kernel, lib, dtype, rows, lengths):
     rng = np.random.default_rng(7)
     say("sinks", dtype, rows)
     c = Case(lib, rng, rows, lengths, 6, 2, 128, 64, dtype, sinks=True, q_scale=0.5)
@@ -142,7 +149,7 @@ def test_sinks(lib, dtype, rows, lengths):
 
 
 @pytest.mark.parametrize("sinks", [False, True])
-def test_rows_that_see_nothing(lib, sinks):
+def test_rows_that_see_nothing(kernel, lib, sinks):
     """Sequences without tokens, and with fewer tokens than rows: zeros; rows behind the last sequence stay."""
     rng = np.random.default_rng(2)
     for rows, lengths in (([1, 2, 5], [0, 0, 3]), ([90, 40], [30, 0])):
@@ -159,7 +166,7 @@ def test_rows_that_see_nothing(lib, sinks):
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("rows,lengths,window", [([1, 8], [300, 40], 0), ([4, 3], [60, 200], 24), ([70, 33], [140, 33], 0), ([100], [150], 40)])
-def test_blocks_of_nan(lib, dtype, d, rows, lengths, window):
+def test_blocks_of_nan(kernel, lib, dtype, d, rows, lengths, window):
     """A NaN reaches the rows that see it, a value's in its own 32 columns, and no other row: not those before it, not those
     whose window has passed it."""
     rng = np.random.default_rng(d + sum(rows))
@@ -172,7 +179,7 @@ def test_blocks_of_nan(lib, dtype, d, rows, lengths, window):
 
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("rows", [5, 60])
-def test_nan_in_the_last_token(lib, d, rows):
+def test_nan_in_the_last_token(kernel, lib, d, rows):
     """Only the last row sees it: a value's NaN its block of columns, a key's all of them."""
     rng = np.random.default_rng(d)
     for in_key in (False, True):
@@ -191,7 +198,7 @@ def test_nan_in_the_last_token(lib, d, rows):
         np.testing.assert_array_equal(got, want)
 
 
-def test_pages_outside_the_pool(lib):
+def test_pages_outside_the_pool(kernel, lib):
     """They read as NaN where a row sees them, and nothing is read there."""
     rng = np.random.default_rng(12)
     for rows, lengths in (([1, 1], [100, 60]), ([40, 3], [100, 60])):
@@ -207,7 +214,7 @@ def test_pages_outside_the_pool(lib):
 
 
 @pytest.mark.parametrize("rows,lengths", [([2, 2, 2], [90, 5, 400]), ([30, 30], [30, 77])])
-def test_strides_and_no_starts(lib, rows, lengths):
+def test_strides_and_no_starts(kernel, lib, rows, lengths):
     rng = np.random.default_rng(5)
     c = Case(lib, rng, rows, lengths, 6, 2, 64, 32, "f16", pad=(6, 10), scale=0.2)
     say("strides", rows)
@@ -220,7 +227,7 @@ def test_strides_and_no_starts(lib, rows, lengths):
 
 
 @pytest.mark.parametrize("rows", [[1], [130]])
-def test_scores_that_rise_and_fall(lib, rows):
+def test_scores_that_rise_and_fall(kernel, lib, rows):
     """Maxima that come early, late and in between, scores over a range of hundreds."""
     rng = np.random.default_rng(6)
     for order in (1, -1, 0):
@@ -240,7 +247,7 @@ def test_scores_that_rise_and_fall(lib, rows):
         c.check()
 
 
-def test_infinite_queries(lib):
+def test_infinite_queries(kernel, lib):
     """An infinity or a NaN in a query makes its own row NaN and no other."""
     rng = np.random.default_rng(15)
     for rows in ([3], [50]):
@@ -258,7 +265,7 @@ def test_infinite_queries(lib):
 
 
 @pytest.mark.parametrize("dtype,v_scale", [("bf16", 2.0 ** 100), ("bf16", 2.0 ** -100), ("f16", 2.0 ** 11), ("f16", 2.0 ** -11)])
-def test_large_and_small_values(lib, dtype, v_scale):
+def test_large_and_small_values(kernel, lib, dtype, v_scale):
     rng = np.random.default_rng(16)
     for rows in ([2], [40]):
         c = Case(lib, rng, rows, [150], 4, 2, 128, 32, dtype, v_scale=v_scale)
@@ -268,7 +275,7 @@ def test_large_and_small_values(lib, dtype, v_scale):
         c.check()
 
 
-def test_shorter_bounds(lib):
+def test_shorter_bounds(kernel, lib):
     """Lengths past max_length count as max_length; rows past max_rows stay."""
     rng = np.random.default_rng(17)
     c = Case(lib, rng, [3, 6], [50, 80], 4, 2, 64, 16, "bf16", max_rows=4)
@@ -300,7 +307,7 @@ def test_every_kernel_and_chunk(lib, d, tile, chunk):
             c.check()
 
 
-def test_same_result_every_time(lib):
+def test_same_result_every_time(kernel, lib):
     rng = np.random.default_rng(18)
     for rows, lengths in (([1, 1], [3000, 10]), ([200], [700])):
         c = Case(lib, rng, rows, lengths, 8, 2, 128, 64, "bf16")
@@ -313,7 +320,7 @@ def test_same_result_every_time(lib):
             np.testing.assert_array_equal(raw, first)
 
 
-def test_a_cache_past_32_bits(lib):
+def test_a_cache_past_32_bits(kernel, lib):
     """Pages whose byte offsets pass 2^32."""
     rng = np.random.default_rng(19)
     for rows in ([1], [40]):
