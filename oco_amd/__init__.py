@@ -1007,7 +1007,8 @@ class CacheBatch:
         p = self.p
         if stride:
             p = Cache.from_buffer_copy(p)
-            p.q_stride = p.k_stride = p.v_stride = stride
+            p.k_stride = p.v_stride = stride
+            p.q_stride = stride if q is not None else 0
         cache_append(self.cache.buffer, self.table, self.lengths, k, v, p, self.starts, q, q_out, positions, rotation, stream)
 
     def read(self, k, v, stream=None):

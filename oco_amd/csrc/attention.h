@@ -42,7 +42,7 @@ struct Half<true> {
     static __device__ __forceinline__ f32x16 product32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
-    static constexpr uint32_t ONE = 0x3f80;
+    static constexpr uint32_t ONE = 0x3f80, LIMIT = 252;  // LIMIT: the last scale whose 6 is a number of the type
 };
 template <>
 struct Half<false> {
@@ -59,8 +59,19 @@ struct Half<false> {
     static __device__ __forceinline__ f32x16 product32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
-    static constexpr uint32_t ONE = 0x3c00;
+    static constexpr uint32_t ONE = 0x3c00, LIMIT = 140;
 };
+// A block's scale, NaN past the limit; and 0x80 in the bytes of a word of
+// scales that are past it (of at least 128).
+template <uint32_t LIMIT>
+__device__ __forceinline__ float block_scale(uint32_t e) {
+    return __uint_as_float(e > LIMIT ? 0x7fc00000u : e << 23);
+}
+template <uint32_t LIMIT>
+__device__ __forceinline__ uint32_t bytes_past(uint32_t x) {
+    return ((x & 0x7f7f7f7fu) + (255 - LIMIT) * 0x01010101u) & x & 0x80808080u;
+}
+
 // Four tokens' pairs of columns -> the two columns' four tokens.
 __device__ __forceinline__ u32x2 low_halves(const uint32_t *c) {
     return u32x2{__builtin_amdgcn_perm(c[1], c[0], 0x05040100), __builtin_amdgcn_perm(c[3], c[2], 0x05040100)};
@@ -110,12 +121,8 @@ __device__ __forceinline__ AttentionTile attention_tile(const CacheSpan &s, uint
     return t;
 }
 
-// exp2 of m - to, 0 for m = -Inf whatever `to` is.
-__device__ __forceinline__ float carry(float m, float to) { return m > -INFINITY ? __builtin_amdgcn_exp2f(m - to) : 0.f; }
-
-// 0x80 in the bytes of a word of scales that are 255 (and in a 254 above one,
-// which no block has).
-__device__ __forceinline__ uint32_t bytes_255(uint32_t x) { return (~x - 0x01010101u) & x & 0x80808080u; }
+// exp2 of m - to, 0 for m = -Inf whatever `to` is (NaN for a sink that is NaN).
+__device__ __forceinline__ float carry(float m, float to) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to); }
 
 // Prompts (attention_prompt.hip; heads of 64 and 128): rows of a tile, tokens of a step.
 constexpr uint32_t PROMPT_ROWS = 128;

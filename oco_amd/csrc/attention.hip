@@ -191,7 +191,7 @@ __global__ __launch_bounds__(256, D * R == 64 ? 4 : D * R == 128 ? 3 : 2) void a
             u32x4 x[2];
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const float scale = cache_scale(D == 256 ? (w < 4 ? k[e].scale & 0xff : k[e].scale >> 8) : k[e].scale & 0xff);
+                const float scale = block_scale<H::LIMIT>(D == 256 ? (w < 4 ? k[e].scale & 0xff : k[e].scale >> 8) : k[e].scale & 0xff);
                 x[e] = u32x4{H::template pair<0>(k[e].w[w], scale), H::template pair<1>(k[e].w[w], scale),
                              H::template pair<2>(k[e].w[w], scale), H::template pair<3>(k[e].w[w], scale)};
             }
@@ -239,13 +239,13 @@ __global__ __launch_bounds__(256, D * R == 64 ? 4 : D * R == 128 ? 3 : 2) void a
 #pragma unroll
         for (int e = 0; e < 2; e++)
             if (lost[e]) v[e].scale = 0xffffffffu;
-        if (__any((bytes_255(v[0].scale) | bytes_255(v[1].scale)) != 0)) {
+        if (__any((bytes_past<H::LIMIT>(v[0].scale) | bytes_past<H::LIMIT>(v[1].scale)) != 0)) {
             // 0 * NaN is NaN: a NaN block enters the product as numbers, and the rows that see
             // it (counted by a product of their own) become NaN in its columns
             u32x4 lost_at;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const uint32_t lo = byte_of(v[i / 2].scale, 2 * i % 4) == 255, hi = byte_of(v[i / 2].scale, 2 * i % 4 + 1) == 255;
+                const uint32_t lo = byte_of(v[i / 2].scale, 2 * i % 4) > H::LIMIT, hi = byte_of(v[i / 2].scale, 2 * i % 4 + 1) > H::LIMIT;
                 lost_at[i] = lo * H::ONE | hi * (H::ONE << 16);
             }
 #pragma unroll
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(256, D * R == 64 ? 4 : D * R == 128 ? 3 : 2) void a
                     for (int j = 0; j < NT; j++) o[r][j][i] = count[i] > 0.f ? __uint_as_float(0x7fc00000u) : o[r][j][i];
             }
 #pragma unroll
-            for (int e = 0; e < 2; e++) v[e].scale ^= bytes_255(v[e].scale);
+            for (int e = 0; e < 2; e++) v[e].scale ^= bytes_past<H::LIMIT>(v[e].scale);
         }
         float scale[8];  // of the tokens' column block
 #pragma unroll
@@ -369,25 +369,48 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
     __shared__ __attribute__((aligned(16))) f32x4 so[GROUPS][LANES * V];
     __shared__ float st[GROUPS];
     const uint32_t row = blockIdx.x / a.heads, head = blockIdx.x % a.heads, group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    const uint64_t index = (uint64_t)blockIdx.x * a.chunks;
+    const float *const ml = a.parts + (uint64_t)a.b.rows * a.heads * a.chunks * D + index * 2;
+    const f32x4 *const parts = (const f32x4 *)(a.parts + index * D) + lane * V;
+    // The first chunks are requested before it is known how many the row has; a place in the workspace that was not
+    // written is read and not used.
+    constexpr uint32_t AHEAD = 4 / V;
+    f32x4 part[AHEAD][V];
+    f32x2 of[AHEAD], tops = {-INFINITY, 0.f};
+    if ((threadIdx.x & 63) < a.chunks) tops = *(const GLOBAL f32x2 *)gp(ml + 2 * (threadIdx.x & 63));
+#pragma unroll
+    for (uint32_t k = 0; k < AHEAD; k++) {
+        const uint32_t c = group + k * GROUPS;
+        if (c < a.chunks) {
+            of[k] = *(const GLOBAL f32x2 *)gp(ml + 2 * c);
+#pragma unroll
+            for (uint32_t j = 0; j < V; j++) part[k][j] = ((const GLOBAL f32x4 *)gp(parts))[(uint64_t)c * (D / 4) + j];
+        }
+    }
     const uint32_t s = cache_sequence(a.b, row);
     if (s >= a.b.sequences) return;
     const CacheSpan span = cache_span(a.b, s);
     if (row - span.first >= span.rows) return;
     const AttentionTile range = attention_tile(span, ((row - span.first) * a.group + head % a.group) / a.tile_rows, a.tile_rows, a.group, a.window);
     const uint32_t used = range.end > range.first ? (range.end - range.first + a.chunk - 1) / a.chunk : 0;
-    const uint64_t index = (uint64_t)blockIdx.x * a.chunks;
-    const float *const ml = a.parts + (uint64_t)a.b.rows * a.heads * a.chunks * D + index * 2;
-    const f32x4 *const parts = (const f32x4 *)(a.parts + index * D) + lane * V;
     const float sink = a.sinks ? a.sinks[head] * 1.44269504088896341f : -INFINITY;
     float top = sink;
-    for (uint32_t c = threadIdx.x & 63; c < used; c += 64) top = fmaxf(top, ml[2 * c]);
+    if ((threadIdx.x & 63) < used) top = fmaxf(top, tops[0]);
+    for (uint32_t c = 64 + (threadIdx.x & 63); c < used; c += 64) top = fmaxf(top, ml[2 * c]);
     top = wave_max(top);
     float total = 0.f;
     f32x4 o[V];
 #pragma unroll
     for (uint32_t j = 0; j < V; j++) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (uint32_t c = group; c < used; c += GROUPS) {
+#pragma unroll
+    for (uint32_t k = 0; k < AHEAD; k++) {
+        if (group + k * GROUPS >= used) break;
+        const float f = carry(of[k][0], top);
+        total += of[k][1] * f;
+#pragma unroll
+        for (uint32_t j = 0; j < V; j++) o[j] += part[k][j] * f;
+    }
+    for (uint32_t c = group + AHEAD * GROUPS; c < used; c += GROUPS) {
         const float f = carry(ml[2 * c], top);
         total += ml[2 * c + 1] * f;
 #pragma unroll
@@ -418,7 +441,7 @@ struct AttentionPlan {
 };
 static AttentionPlan attention_plan(const oco_cache *p) {
     AttentionPlan l;
-    const uint64_t rows = (uint64_t)p->max_rows * (p->heads / p->kv_heads);
+    const uint64_t rows = (uint64_t)(p->max_rows < p->rows ? p->max_rows : p->rows) * (p->heads / p->kv_heads);
     // Tiles of 16 rows while that is all, of 32 beyond (of 16 where the second one would be half empty).  With narrow heads
     // tiles of 128 of the prompts' kernel from 256 of them on, one per compute unit.  us, tiles of 16 / 32 / 128:
     // 32 sequences of 5 x 4 rows over 8000 tokens, 128 wide 115 / 84 / 141; 8 of 5 x 8 rows, 64 wide 20.7 / 22.1 / 33;
@@ -481,7 +504,7 @@ static int attention_launch(const AttentionArgs &a, const AttentionPlan &l, hipS
 static const char *attention_problem(const oco_cache *p) {
     if (const char *why = cache_problem(p)) return why;
     if (p->heads == 0) return "no heads";
-    if ((uint64_t)p->rows * p->heads > 0x7fffffffull) return "too many rows for one call";
+    if ((uint64_t)p->rows * p->heads > 0x7fffffffull || (uint64_t)p->sequences * p->kv_heads > 0x7fffffffull) return "too many rows for one call";
     return nullptr;
 }
 

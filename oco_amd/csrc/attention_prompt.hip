@@ -122,7 +122,7 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(AttentionArgs 
         x.lost = p.lost;
     };
     auto convert_keys = [&](const Raw &x, uint32_t into) {
-        const float ks = cache_scale(x.lost ? 255 : x.scale);
+        const float ks = block_scale<H::LIMIT>(x.lost ? 255 : x.scale);
 #pragma unroll
         for (int i = 0; i < (int)KB / 4; i++)
             keys[into][kt * KROW + kp * (KB / 4) + i] = u32x4{H::template pair<0>(x.w[i], ks), H::template pair<1>(x.w[i], ks),
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(AttentionArgs 
         uint32_t vs = x.lost ? 0xffffffffu : x.scale;
         // a NaN block enters as numbers, for 0 * NaN is NaN; without a branch, which would keep the
         // products before it from running beside
-        const uint32_t bad = bytes_255(vs);
+        const uint32_t bad = bytes_past<H::LIMIT>(vs);
         vs ^= bad;
         flags[__any(bad != 0) ? into : 2] = number;
         float scale[4];
@@ -229,7 +229,7 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(AttentionArgs 
                 const uint32_t page = table[t / a.b.page_size];
                 for (uint32_t b = 0; b < D / 32; b++)
                     if (page >= a.b.pages ||
-                        a.cache[((uint64_t)page * a.b.kv_heads + h) * head_bytes + cache_value_scale_at(a.b.page_size, t % a.b.page_size, b, D)] == 255)
+                        a.cache[((uint64_t)page * a.b.kv_heads + h) * head_bytes + cache_value_scale_at(a.b.page_size, t % a.b.page_size, b, D)] > H::LIMIT)
                         bad |= 1u << b;
             }
 #pragma unroll

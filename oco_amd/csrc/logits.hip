@@ -20,8 +20,14 @@ struct LogitsArgs {
     uint32_t vocabulary, chunks, history_stride, bias_stride, mask_stride, group, mask_group;
 };
 
-template <class T, uint32_t THREADS, uint32_t CHUNK>
-__global__ __launch_bounds__(THREADS) void logits_kernel(LogitsArgs a) {
+// Words per workgroup: every workgroup of a row reads its whole history, which costs little (64 rows of 151936 f32 words:
+// 14.5 us without one, 15.0 with 512 ids, 18.2 with 8192), and 1024 threads on 16384 words are slower but there
+// (15.1, 15.8, 17.6).
+constexpr uint32_t LOGITS_CHUNK = 4096;
+
+template <class T>
+__global__ __launch_bounds__(256) void logits_kernel(LogitsArgs a) {
+    constexpr uint32_t THREADS = 256, CHUNK = LOGITS_CHUNK;
     __shared__ __attribute__((aligned(16))) uint32_t marks[CHUNK];
     const uint32_t row = blockIdx.x / a.chunks, first = blockIdx.x % a.chunks * CHUNK, g = row / a.group;
     const uint32_t size = min(CHUNK, a.vocabulary - first);
@@ -45,9 +51,18 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(LogitsArgs a) {
             presence = p[2];
             const uint32_t n = a.history_lengths ? min(a.history_lengths[g], a.history_stride) : a.history_stride;
             const uint32_t *const ids = a.history + (uint64_t)g * a.history_stride;
-            for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-                const uint32_t at = ids[i] - first;
-                if (at < size) atomicAdd(&marks[at], 1u);
+            for (uint32_t i = 4 * threadIdx.x; i < n; i += 4 * THREADS) {
+                u32x4 id = {first - 1, first - 1, first - 1, first - 1};
+                if (i + 4 <= n) {
+                    id = *(const GLOBAL u32x4_u *)gp(ids + i);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 3; j++)
+                        if (i + j < n) id[j] = ids[i + j];
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (id[j] - first < size) atomicAdd(&marks[id[j] - first], 1u);
             }
         }
         __syncthreads();
@@ -81,10 +96,9 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(LogitsArgs a) {
 
 template <class T>
 static int logits_launch(LogitsArgs a, uint32_t rows, hipStream_t stream) {
-    constexpr uint32_t CHUNK = 4096;
-    a.chunks = (a.vocabulary + CHUNK - 1) / CHUNK;
+    a.chunks = (a.vocabulary + LOGITS_CHUNK - 1) / LOGITS_CHUNK;
     if ((uint64_t)rows * a.chunks > 0x7fffffffull) return fail(OCO_ERR_INVALID, "oco_logits_adjust: %u rows", rows);
-    hipLaunchKernelGGL((logits_kernel<T, 256, CHUNK>), dim3(rows * a.chunks), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((logits_kernel<T>), dim3(rows * a.chunks), dim3(256), 0, stream, a);
     return launch_check("oco_logits_adjust");
 }
 

@@ -198,6 +198,76 @@ def test_nan_in_the_last_token(kernel, lib, d, rows):
         np.testing.assert_array_equal(got, want)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_pages_of_anything(kernel, lib, dtype):
+    """Memory that no token was written to, behind the last token and in pages of nobody, whatever it holds."""
+    rng = np.random.default_rng(21)
+    for rows, lengths in (([1, 3], [37, 70]), ([45], [75])):
+        for fill in (0xFD, 0xFE, 0x8D, 0xC8, 0x00, None):
+            c = Case(lib, rng, rows, lengths, 4, 2, 128, 32, dtype, window=50)
+            empty = np.ones(c.pool.bytes.shape, bool)
+            for s, n in enumerate(lengths):  # a pool that marks what the tokens take
+                for t in range(n):
+                    page, slot = c.b.place(s, t)
+                    mark = Pool(1, 1, 32, 128)
+                    mark.bytes[:] = 0
+                    one = (np.full(128, 15, np.uint8), np.full(4, 255, np.uint8))
+                    mark.put(0, slot, 0, one, one)
+                    empty[page] &= mark.bytes[0] == 0
+            noise = rng.integers(0, 256, empty.shape).astype(np.uint8) if fill is None else np.full(empty.shape, fill, np.uint8)
+            c.dev[1].upload(np.where(empty, noise, c.pool.bytes))
+            say("anything", dtype, rows, fill)
+            c.call()
+            lib.synchronize()
+            got = c.check()
+            assert not np.isnan(got).any()
+
+
+def test_blocks_past_f16(kernel, lib):
+    """In f16 a block that the type cannot hold is NaN to the rows that see it, and to no other."""
+    rng = np.random.default_rng(22)
+    for rows in ([3], [45]):
+        c = Case(lib, rng, rows, [90], 4, 2, 64, 16, "f16")
+        for at, (what, t, scale) in enumerate((("v", 89, 141), ("k", 89, 200), ("v", 88, 252))):
+            if what == "k" and rows == [3]:
+                continue
+            page, slot = c.b.place(0, t)
+            c.pool.bytes[page, at % 2, 16 * 64 + (slot * 2 if what == "k" else 32 + slot // 4 * 8 + slot % 4)] = scale
+            (c.k if what == "k" else c.v)[0][t, at % 2, :32] = np.nan
+        c.dev[1].upload(c.pool.bytes)
+        say("past f16", rows)
+        c.call()
+        lib.synchronize()
+        got = c.check()
+        assert np.isnan(got[-1]).any() and not np.isnan(got[-3]).any()
+
+
+def test_sinks_that_are_nan(kernel, lib):
+    rng = np.random.default_rng(23)
+    for rows, lengths in (([1], [3000]), ([40], [60])):
+        c = Case(lib, rng, rows, lengths, 4, 2, 64, 16, "bf16", sinks=True)
+        c.sinks[2] = np.nan
+        c.dev[5].upload(c.sinks)
+        say("nan sink", rows)
+        c.call()
+        lib.synchronize()
+        c.sinks[2] = 0.0
+        raw = values(c.out.read(np.uint8), "bf16", c.q.shape)
+        assert np.isnan(raw[:, 2]).all() and not np.isnan(raw[:, [0, 1, 3]]).any()
+
+
+@pytest.mark.parametrize("rows,lengths", [([1, 2], [2000, 30]), ([60], [100]), ([6], [1500])])
+def test_in_the_place_of_the_queries(kernel, lib, rows, lengths):
+    rng = np.random.default_rng(24)
+    c = Case(lib, rng, rows, lengths, 8, 2, 128, 32, "bf16", sinks=True)
+    c.call()
+    q, cache, table, lens, starts, sinks = c.dev
+    say("in place", rows)
+    lib.cache_attention(q, cache, table, lens, q, c.p, starts=starts, sinks=sinks, workspace=c.work.ptr if c.need else None, workspace_bytes=c.need)
+    lib.synchronize()
+    np.testing.assert_array_equal(q.download(np.uint8), c.out.read(np.uint8))
+
+
 def test_pages_outside_the_pool(kernel, lib):
     """They read as NaN where a row sees them, and nothing is read there."""
     rng = np.random.default_rng(12)

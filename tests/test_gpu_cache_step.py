@@ -99,7 +99,6 @@ def test_step(lib, rows, lengths):
         prefix = st.cache.batch(st.keep[0], dev(lib, np.array(before, np.uint32)), len(rows), sum(before), max(before), max(lengths), b.stride, HEADS,
                                 starts=dev(lib, starts))
         buf = dev(lib, raw)
-        prefix.p.heads = KV  # no queries: the stride of the keys and values is that of their rows
         prefix.append(buf.ptr, buf.ptr + KV * D * 2, stride=2 * KV * D)
         for s in range(len(rows)):
             part = old[starts[s]:starts[s + 1]]
