@@ -436,32 +436,33 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
 // ---- choices and launches -------------------------------------------------------------------
 
 struct AttentionPlan {
-    uint32_t tile, tiles, chunks, chunk;  // tile: of 16 rows
+    uint32_t tile, tiles, chunks, chunk;  // tile: its rows / 16
     uint64_t bytes;
 };
 static AttentionPlan attention_plan(const oco_cache *p) {
     AttentionPlan l;
     const uint64_t rows = (uint64_t)(p->max_rows < p->rows ? p->max_rows : p->rows) * (p->heads / p->kv_heads);
     // Tiles of 16 rows while that is all, of 32 beyond (of 16 where the second one would be half empty).  With narrow heads
-    // tiles of 128 of the prompts' kernel from 256 of them on, one per compute unit.  us, tiles of 16 / 32 / 128:
+    // the prompts' kernel: tiles of 128 rows from 256 of them on, one per compute unit, and of 256 from 512 of those on.  us,
+    // tiles of 16 / 32 / 128 / 256:
     // 32 sequences of 5 x 4 rows over 8000 tokens, 128 wide 115 / 84 / 141; 8 of 5 x 8 rows, 64 wide 20.7 / 22.1 / 33;
-    // 4 of 128 x 4 rows over 2000 (128 tiles) 41 / 33 / 49, 16 of 64 x 4 over 4000 (256 tiles) 142 / 108 / 86, 64 of 32 x 4
-    // over 1000 (512) 92 / 75 / 49; 1000 x 4 rows from the start on (256) 26 / 24 / 28; 4096 x 4 rows over 8192 722 / 569 /
-    // 392, 256 wide (16 heads) 623 / 443 / 715.
+    // 4 of 128 x 4 rows over 2000 (128 tiles of 128) 41 / 33 / 49; 16 of 64 x 4 over 4000 (256, 128 of 256) 142 / 108 / 86 / 113;
+    // 64 of 32 x 4 over 1000 (512) 92 / 75 / 49; 2048 x 4 rows from the start on (512, 256 of 256) 65 with 32 / 52 / 63;
+    // 4096 x 4 rows over 8192 (512 of 256) 715 / 567 / 381 / 365, 256 wide (16 heads) 623 / 443.
     int32_t knob[4];
     const int set = plan_override(OCO_KNOB_ATTENTION, knob);
     const bool narrow = p->head_dim <= 128;
-    const uint64_t wide_tiles = (rows + PROMPT_ROWS - 1) / PROMPT_ROWS * p->kv_heads * p->sequences;
+    const uint64_t heads = (uint64_t)p->kv_heads * p->sequences;
     l.tile = rows <= 16 || (rows > 32 && rows <= 48) ? 1 : 2;
-    if (narrow && rows >= PROMPT_ROWS && wide_tiles >= 256) l.tile = PROMPT_ROWS / 16;
-    if (set && (knob[0] == 1 || knob[0] == 2 || (knob[0] == (int)PROMPT_ROWS / 16 && narrow))) l.tile = (uint32_t)knob[0];
+    if (narrow && rows >= 128 && (rows + 127) / 128 * heads >= 256) l.tile = (rows + 255) / 256 * heads >= 512 ? 16 : 8;
+    if (set && (knob[0] == 1 || knob[0] == 2 || ((knob[0] == 8 || knob[0] == 16) && narrow))) l.tile = (uint32_t)knob[0];
     l.tiles = (uint32_t)((rows + 16 * l.tile - 1) / (16 * l.tile));
     // the most tokens that a tile sees
     const uint64_t tile_tokens = (16 * l.tile + p->heads / p->kv_heads - 1) / (p->heads / p->kv_heads);
     uint64_t seen = p->max_length;
     if (p->window && p->window + tile_tokens + 31 < seen) seen = p->window + tile_tokens + 31;
     const uint64_t blocks = (uint64_t)p->sequences * p->kv_heads * l.tiles;
-    const bool prompt = l.tile == PROMPT_ROWS / 16;
+    const bool prompt = l.tile >= 8;
     // Chunks until the card is full: 3072 workgroups of few rows, of at least two steps per wavefront (32 sequences of up to
     // 16384 tokens: 1152 to 2048 tokens a chunk 75 to 78 us, 4096 74 to 95 by how they divide, 256 104; one of 4101: 256
     // tokens 9.2, 512 10.9), 512 of a prompt's tiles.

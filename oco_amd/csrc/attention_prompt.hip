@@ -1,28 +1,41 @@
 // Attention over the paged cache for many rows: the matrix cores' side.
 //
-// A workgroup's four wavefronts hold 32 rows each and share steps of 64 tokens
-// whose codes are converted once for all of them into LDS:
-// keys as rows, values transposed, so that both products read 16 bytes per
-// lane.  Two buffers, one barrier per step: the next step's codes are on their
-// way while this one is computed.  As in the kernel for few rows a lane is a
-// row throughout (here of two), and the products' inner indexes are in the order
-// in which the scores leave the first product.
+// A workgroup's four or eight wavefronts hold 32 rows each and share steps of
+// 64 tokens, whose codes are converted once for all of them into LDS: keys as
+// rows, values transposed, so that both products read 16 bytes per lane.  As
+// in the kernel for few rows a lane is a row throughout (here of two), and the
+// products' inner indexes are in the order in which the scores leave the first
+// product.  A wavefront converts 16 tokens of a buffer, which lie in one page.
 //
-// A wavefront converts 16 tokens of a step, which lie in one page.
+// Bound by how well matrix cores, vector units and LDS run beside each other,
+// each about half of the time busy with the two wavefronts per SIMD that the
+// registers leave: a step of a wavefront is 32 products of 32 x 32 x 16 (1024
+// clocks), 32 KB from LDS, 32 exponentials per lane and its share of the
+// conversions (190 to 210 vector instructions).  So a step computes the next
+// one's scores beside its own exponentials and converts beside the second
+// product, in groups that each request the next group's fragments (4096 rows
+// of 32 heads over 8192 tokens: 670 us with the steps one after the other and
+// in three chunks, 476 whole, 435 with the scores of the next step, 412 in
+// groups and without copies between turns, 381 with the chunk grid by tile).
+// Eight wavefronts on twice the tokens halve the conversions' share: 365 us,
+// 1.13 PFLOP/s (a large library product of bf16 reaches 1.2 to 1.35), 807 over
+// 16000 tokens.  Measured and lost: wavefront priorities around the products
+// (no change), other paddings of the rows in LDS (413 to 430 against 412).
 #include "attention.h"
 
 namespace oco {
 
-template <uint32_t D, bool BF>
-__global__ __launch_bounds__(256, 2) void attention_prompt_kernel(AttentionArgs a, uint32_t tiles) {
+template <uint32_t D, bool BF, int W>
+__global__ __launch_bounds__(64 * W, 2) void attention_prompt_kernel(AttentionArgs a, uint32_t tiles) {
     using H = Half<BF>;
-    constexpr uint32_t KT = PROMPT_STEP;
+    constexpr uint32_t KT = 64, BT = 16 * W;  // tokens of a step, of a buffer: a step or two
+    constexpr int SUBS = BT / KT;
     constexpr int KN = KT / 32, NS = D / 16, NO = D / 32;       // key tiles, key steps, column tiles
     constexpr uint32_t PIECE = D / 16;                          // columns of a value's piece
     // rows of 16-byte pieces, one piece of padding: eight consecutive rows fall into different banks
-    constexpr uint32_t KROW = D / 8 + 1, VROW = KT / 8 + 1;
-    __shared__ __attribute__((aligned(16))) u32x4 keys[2][KT * KROW], values[2][D * VROW];
-    __shared__ uint32_t flags[3];  // the step, from 1, whose values hold a block of NaN; the last one is not read
+    constexpr uint32_t KROW = D / 8 + 1, VROW = BT / 8 + 1;
+    __shared__ __attribute__((aligned(16))) u32x4 keys[2][BT * KROW], values[2][D * VROW];
+    __shared__ uint32_t flags[3];  // the buffer's number, from 1, whose values hold a block of NaN; the last one is not read
 
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, g = lane >> 5;
     uint32_t id = blockIdx.x;
@@ -32,7 +45,7 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(AttentionArgs 
     id /= a.chunks;
     const uint32_t s = id % a.b.sequences, tile = tiles - 1 - id / a.b.sequences;
     const CacheSpan span = cache_span(a.b, s);
-    const AttentionTile range = attention_tile(span, tile, PROMPT_ROWS, a.group, a.window);
+    const AttentionTile range = attention_tile(span, tile, 32 * W, a.group, a.window);
     const uint32_t rows = range.rows;
     if (range.first_row >= rows) return;
     const int32_t before = (int32_t)span.length - (int32_t)span.rows;
@@ -72,9 +85,9 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(AttentionArgs 
     const uint32_t k_at = kt % 16 * (D / 2) + kp * KB, ks_at = a.b.page_size * D + kt % 16 * (D / 32) + kp * KB / 16;
     const uint32_t v_at = a.b.page_size * (D / 2) + vg % 4 * (2 * D) + vm * (D / 8);
     const uint32_t vs_at = a.b.page_size * D + a.b.page_size * (D / 32) + vg % 4 * (D / 8) + vm * D / 512 * 4;
-    uint32_t page_of = 0, slot_of = 0;  // lane i: of step 64 c + i
+    uint32_t page_of = 0, slot_of = 0;  // lane i: of buffer 64 c + i
     auto read_table = [&](uint32_t step) {
-        const uint32_t t = first + (step + lane) * KT + 16 * half;  // step: the first of 64
+        const uint32_t t = first + (step + lane) * BT + 16 * half;  // step: the first of 64
         page_of = t < end ? table[t / a.b.page_size] : 0;
         slot_of = t % a.b.page_size;
     };
@@ -154,7 +167,7 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(AttentionArgs 
             out[((2 * b + 1) * 16 + vm) * (2 * VROW)] = high_halves(c);
         }
     };
-    auto scores = [&](f32x16 *sc, uint32_t from) {
+    auto scores = [&](f32x16 *sc) {  // of the first step
 #pragma unroll
         for (int k = 0; k < KN; k++)
 #pragma unroll
@@ -162,12 +175,13 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(AttentionArgs 
 #pragma unroll
         for (int i = 0; i < NS; i++)
 #pragma unroll
-            for (int k = 0; k < KN; k++) sc[k] = H::product32(keys[from][(32 * k + n) * KROW + 2 * i + g], q[i], sc[k]);
+            for (int k = 0; k < KN; k++) sc[k] = H::product32(keys[0][(32 * k + n) * KROW + 2 * i + g], q[i], sc[k]);
     };
 
-    // Step i computes the scores of step i + 1 beside the probabilities of its own, and converts the
-    // keys of step i + 2 and the values of step i + 1; the ones after those are on their way.  Past
-    // the last step the first one's page is read again.
+    // A step computes the scores of the next one beside its own probabilities.  With a step per buffer it
+    // converts the keys of the buffer after the next and the values of the next; with two, the first
+    // one the next buffer's keys and the second its values.  The ones after those are on their way.
+    // Past the last buffer the first page is read again.
     const uint32_t steps = end > first ? (end - first + KT - 1) / KT : 0;
     Raw rk, rv;
     Place ahead;
@@ -179,22 +193,33 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(AttentionArgs 
         request_values(rv, p);
         p = find(1);
         Raw second;
-        request_keys(second, p);
+        if constexpr (SUBS == 1) request_keys(second, p);
         convert_keys(rk, 0);
         if (threadIdx.x < 2) flags[threadIdx.x] = 0;
         __syncthreads();
         convert_values(rv, 0, 1);
         request_values(rv, p);
-        ahead = find(2);
-        request_keys(rk, ahead);
-        convert_keys(second, 1);
+        if constexpr (SUBS == 1) {
+            ahead = find(2);
+            request_keys(rk, ahead);
+            convert_keys(second, 1);
+        } else {
+            request_keys(rk, p);
+        }
         __syncthreads();
-        scores(sc, 0);
+        scores(sc);
     }
-    // step, its scores, where the next step's go, the buffer of its values
-    auto compute = [&](const uint32_t step, f32x16 *sc, f32x16 *next, const uint32_t buffer) {
-        const uint32_t t0 = first + step * KT;
-        if ((step + 3) % 64 == 0) read_table(step + 3);
+    // step, its scores, where the next step's go, its buffer's number and place, its place in the buffer
+    auto compute = [&](const uint32_t step, f32x16 *sc, f32x16 *next, const uint32_t number, const uint32_t buffer, const int sub) {
+        const uint32_t t0 = first + step * KT, next_buffer = sub + 1 == SUBS ? buffer ^ 1 : buffer;
+        const int next_sub = sub + 1 == SUBS ? 0 : sub + 1;
+        const u32x4 *const next_keys = &keys[next_buffer][(next_sub * KT + n) * KROW + g];
+        const u32x4 *const own_values = &values[buffer][n * VROW + sub * (KT / 8) + g];
+        if constexpr (SUBS == 1) {
+            if ((step + 3) % 64 == 0) read_table(step + 3);
+        } else {
+            if (sub == 0 && (number + 2) % 64 == 0) read_table(number + 2);
+        }
         if ((int32_t)(t0 + KT) - 1 > least || t0 + KT > end || (a.window && (int32_t)t0 + (int32_t)a.window <= most)) {
 #pragma unroll
             for (int k = 0; k < KN; k++)
@@ -221,7 +246,7 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(AttentionArgs 
 #pragma unroll
             for (int j = 0; j < NO; j++) o[j] *= f;
         }
-        if (flags[buffer] == step + 1) {
+        if (flags[buffer] == number + 1) {
             // rows that see a block of NaN: every lane looks at the step's tokens itself
             uint32_t bad = 0;
             for (uint32_t t = t0; t < min(t0 + KT, end); t++) {
@@ -249,16 +274,16 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(AttentionArgs 
         for (int k = 0; k < KN; k++) {
 #pragma unroll
             for (int i = 0; i < 16; i++) next[k][i] = 0.f;
-            kf[0][k] = keys[buffer ^ 1][(32 * k + n) * KROW + g];
+            kf[0][k] = next_keys[32 * k * KROW];
         }
 #pragma unroll
         for (int i = 0; i < NS; i++) {
             if (i + 1 < NS) {
 #pragma unroll
-                for (int k = 0; k < KN; k++) kf[(i + 1) % 2][k] = keys[buffer ^ 1][(32 * k + n) * KROW + 2 * (i + 1) + g];
+                for (int k = 0; k < KN; k++) kf[(i + 1) % 2][k] = next_keys[32 * k * KROW + 2 * (i + 1)];
             } else {
 #pragma unroll
-                for (int j = 0; j < NO; j++) vf[0][j] = values[buffer][(32 * j + n) * VROW + g];
+                for (int j = 0; j < NO; j++) vf[0][j] = own_values[32 * j * VROW];
             }
 #pragma unroll
             for (int k = 0; k < KN; k++) next[k] = H::product32(kf[i % 2][k], q[i], next[k]);
@@ -277,27 +302,46 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(AttentionArgs 
         for (int t = 0; t < 2 * KN; t++) {
             if (t + 1 < 2 * KN) {
 #pragma unroll
-                for (int j = 0; j < NO; j++) vf[(t + 1) % 2][j] = values[buffer][(32 * j + n) * VROW + 2 * (t + 1) + g];
+                for (int j = 0; j < NO; j++) vf[(t + 1) % 2][j] = own_values[32 * j * VROW + 2 * (t + 1)];
             }
 #pragma unroll
             for (int j = 0; j < NO; j++) o[j] = H::product32(vf[t % 2][j], p[t], o[j]);
-            if (t == 0) {
-                convert_keys(rk, buffer);
-            } else if (t == KN) {
-                convert_values(rv, buffer ^ 1, step + 2);
-                request_values(rv, ahead);
-                ahead = find(step + 3);
-                request_keys(rk, ahead);
+            if constexpr (SUBS == 1) {
+                if (t == 0) {
+                    convert_keys(rk, buffer);
+                } else if (t == KN) {
+                    convert_values(rv, buffer ^ 1, number + 2);
+                    request_values(rv, ahead);
+                    ahead = find(step + 3);
+                    request_keys(rk, ahead);
+                }
+            } else if (t == 1) {
+                if (sub == 0) {
+                    convert_keys(rk, buffer ^ 1);
+                    ahead = find(number + 2);
+                    request_keys(rk, ahead);
+                } else {
+                    convert_values(rv, buffer ^ 1, number + 2);
+                    request_values(rv, ahead);
+                }
             }
             if (t + 1 < 2 * KN && (t == 0 || t + 1 == KN)) __builtin_amdgcn_sched_barrier(0);
         }
         __syncthreads();
     };
     f32x16 other[KN];
-    for (uint32_t step = 0; step < steps; step += 2) {
-        compute(step, sc, other, 0);
-        if (step + 1 == steps) break;
-        compute(step + 1, other, sc, 1);
+    if constexpr (SUBS == 1) {
+        for (uint32_t step = 0; step < steps; step += 2) {
+            compute(step, sc, other, step, 0, 0);
+            if (step + 1 == steps) break;
+            compute(step + 1, other, sc, step + 1, 1, 0);
+        }
+    } else {
+        for (uint32_t step = 0, number = 0; step < steps; step += 2, number++) {
+            compute(step, sc, other, number, number & 1, 0);
+            if (step + 1 == steps) break;
+            compute(step + 1, other, sc, number, number & 1, 1);
+        }
     }
     if (!live) return;
     {
@@ -338,15 +382,23 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(AttentionArgs 
 }
 
 int attention_prompt_launch(const AttentionArgs &a, uint32_t head_dim, bool bf, uint32_t tiles, uint32_t grid, hipStream_t stream) {
-#define GO(D)                                                                                                             \
-    if (bf)                                                                                                               \
-        hipLaunchKernelGGL((attention_prompt_kernel<D, true>), dim3(grid), dim3(256), 0, stream, a, tiles);               \
-    else                                                                                                                  \
-        hipLaunchKernelGGL((attention_prompt_kernel<D, false>), dim3(grid), dim3(256), 0, stream, a, tiles);
+#define GO(D, BF)                                                                                                                     \
+    if (a.tile_rows == 256)                                                                                                           \
+        hipLaunchKernelGGL((attention_prompt_kernel<D, BF, 8>), dim3(grid), dim3(512), 0, stream, a, tiles);                          \
+    else                                                                                                                              \
+        hipLaunchKernelGGL((attention_prompt_kernel<D, BF, 4>), dim3(grid), dim3(256), 0, stream, a, tiles);
     if (head_dim == 64) {
-        GO(64)
+        if (bf) {
+            GO(64, true)
+        } else {
+            GO(64, false)
+        }
     } else {
-        GO(128)
+        if (bf) {
+            GO(128, true)
+        } else {
+            GO(128, false)
+        }
     }
 #undef GO
     return launch_check("oco_cache_attention (prompt)");

@@ -10,9 +10,9 @@ pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 
 
-@pytest.fixture(params=[0, 8], ids=["", "prompt"])
+@pytest.fixture(params=[0, 8, 16], ids=["", "prompt", "long"])
 def kernel(request, lib):
-    """The kernel that the rule takes, and the one of long prompts (which heads of 256 do not have)."""
+    """The kernel that the rule takes, and the two of prompts (which heads of 256 do not have)."""
     with lib.overridden(lib.Knob.ATTENTION, (request.param,)):
         yield request.param
 
@@ -363,7 +363,7 @@ def test_shorter_bounds(kernel, lib):
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
-@pytest.mark.parametrize("tile", [1, 2, 8])
+@pytest.mark.parametrize("tile", [1, 2, 8, 16])
 @pytest.mark.parametrize("chunk", [0, 128, 384])
 def test_every_kernel_and_chunk(lib, d, tile, chunk):
     """Each kernel on few and many rows, whole and in chunks, with windows that begin inside a step."""
