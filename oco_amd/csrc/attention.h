@@ -36,6 +36,10 @@ struct Half<true> {
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
     }
+    // c + the pair's two values
+    static __device__ __forceinline__ float add(uint32_t pair, float c) {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), bf16x2{(__bf16)1.f, (__bf16)1.f}, c, false);
+    }
     static __device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
@@ -52,6 +56,9 @@ struct Half<false> {
     }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+    }
+    static __device__ __forceinline__ float add(uint32_t pair, float c) {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), f16x2{(_Float16)1.f, (_Float16)1.f}, c, false);
     }
     static __device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);

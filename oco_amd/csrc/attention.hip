@@ -233,8 +233,9 @@ __global__ __launch_bounds__(256, D * R == 64 ? 4 : D * R == 128 ? 3 : 2) void a
             float u[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) u[i] = __builtin_amdgcn_exp2f(fmaf(sc[r][i / 4][i % 4], a.c, -ref));
-            l[r] += ((u[0] + u[1]) + (u[2] + u[3])) + ((u[4] + u[5]) + (u[6] + u[7]));
             p[r] = u32x4{H::pack(u[0], u[1]), H::pack(u[2], u[3]), H::pack(u[4], u[5]), H::pack(u[6], u[7])};
+            // of the rounded probabilities: their roundings cancel where few tokens have all the weight
+            l[r] += H::add(p[r].y, H::add(p[r].x, 0.f)) + H::add(p[r].w, H::add(p[r].z, 0.f));
         }
 #pragma unroll
         for (int e = 0; e < 2; e++)

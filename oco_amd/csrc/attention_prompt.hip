@@ -269,7 +269,7 @@ __global__ __launch_bounds__(64 * W, 2) void attention_prompt_kernel(AttentionAr
         // the conversions.  Each group requests the next one's fragments, and nothing moves across groups.
         const float ref = m > -INFINITY ? m : 0.f;
         u32x4 p[2 * KN], kf[2][KN], vf[2][NO];
-        float sum = 0.f;
+        float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < KN; k++) {
 #pragma unroll
@@ -292,12 +292,15 @@ __global__ __launch_bounds__(64 * W, 2) void attention_prompt_kernel(AttentionAr
             for (int e = E * i; e < E * i + E; e++) {
                 const float u = __builtin_amdgcn_exp2f(fmaf(sc[e / 16][e % 16], a.c, -ref));
                 sc[e / 16][e % 16] = u;
-                sum += u;
-                if (e % 2) p[e / 8][e % 8 / 2] = H::pack(sc[e / 16][e % 16 - 1], u);
+                if (e % 2) {
+                    const uint32_t pair = H::pack(sc[e / 16][e % 16 - 1], u);
+                    p[e / 8][e % 8 / 2] = pair;
+                    sum[e / 2 % 2] = H::add(pair, sum[e / 2 % 2]);  // the rounded probabilities, as they weigh
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        l += sum;
+        l += sum[0] + sum[1];
 #pragma unroll
         for (int t = 0; t < 2 * KN; t++) {
             if (t + 1 < 2 * KN) {
