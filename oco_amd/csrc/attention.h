@@ -1,14 +1,13 @@
 // Attention over the paged cache: what its kernels share.
 #pragma once
 #include "cache.h"
+#include "eight.h"
 
 namespace oco {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 struct AttentionArgs {

@@ -7,7 +7,7 @@
 // the last bias for it (from 1) in the upper 12.  Maxima and counts do not
 // hang on the order of the atomics.  Then the chunk passes through registers
 // once.
-#include "rows.h"
+#include "eight.h"
 
 namespace oco {
 
@@ -20,9 +20,10 @@ struct LogitsArgs {
     uint32_t vocabulary, chunks, history_stride, bias_stride, mask_stride, group, mask_group;
 };
 
-// Words per workgroup: every workgroup of a row reads its whole history, which costs little (64 rows of 151936 f32 words:
-// 14.5 us without one, 15.0 with 512 ids, 18.2 with 8192), and 1024 threads on 16384 words are slower but there
-// (15.1, 15.8, 17.6).
+// Words per workgroup.  Every workgroup of a row reads its whole history, which costs little: 64 rows of 151936 f32 words
+// take 15.1 us with 512 ids and no mask (5.2 TB/s), 16.6 with 2048 and a mask, 19.3 with 8192 (bf16, 2048 ids: 13.9).
+// 1024 threads on 16384 words: 15.8 with 512 ids, 17.6 with 8192.  Copying the chunk while the ids are read, and mending
+// the marked words after it: 16.8 with 2048, 22.2 with 8192, 13.4 in bf16.
 constexpr uint32_t LOGITS_CHUNK = 4096;
 
 template <class T>
@@ -90,7 +91,12 @@ __global__ __launch_bounds__(256) void logits_kernel(LogitsArgs a) {
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = (m >> j) & 1 ? v[j] : -INFINITY;
         }
-        store_run(out, c, size, v);
+        Eight<T> y;
+        y.round(v);
+        if (c + 8 <= size)
+            y.store(out + c);
+        else
+            y.store_some(out + c, size - c);
     }
 }
 

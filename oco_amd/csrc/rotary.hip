@@ -8,11 +8,9 @@
 // does.  One token's pairs are the same for all its heads, so a workgroup
 // takes one token (or a slice of its heads) and keeps them in LDS.
 #include "cache.h"
+#include "eight.h"
 
 namespace oco {
-
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 // cos and sin of a: a - k pi/2 with pi/2 in two parts, then Taylor series for
 // |r| <= pi/4, whose first terms left out are r^19 / 19! and r^20 / 20! (1e-19).
@@ -82,61 +80,8 @@ __device__ __forceinline__ HeadUnits head_units(const Rotation &r, uint32_t head
 struct Unit {
     float a[8], b[8];
 };
-// The same as they are loaded.
-template <class T>
-struct Eight {
-    u32x4 w[sizeof(T) / 2];
-    __device__ __forceinline__ void load(const T *p) {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; i++) w[i] = ((const GLOBAL u32x4_u *)gp((const u32x4_u *)p))[i];
-    }
-    __device__ __forceinline__ void values(float *v) const {
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint32_t u = sizeof(T) == 4 ? w[j / 4 % (sizeof(T) / 2)][j % 4] : w[0][j / 2];
-            if constexpr (sizeof(T) == 4)
-                v[j] = __uint_as_float(u);
-            else if constexpr (std::is_same_v<T, bf16_t>)
-                v[j] = __uint_as_float(j % 2 ? u & 0xffff0000u : u << 16);
-            else
-                v[j] = half_bits_to_f32(j % 2 ? u >> 16 : u & 0xffff);
-        }
-    }
-    // rounded by the hardware's conversions
-    __device__ __forceinline__ void round(const float *v) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            if constexpr (sizeof(T) == 4) {
-                w[j / 4][j % 4] = __float_as_uint(v[j]);
-            } else if (j % 2 == 0) {
-                if constexpr (std::is_same_v<T, bf16_t>)
-                    w[0][j / 2] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)v[j], (__bf16)v[j + 1]});
-                else
-                    w[0][j / 2] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)v[j], (_Float16)v[j + 1]});
-            }
-        }
-    }
-    // Past the caches, where rows still to be read stay: 8192 rows of 32 x 128 f16 33.4 -> 24.1 us, 8192 tokens appended and
-    // read back 55 -> 47; the attention that reads the turned queries next takes as long (64 sequences of one token after
-    // their append 21.7 us either way, 8192 tokens 574 against 569).  Loads past them lost (24 -> 31).
-    __device__ __forceinline__ void store(T *p) const {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; i++) __builtin_nontemporal_store(w[i], (GLOBAL u32x4_u *)gp((u32x4_u *)p) + i);
-    }
-    // the first n of them (LDS or memory)
-    __device__ __forceinline__ void store_some(T *p, uint32_t n) const {
-#pragma unroll
-        for (uint32_t j = 0; j < 8; j++) {
-            if (j >= n) break;
-            if constexpr (sizeof(T) == 4)
-                p[j] = __uint_as_float(w[j / 4][j % 4]);
-            else
-                p[j].bits = (uint16_t)(w[0][j / 2] >> (16 * (j % 2)));
-        }
-    }
-};
 template <class T, bool INTERLEAVED>
-struct RawUnit {
+struct RawUnit {  // the same as they are loaded
     Eight<T> a, b;
     __device__ __forceinline__ void values(Unit &x) const {
         a.values(x.a);
@@ -182,14 +127,17 @@ __device__ __forceinline__ void turn_unit(Unit &x, const UnitPlace &p, const Rot
         for (int j = 0; j < 4; j++) turn_pair(x.a[2 * j], x.a[2 * j + 1], table[WHOLE ? first + j : min(first + j, last)]);
     }
 }
+// Past the caches, where rows still to be read stay: 8192 rows of 32 x 128 f16 33.4 -> 24.1 us, 8192 tokens appended and
+// read back 55 -> 47; the attention that reads the turned queries next takes as long (64 sequences of one token after
+// their append 21.7 us either way, 8192 tokens 574 against 569).  Loads past them lost (24 -> 31).
 template <class T>
 __device__ __forceinline__ void store_unit(T *head, const Unit &x, const UnitPlace &p, const Rotation &r) {
     Eight<T> y;
     y.round(x.a);
-    y.store(head + p.first);
+    y.stream(head + p.first);
     if (p.pairs) {
         y.round(x.b);
-        y.store(head + p.first + r.dim / 2);
+        y.stream(head + p.first + r.dim / 2);
     }
 }
 template <class T>
@@ -459,10 +407,10 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
         Eight<T> y;
         cache_dequantize(key, key_scale, x);
         y.round(x);
-        y.store(k + 8 * i);
+        y.stream(k + 8 * i);
         cache_dequantize(value, value_scale, x);
         y.round(x);
-        y.store(v + 8 * i);
+        y.stream(v + 8 * i);
     }
 }
 
