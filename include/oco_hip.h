@@ -109,7 +109,7 @@ typedef enum oco_knob {
                                      kernel (default: by size, among these and the few-row kernel) */
     OCO_KNOB_FP8 = 13,            /* 8-bit products: 0 the few-row kernel (up to 64 rows), 128 or 256 tiles of that size;
                                      second value (optional): K parts of the tiles */
-    OCO_KNOB_ATTENTION = 14,      /* cache attention: rows per tile / 16 (1, 2 or 8; 0: by the rule); second value (optional): tokens per
+    OCO_KNOB_ATTENTION = 14,      /* cache attention: rows per tile / 16 (1, 2, 8 or 16; 0: by the rule); second value (optional): tokens per
                                      chunk, a multiple of 128 */
     OCO_KNOB_COUNT = 15
 } oco_knob;

@@ -983,6 +983,8 @@ class PagedCache:
         page = cache_page_bytes(Cache(head_dim=head_dim, kv_heads=kv_heads, page_size=page_size))
         if page == 0:
             raise ValueError(f"no cache of {kv_heads} heads of {head_dim} in pages of {page_size} tokens")
+        if buffer is not None and buffer.nbytes < pages * page:
+            raise ValueError(f"{buffer.nbytes} bytes for {pages} pages of {page}")
         self.buffer = DeviceBuffer(pages * page) if buffer is None else buffer
 
     def batch(self, table, lengths, sequences: int, rows: int, max_rows: int, max_length: int, table_stride: int, heads: int,

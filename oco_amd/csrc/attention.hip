@@ -542,6 +542,7 @@ extern "C" int oco_cache_attention(const void *q, const void *pages, const uint3
     a.parts = (float *)workspace;
     a.q_stride = p->q_stride ? p->q_stride : (uint64_t)p->heads * p->head_dim;
     a.out_stride = p->out_stride ? p->out_stride : (uint64_t)p->heads * p->head_dim;
+    if (q == out && a.q_stride != a.out_stride) return fail(OCO_ERR_INVALID, "oco_cache_attention: in place with another stride");
     a.heads = p->heads;
     a.group = p->heads / p->kv_heads;
     a.window = p->window >= p->max_length ? 0 : p->window;

@@ -79,6 +79,9 @@ def test_attention():
     refused(attention(cache(dtype=0)), "type 0", 2)
     refused(attention(cache(heads=0)), "no heads")
     refused(attention(cache(rows=1 << 30)), "too many rows")
+    refused(attention(cache(sequences=1 << 31)), "too many rows")
+    refused(attention(cache(q_stride=2000)), "in place")
+    refused(attention(cache(out_stride=1032)), "in place")
     p = cache(sequences=1, rows=1, max_rows=1, max_length=100000, table_stride=2000)
     need = oco.cache_attention_workspace(p)
     assert need > 0 and need % 16 == 0
@@ -86,6 +89,15 @@ def test_attention():
     refused(attention(p, work=None), "workspace")
     refused(attention(p, work=ODD), "workspace")
     assert oco.cache_attention_workspace(cache(max_length=10)) == 0
+
+
+def test_pool_in_a_buffer_that_is_too_small():
+    class Small:
+        nbytes = 10 * 2 * 64 * (128 + 8) - 1
+    with pytest.raises(ValueError, match="for 10 pages"):
+        oco.PagedCache(10, 128, 2, 64, buffer=Small())
+    with pytest.raises(ValueError, match="no cache"):
+        oco.PagedCache(10, 96, 2, 64, buffer=Small())
 
 
 def test_rotate():
