@@ -20,7 +20,9 @@ struct AttentionArgs {
     uint64_t q_stride, out_stride;
     uint32_t heads, group, window;
     uint32_t tile_rows;      // rows of a tile
-    uint32_t chunks, chunk;  // parts of a tile's tokens, each of `chunk` tokens
+    uint32_t chunks, chunk;  // parts of a tile's tokens, at most, and the tokens of each, at least (attention_chunk)
+    uint32_t seen;           // the most tokens that a tile sees
+    uint32_t works, pieces[2];  // of attention_chunk; works 0: chunks have `chunk` tokens
     float c;                 // scale * log2(e)
 };
 
@@ -105,6 +107,41 @@ __device__ __forceinline__ float row_sum(float v) {
     v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
     auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+__device__ __forceinline__ float half_sum(float v) {  // over l and l ^ 32
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// Over the wavefront, uniform.
+__device__ __forceinline__ uint32_t wave_total(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, true);
+    return (uint32_t)(__builtin_amdgcn_readlane((int)v, 0) + __builtin_amdgcn_readlane((int)v, 16) + __builtin_amdgcn_readlane((int)v, 32) +
+                      __builtin_amdgcn_readlane((int)v, 48));
+}
+
+// Up to this lane.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
+// The tokens of a chunk, from the lengths as they are (of at most 64 sequences; n: what a lane's own has to be read of): all
+// of them over 2^32 / pieces[0], or pieces[1] from `works` times 128 tokens on.  Integers, for the join has to find the same.
+__device__ __forceinline__ uint32_t attention_chunk(const AttentionArgs &a, uint32_t &n) {
+    const uint32_t lane = threadIdx.x & 63;
+    n = lane < a.b.sequences ? min(a.b.lengths[lane], a.seen) : 0;
+    const uint32_t all = wave_total((n + 127) / 128);
+    return max(a.chunk, min(__umulhi(all, all < a.works ? a.pieces[0] : a.pieces[1]) + 1, 1u << 23) * 128);
 }
 
 // A tile of a sequence's rows (a token's query heads of one key-value head

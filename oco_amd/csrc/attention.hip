@@ -95,15 +95,27 @@ __global__ __launch_bounds__(256, D * R == 64 ? 4 : D * R == 128 ? 3 : 2) void a
     uint32_t id = blockIdx.x;
     const uint32_t h = id % a.b.kv_heads;
     id /= a.b.kv_heads;
-    const uint32_t chunk = id % a.chunks;
-    id /= a.chunks;
-    const uint32_t s = id % a.b.sequences, tile = tiles - 1 - id / a.b.sequences;
+    uint32_t s, tile, chunk, size = a.chunk;
+    if (a.works) {  // one tile; the chunks that there are come first
+        uint32_t n;
+        size = attention_chunk(a, n);
+        const uint32_t parts = (threadIdx.x & 63) < a.b.sequences ? max((n + size - 1) / size, 1u) : 0, to = wave_scan(parts);
+        s = __builtin_popcountll(__ballot(to <= id));
+        if (s >= a.b.sequences) return;
+        chunk = id - (uint32_t)(__builtin_amdgcn_readlane((int)to, s) - __builtin_amdgcn_readlane((int)parts, s));
+        tile = 0;
+    } else {
+        chunk = id % a.chunks;
+        id /= a.chunks;
+        s = id % a.b.sequences;
+        tile = tiles - 1 - id / a.b.sequences;
+    }
     const CacheSpan span = cache_span(a.b, s);
     const AttentionTile range = attention_tile(span, tile, 16 * R, a.group, a.window);
     const uint32_t row0 = range.first_row, rows = range.rows;
     if (row0 >= rows) return;
     const int32_t least = range.least, most = range.most;
-    const uint32_t first = range.first + chunk * a.chunk, end = min(first + a.chunk, range.end);  // this chunk's tokens
+    const uint32_t first = range.first + chunk * size, end = min(first + size, range.end);  // this chunk's tokens
     if (chunk && first >= range.end) return;  // the tile has fewer chunks
     const uint32_t head_bytes = cache_head_bytes(a.b.page_size, D);
     const uint32_t *const table = a.b.table + (uint64_t)s * a.b.table_stride;
@@ -360,17 +372,19 @@ __global__ __launch_bounds__(256, D * R == 64 ? 4 : D * R == 128 ? 3 : 2) void a
     }
 }
 
-// ---- chunks joined: a workgroup per row and head ------------------------------------------
+// ---- chunks joined: a workgroup per row and head, or a wavefront -------------------------
 
-// Eight groups of 32 lanes (D = 64: 16 of 16) take the chunks in turn.
-template <uint32_t D, bool BF>
+// Groups of 32 lanes (D = 64: 16) take the chunks in turn.  W = 4: a workgroup per row and head, the least latency; W = 1:
+// a wavefront, from 2048 of them on, where the lookups of a row's place bound it (160 rows of 64 heads of 64 in 6 chunks:
+// 62.7 -> 53.7 us with the attention; 64 rows of 32 of 128 20.9 -> 19.5; 32 rows of 32 40.2, 40.8 so).
+template <uint32_t D, bool BF, int W>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
-    constexpr uint32_t N = D / 64, LANES = D / (4 * (N > 1 ? N / 2 : 1)), GROUPS = 256 / LANES;  // 16, 32 and 32 lanes
+    constexpr uint32_t N = D / 64, LANES = D / (4 * (N > 1 ? N / 2 : 1)), GROUPS = 64 * W / LANES;  // 16, 32 and 32 lanes
     constexpr uint32_t V = D / LANES / 4;                                                            // of 4, 4 and 8 values
-    __shared__ __attribute__((aligned(16))) f32x4 so[GROUPS][LANES * V];
-    __shared__ float st[GROUPS];
-    const uint32_t row = blockIdx.x / a.heads, head = blockIdx.x % a.heads, group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
-    const uint64_t index = (uint64_t)blockIdx.x * a.chunks;
+    const uint32_t item = W == 1 ? blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
+    const uint32_t row = item / a.heads, head = item % a.heads, group = threadIdx.x % (64 * W) / LANES, lane = threadIdx.x % LANES;
+    if (W == 1 && row >= a.b.rows) return;
+    const uint64_t index = (uint64_t)item * a.chunks;
     const float *const ml = a.parts + (uint64_t)a.b.rows * a.heads * a.chunks * D + index * 2;
     const f32x4 *const parts = (const f32x4 *)(a.parts + index * D) + lane * V;
     // The first chunks are requested before it is known how many the row has; a place in the workspace that was not
@@ -393,7 +407,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
     const CacheSpan span = cache_span(a.b, s);
     if (row - span.first >= span.rows) return;
     const AttentionTile range = attention_tile(span, ((row - span.first) * a.group + head % a.group) / a.tile_rows, a.tile_rows, a.group, a.window);
-    const uint32_t used = range.end > range.first ? (range.end - range.first + a.chunk - 1) / a.chunk : 0;
+    uint32_t n, size = a.chunk;
+    if (a.works) size = attention_chunk(a, n);
+    const uint32_t used = range.end > range.first ? (range.end - range.first + size - 1) / size : 0;
     const float sink = a.sinks ? a.sinks[head] * 1.44269504088896341f : -INFINITY;
     float top = sink;
     if ((threadIdx.x & 63) < used) top = fmaxf(top, tops[0]);
@@ -417,27 +433,41 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
 #pragma unroll
         for (uint32_t j = 0; j < V; j++) o[j] += parts[(uint64_t)c * (D / 4) + j] * f;
     }
+    uint16_t *const out = (uint16_t *)a.out + (uint64_t)row * a.out_stride + (uint64_t)head * D;
+    if constexpr (W == 1) {
+        total = (GROUPS == 4 ? row_sum(total) : half_sum(total)) + carry(sink, top);
+        const float f = total > 0.f || total != total ? 1.f / total : 0.f;
 #pragma unroll
-    for (uint32_t j = 0; j < V; j++) so[group][lane * V + j] = o[j];
-    if (lane == 0) st[group] = total;
-    __syncthreads();
-    if (threadIdx.x >= D / 4) return;
-    f32x4 sum = so[0][threadIdx.x];
-    total = carry(sink, top) + st[0];
+        for (uint32_t j = 0; j < V; j++) {
 #pragma unroll
-    for (uint32_t i = 1; i < GROUPS; i++) {
-        sum += so[i][threadIdx.x];
-        total += st[i];
+            for (int i = 0; i < 4; i++) o[j][i] = (GROUPS == 4 ? row_sum(o[j][i]) : half_sum(o[j][i])) * f;
+            if (group == 0) *(GLOBAL u32x2_u *)gp(out + 4 * (lane * V + j)) = u32x2_u{Half<BF>::pack(o[j][0], o[j][1]), Half<BF>::pack(o[j][2], o[j][3])};
+        }
+    } else {
+        __shared__ __attribute__((aligned(16))) f32x4 so[GROUPS][LANES * V];
+        __shared__ float st[GROUPS];
+#pragma unroll
+        for (uint32_t j = 0; j < V; j++) so[group][lane * V + j] = o[j];
+        if (lane == 0) st[group] = total;
+        __syncthreads();
+        if (threadIdx.x >= D / 4) return;
+        f32x4 sum = so[0][threadIdx.x];
+        total = carry(sink, top) + st[0];
+#pragma unroll
+        for (uint32_t i = 1; i < GROUPS; i++) {
+            sum += so[i][threadIdx.x];
+            total += st[i];
+        }
+        const float f = total > 0.f || total != total ? 1.f / total : 0.f;
+        *(GLOBAL u32x2_u *)gp(out + 4 * threadIdx.x) = u32x2_u{Half<BF>::pack(sum[0] * f, sum[1] * f), Half<BF>::pack(sum[2] * f, sum[3] * f)};
     }
-    const float f = total > 0.f || total != total ? 1.f / total : 0.f;
-    uint16_t *const out = (uint16_t *)a.out + (uint64_t)row * a.out_stride + (uint64_t)head * D + 4 * threadIdx.x;
-    *(GLOBAL u32x2_u *)gp(out) = u32x2_u{Half<BF>::pack(sum[0] * f, sum[1] * f), Half<BF>::pack(sum[2] * f, sum[3] * f)};
 }
 
 // ---- choices and launches -------------------------------------------------------------------
 
 struct AttentionPlan {
     uint32_t tile, tiles, chunks, chunk;  // tile: its rows / 16
+    uint32_t seen, works, pieces[2];  // as in AttentionArgs
     uint64_t bytes;
 };
 static AttentionPlan attention_plan(const oco_cache *p) {
@@ -462,11 +492,11 @@ static AttentionPlan attention_plan(const oco_cache *p) {
     const uint64_t tile_tokens = (16 * l.tile + p->heads / p->kv_heads - 1) / (p->heads / p->kv_heads);
     uint64_t seen = p->max_length;
     if (p->window && p->window + tile_tokens + 31 < seen) seen = p->window + tile_tokens + 31;
+    l.seen = (uint32_t)seen;
     const uint64_t blocks = (uint64_t)p->sequences * p->kv_heads * l.tiles;
     const bool prompt = l.tile >= 8;
-    // Chunks until the card is full: 3072 workgroups of few rows, of at least two steps per wavefront (32 sequences of up to
-    // 16384 tokens: 1152 to 2048 tokens a chunk 75 to 78 us, 4096 74 to 95 by how they divide, 256 104; one of 4101: 256
-    // tokens 9.2, 512 10.9), 512 of a prompt's tiles.
+    // Chunks at most and their tokens at least: 3072 workgroups of few rows, of at least two steps per wavefront (one sequence
+    // of 4101: 256 tokens 8.5 us, 384 9.1, 512 9.7), 512 of a prompt's tiles.
     const uint64_t wanted = prompt ? 512 : 3072;
     uint64_t chunks = blocks ? (wanted + blocks - 1) / blocks : 1;
     const uint64_t least = prompt ? 512 : 256;
@@ -481,6 +511,23 @@ static AttentionPlan attention_plan(const oco_cache *p) {
     if (l.chunk == 0) l.chunk = 128;
     l.chunks = (uint32_t)((seen + l.chunk - 1) / l.chunk);
     if (l.chunks < 1) l.chunks = 1;
+    // Where a sequence has one tile and there is enough to do, the kernel chooses the chunks' tokens from the lengths as they
+    // are (attention_chunk) and numbers the chunks that there are one after the other, for workgroups that end at once leave
+    // others unevenly spread.  Then as many workgroups fit the card as it holds (twice that of tiles of 32, which compute
+    // more), or two per compute unit where that leaves them under 680 tokens.  us, 3072 workgroups at most -> so, 128 wide:
+    // 8 sequences of 4101 tokens 17.1 -> 15.2, 32 41.4 -> 37.5, 32 of up to 4101 26.9 -> 25.0, 64 of up to 1001 21.6 -> 19.4,
+    // 32 of up to 16384 80.1 -> 74.9 (4 per compute unit 86.6, 6 75.7), one of 64001 31.6 -> 21.5 (3: 23.3); 256 wide, 2 per
+    // compute unit 80.2 -> 72.8 (3: 82.2); 64 wide, 4 54.4 -> 49.3 (3: 53.3); 5 x 4 rows, 4 112.9 -> 104.4 (2: 121.2).
+    l.works = 0;
+    if (l.chunks > 1 && !(set > 1 && knob[1] > 0) && !prompt && l.tiles == 1 && p->sequences <= 64 &&
+        (uint64_t)p->sequences * seen * p->kv_heads > 640 * 256) {
+        const uint32_t resident = l.tile == 1 ? (p->head_dim == 64 ? 4 : p->head_dim == 128 ? 3 : 2) : 2 * (p->head_dim == 64 ? 3 : 2);
+        l.works = 2048 * 256 / 128 / p->kv_heads + 1;
+        for (int i = 0; i < 2; i++) {  // 2^32 / parts, half a part of each sequence left for its last one
+            const uint32_t all = 256 * (i ? resident : 2) / p->kv_heads, parts = all > p->sequences / 2 + 1 ? all - p->sequences / 2 : 1;
+            l.pieces[i] = parts > 1 ? 0xffffffffu / parts + 1 : 0xffffffffu;
+        }
+    }
     l.bytes = l.chunks > 1 ? (uint64_t)p->rows * p->heads * l.chunks * (p->head_dim + 2) * 4 : 0;
     return l;
 }
@@ -497,7 +544,10 @@ static int attention_launch(const AttentionArgs &a, const AttentionPlan &l, hipS
         OCO_TRY(attention_prompt_launch(a, D, BF, l.tiles, (uint32_t)grid, stream));
     OCO_TRY(launch_check("oco_cache_attention"));
     if (l.chunks > 1) {
-        hipLaunchKernelGGL((attention_join_kernel<D, BF>), dim3(a.b.rows * a.heads), dim3(256), 0, stream, a);
+        if (a.b.rows * a.heads >= 2048)
+            hipLaunchKernelGGL((attention_join_kernel<D, BF, 1>), dim3((a.b.rows * a.heads + 3) / 4), dim3(256), 0, stream, a);
+        else
+            hipLaunchKernelGGL((attention_join_kernel<D, BF, 4>), dim3(a.b.rows * a.heads), dim3(256), 0, stream, a);
         OCO_TRY(launch_check("oco_cache_attention (join)"));
     }
     return OCO_OK;
@@ -549,6 +599,9 @@ extern "C" int oco_cache_attention(const void *q, const void *pages, const uint3
     a.tile_rows = 16 * l.tile;
     a.chunks = l.chunks;
     a.chunk = l.chunk;
+    a.seen = l.seen;
+    a.works = l.works;
+    for (int i = 0; i < 2; i++) a.pieces[i] = l.pieces[i];
     a.c = (p->scale != 0.f ? p->scale : 1.f / sqrtf((float)p->head_dim)) * 1.44269504088896341f;
     hipStream_t st = (hipStream_t)stream;
     const bool bf = p->dtype == OCO_DT_BF16;

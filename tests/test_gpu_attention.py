@@ -408,3 +408,54 @@ def test_a_cache_past_32_bits(kernel, lib):
         lib.synchronize()
         c.check()
         big.free()
+
+
+@pytest.mark.parametrize("d,rows,window", [(64, 8, 0), (64, 1, 700), (128, 16, 0), (256, 3, 0)])
+@pytest.mark.parametrize("sequences", [1, 3, 20, 64, 65])
+def test_chunks_by_the_lengths(lib, d, rows, window, sequences):
+    """Bounds far past the lengths, as a captured step has them: chunks follow the lengths, of sequences without rows or tokens too."""
+    rng = np.random.default_rng(d + sequences)
+    n = [int(i) for i in rng.integers(0 if sequences > 3 else 1, rows + 1, sequences)]
+    lengths = [int(i) for i in rng.integers(0, 1500 if sequences < 20 else 300, sequences)]
+    c = Case(lib, rng, n, lengths, 4, 2, d, 16, "bf16", window=window, sinks=True, holes=sequences % 2, max_rows=rows)
+    c.p.max_length = 100000 // sequences
+    stride = c.p.max_length // 16 + 1
+    c.p.table_stride = stride
+    c.dev[2] = dev(lib, np.ascontiguousarray(np.pad(c.b.table, ((0, 0), (0, stride - c.b.table.shape[1])))))
+    c.need = lib.cache_attention_workspace(c.p)
+    c.work = Guarded(lib, c.need)
+    assert c.need
+    say("chunks", d, n[:8], lengths[:8])
+    c.call()
+    lib.synchronize()
+    c.check()
+
+
+@pytest.mark.parametrize("d,rows,heads,kv", [(64, 1, 16, 8), (128, 1, 16, 4), (128, 8, 16, 4), (256, 1, 8, 8)])
+@pytest.mark.parametrize("even", [False, True])
+def test_long_sequences_in_chunks(lib, d, rows, heads, kv, even):
+    """As in chunks of 4096 tokens, each within the roundings of its probabilities and of its result."""
+    rng = np.random.default_rng(d + rows + even)
+    S, P, longest = 12, 64, 20000
+    lengths = np.full(S, longest) if even else rng.integers(rows, longest, S)
+    p = lib.Cache(head_dim=d, heads=heads, kv_heads=kv, page_size=P, pages=40, sequences=S, rows=S * rows, max_rows=rows, max_length=longest,
+                  table_stride=longest // P + 1, dtype=1)
+    pool = rng.integers(0, 256, (40, kv, P * d + P * d // 16), dtype=np.uint8)
+    pool[:, :, P * d:] = rng.integers(124, 128, pool[:, :, P * d:].shape)
+    buffers = [dev(lib, stored(rng.normal(size=(S * rows, heads * d)), "bf16")[0]), dev(lib, pool), dev(lib, rng.integers(0, 40, (S, p.table_stride)).astype(np.uint32)),
+               dev(lib, lengths.astype(np.uint32))]
+    got = []
+    for knob in ((0, 4096), (0,)):
+        with lib.overridden(lib.Knob.ATTENTION, knob):
+            need = lib.cache_attention_workspace(p)
+            work, out = Guarded(lib, need), Guarded(lib, S * rows * heads * d * 2)
+            say("long", d, rows, even, knob)
+            lib.cache_attention(buffers[0], buffers[1], buffers[2], buffers[3], out.ptr, p, workspace=work.ptr, workspace_bytes=need)
+            lib.synchronize()
+            work.read(np.uint8)
+            got.append(values(out.read(np.uint8), "bf16", (S * rows, heads, d)))
+    # values up to 6 * 2: each side's probabilities round by half a step of bf16, of weights that add up to 1, and its result
+    # by half a step of itself; f32 sums of 20000 terms, 2 * 2^-24 a term, and of scores up to about 500
+    assert np.isfinite(got[0]).all()
+    bound = 12 * (2.0 ** -8 + 20000 * 2.0 ** -23 + 4 * 500 * 2.0 ** -23)
+    assert np.abs(got[0] - got[1]).max() <= 2 * bound + 2.0 ** -8 * (np.abs(got[0]).max() + np.abs(got[1]).max())
