@@ -109,7 +109,7 @@ typedef enum oco_knob {
                                      kernel (default: by size, among these and the few-row kernel) */
     OCO_KNOB_FP8 = 13,            /* 8-bit products: 0 the few-row kernel (up to 64 rows), 128 or 256 tiles of that size;
                                      second value (optional): K parts of the tiles */
-    OCO_KNOB_ATTENTION = 14,      /* cache attention: rows per tile / 16 (1, 2, 8 or 16; 0: by the rule); second value (optional): tokens per
+    OCO_KNOB_ATTENTION = 14,      /* cache attention: rows per tile / 16 (1, 2, 3, 8 or 16; 0: by the rule); second value (optional): tokens per
                                      chunk, a multiple of 128 */
     OCO_KNOB_COUNT = 15
 } oco_knob;
@@ -726,7 +726,9 @@ int oco_cache_read(const void *pages, const uint32_t *table, const uint32_t *sta
  * page that is not in the pool reads as NaN, and so does, in f16, a block with
  * a scale past 2^13 (append gives it values past 65504 alone).  q and out are
  * bf16 or f16; the probabilities are rounded to that type, sums are f32.  out
- * may be q where their strides agree.
+ * may be q where their strides agree.  How the tokens are split over
+ * workgroups, and with it the roundings, goes by the whole batch; the same
+ * call gives the same bits.
  *   workspace: oco_cache_attention_workspace bytes (0 for a description that is
  *   refused, and where none is needed), 16-byte aligned; calls sharing one must be ordered */
 uint64_t oco_cache_attention_workspace(const oco_cache *p);

@@ -16,13 +16,15 @@ struct AttentionArgs {
     const void *q;
     void *out;
     const float *sinks;
-    float *parts;  // [rows][heads][chunks][D], then m and l [rows][heads][chunks][2]
+    float *parts;  // [rows][heads][chunks][D], then m and l [rows][heads][chunks][2], then a chunk's tokens (u32)
     uint64_t q_stride, out_stride;
     uint32_t heads, group, window;
     uint32_t tile_rows;      // rows of a tile
     uint32_t chunks, chunk;  // parts of a tile's tokens, at most, and the tokens of each, at least (attention_chunk)
     uint32_t seen;           // the most tokens that a tile sees
-    uint32_t works, pieces[2];  // of attention_chunk; works 0: chunks have `chunk` tokens
+    uint32_t works;          // 0: chunks have `chunk` tokens; else attention_chunk's: what is more goes into
+    uint32_t pieces[2];      // pieces[1] chunks, what is less into pieces[0]
+    float inverse[2], relaxed[2];  // of pieces, and of as many less half a piece per sequence
     float c;                 // scale * log2(e)
 };
 
@@ -135,13 +137,36 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
     return v;
 }
 
-// The tokens of a chunk, from the lengths as they are (of at most 64 sequences; n: what a lane's own has to be read of): all
-// of them over 2^32 / pieces[0], or pieces[1] from `works` times 128 tokens on.  Integers, for the join has to find the same.
-__device__ __forceinline__ uint32_t attention_chunk(const AttentionArgs &a, uint32_t &n) {
-    const uint32_t lane = threadIdx.x & 63;
-    n = lane < a.b.sequences ? min(a.b.lengths[lane], a.seen) : 0;
-    const uint32_t all = wave_total((n + 127) / 128);
-    return max(a.chunk, min(__umulhi(all, all < a.works ? a.pieces[0] : a.pieces[1]) + 1, 1u << 23) * 128);
+// A workgroup's sequence and chunk where chunks are sized by the lengths as they are (of at most 64 sequences, a lane's
+// each) and numbered one after the other: the least of a few sizes that leave no more chunks than wanted.
+struct AttentionPart {
+    uint32_t sequence, chunk, size;  // sequence past the last one: there is none
+    CacheSpan span;
+};
+__device__ __forceinline__ AttentionPart attention_part(const AttentionArgs &a, uint32_t id) {
+    const uint32_t lane = threadIdx.x & 63, mine = min(lane, a.b.sequences - 1);
+    const CacheSpan own = cache_span(a.b, mine);
+    const uint32_t n = lane < a.b.sequences ? min(own.length, a.seen) : 0, units = (n + 127) / 128;
+    const uint32_t all = wave_total(units), k = all < a.works ? 0 : 1;
+    const float least = fmaxf(ceilf((float)all * a.inverse[k]), 1.f);
+    float size = fmaxf(least, ceilf((float)all * a.relaxed[k]));
+#pragma unroll
+    for (int j = 0; j < 3; j++) {
+        const float c = ceilf(least * (1.f + 0.125f * j));
+        if (wave_total((uint32_t)ceilf((float)units * (__builtin_amdgcn_rcpf(c) * 0.9999998f))) <= a.pieces[k]) {
+            size = c;
+            break;
+        }
+    }
+    AttentionPart p;
+    p.size = max(a.chunk, (uint32_t)fminf(size, 8388608.f) * 128);
+    const uint32_t parts = lane < a.b.sequences ? max((n + p.size - 1) / p.size, 1u) : 0, to = wave_scan(parts);
+    p.sequence = __builtin_popcountll(__ballot(to <= id));
+    const uint32_t s = min(p.sequence, 63u);
+    p.chunk = id - (uint32_t)(__builtin_amdgcn_readlane((int)to, s) - __builtin_amdgcn_readlane((int)parts, s));
+    p.span = CacheSpan{(uint32_t)__builtin_amdgcn_readlane((int)own.first, s), (uint32_t)__builtin_amdgcn_readlane((int)own.rows, s),
+                       (uint32_t)__builtin_amdgcn_readlane((int)own.length, s)};
+    return p;
 }
 
 // A tile of a sequence's rows (a token's query heads of one key-value head

@@ -86,7 +86,8 @@ __device__ __forceinline__ Halves load_halves(const uint32_t *table, uint32_t t0
     return h;
 }
 
-template <uint32_t D, bool BF, int R>
+// FIT: chunks by the lengths (attention_part), one tile per sequence.
+template <uint32_t D, bool BF, int R, bool FIT>
 __global__ __launch_bounds__(256, D * R == 64 ? 4 : D * R == 128 ? 3 : 2) void attention_kernel(AttentionArgs a, uint32_t tiles) {
     constexpr int KW = D / 32, NT = D / 16;  // key words per lane and token; tiles of 16 columns
     using H = Half<BF>;
@@ -96,21 +97,23 @@ __global__ __launch_bounds__(256, D * R == 64 ? 4 : D * R == 128 ? 3 : 2) void a
     const uint32_t h = id % a.b.kv_heads;
     id /= a.b.kv_heads;
     uint32_t s, tile, chunk, size = a.chunk;
-    if (a.works) {  // one tile; the chunks that there are come first
-        uint32_t n;
-        size = attention_chunk(a, n);
-        const uint32_t parts = (threadIdx.x & 63) < a.b.sequences ? max((n + size - 1) / size, 1u) : 0, to = wave_scan(parts);
-        s = __builtin_popcountll(__ballot(to <= id));
-        if (s >= a.b.sequences) return;
-        chunk = id - (uint32_t)(__builtin_amdgcn_readlane((int)to, s) - __builtin_amdgcn_readlane((int)parts, s));
+    CacheSpan span;
+    if constexpr (FIT) {
+        const AttentionPart part = attention_part(a, id);
+        s = part.sequence;
+        chunk = part.chunk;
+        size = part.size;
+        span = part.span;
         tile = 0;
+        if (blockIdx.x == 0 && threadIdx.x == 0) *gp((uint32_t *)(a.parts + (uint64_t)a.b.rows * a.heads * a.chunks * (D + 2))) = size;
+        if (s >= a.b.sequences) return;
     } else {
         chunk = id % a.chunks;
         id /= a.chunks;
         s = id % a.b.sequences;
         tile = tiles - 1 - id / a.b.sequences;
+        span = cache_span(a.b, s);
     }
-    const CacheSpan span = cache_span(a.b, s);
     const AttentionTile range = attention_tile(span, tile, 16 * R, a.group, a.window);
     const uint32_t row0 = range.first_row, rows = range.rows;
     if (row0 >= rows) return;
@@ -155,7 +158,7 @@ __global__ __launch_bounds__(256, D * R == 64 ? 4 : D * R == 128 ? 3 : 2) void a
     }
     // A step's tokens are requested before the step before it is computed; where that does not leave the
     // registers for it (STAGED), the keys once that step's are used up, and its values likewise.
-    constexpr bool STAGED = D * R >= 512;  // 256 wide, 32 rows
+    constexpr bool STAGED = D * R >= 384;  // 256 wide, 32 rows
     struct Step {
         Keys<D> k[2];
         Values<D> v[2];
@@ -402,13 +405,12 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
             for (uint32_t j = 0; j < V; j++) part[k][j] = ((const GLOBAL f32x4 *)gp(parts))[(uint64_t)c * (D / 4) + j];
         }
     }
+    const uint32_t size = a.works ? *gp((const uint32_t *)(a.parts + (uint64_t)a.b.rows * a.heads * a.chunks * (D + 2))) : a.chunk;
     const uint32_t s = cache_sequence(a.b, row);
     if (s >= a.b.sequences) return;
     const CacheSpan span = cache_span(a.b, s);
     if (row - span.first >= span.rows) return;
     const AttentionTile range = attention_tile(span, ((row - span.first) * a.group + head % a.group) / a.tile_rows, a.tile_rows, a.group, a.window);
-    uint32_t n, size = a.chunk;
-    if (a.works) size = attention_chunk(a, n);
     const uint32_t used = range.end > range.first ? (range.end - range.first + size - 1) / size : 0;
     const float sink = a.sinks ? a.sinks[head] * 1.44269504088896341f : -INFINITY;
     float top = sink;
@@ -468,33 +470,20 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
 struct AttentionPlan {
     uint32_t tile, tiles, chunks, chunk;  // tile: its rows / 16
     uint32_t seen, works, pieces[2];  // as in AttentionArgs
+    uint64_t grid;                    // workgroups per head
     uint64_t bytes;
 };
-static AttentionPlan attention_plan(const oco_cache *p) {
+// The tiles' split along the tokens.
+static AttentionPlan attention_split(const oco_cache *p, uint32_t tile, uint64_t rows, uint32_t chunk) {
     AttentionPlan l;
-    const uint64_t rows = (uint64_t)(p->max_rows < p->rows ? p->max_rows : p->rows) * (p->heads / p->kv_heads);
-    // Tiles of 16 rows while that is all, of 32 beyond (of 16 where the second one would be half empty).  With narrow heads
-    // the prompts' kernel: tiles of 128 rows from 256 of them on, one per compute unit, and of 256 from 512 of those on.  us,
-    // tiles of 16 / 32 / 128 / 256:
-    // 32 sequences of 5 x 4 rows over 8000 tokens, 128 wide 115 / 84 / 141; 8 of 5 x 8 rows, 64 wide 20.7 / 22.1 / 33;
-    // 4 of 128 x 4 rows over 2000 (128 tiles of 128) 41 / 33 / 49; 16 of 64 x 4 over 4000 (256, 128 of 256) 142 / 108 / 86 / 113;
-    // 64 of 32 x 4 over 1000 (512) 92 / 75 / 49; 2048 x 4 rows from the start on (512, 256 of 256) 65 with 32 / 52 / 63;
-    // 4096 x 4 rows over 8192 (512 of 256) 715 / 567 / 381 / 365, 256 wide (16 heads) 623 / 443.
-    int32_t knob[4];
-    const int set = plan_override(OCO_KNOB_ATTENTION, knob);
-    const bool narrow = p->head_dim <= 128;
-    const uint64_t heads = (uint64_t)p->kv_heads * p->sequences;
-    l.tile = rows <= 16 || (rows > 32 && rows <= 48) ? 1 : 2;
-    if (narrow && rows >= 128 && (rows + 127) / 128 * heads >= 256) l.tile = (rows + 255) / 256 * heads >= 512 ? 16 : 8;
-    if (set && (knob[0] == 1 || knob[0] == 2 || ((knob[0] == 8 || knob[0] == 16) && narrow))) l.tile = (uint32_t)knob[0];
-    l.tiles = (uint32_t)((rows + 16 * l.tile - 1) / (16 * l.tile));
-    // the most tokens that a tile sees
-    const uint64_t tile_tokens = (16 * l.tile + p->heads / p->kv_heads - 1) / (p->heads / p->kv_heads);
+    l.tile = tile;
+    l.tiles = (uint32_t)((rows + 16 * tile - 1) / (16 * tile));
+    const uint64_t tile_tokens = (16 * tile + p->heads / p->kv_heads - 1) / (p->heads / p->kv_heads);
     uint64_t seen = p->max_length;
     if (p->window && p->window + tile_tokens + 31 < seen) seen = p->window + tile_tokens + 31;
     l.seen = (uint32_t)seen;
     const uint64_t blocks = (uint64_t)p->sequences * p->kv_heads * l.tiles;
-    const bool prompt = l.tile >= 8;
+    const bool prompt = tile >= 8;
     // Chunks at most and their tokens at least: 3072 workgroups of few rows, of at least two steps per wavefront (one sequence
     // of 4101: 256 tokens 8.5 us, 384 9.1, 512 9.7), 512 of a prompt's tiles.
     const uint64_t wanted = prompt ? 512 : 3072;
@@ -505,43 +494,92 @@ static AttentionPlan attention_plan(const oco_cache *p) {
     const uint64_t part = (uint64_t)p->rows * p->heads * (p->head_dim + 2) * 4;
     if (part && (16ull << 20) / part < most) most = (16ull << 20) / part;
     if (chunks > most) chunks = most;
+    // Whole where the join costs more than a split saves (us, split / whole, 128 wide, tokens x tiles: 505 x 8 8.8 / 6.7, 755 x 8
+    // 8.5 / 8.2, 1005 x 8 8.4 / 9.6; 505 x 256 12.2 / 7.9, 1255 x 256 15.8 / 13.1, 3005 x 256 28.6 / 29.8; 3005 x 512 47.8 /
+    // 41.6; up to 2005 x 256 17.2 / 18.0; 256 wide 755 x 32 10.0 / 11.1, 1255 x 128 19.4 / 16.6)
+    const uint64_t whole = blocks > 512 ? 3072 : 6 * blocks;
+    if (!prompt && seen <= (whole > 768 ? whole : p->head_dim > 128 ? 512 : 768)) chunks = 1;
     if (chunks < 1) chunks = 1;
-    l.chunk = (uint32_t)(((seen + chunks - 1) / chunks + 127) / 128 * 128);
-    if (set > 1 && knob[1] > 0 && knob[1] % 128 == 0) l.chunk = (uint32_t)knob[1];
+    l.chunk = chunk ? chunk : (uint32_t)(((seen + chunks - 1) / chunks + 127) / 128 * 128);
     if (l.chunk == 0) l.chunk = 128;
     l.chunks = (uint32_t)((seen + l.chunk - 1) / l.chunk);
     if (l.chunks < 1) l.chunks = 1;
-    // Where a sequence has one tile and there is enough to do, the kernel chooses the chunks' tokens from the lengths as they
-    // are (attention_chunk) and numbers the chunks that there are one after the other, for workgroups that end at once leave
-    // others unevenly spread.  Then as many workgroups fit the card as it holds (twice that of tiles of 32, which compute
-    // more), or two per compute unit where that leaves them under 680 tokens.  us, 3072 workgroups at most -> so, 128 wide:
-    // 8 sequences of 4101 tokens 17.1 -> 15.2, 32 41.4 -> 37.5, 32 of up to 4101 26.9 -> 25.0, 64 of up to 1001 21.6 -> 19.4,
-    // 32 of up to 16384 80.1 -> 74.9 (4 per compute unit 86.6, 6 75.7), one of 64001 31.6 -> 21.5 (3: 23.3); 256 wide, 2 per
-    // compute unit 80.2 -> 72.8 (3: 82.2); 64 wide, 4 54.4 -> 49.3 (3: 53.3); 5 x 4 rows, 4 112.9 -> 104.4 (2: 121.2).
-    l.works = 0;
-    if (l.chunks > 1 && !(set > 1 && knob[1] > 0) && !prompt && l.tiles == 1 && p->sequences <= 64 &&
-        (uint64_t)p->sequences * seen * p->kv_heads > 640 * 256) {
-        const uint32_t resident = l.tile == 1 ? (p->head_dim == 64 ? 4 : p->head_dim == 128 ? 3 : 2) : 2 * (p->head_dim == 64 ? 3 : 2);
-        l.works = 2048 * 256 / 128 / p->kv_heads + 1;
-        for (int i = 0; i < 2; i++) {  // 2^32 / parts, half a part of each sequence left for its last one
-            const uint32_t all = 256 * (i ? resident : 2) / p->kv_heads, parts = all > p->sequences / 2 + 1 ? all - p->sequences / 2 : 1;
-            l.pieces[i] = parts > 1 ? 0xffffffffu / parts + 1 : 0xffffffffu;
+    l.grid = (uint64_t)p->sequences * l.tiles * l.chunks;
+    l.pieces[0] = l.pieces[1] = l.works = 0;
+    // With one tile per sequence and enough to do, over 640 tokens of a head for each compute unit, the kernel sizes the
+    // chunks by the lengths as they are, which may be far under max_length and far apart, and numbers those that there are one
+    // after the other: workgroups that end at once leave the others unevenly spread.  As many as the card holds at once
+    // (twice as many of 32 rows), or two per compute unit where that leaves them under 700 tokens or so.
+    // us, by max_length alone -> so, 128 wide, a row of 4 heads: 8 sequences of 4101 tokens 17.1 -> 15.4, 32 of them 41.4 ->
+    // 36.3, 32 of up to 4101 26.9 -> 23.4, 64 of up to 1001 21.6 -> 19.6, one of 64001 31.6 -> 21.7 (3 per compute unit 23.7),
+    // 32 of up to 16384 80.1 -> 76 (2: 83.6, 4: 88.5); 256 wide, 2 80.2 -> 73.2 (3: 84.4); 64 wide, 4 54.4 -> 50.8 (3: 56.4);
+    // 5 x 4 rows, 4 112.9 -> 105.7 (2: 121.1).
+    const uint64_t all = (uint64_t)p->sequences * ((seen + 127) / 128);
+    if (l.chunks > 1 && !chunk && !prompt && l.tiles == 1 && p->sequences <= 64 && all * p->kv_heads > 640 * 2) {
+        const uint32_t held = p->head_dim == 64 ? 4 : p->head_dim == 128 ? 3 : 2, per[2] = {2, tile == 1 ? held : tile == 2 ? 4 : 2};
+        l.works = 2048 * 2 / p->kv_heads + 1;
+        uint64_t grid = 0;
+        for (uint32_t i = 0; i < 2; i++) {
+            l.pieces[i] = 256 * per[i] / p->kv_heads;
+            if (l.pieces[i] == 0) l.pieces[i] = 1;
+            // sizes of at least all / pieces make pieces and one per sequence at most
+            if ((i == 0 || all >= l.works) && l.pieces[i] + p->sequences + 1 > grid) grid = l.pieces[i] + p->sequences + 1;
         }
+        if (grid < l.grid) l.grid = grid;
     }
-    l.bytes = l.chunks > 1 ? (uint64_t)p->rows * p->heads * l.chunks * (p->head_dim + 2) * 4 : 0;
+    l.bytes = l.chunks > 1 ? (uint64_t)p->rows * p->heads * l.chunks * (p->head_dim + 2) * 4 + 16 : 0;
     return l;
+}
+
+static AttentionPlan attention_plan(const oco_cache *p) {
+    const uint64_t rows = (uint64_t)(p->max_rows < p->rows ? p->max_rows : p->rows) * (p->heads / p->kv_heads);
+    // Tiles of 16 rows while that is all, of 32 beyond (of 16 where the second one would be half empty, or one of 48 with
+    // over 3000 tokens of a head for each compute unit).  With narrow heads the prompts' kernel: tiles of 128 rows from 256
+    // of them on, one per compute unit, and of 256 from 512 of those on.  us, tiles of 16 / 32 / 128 / 256:
+    // 32 sequences of 5 x 4 rows over 8000 tokens, 128 wide 115 / 84 / 141; 8 of 5 x 8 rows, 64 wide 20.7 / 22.1 / 33;
+    // 4 of 128 x 4 rows over 2000 (128 tiles of 128) 41 / 33 / 49; 16 of 64 x 4 over 4000 (256, 128 of 256) 142 / 108 / 86 / 113;
+    // 64 of 32 x 4 over 1000 (512) 92 / 75 / 49; 2048 x 4 rows from the start on (512, 256 of 256) 65 with 32 / 52 / 63;
+    // 4096 x 4 rows over 8192 (512 of 256) 715 / 567 / 381 / 365, 256 wide (16 heads) 623 / 443.
+    // Tiles of 16 / 48, 5 x 8 rows: 32 sequences of 4005 tokens, 64 wide 54 / 42, 128 wide 85 / 59, of up to 8192 64 wide 63 / 59,
+    // 128 wide 89 / 76; 8 of up to 8192, 64 wide 20.7 / 21.8; two of 2000 9.3 / 11.6.
+    int32_t knob[4];
+    const int set = plan_override(OCO_KNOB_ATTENTION, knob);
+    const bool narrow = p->head_dim <= 128;
+    const uint64_t heads = (uint64_t)p->kv_heads * p->sequences;
+    uint32_t tile = rows <= 16 || (rows > 32 && rows <= 48) ? 1 : 2;
+    if (narrow && rows > 32 && rows <= 48 && heads * p->max_length > 3000 * 256) tile = 3;
+    if (narrow && rows >= 128 && (rows + 127) / 128 * heads >= 256) tile = (rows + 255) / 256 * heads >= 512 ? 16 : 8;
+    if (set && (knob[0] == 1 || knob[0] == 2 || ((knob[0] == 3 || knob[0] == 8 || knob[0] == 16) && narrow))) tile = (uint32_t)knob[0];
+    const uint32_t chunk = set > 1 && knob[1] > 0 && knob[1] % 128 == 0 ? (uint32_t)knob[1] : 0;
+    return attention_split(p, tile, rows, chunk);
 }
 
 template <uint32_t D, bool BF>
 static int attention_launch(const AttentionArgs &a, const AttentionPlan &l, hipStream_t stream) {
-    const uint64_t grid = (uint64_t)a.b.sequences * a.b.kv_heads * l.tiles * l.chunks;
+    const uint64_t grid = l.grid * a.b.kv_heads;
     if (grid > 0x7fffffffull) return fail(OCO_ERR_INVALID, "oco_cache_attention: too many rows for one call");
-    if (l.tile == 1)
-        hipLaunchKernelGGL((attention_kernel<D, BF, 1>), dim3((uint32_t)grid), dim3(256), 0, stream, a, l.tiles);
-    else if (l.tile == 2)
-        hipLaunchKernelGGL((attention_kernel<D, BF, 2>), dim3((uint32_t)grid), dim3(256), 0, stream, a, l.tiles);
-    else
+#define GO(R, FIT) hipLaunchKernelGGL((attention_kernel<D, BF, R, FIT>), dim3((uint32_t)grid), dim3(256), 0, stream, a, l.tiles)
+    if (l.tile >= 8) {
         OCO_TRY(attention_prompt_launch(a, D, BF, l.tiles, (uint32_t)grid, stream));
+    } else if (l.tile == 3) {
+        if constexpr (D <= 128) {
+            if (l.works)
+                GO(3, true);
+            else
+                GO(3, false);
+        }
+    } else if (l.tile == 2) {
+        if (l.works)
+            GO(2, true);
+        else
+            GO(2, false);
+    } else {
+        if (l.works)
+            GO(1, true);
+        else
+            GO(1, false);
+    }
+#undef GO
     OCO_TRY(launch_check("oco_cache_attention"));
     if (l.chunks > 1) {
         if (a.b.rows * a.heads >= 2048)
@@ -601,7 +639,11 @@ extern "C" int oco_cache_attention(const void *q, const void *pages, const uint3
     a.chunk = l.chunk;
     a.seen = l.seen;
     a.works = l.works;
-    for (int i = 0; i < 2; i++) a.pieces[i] = l.pieces[i];
+    for (int i = 0; i < 2; i++) {
+        a.pieces[i] = l.pieces[i];
+        a.inverse[i] = 1.f / (float)l.pieces[i];
+        a.relaxed[i] = l.pieces[i] > p->sequences / 2 + 1 ? 1.f / (float)(l.pieces[i] - p->sequences / 2) : 1.f;
+    }
     a.c = (p->scale != 0.f ? p->scale : 1.f / sqrtf((float)p->head_dim)) * 1.44269504088896341f;
     hipStream_t st = (hipStream_t)stream;
     const bool bf = p->dtype == OCO_DT_BF16;
