@@ -110,9 +110,17 @@ __global__ __launch_bounds__(256, D * R == 64 ? 4 : D * R == 128 ? 3 : 2) void a
     } else {
         chunk = id % a.chunks;
         id /= a.chunks;
-        s = id % a.b.sequences;
-        tile = tiles - 1 - id / a.b.sequences;
-        span = cache_span(a.b, s);
+        if constexpr (R == 2) {
+            const AttentionPlace place = attention_place<16 * R>(a, id, tiles);
+            s = place.sequence;
+            tile = place.tile;
+            span = place.span;
+            if (s >= a.b.sequences) return;
+        } else {  // three tiles at most, by the rule
+            s = id % a.b.sequences;
+            tile = tiles - 1 - id / a.b.sequences;
+            span = cache_span(a.b, s);
+        }
     }
     const AttentionTile range = attention_tile(span, tile, 16 * R, a.group, a.window);
     const uint32_t row0 = range.first_row, rows = range.rows;
@@ -474,7 +482,7 @@ struct AttentionPlan {
     uint64_t bytes;
 };
 // The tiles' split along the tokens.
-static AttentionPlan attention_split(const oco_cache *p, uint32_t tile, uint64_t rows, uint32_t chunk) {
+static AttentionPlan attention_split(const oco_cache *p, uint32_t tile, uint64_t rows, uint32_t chunk, bool starts) {
     AttentionPlan l;
     l.tile = tile;
     l.tiles = (uint32_t)((rows + 16 * tile - 1) / (16 * tile));
@@ -505,6 +513,8 @@ static AttentionPlan attention_split(const oco_cache *p, uint32_t tile, uint64_t
     l.chunks = (uint32_t)((seen + l.chunk - 1) / l.chunk);
     if (l.chunks < 1) l.chunks = 1;
     l.grid = (uint64_t)p->sequences * l.tiles * l.chunks;
+    const uint64_t places = (uint64_t)p->rows * (p->heads / p->kv_heads) / (16 * tile) + p->sequences;
+    if (tile != 1 && tile != 3 && attention_counts(p->sequences, starts, l.tiles) && places * l.chunks < l.grid) l.grid = places * l.chunks;
     l.pieces[0] = l.pieces[1] = l.works = 0;
     // With one tile per sequence and enough to do, over 640 tokens of a head for each compute unit, the kernel sizes the
     // chunks by the lengths as they are, which may be far under max_length and far apart, and numbers those that there are one
@@ -531,7 +541,7 @@ static AttentionPlan attention_split(const oco_cache *p, uint32_t tile, uint64_t
     return l;
 }
 
-static AttentionPlan attention_plan(const oco_cache *p) {
+static AttentionPlan attention_plan(const oco_cache *p, bool starts) {
     const uint64_t rows = (uint64_t)(p->max_rows < p->rows ? p->max_rows : p->rows) * (p->heads / p->kv_heads);
     // Tiles of 16 rows while that is all, of 32 beyond (of 16 where the second one would be half empty, or one of 48 with
     // over 3000 tokens of a head for each compute unit).  With narrow heads the prompts' kernel: tiles of 128 rows from 256
@@ -551,7 +561,7 @@ static AttentionPlan attention_plan(const oco_cache *p) {
     if (narrow && rows >= 128 && (rows + 127) / 128 * heads >= 256) tile = (rows + 255) / 256 * heads >= 512 ? 16 : 8;
     if (set && (knob[0] == 1 || knob[0] == 2 || ((knob[0] == 3 || knob[0] == 8 || knob[0] == 16) && narrow))) tile = (uint32_t)knob[0];
     const uint32_t chunk = set > 1 && knob[1] > 0 && knob[1] % 128 == 0 ? (uint32_t)knob[1] : 0;
-    return attention_split(p, tile, rows, chunk);
+    return attention_split(p, tile, rows, chunk, starts);
 }
 
 template <uint32_t D, bool BF>
@@ -603,7 +613,7 @@ static const char *attention_problem(const oco_cache *p) {
 using namespace oco;
 
 extern "C" uint64_t oco_cache_attention_workspace(const oco_cache *p) {
-    return p && !attention_problem(p) ? attention_plan(p).bytes : 0;
+    return p && !attention_problem(p) ? attention_plan(p, false).bytes : 0;
 }
 
 extern "C" int oco_cache_attention(const void *q, const void *pages, const uint32_t *table, const uint32_t *starts,
@@ -617,7 +627,7 @@ extern "C" int oco_cache_attention(const void *q, const void *pages, const uint3
     if ((uintptr_t)pages & 15u) return fail(OCO_ERR_INVALID, "oco_cache_attention: pages must be 16-byte aligned");
     if (!starts && p->rows % p->sequences)
         return fail(OCO_ERR_INVALID, "oco_cache_attention: %u rows of %u sequences without starts", p->rows, p->sequences);
-    const AttentionPlan l = attention_plan(p);
+    const AttentionPlan l = attention_plan(p, starts);
     if (l.bytes && (!workspace || ((uintptr_t)workspace & 15u) || workspace_bytes < l.bytes))
         return fail(OCO_ERR_INVALID, "oco_cache_attention: workspace of %llu bytes, need %llu, 16-byte aligned",
                     (unsigned long long)workspace_bytes, (unsigned long long)l.bytes);

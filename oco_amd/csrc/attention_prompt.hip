@@ -43,8 +43,10 @@ __global__ __launch_bounds__(64 * W, 2) void attention_prompt_kernel(AttentionAr
     id /= a.b.kv_heads;
     const uint32_t chunk = id % a.chunks;
     id /= a.chunks;
-    const uint32_t s = id % a.b.sequences, tile = tiles - 1 - id / a.b.sequences;
-    const CacheSpan span = cache_span(a.b, s);
+    const AttentionPlace place = attention_place<32 * W>(a, id, tiles);
+    const uint32_t s = place.sequence, tile = place.tile;
+    const CacheSpan span = place.span;
+    if (s >= a.b.sequences) return;
     const AttentionTile range = attention_tile(span, tile, 32 * W, a.group, a.window);
     const uint32_t rows = range.rows;
     if (range.first_row >= rows) return;

@@ -458,3 +458,21 @@ def test_long_sequences_in_chunks(lib, d, rows, heads, kv, even):
     assert np.isfinite(got[0]).all()
     bound = 12 * (2.0 ** -8 + 20000 * 2.0 ** -23 + 4 * 500 * 2.0 ** -23)
     assert np.abs(got[0] - got[1]).max() <= 2 * bound + 2.0 ** -8 * (np.abs(got[0]).max() + np.abs(got[1]).max())
+
+
+@pytest.mark.parametrize("d,window", [(64, 0), (128, 50), (256, 0)])
+@pytest.mark.parametrize("sequences,most", [(2, 200), (5, 200), (64, 30), (65, 30)])
+def test_tiles_of_uneven_batches(kernel, lib, d, window, sequences, most):
+    """Some sequences with many tiles, some with one and some with none; rows behind the last one stay."""
+    rng = np.random.default_rng(d + sequences)
+    rows = [int(most * r ** 3) for r in rng.random(sequences)]
+    rows[int(rng.integers(sequences))] = most
+    rows[-1] = 0
+    lengths = [n + int(rng.integers(0, 90)) for n in rows]
+    lengths[0] = max(rows[0] - 3, 0)  # its first rows have no token
+    say("uneven", d, rows[:10])
+    c = Case(lib, rng, rows, lengths, 4, 1, d, 16, "bf16", window=window, sinks=True, extra_rows=3, holes=1)
+    c.call()
+    lib.synchronize()
+    c.check()
+    assert np.all(np.ascontiguousarray(c.out.read(np.uint8)[sum(rows) * 4 * d * 2:]).view(np.uint32) == 0x7FC12345)
