@@ -185,33 +185,37 @@ __device__ __forceinline__ AttentionPlace attention_place(const AttentionArgs &a
     return p;
 }
 
-// A workgroup's sequence and chunk where chunks are sized by the lengths as they are (of at most 64 sequences, a lane's
-// each) and numbered one after the other: the least of a few sizes that leave no more chunks than wanted.
+// A workgroup's sequence, tile and chunk where chunks are sized by the lengths as they are (of at most 64 sequences, a
+// lane's each) and numbered one after the other: the least of a few sizes that leave no more chunks than wanted.
 struct AttentionPart {
-    uint32_t sequence, chunk, size;  // sequence past the last one: there is none
+    uint32_t sequence, tile, chunk, size;  // sequence past the last one: there is none
     CacheSpan span;
 };
+template <uint32_t TILE>
 __device__ __forceinline__ AttentionPart attention_part(const AttentionArgs &a, uint32_t id) {
     const uint32_t lane = threadIdx.x & 63, mine = min(lane, a.b.sequences - 1);
     const CacheSpan own = cache_span(a.b, mine);
     const uint32_t n = lane < a.b.sequences ? min(own.length, a.seen) : 0, units = (n + 127) / 128;
-    const uint32_t all = wave_total(units), k = all < a.works ? 0 : 1;
+    const uint32_t tiles = lane < a.b.sequences ? (own.rows * a.group + TILE - 1) / TILE : 0;
+    const uint32_t all = wave_total(units * tiles), k = all < a.works ? 0 : 1;
     const float least = fmaxf(ceilf((float)all * a.inverse[k]), 1.f);
     float size = fmaxf(least, ceilf((float)all * a.relaxed[k]));
 #pragma unroll
     for (int j = 0; j < 3; j++) {
         const float c = ceilf(least * (1.f + 0.125f * j));
-        if (wave_total((uint32_t)ceilf((float)units * (__builtin_amdgcn_rcpf(c) * 0.9999998f))) <= a.pieces[k]) {
+        if (wave_total((uint32_t)ceilf((float)units * (__builtin_amdgcn_rcpf(c) * 0.9999998f)) * tiles) <= a.pieces[k]) {
             size = c;
             break;
         }
     }
     AttentionPart p;
     p.size = max(a.chunk, (uint32_t)fminf(size, 8388608.f) * 128);
-    const uint32_t parts = lane < a.b.sequences ? max((n + p.size - 1) / p.size, 1u) : 0, to = wave_scan(parts);
+    const uint32_t parts = max((n + p.size - 1) / p.size, 1u) * tiles, to = wave_scan(parts);
     p.sequence = __builtin_popcountll(__ballot(to <= id));
-    const uint32_t s = min(p.sequence, 63u);
-    p.chunk = id - (uint32_t)(__builtin_amdgcn_readlane((int)to, s) - __builtin_amdgcn_readlane((int)parts, s));
+    const uint32_t s = min(p.sequence, 63u), rest = id - (uint32_t)(__builtin_amdgcn_readlane((int)to, s) - __builtin_amdgcn_readlane((int)parts, s));
+    const uint32_t of = max((uint32_t)__builtin_amdgcn_readlane((int)tiles, s), 1u);
+    p.tile = rest % of;
+    p.chunk = rest / of;
     p.span = CacheSpan{(uint32_t)__builtin_amdgcn_readlane((int)own.first, s), (uint32_t)__builtin_amdgcn_readlane((int)own.rows, s),
                        (uint32_t)__builtin_amdgcn_readlane((int)own.length, s)};
     return p;

@@ -86,7 +86,7 @@ __device__ __forceinline__ Halves load_halves(const uint32_t *table, uint32_t t0
     return h;
 }
 
-// FIT: chunks by the lengths (attention_part), one tile per sequence.
+// FIT: chunks by the lengths (attention_part).
 template <uint32_t D, bool BF, int R, bool FIT>
 __global__ __launch_bounds__(256, D * R == 64 ? 4 : D * R == 128 ? 3 : 2) void attention_kernel(AttentionArgs a, uint32_t tiles) {
     constexpr int KW = D / 32, NT = D / 16;  // key words per lane and token; tiles of 16 columns
@@ -99,12 +99,12 @@ __global__ __launch_bounds__(256, D * R == 64 ? 4 : D * R == 128 ? 3 : 2) void a
     uint32_t s, tile, chunk, size = a.chunk;
     CacheSpan span;
     if constexpr (FIT) {
-        const AttentionPart part = attention_part(a, id);
+        const AttentionPart part = attention_part<16 * R>(a, id);
         s = part.sequence;
         chunk = part.chunk;
         size = part.size;
         span = part.span;
-        tile = 0;
+        tile = part.tile;
         if (blockIdx.x == 0 && threadIdx.x == 0) *gp((uint32_t *)(a.parts + (uint64_t)a.b.rows * a.heads * a.chunks * (D + 2))) = size;
         if (s >= a.b.sequences) return;
     } else {
@@ -516,24 +516,28 @@ static AttentionPlan attention_split(const oco_cache *p, uint32_t tile, uint64_t
     const uint64_t places = (uint64_t)p->rows * (p->heads / p->kv_heads) / (16 * tile) + p->sequences;
     if (tile != 1 && tile != 3 && attention_counts(p->sequences, starts, l.tiles) && places * l.chunks < l.grid) l.grid = places * l.chunks;
     l.pieces[0] = l.pieces[1] = l.works = 0;
-    // With one tile per sequence and enough to do, over 640 tokens of a head for each compute unit, the kernel sizes the
+    // With few tiles per sequence and enough to do, over 640 tokens of a head for each compute unit, the kernel sizes the
     // chunks by the lengths as they are, which may be far under max_length and far apart, and numbers those that there are one
-    // after the other: workgroups that end at once leave the others unevenly spread.  As many as the card holds at once
-    // (twice as many of 32 rows), or two per compute unit where that leaves them under 700 tokens or so.
-    // us, by max_length alone -> so, 128 wide, a row of 4 heads: 8 sequences of 4101 tokens 17.1 -> 15.4, 32 of them 41.4 ->
-    // 36.3, 32 of up to 4101 26.9 -> 23.4, 64 of up to 1001 21.6 -> 19.6, one of 64001 31.6 -> 21.7 (3 per compute unit 23.7),
-    // 32 of up to 16384 80.1 -> 76 (2: 83.6, 4: 88.5); 256 wide, 2 80.2 -> 73.2 (3: 84.4); 64 wide, 4 54.4 -> 50.8 (3: 56.4);
-    // 5 x 4 rows, 4 112.9 -> 105.7 (2: 121.1).
-    const uint64_t all = (uint64_t)p->sequences * ((seen + 127) / 128);
-    if (l.chunks > 1 && !chunk && !prompt && l.tiles == 1 && p->sequences <= 64 && all * p->kv_heads > 640 * 2) {
-        const uint32_t held = p->head_dim == 64 ? 4 : p->head_dim == 128 ? 3 : 2, per[2] = {2, tile == 1 ? held : tile == 2 ? 4 : 2};
+    // after the other: workgroups that end at once leave the others unevenly spread.  As many as the card holds at once (or
+    // twice as many, of 32 rows where that is not two per sequence), or two per compute unit where that leaves them under 700
+    // tokens or so.
+    // us, by max_length alone -> so, 128 wide, a row of 4 heads: 8 sequences of 4101 tokens 17.1 -> 15.0, 32 of them 41.4 ->
+    // 35.6, 32 of up to 4101 26.9 -> 22.9, one of 64001 31.6 -> 21.2 (3 per compute unit 23.7), 32 of up to 16384 80.1 -> 76 (2:
+    // 83.6, 4: 88.5); 256 wide, 2 80.2 -> 72.4 (3: 84.4); 64 wide, 4 54.4 -> 49.8 (3: 56.4); 5 x 4 rows, 4 112.9 -> 105 (2: 121);
+    // 16 x 8 rows of 8 sequences, 2 52.3 -> 45.4 (4: 52.2); 64 wide, 8 x 8 rows of 16, 3 39.0 -> 36.5 (2: 40.2, 4: 39.4), 5 x 8 rows
+    // of 8 20.8 -> 20.1.
+    const uint64_t all = (uint64_t)p->sequences * l.tiles * ((seen + 127) / 128);
+    if (l.chunks > 1 && !chunk && !prompt && l.tiles <= 4 && p->sequences <= 64 && all * p->kv_heads > 640 * 2) {
+        const uint32_t held = tile == 1 ? (p->head_dim == 64 ? 4 : p->head_dim == 128 ? 3 : 2) : tile == 2 && p->head_dim == 64 ? 3 : 2;
+        const uint32_t per[2] = {2, tile == 2 && 2ull * p->sequences * p->kv_heads >= 256 * held ? 2 * held : held};
         l.works = 2048 * 2 / p->kv_heads + 1;
         uint64_t grid = 0;
         for (uint32_t i = 0; i < 2; i++) {
             l.pieces[i] = 256 * per[i] / p->kv_heads;
             if (l.pieces[i] == 0) l.pieces[i] = 1;
-            // sizes of at least all / pieces make pieces and one per sequence at most
-            if ((i == 0 || all >= l.works) && l.pieces[i] + p->sequences + 1 > grid) grid = l.pieces[i] + p->sequences + 1;
+            // sizes of at least all / pieces make pieces and one per tile at most
+            const uint64_t parts = l.pieces[i] + (uint64_t)p->sequences * l.tiles + 1;
+            if ((i == 0 || all >= l.works) && parts > grid) grid = parts;
         }
         if (grid < l.grid) l.grid = grid;
     }
@@ -652,7 +656,7 @@ extern "C" int oco_cache_attention(const void *q, const void *pages, const uint3
     for (int i = 0; i < 2; i++) {
         a.pieces[i] = l.pieces[i];
         a.inverse[i] = 1.f / (float)l.pieces[i];
-        a.relaxed[i] = l.pieces[i] > p->sequences / 2 + 1 ? 1.f / (float)(l.pieces[i] - p->sequences / 2) : 1.f;
+        a.relaxed[i] = l.pieces[i] > p->sequences * l.tiles / 2 + 1 ? 1.f / (float)(l.pieces[i] - p->sequences * l.tiles / 2) : 1.f;
     }
     a.c = (p->scale != 0.f ? p->scale : 1.f / sqrtf((float)p->head_dim)) * 1.44269504088896341f;
     hipStream_t st = (hipStream_t)stream;

@@ -476,3 +476,24 @@ def test_tiles_of_uneven_batches(kernel, lib, d, window, sequences, most):
     lib.synchronize()
     c.check()
     assert np.all(np.ascontiguousarray(c.out.read(np.uint8)[sum(rows) * 4 * d * 2:]).view(np.uint32) == 0x7FC12345)
+
+
+@pytest.mark.parametrize("d,heads,rows", [(64, 20, 5), (128, 16, 6), (128, 4, 40), (256, 4, 17)])
+@pytest.mark.parametrize("sequences", [2, 7, 40])
+def test_chunks_and_tiles_by_the_lengths(lib, d, heads, rows, sequences):
+    """As test_chunks_by_the_lengths, where sequences have up to four tiles."""
+    rng = np.random.default_rng(d + heads + sequences)
+    n = [int(i) for i in rng.integers(0, rows + 1, sequences)]
+    n[int(rng.integers(sequences))] = rows
+    lengths = [int(i) for i in rng.integers(0, 1500 if sequences < 20 else 200, sequences)]
+    c = Case(lib, rng, n, lengths, heads, 2, d, 16, "bf16", sinks=True, holes=sequences % 2, max_rows=rows, extra_rows=1)
+    c.p.max_length = 100000 // sequences
+    stride = c.p.max_length // 16 + 1
+    c.p.table_stride = stride
+    c.dev[2] = dev(lib, np.ascontiguousarray(np.pad(c.b.table, ((0, 0), (0, stride - c.b.table.shape[1])))))
+    c.need = lib.cache_attention_workspace(c.p)
+    c.work = Guarded(lib, c.need)
+    say("chunks and tiles", d, heads, n[:8], lengths[:8])
+    c.call()
+    lib.synchronize()
+    c.check()
