@@ -414,9 +414,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
         }
     }
     const uint32_t size = a.works ? *gp((const uint32_t *)(a.parts + (uint64_t)a.b.rows * a.heads * a.chunks * (D + 2))) : a.chunk;
-    const uint32_t s = cache_sequence(a.b, row);
-    if (s >= a.b.sequences) return;
-    const CacheSpan span = cache_span(a.b, s);
+    const CacheRow at_row = cache_row(a.b, row);
+    const CacheSpan span = at_row.span;
+    if (at_row.sequence >= a.b.sequences) return;
     if (row - span.first >= span.rows) return;
     const AttentionTile range = attention_tile(span, ((row - span.first) * a.group + head % a.group) / a.tile_rows, a.tile_rows, a.group, a.window);
     const uint32_t used = range.end > range.first ? (range.end - range.first + size - 1) / size : 0;

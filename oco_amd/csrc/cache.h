@@ -44,6 +44,31 @@ __device__ __forceinline__ uint32_t cache_sequence(const CacheBatch &b, uint32_t
     }
 }
 
+// A row's sequence (b.sequences: none), rows and tokens, by one wavefront, uniform: of up to 64 sequences a lane's starts and
+// length are read at once, for every load that waits for another is a microsecond of a small call.
+struct CacheRow {
+    uint32_t sequence;
+    CacheSpan span;
+};
+__device__ __forceinline__ CacheRow cache_row(const CacheBatch &b, uint32_t row) {
+    CacheRow r;
+    if (b.starts && b.sequences <= 64) {
+        const uint32_t lane = threadIdx.x & 63, start = b.starts[min(lane, b.sequences - 1)], length = b.lengths[min(lane, b.sequences - 1)];
+        const uint32_t last = b.starts[b.sequences];
+        const uint32_t c = __builtin_popcountll(__ballot(lane < b.sequences && start <= row));
+        r.sequence = c ? c - 1 : b.sequences;
+        const uint32_t s = c ? c - 1 : 0;
+        r.span.first = min((uint32_t)__builtin_amdgcn_readlane((int)start, s), b.rows);
+        const uint32_t next = c == b.sequences ? last : (uint32_t)__builtin_amdgcn_readlane((int)start, c);
+        r.span.rows = min(min(max(next, r.span.first), b.rows) - r.span.first, b.max_rows);
+        r.span.length = min((uint32_t)__builtin_amdgcn_readlane((int)length, s), b.max_length);
+    } else {
+        r.sequence = cache_sequence(b, row);
+        r.span = cache_span(b, min(r.sequence, b.sequences - 1));
+    }
+    return r;
+}
+
 // A head's bytes in a page, and where a token's parts are in them.  D: head_dim.
 __host__ __device__ constexpr uint32_t cache_head_bytes(uint32_t page_size, uint32_t d) { return page_size * d + page_size * d / 16; }
 __device__ __forceinline__ uint32_t cache_key_at(uint32_t t, uint32_t word, uint32_t d) { return t * (d / 2) + 4 * word; }

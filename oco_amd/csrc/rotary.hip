@@ -300,9 +300,10 @@ __global__ __launch_bounds__(256, 4) void append_kernel(AppendArgs a) {
     for (int i = 0; i < 2; i++) first_values[i].load(v + 8 * min(lane + 64 * i, heads * WORDS - 1));
     uint32_t page = 0xffffffffu, t = 0;
     const bool mine = turn_heads<T, INTERLEAVED>(lane, 64, heads * group, D, n, a.r, table, [&](uint32_t h) { return q + h * D; }, [&](uint32_t h) { return q_out + h * D; }, [&] {
-        const uint32_t s = cache_sequence(a.b, row);
+        const CacheRow at_row = cache_row(a.b, row);
+        const uint32_t s = at_row.sequence;
+        const CacheSpan span = at_row.span;
         if (s >= a.b.sequences) return false;
-        const CacheSpan span = cache_span(a.b, s);
         if (row - span.first >= span.rows) return false;
         const uint32_t back = span.rows - (row - span.first);  // the row's place from the end
         const bool token = span.length >= back;
@@ -368,9 +369,10 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
     const uint32_t id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = id / a.parts;
     const uint32_t lane = id % a.parts * 64 + (threadIdx.x & 63), step = 64 * a.parts;
     if (row >= a.b.rows) return;
-    const uint32_t s = cache_sequence(a.b, row);
+    const CacheRow at_row = cache_row(a.b, row);
+    const uint32_t s = at_row.sequence;
+    const CacheSpan span = at_row.span;
     if (s >= a.b.sequences) return;
-    const CacheSpan span = cache_span(a.b, s);
     if (row - span.first >= span.rows) return;
     const uint32_t back = span.rows - (row - span.first);
     const bool token = span.length >= back;
