@@ -17,6 +17,13 @@
 // E2M1 times a power of two is exact in bf16 and f16 (an f16 model's cache
 // stays in range), so codes go to the matrix instruction through the hardware's
 // conversion, two values per instruction, with their scale.
+//
+// Bound by memory for single tokens of many long sequences (32 of up to 16384,
+// 8 heads of 128: 338 MB in 75 us, 4.5 TB/s), by two launches and three loads
+// that wait for each other for one (4101 tokens 8.5 to 9), and by issue where
+// several tiles convert the same codes: per step of 16 rows and 64 columns
+// about 190 vector instructions of 4 clocks beside 128 clocks of products (8
+// sequences of up to 5 rows of 64 heads 20 us; 1700 rows 256 wide 55 us).
 #include "attention.h"
 
 namespace oco {
@@ -492,9 +499,9 @@ static AttentionPlan attention_split(const oco_cache *p, uint32_t tile, uint64_t
     l.seen = (uint32_t)seen;
     const uint64_t blocks = (uint64_t)p->sequences * p->kv_heads * l.tiles;
     const bool prompt = tile >= 8;
-    // Chunks at most and their tokens at least: 3072 workgroups of few rows, of at least two steps per wavefront (one sequence
-    // of 4101: 256 tokens 8.5 us, 384 9.1, 512 9.7), 512 of a prompt's tiles.
-    const uint64_t wanted = prompt ? 512 : 3072;
+    // Chunks at most and their tokens at least: twelve workgroups of few rows per compute unit, of at least two steps per
+    // wavefront (one sequence of 4101: 256 tokens 8.5 us, 384 9.1, 512 9.7), two of a prompt's tiles.
+    const uint64_t wanted = 256 * (prompt ? 2 : 12);
     uint64_t chunks = blocks ? (wanted + blocks - 1) / blocks : 1;
     const uint64_t least = prompt ? 512 : 256;
     uint64_t most = (seen + least - 1) / least;
@@ -505,7 +512,7 @@ static AttentionPlan attention_split(const oco_cache *p, uint32_t tile, uint64_t
     // Whole where the join costs more than a split saves (us, split / whole, 128 wide, tokens x tiles: 505 x 8 8.8 / 6.7, 755 x 8
     // 8.5 / 8.2, 1005 x 8 8.4 / 9.6; 505 x 256 12.2 / 7.9, 1255 x 256 15.8 / 13.1, 3005 x 256 28.6 / 29.8; 3005 x 512 47.8 /
     // 41.6; up to 2005 x 256 17.2 / 18.0; 256 wide 755 x 32 10.0 / 11.1, 1255 x 128 19.4 / 16.6)
-    const uint64_t whole = blocks > 512 ? 3072 : 6 * blocks;
+    const uint64_t whole = 6 * (blocks < 512 ? blocks : 512);
     if (!prompt && seen <= (whole > 768 ? whole : p->head_dim > 128 ? 512 : 768)) chunks = 1;
     if (chunks < 1) chunks = 1;
     l.chunk = chunk ? chunk : (uint32_t)(((seen + chunks - 1) / chunks + 127) / 128 * 128);
