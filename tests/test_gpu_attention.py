@@ -497,3 +497,29 @@ def test_chunks_and_tiles_by_the_lengths(lib, d, heads, rows, sequences):
     c.call()
     lib.synchronize()
     c.check()
+
+
+def test_chunks_in_a_graph(lib):
+    """A captured call follows lengths that change between its replays, with eager calls in between."""
+    rng = np.random.default_rng(23)
+    c = Case(lib, rng, [1, 3, 2, 1, 4], [900, 40, 1400, 7, 300], 4, 2, 64, 16, "bf16", sinks=True)
+    c.p.max_length, c.p.table_stride = 40000, 2500
+    c.dev[2] = dev(lib, np.ascontiguousarray(np.pad(c.b.table, ((0, 0), (0, 2500 - c.b.table.shape[1])))))
+    c.need = lib.cache_attention_workspace(c.p)
+    c.work = Guarded(lib, c.need)
+    assert c.need
+    stream, longest = lib.Stream(), list(c.b.lengths)
+    c.call(stream)
+    stream.sync()
+    graph = lib.Graph(stream, lambda: c.call(stream))
+    for turn in range(4):
+        say("replay", turn)
+        c.b.lengths = [int(rng.integers(n, most + 1)) for n, most in zip(c.b.rows, longest)]
+        c.dev[3].upload(np.array(c.b.lengths, np.uint32))
+        graph.launch()
+        stream.sync()
+        got = c.out.read(np.uint8).copy()
+        c.check()
+        c.call()
+        lib.synchronize()
+        np.testing.assert_array_equal(got, c.out.read(np.uint8))
