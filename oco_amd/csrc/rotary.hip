@@ -585,11 +585,12 @@ extern "C" int oco_cache_append(void *pages, const uint32_t *table, const uint32
     if (q && q == q_out && a.q_stride != a.out_stride) return fail(OCO_ERR_INVALID, "oco_cache_append: queries in place with another stride");
     a.heads = p->heads;
     a.r = rotation_of(rotation);
-    // few tokens: their heads over 1024 wavefronts, one per SIMD, down to one each (64 tokens of 8 heads 6.0 us, 7.6 by one
-    // each; 512 appended and read back 10.6, 12.1; over 4096, whose tables of angles cost more, 12.5, and 1300 of 64 wide 16.1
-    // against 13.7)
+    // few tokens: their heads over 1024 wavefronts, one per SIMD, down to one each, and halved under 2048 of them.  us:
+    // 64 tokens of 8 heads 6.0, by one each 7.6; 512 appended and read back 10.1, 12.1, over 2048 10.5; 1500 12.9, 14.1; about
+    // 1300 of 64 wide 13.0, 13.7, over 4096 16.1
+    uint32_t parts = 1;
     a.part_heads = APPEND_VALUES / p->head_dim;
-    while (a.part_heads > 1 && (uint64_t)p->rows * ((p->kv_heads + a.part_heads - 1) / a.part_heads) < 1024) a.part_heads /= 2;
+    while (a.part_heads > 1 && (uint64_t)p->rows * (parts = (p->kv_heads + a.part_heads - 1) / a.part_heads) < (parts == 1 ? 2048 : 1024)) a.part_heads /= 2;
     a.parts = (p->kv_heads + a.part_heads - 1) / a.part_heads;
     if ((uint64_t)p->rows * a.parts > 0x7fffffffull) return fail(OCO_ERR_INVALID, "oco_cache_append: %u rows", p->rows);
     const dim3 grid((uint32_t)(((uint64_t)p->rows * a.parts + 3) / 4));
