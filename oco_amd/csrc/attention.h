@@ -185,39 +185,66 @@ __device__ __forceinline__ AttentionPlace attention_place(const AttentionArgs &a
     return p;
 }
 
-// A workgroup's sequence, tile and chunk where chunks are sized by the lengths as they are (of at most 64 sequences, a
-// lane's each) and numbered one after the other: the least of a few sizes that leave no more chunks than wanted.
+// A workgroup's sequence, tile and chunk where chunks are sized by the lengths as they are (of at most 64 M sequences, a
+// lane's M each) and numbered one after the other: the least of a few sizes that leave no more chunks than wanted.
 struct AttentionPart {
     uint32_t sequence, tile, chunk, size;  // sequence past the last one: there is none
     CacheSpan span;
 };
-template <uint32_t TILE>
+template <uint32_t TILE, int M>
 __device__ __forceinline__ AttentionPart attention_part(const AttentionArgs &a, uint32_t id) {
-    const uint32_t lane = threadIdx.x & 63, mine = min(lane, a.b.sequences - 1);
-    const CacheSpan own = cache_span(a.b, mine);
-    const uint32_t n = lane < a.b.sequences ? min(own.length, a.seen) : 0, units = (n + 127) / 128;
-    const uint32_t tiles = lane < a.b.sequences ? (own.rows * a.group + TILE - 1) / TILE : 0;
-    const uint32_t all = wave_total(units * tiles), k = all < a.works ? 0 : 1;
+    const uint32_t lane = threadIdx.x & 63;
+    CacheSpan own[M];
+    uint32_t units[M], tiles[M], parts[M], of_lane = 0;
+#pragma unroll
+    for (int i = 0; i < M; i++) {
+        const uint32_t s = lane * M + i;
+        own[i] = cache_span(a.b, min(s, a.b.sequences - 1));
+        units[i] = (min(own[i].length, a.seen) + 127) / 128;
+        tiles[i] = s < a.b.sequences ? (own[i].rows * a.group + TILE - 1) / TILE : 0;
+        of_lane += units[i] * tiles[i];
+    }
+    const uint32_t all = wave_total(of_lane), k = all < a.works ? 0 : 1;
     const float least = fmaxf(ceilf((float)all * a.inverse[k]), 1.f);
     float size = fmaxf(least, ceilf((float)all * a.relaxed[k]));
 #pragma unroll
     for (int j = 0; j < 3; j++) {
-        const float c = ceilf(least * (1.f + 0.125f * j));
-        if (wave_total((uint32_t)ceilf((float)units * (__builtin_amdgcn_rcpf(c) * 0.9999998f)) * tiles) <= a.pieces[k]) {
+        const float c = ceilf(least * (1.f + 0.125f * j)), by = __builtin_amdgcn_rcpf(c) * 0.9999998f;
+        of_lane = 0;
+#pragma unroll
+        for (int i = 0; i < M; i++) of_lane += (uint32_t)ceilf((float)units[i] * by) * tiles[i];
+        if (wave_total(of_lane) <= a.pieces[k]) {
             size = c;
             break;
         }
     }
     AttentionPart p;
     p.size = max(a.chunk, (uint32_t)fminf(size, 8388608.f) * 128);
-    const uint32_t parts = max((n + p.size - 1) / p.size, 1u) * tiles, to = wave_scan(parts);
-    p.sequence = __builtin_popcountll(__ballot(to <= id));
-    const uint32_t s = min(p.sequence, 63u), rest = id - (uint32_t)(__builtin_amdgcn_readlane((int)to, s) - __builtin_amdgcn_readlane((int)parts, s));
-    const uint32_t of = max((uint32_t)__builtin_amdgcn_readlane((int)tiles, s), 1u);
+    of_lane = 0;
+#pragma unroll
+    for (int i = 0; i < M; i++) {
+        parts[i] = max((min(own[i].length, a.seen) + p.size - 1) / p.size, 1u) * tiles[i];
+        of_lane += parts[i];
+    }
+    const uint32_t to = wave_scan(of_lane), c = __builtin_popcountll(__ballot(to <= id)), s = min(c, 63u);
+    uint32_t rest = id - (uint32_t)(__builtin_amdgcn_readlane((int)to, s) - __builtin_amdgcn_readlane((int)of_lane, s)), of = 1;
+    p.sequence = a.b.sequences;
+    p.span = CacheSpan{0, 0, 0};
+    bool found = c == 64;
+#pragma unroll
+    for (int i = 0; i < M; i++) {
+        const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)parts[i], s);
+        if (!found && rest < n) {
+            found = true;
+            p.sequence = s * M + i;
+            of = (uint32_t)__builtin_amdgcn_readlane((int)tiles[i], s);
+            p.span = CacheSpan{(uint32_t)__builtin_amdgcn_readlane((int)own[i].first, s), (uint32_t)__builtin_amdgcn_readlane((int)own[i].rows, s),
+                               (uint32_t)__builtin_amdgcn_readlane((int)own[i].length, s)};
+        }
+        rest -= found ? 0 : n;
+    }
     p.tile = rest % of;
     p.chunk = rest / of;
-    p.span = CacheSpan{(uint32_t)__builtin_amdgcn_readlane((int)own.first, s), (uint32_t)__builtin_amdgcn_readlane((int)own.rows, s),
-                       (uint32_t)__builtin_amdgcn_readlane((int)own.length, s)};
     return p;
 }
 

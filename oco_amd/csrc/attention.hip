@@ -106,7 +106,7 @@ __global__ __launch_bounds__(256, D * R == 64 ? 4 : D * R == 128 ? 3 : 2) void a
     uint32_t s, tile, chunk, size = a.chunk;
     CacheSpan span;
     if constexpr (FIT) {
-        const AttentionPart part = attention_part<16 * R>(a, id);
+        const AttentionPart part = a.b.sequences <= 64 ? attention_part<16 * R, 1>(a, id) : attention_part<16 * R, 4>(a, id);
         s = part.sequence;
         chunk = part.chunk;
         size = part.size;
@@ -511,8 +511,9 @@ static AttentionPlan attention_split(const oco_cache *p, uint32_t tile, uint64_t
     if (chunks > most) chunks = most;
     // Whole where the join costs more than a split saves (us, split / whole, 128 wide, tokens x tiles: 505 x 8 8.8 / 6.7, 755 x 8
     // 8.5 / 8.2, 1005 x 8 8.4 / 9.6; 505 x 256 12.2 / 7.9, 1255 x 256 15.8 / 13.1, 3005 x 256 28.6 / 29.8; 3005 x 512 47.8 /
-    // 41.6; up to 2005 x 256 17.2 / 18.0; 256 wide 755 x 32 10.0 / 11.1, 1255 x 128 19.4 / 16.6)
-    const uint64_t whole = 6 * (blocks < 512 ? blocks : 512);
+    // 41.6; up to 2005 x 256 17.2 / 18.0; 256 wide 755 x 32 10.0 / 11.1, 1255 x 128 19.4 / 16.6;
+    // up to 8005 x 1024 128 / 153, up to 4005 x 2048 164 / 138)
+    const uint64_t whole = blocks < 512 ? 6 * blocks : blocks < 1024 ? 6 * 512 : 3 * (blocks < 4096 ? blocks : 4096);
     if (!prompt && seen <= (whole > 768 ? whole : p->head_dim > 128 ? 512 : 768)) chunks = 1;
     if (chunks < 1) chunks = 1;
     l.chunk = chunk ? chunk : (uint32_t)(((seen + chunks - 1) / chunks + 127) / 128 * 128);
@@ -525,18 +526,20 @@ static AttentionPlan attention_split(const oco_cache *p, uint32_t tile, uint64_t
     l.pieces[0] = l.pieces[1] = l.works = 0;
     // With few tiles per sequence and enough to do, over 640 tokens of a head for each compute unit, the kernel sizes the
     // chunks by the lengths as they are, which may be far under max_length and far apart, and numbers those that there are one
-    // after the other: workgroups that end at once leave the others unevenly spread.  As many as the card holds at once (or
-    // twice as many, of 32 rows where that is not two per sequence), or two per compute unit where that leaves them under 700
-    // tokens or so.
+    // after the other: workgroups that end at once leave the others unevenly spread.  As many as the card holds at once, or a
+    // multiple of it, or two per compute unit where that leaves them under 700 tokens or so.  From 1024 tiles of more than 64
+    // sequences on the gaps cost less than the count (96 sequences of up to 8005 126 -> 102, 128 128 -> 132).
     // us, by max_length alone -> so, 128 wide, a row of 4 heads: 8 sequences of 4101 tokens 17.1 -> 15.0, 32 of them 41.4 ->
     // 35.6, 32 of up to 4101 26.9 -> 22.9, one of 64001 31.6 -> 21.2 (3 per compute unit 23.7), 32 of up to 16384 80.1 -> 76 (2:
     // 83.6, 4: 88.5); 256 wide, 2 80.2 -> 72.4 (3: 84.4); 64 wide, 4 54.4 -> 49.8 (3: 56.4); 5 x 4 rows, 4 112.9 -> 105 (2: 121);
     // 16 x 8 rows of 8 sequences, 2 52.3 -> 45.4 (4: 52.2); 64 wide, 8 x 8 rows of 16, 3 39.0 -> 36.5 (2: 40.2, 4: 39.4), 5 x 8 rows
     // of 8 20.8 -> 20.1.
     const uint64_t all = (uint64_t)p->sequences * l.tiles * ((seen + 127) / 128);
-    if (l.chunks > 1 && !chunk && !prompt && l.tiles <= 4 && p->sequences <= 64 && all * p->kv_heads > 640 * 2) {
+    if (l.chunks > 1 && !chunk && !prompt && l.tiles <= 4 && (p->sequences <= 64 || (p->sequences <= 256 && blocks < 1024)) && all * p->kv_heads > 640 * 2) {
         const uint32_t held = tile == 1 ? (p->head_dim == 64 ? 4 : p->head_dim == 128 ? 3 : 2) : tile == 2 && p->head_dim == 64 ? 3 : 2;
-        const uint32_t per[2] = {2, tile == 2 && 2ull * p->sequences * p->kv_heads >= 256 * held ? 2 * held : held};
+        // half a workgroup for each sequence's last chunk has to be small beside them
+        const uint64_t times = 2ull * p->sequences * p->kv_heads / (256 * held) + (tile == 2 ? 1 : 0);
+        const uint32_t per[2] = {2, held * (uint32_t)(times < 1 ? 1 : times)};
         l.works = 2048 * 2 / p->kv_heads + 1;
         uint64_t grid = 0;
         for (uint32_t i = 0; i < 2; i++) {

@@ -411,7 +411,7 @@ def test_a_cache_past_32_bits(kernel, lib):
 
 
 @pytest.mark.parametrize("d,rows,window", [(64, 8, 0), (64, 1, 700), (128, 16, 0), (256, 3, 0), (64, 2, 1500), (128, 24, 0)])
-@pytest.mark.parametrize("sequences", [1, 3, 20, 64, 65])
+@pytest.mark.parametrize("sequences", [1, 3, 20, 64, 65, 200])
 def test_chunks_by_the_lengths(lib, d, rows, window, sequences):
     """Bounds far past the lengths, as a captured step has them: chunks follow the lengths, of sequences without rows or tokens too."""
     rng = np.random.default_rng(d + sequences)
