@@ -559,11 +559,14 @@ static AttentionPlan attention_plan(const oco_cache *p, bool starts) {
     const uint64_t rows = (uint64_t)(p->max_rows < p->rows ? p->max_rows : p->rows) * (p->heads / p->kv_heads);
     // Tiles of 16 rows while that is all, of 32 beyond (of 16 where the second one would be half empty, or one of 48 with
     // over 3000 tokens of a head for each compute unit).  With narrow heads the prompts' kernel: tiles of 128 rows from 256
-    // of them on, one per compute unit, and of 256 from 512 of those on.  us, tiles of 16 / 32 / 128 / 256:
+    // of them on, one per compute unit, and of 256 from 512 on where all are alike: 128 wide, one or two sequences, no window.
+    // us, tiles of 16 / 32 / 128 / 256:
     // 32 sequences of 5 x 4 rows over 8000 tokens, 128 wide 115 / 84 / 141; 8 of 5 x 8 rows, 64 wide 20.7 / 22.1 / 33;
     // 4 of 128 x 4 rows over 2000 (128 tiles of 128) 41 / 33 / 49; 16 of 64 x 4 over 4000 (256, 128 of 256) 142 / 108 / 86 / 113;
-    // 64 of 32 x 4 over 1000 (512) 92 / 75 / 49; 2048 x 4 rows from the start on (512, 256 of 256) 65 with 32 / 52 / 63;
-    // 4096 x 4 rows over 8192 (512 of 256) 715 / 567 / 381 / 365, 256 wide (16 heads) 623 / 443.
+    // 64 of 32 x 4 over 1000 (512) 92 / 75 / 49 / 80; 2048 x 4 rows from the start on (512, 256 of 256) 65 with 32 / 52 / 63;
+    // 4096 x 4 rows over 8192 (512 of 256) 715 / 567 / 376 / 365, 4096 from the start on 147 / 138, 8192 505 / 507, with a window
+    // of 2048 252 / 272, 64 wide 328 / 339; 4 sequences of up to 1000 x 4 rows after 3000 142 / 150, 4 of up to 4096 after 4096
+    // 1020 / 1047; 256 wide (16 heads) 623 / 443.
     // Tiles of 16 / 48, 5 x 8 rows: 32 sequences of 4005 tokens, 64 wide 54 / 42, 128 wide 85 / 59, of up to 8192 64 wide 63 / 59,
     // 128 wide 89 / 76; 8 of up to 8192, 64 wide 20.7 / 21.8; two of 2000 9.3 / 11.6.
     int32_t knob[4];
@@ -572,8 +575,10 @@ static AttentionPlan attention_plan(const oco_cache *p, bool starts) {
     const uint64_t heads = (uint64_t)p->kv_heads * p->sequences;
     uint32_t tile = rows <= 16 || (rows > 32 && rows <= 48) ? 1 : 2;
     if (narrow && rows > 32 && rows <= 48 && heads * p->max_length > 3000 * 256) tile = 3;
-    if (narrow && rows >= 128 && (rows + 127) / 128 * heads >= 256) tile = (rows + 255) / 256 * heads >= 512 ? 16 : 8;
-    if (set && (knob[0] == 1 || knob[0] == 2 || ((knob[0] == 3 || knob[0] == 8 || knob[0] == 16) && narrow))) tile = (uint32_t)knob[0];
+    const uint64_t total = (uint64_t)p->rows * (p->heads / p->kv_heads);  // of all sequences
+    const bool wide_tiles = p->head_dim == 128 && p->sequences <= 2 && (p->window == 0 || p->window >= p->max_length);
+    if (narrow && rows >= 128 && (total / 64 + p->sequences) * p->kv_heads >= 512) tile = wide_tiles && total / 256 * p->kv_heads >= 512 ? 16 : 8;
+    if (set && (knob[0] == 1 || knob[0] == 2 || ((knob[0] == 3 || knob[0] == 8) && narrow) || (knob[0] == 16 && p->head_dim == 128))) tile = (uint32_t)knob[0];
     const uint32_t chunk = set > 1 && knob[1] > 0 && knob[1] % 128 == 0 ? (uint32_t)knob[1] : 0;
     return attention_split(p, tile, rows, chunk, starts);
 }

@@ -387,23 +387,22 @@ __global__ __launch_bounds__(64 * W, 2) void attention_prompt_kernel(AttentionAr
 }
 
 int attention_prompt_launch(const AttentionArgs &a, uint32_t head_dim, bool bf, uint32_t tiles, uint32_t grid, hipStream_t stream) {
-#define GO(D, BF)                                                                                                                     \
-    if (a.tile_rows == 256)                                                                                                           \
-        hipLaunchKernelGGL((attention_prompt_kernel<D, BF, 8>), dim3(grid), dim3(512), 0, stream, a, tiles);                          \
-    else                                                                                                                              \
-        hipLaunchKernelGGL((attention_prompt_kernel<D, BF, 4>), dim3(grid), dim3(256), 0, stream, a, tiles);
+#define GO(D, BF, W) hipLaunchKernelGGL((attention_prompt_kernel<D, BF, W>), dim3(grid), dim3(64 * W), 0, stream, a, tiles)
     if (head_dim == 64) {
-        if (bf) {
-            GO(64, true)
-        } else {
-            GO(64, false)
-        }
+        if (bf)
+            GO(64, true, 4);
+        else
+            GO(64, false, 4);
+    } else if (a.tile_rows == 256) {
+        if (bf)
+            GO(128, true, 8);
+        else
+            GO(128, false, 8);
     } else {
-        if (bf) {
-            GO(128, true)
-        } else {
-            GO(128, false)
-        }
+        if (bf)
+            GO(128, true, 4);
+        else
+            GO(128, false, 4);
     }
 #undef GO
     return launch_check("oco_cache_attention (prompt)");
