@@ -488,8 +488,8 @@ struct AttentionPlan {
     uint64_t grid;                    // workgroups per head
     uint64_t bytes;
 };
-// The tiles' split along the tokens.
-static AttentionPlan attention_split(const oco_cache *p, uint32_t tile, uint64_t rows, uint32_t chunk, bool starts) {
+// The tiles' split along the tokens (split: chunks of a prompt's tiles; chunk: their tokens, if not 0).
+static AttentionPlan attention_split(const oco_cache *p, uint32_t tile, uint64_t rows, uint32_t split, uint32_t chunk, bool starts) {
     AttentionPlan l;
     l.tile = tile;
     l.tiles = (uint32_t)((rows + 16 * tile - 1) / (16 * tile));
@@ -500,15 +500,16 @@ static AttentionPlan attention_split(const oco_cache *p, uint32_t tile, uint64_t
     const uint64_t blocks = (uint64_t)p->sequences * p->kv_heads * l.tiles;
     const bool prompt = tile >= 8;
     // Chunks at most and their tokens at least: twelve workgroups of few rows per compute unit, of at least two steps per
-    // wavefront (one sequence of 4101: 256 tokens 8.5 us, 384 9.1, 512 9.7), two of a prompt's tiles.
-    const uint64_t wanted = 256 * (prompt ? 2 : 12);
-    uint64_t chunks = blocks ? (wanted + blocks - 1) / blocks : 1;
-    const uint64_t least = prompt ? 512 : 256;
-    uint64_t most = (seen + least - 1) / least;
-    // what the chunks write and the join reads, in proportion to the rows: 16 MB at most
-    const uint64_t part = (uint64_t)p->rows * p->heads * (p->head_dim + 2) * 4;
-    if (part && (16ull << 20) / part < most) most = (16ull << 20) / part;
-    if (chunks > most) chunks = most;
+    // wavefront (one sequence of 4101: 256 tokens 8.5 us, 384 9.1, 512 9.7).
+    uint64_t chunks = split;
+    if (!prompt) {
+        chunks = blocks ? (12 * 256 + blocks - 1) / blocks : 1;
+        uint64_t most = (seen + 255) / 256;
+        // what the chunks write and the join reads, in proportion to the rows: 16 MB at most
+        const uint64_t part = (uint64_t)p->rows * p->heads * (p->head_dim + 2) * 4;
+        if (part && (16ull << 20) / part < most) most = (16ull << 20) / part;
+        if (chunks > most) chunks = most;
+    }
     // Whole where the join costs more than a split saves (us, split / whole, 128 wide, tokens x tiles: 505 x 8 8.8 / 6.7, 755 x 8
     // 8.5 / 8.2, 1005 x 8 8.4 / 9.6; 505 x 256 12.2 / 7.9, 1255 x 256 15.8 / 13.1, 3005 x 256 28.6 / 29.8; 3005 x 512 47.8 /
     // 41.6; up to 2005 x 256 17.2 / 18.0; 256 wide 755 x 32 10.0 / 11.1, 1255 x 128 19.4 / 16.6;
@@ -578,9 +579,23 @@ static AttentionPlan attention_plan(const oco_cache *p, bool starts) {
     const uint64_t total = (uint64_t)p->rows * (p->heads / p->kv_heads);  // of all sequences
     const bool wide_tiles = p->head_dim == 128 && p->sequences <= 2 && (p->window == 0 || p->window >= p->max_length);
     if (narrow && rows >= 128 && (total / 64 + p->sequences) * p->kv_heads >= 512) tile = wide_tiles && total / 256 * p->kv_heads >= 512 ? 16 : 8;
+    // Fewer tiles of 128 than compute units over a long context: chunks of them until the card's 512 places are full or
+    // nearly so, of 1536 tokens at least.  us, tiles of 32 / so: 512 rows of 32 heads after 8000 tokens (4 chunks) 109 / 92, 256
+    // after 16000 (8) 118 / 88, 128 after 32000 (16) 126 / 86, 700 after 16000 (5) 314 / 242, 4 of 128 after 8000 (4) 105 / 93;
+    // 512 after 2000 35 / 47.
+    uint32_t split = 1;
+    const uint64_t alike = (rows + 127) / 128 * heads, half = (total / 64 + p->sequences) * p->kv_heads / 2, estimate = alike < half ? alike : half;
+    const uint64_t reach = p->window ? (p->window < p->max_length ? p->window : p->max_length) : p->max_length;
+    if (narrow && rows >= 128 && estimate < 256) {
+        while (split < 64 && 20 * split * estimate < 17 * ((split * estimate + 511) / 512) * 512) split++;
+        if (reach / split >= 1536)
+            tile = 8;
+        else
+            split = 1;
+    }
     if (set && (knob[0] == 1 || knob[0] == 2 || ((knob[0] == 3 || knob[0] == 8) && narrow) || (knob[0] == 16 && p->head_dim == 128))) tile = (uint32_t)knob[0];
     const uint32_t chunk = set > 1 && knob[1] > 0 && knob[1] % 128 == 0 ? (uint32_t)knob[1] : 0;
-    return attention_split(p, tile, rows, chunk, starts);
+    return attention_split(p, tile, rows, split, chunk, starts);
 }
 
 template <uint32_t D, bool BF>

@@ -523,3 +523,16 @@ def test_chunks_in_a_graph(lib):
         c.call()
         lib.synchronize()
         np.testing.assert_array_equal(got, c.out.read(np.uint8))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows,lengths,window", [([40], [6500], 0), ([70, 0, 33], [3500, 10, 3300], 0), ([35], [6000], 4000)])
+def test_prompt_chunks_after_long_contexts(lib, d, rows, lengths, window):
+    """A chunk of a prompt after a long context, which is split along its tokens."""
+    rng = np.random.default_rng(d + sum(rows))
+    say("prompt chunks", d, rows, lengths, window)
+    c = Case(lib, rng, rows, lengths, 4, 1, d, 32, "bf16", window=window, sinks=True, extra_rows=1)
+    assert c.need
+    c.call()
+    lib.synchronize()
+    c.check()
