@@ -513,8 +513,9 @@ static AttentionPlan attention_split(const oco_cache *p, uint32_t tile, uint64_t
     // Whole where the join costs more than a split saves (us, split / whole, 128 wide, tokens x tiles: 505 x 8 8.8 / 6.7, 755 x 8
     // 8.5 / 8.2, 1005 x 8 8.4 / 9.6; 505 x 256 12.2 / 7.9, 1255 x 256 15.8 / 13.1, 3005 x 256 28.6 / 29.8; 3005 x 512 47.8 /
     // 41.6; up to 2005 x 256 17.2 / 18.0; 256 wide 755 x 32 10.0 / 11.1, 1255 x 128 19.4 / 16.6;
-    // up to 8005 x 1024 128 / 153, up to 4005 x 2048 164 / 138)
-    const uint64_t whole = blocks < 512 ? 6 * blocks : blocks < 1024 ? 6 * 512 : 3 * (blocks < 4096 ? blocks : 4096);
+    // up to 8005 x 1024 128 / 153, up to 4005 x 2048 164 / 138; tiles of 32 rows, which join more, 1304 x 104 19.7 / 16.5, 2200 x 200
+    // 31.1 / 23.9, 2505 x 256 37.5 / 30.8, up to 2505 x 256 26.6 / 28.5)
+    const uint64_t several = (tile == 1 ? 6 : 12) * blocks, whole = blocks < 1024 ? (several < 6 * 512 ? several : 6 * 512) : 3 * (blocks < 4096 ? blocks : 4096);
     if (!prompt && seen <= (whole > 768 ? whole : p->head_dim > 128 ? 512 : 768)) chunks = 1;
     if (chunks < 1) chunks = 1;
     l.chunk = chunk ? chunk : (uint32_t)(((seen + chunks - 1) / chunks + 127) / 128 * 128);
