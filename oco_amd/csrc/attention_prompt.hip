@@ -210,6 +210,8 @@ __global__ __launch_bounds__(64 * W, 2) void attention_prompt_kernel(AttentionAr
         }
         __syncthreads();
         scores(sc);
+        // step 0 converts the keys of step 2 over those that every wavefront has just read
+        if constexpr (SUBS == 1) __syncthreads();
     }
     // step, its scores, where the next step's go, its buffer's number and place, its place in the buffer
     auto compute = [&](const uint32_t step, f32x16 *sc, f32x16 *next, const uint32_t number, const uint32_t buffer, const int sub) {

@@ -536,3 +536,32 @@ def test_prompt_chunks_after_long_contexts(lib, d, rows, lengths, window):
     c.call()
     lib.synchronize()
     c.check()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows,lengths,window,chunk", [([200], [460], 0, 0), ([130, 0, 150], [330, 5, 500], 0, 0), ([150], [900], 300, 0), ([140], [1500], 0, 256)])
+def test_first_step_of_every_wavefront(lib, d, rows, lengths, window, chunk):
+    """Tiles of 128 rows, where the third step's keys take the place of the first one's: of a tile's or chunk's tokens the
+    first 64 have other keys than all others, so that a wavefront that met them late would give them other weights."""
+    rng = np.random.default_rng(d + sum(rows))
+    with lib.overridden(lib.Knob.ATTENTION, (8, chunk)):
+        c = Case(lib, rng, rows, lengths, 32, 4, d, 16, "bf16", window=window, q_scale=4.0)
+        side = np.sign(rng.normal(size=d))
+        for s, n in enumerate(lengths):
+            k = rng.normal(size=(n, 4, d)) * 0.5 + np.where(np.arange(n) % 256 < 64, 1.0, -1.0)[:, None, None] * side
+            v = rng.normal(size=(n, 4, d)) + np.where(np.arange(n) % 256 < 64, 4.0, -4.0)[:, None, None]
+            k, v = quantize(k), quantize(v)
+            for t in range(n):
+                page, slot = c.b.place(s, t)
+                for j in range(4):
+                    c.pool.put(page, slot, j, (k[0][t, j], k[1][t, j]), (v[0][t, j], v[1][t, j]))
+            c.k[s], c.v[s] = dequantize(*k), dequantize(*v)
+        c.dev[1].upload(c.pool.bytes)
+        first = None
+        for _ in range(3):
+            say("first step", d, rows, lengths, window, chunk)
+            c.call()
+            lib.synchronize()
+            got = c.check()
+            first = got if first is None else first
+            np.testing.assert_array_equal(got, first)
