@@ -139,7 +139,8 @@ __global__ __launch_bounds__(256, D * R == 64 ? 4 : D * R == 128 ? 3 : 2) void a
     const uint32_t *const table = a.b.table + (uint64_t)s * a.b.table_stride;
     uint32_t t0 = first + 32 * wave, step = 0;
     Halves halves = load_halves(table, t0, 128, end, a.b.page_size);
-    // the rows' positions (-1: no token, and no row)
+    // the rows' positions (-1: no token). A lane without a row is the last row once more, and is not written: such lanes take
+    // part in the votes on the maxima, and a row of another tile may already be the result where that takes the queries' place.
     int32_t at[R];
     constexpr bool SHARED = R > 1;  // the queries in LDS, by fragment
     constexpr int QF = SHARED ? R * KW * 64 : 1, OF = 4 * NT * 64;
@@ -147,10 +148,8 @@ __global__ __launch_bounds__(256, D * R == 64 ? 4 : D * R == 128 ? 3 : 2) void a
     u32x4 q[R][SHARED ? 1 : KW];
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        const uint32_t i = row0 + 16 * r + n;
-        const bool live = i < rows;
-        const uint32_t token = live ? i / a.group : 0, head = h * a.group + (live ? i % a.group : 0);
-        at[r] = live ? (int32_t)(span.length + token) - (int32_t)span.rows : -1;
+        const uint32_t i = min(row0 + 16 * r + n, rows - 1), token = i / a.group, head = h * a.group + i % a.group;
+        at[r] = (int32_t)(span.length + token) - (int32_t)span.rows;
         const uint16_t *const row = (const uint16_t *)a.q + (uint64_t)(span.first + token) * a.q_stride + (uint64_t)head * D + g * (D / 4);
         if constexpr (SHARED) {
             if (r == (int)wave)

@@ -56,11 +56,12 @@ __global__ __launch_bounds__(64 * W, 2) void attention_prompt_kernel(AttentionAr
     const uint32_t head_bytes = cache_head_bytes(a.b.page_size, D);
     const uint32_t *const table = a.b.table + (uint64_t)s * a.b.table_stride;
 
-    // this lane's row
-    const uint32_t row0 = range.first_row + 32 * wave, i0 = row0 + n;
-    const bool live = i0 < rows;
-    const uint32_t token = live ? i0 / a.group : 0, head = h * a.group + (live ? i0 % a.group : 0);
-    const int32_t at = live ? before + (int32_t)token : -1;
+    // this lane's row, or the last one once more (as in the kernel for few rows)
+    const uint32_t row0 = range.first_row + 32 * wave;
+    const bool live = row0 + n < rows;
+    const uint32_t i0 = live ? row0 + n : rows - 1;
+    const uint32_t token = i0 / a.group, head = h * a.group + i0 % a.group;
+    const int32_t at = before + (int32_t)token;
     const int32_t least = before + (int32_t)(row0 / a.group), most = before + (int32_t)((min(row0 + 32, rows) - 1) / a.group);
     u32x4 q[NS];
     {

@@ -565,3 +565,22 @@ def test_first_step_of_every_wavefront(lib, d, rows, lengths, window, chunk):
             got = c.check()
             first = got if first is None else first
             np.testing.assert_array_equal(got, first)
+
+
+@pytest.mark.parametrize("tile,d,rows", [(1, 64, 20), (2, 64, 40), (2, 256, 40), (3, 128, 52), (8, 64, 132), (8, 128, 132), (16, 128, 260)])
+def test_rows_of_a_tile_that_is_not_full(lib, tile, d, rows):
+    """The lanes without a row take nothing from other rows, which may be written meanwhile where the result takes the queries'
+    place: whatever a sequence's first query is, the rows of its last tile have the same bits."""
+    rng = np.random.default_rng(d + rows)
+    with lib.overridden(lib.Knob.ATTENTION, (tile,)):
+        c = Case(lib, rng, [rows], [1200], 2, 2, d, 16, "bf16")
+        raw, last, got = c.dev[0].download(np.uint16).reshape(rows, 2 * d), rows // (16 * tile) * 16 * tile, []
+        for scale in (0.0, 50.0):
+            first = stored(np.random.default_rng(1).normal(size=2 * d) * scale, "bf16")
+            raw[0], c.q[0] = first[0].view(np.uint16), first[1].reshape(2, d)
+            c.dev[0].upload(raw)
+            say("first query", tile, d, scale)
+            c.call()
+            lib.synchronize()
+            got.append(c.check()[last:])
+        np.testing.assert_array_equal(*got)
