@@ -722,13 +722,13 @@ int oco_cache_read(const void *pages, const uint32_t *table, const uint32_t *sta
  * (its own position and before, within the window) of scale * q[r][h] . key_t,
  * of head h / (heads / kv_heads).  sinks: f32 [heads], one more score per head
  * that takes part in the sum and has no value, or NULL.  A row that sees
- * nothing is 0; what it does not see (a NaN among it) has no effect on it; a
- * page that is not in the pool reads as NaN, and so does, in f16, a block with
- * a scale past 2^13 (append gives it values past 65504 alone).  q and out are
- * bf16 or f16; the probabilities are rounded to that type, sums are f32.  out
- * may be q where their strides agree.  How the tokens are split over
- * workgroups, and with it the roundings, goes by the whole batch; the same
- * call gives the same bits.
+ * nothing is 0, one whose scores are all -Inf is NaN; what a row does not see
+ * (a NaN among it) has no effect on it; a page that is not in the pool reads as
+ * NaN, and so does, in f16, a block with a scale past 2^13 (append gives it
+ * values past 65504 alone).  q and out are bf16 or f16; the probabilities are
+ * rounded to that type, sums are f32.  out may be q where their strides agree.
+ * How the tokens are split over workgroups, and with it the roundings, goes by
+ * the whole batch; the same call gives the same bits.
  *   workspace: oco_cache_attention_workspace bytes (0 for a description that is
  *   refused, and where none is needed), 16-byte aligned; calls sharing one must be ordered */
 uint64_t oco_cache_attention_workspace(const oco_cache *p);

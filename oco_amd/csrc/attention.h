@@ -271,6 +271,12 @@ __device__ __forceinline__ AttentionTile attention_tile(const CacheSpan &s, uint
 // exp2 of m - to, 0 for m = -Inf whatever `to` is (NaN for a sink that is NaN).
 __device__ __forceinline__ float carry(float m, float to) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to); }
 
+// part / total. A total of 0 is a row that sees nothing (0), or whose scores are all -Inf and have no softmax (NaN): a finite
+// one makes it 1 or nearly so at least.
+__device__ __forceinline__ float part_of(float part, float total, bool sees) {
+    return total > 0.f || total != total ? part / total : sees ? __uint_as_float(0x7fc00000u) : 0.f;
+}
+
 // Prompts (attention_prompt.hip; heads of 64 and 128), in tiles of 128 rows, or of 256 where heads are 128 wide.
 int attention_prompt_launch(const AttentionArgs &a, uint32_t head_dim, bool bf, uint32_t tiles, uint32_t grid, hipStream_t stream);
 

@@ -380,7 +380,7 @@ __global__ __launch_bounds__(256, D * R == 64 ? 4 : D * R == 128 ? 3 : 2) void a
                 end_top = fmaxf(top, sink);
                 total = total * carry(top, end_top) + carry(sink, end_top);
             }
-            const float by = total > 0.f || total != total ? carry(top, end_top) / total : 0.f;
+            const float by = part_of(carry(top, end_top), total, at[r] >= 0);
             uint16_t *const out = (uint16_t *)a.out + (uint64_t)row * a.out_stride + (uint64_t)head * D + column;
 #pragma unroll
             for (int j = 0; j < NT / 4; j++)
@@ -426,6 +426,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
     if (row - span.first >= span.rows) return;
     const AttentionTile range = attention_tile(span, ((row - span.first) * a.group + head % a.group) / a.tile_rows, a.tile_rows, a.group, a.window);
     const uint32_t used = range.end > range.first ? (range.end - range.first + size - 1) / size : 0;
+    const bool sees = span.length + (row - span.first) >= span.rows;
     const float sink = a.sinks ? a.sinks[head] * 1.44269504088896341f : -INFINITY;
     float top = sink;
     if ((threadIdx.x & 63) < used) top = fmaxf(top, tops[0]);
@@ -452,7 +453,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
     uint16_t *const out = (uint16_t *)a.out + (uint64_t)row * a.out_stride + (uint64_t)head * D;
     if constexpr (W == 1) {
         total = (GROUPS == 4 ? row_sum(total) : half_sum(total)) + carry(sink, top);
-        const float f = total > 0.f || total != total ? 1.f / total : 0.f;
+        const float f = part_of(1.f, total, sees);
 #pragma unroll
         for (uint32_t j = 0; j < V; j++) {
 #pragma unroll
@@ -474,7 +475,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
             sum += so[i][threadIdx.x];
             total += st[i];
         }
-        const float f = total > 0.f || total != total ? 1.f / total : 0.f;
+        const float f = part_of(1.f, total, sees);
         *(GLOBAL u32x2_u *)gp(out + 4 * threadIdx.x) = u32x2_u{Half<BF>::pack(sum[0] * f, sum[1] * f), Half<BF>::pack(sum[2] * f, sum[3] * f)};
     }
 }

@@ -368,7 +368,7 @@ __global__ __launch_bounds__(64 * W, 2) void attention_prompt_kernel(AttentionAr
             top = fmaxf(m, sink);
             total = l * carry(m, top) + carry(sink, top);
         }
-        by = total > 0.f || total != total ? carry(m, top) / total : 0.f;
+        by = part_of(carry(m, top), total, at >= 0);
     }
     // accumulator row 16 c + m is column PIECE m + c: a lane has all columns of a piece
 #pragma unroll

@@ -584,3 +584,37 @@ def test_rows_of_a_tile_that_is_not_full(lib, tile, d, rows):
             lib.synchronize()
             got.append(c.check()[last:])
         np.testing.assert_array_equal(*got)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows,lengths", [([1, 2], [3000, 2]), ([45, 3], [50, 1]), ([300], [300])])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_scores_that_are_all_minus_infinity(kernel, lib, d, rows, lengths, sinks):
+    """Such a row has no softmax and is NaN, or 0 where a sink takes all the weight; a row that sees nothing is 0 either way."""
+    rng = np.random.default_rng(d + sum(rows))
+    c = Case(lib, rng, rows, lengths, 4, 2, d, 16, "bf16", sinks=sinks)
+    for s, n in enumerate(lengths):  # keys that are positive in column 3
+        k = np.abs(c.k[s])
+        k[:, :, 3] = 1.0 + (k[:, :, 3] > 1)
+        ck, cv = quantize(k), quantize(c.v[s])
+        for t in range(n):
+            page, slot = c.b.place(s, t)
+            for j in range(2):
+                c.pool.put(page, slot, j, (ck[0][t, j], ck[1][t, j]), (cv[0][t, j], cv[1][t, j]))
+        c.k[s], c.v[s] = dequantize(*ck), dequantize(*cv)
+        assert (c.k[s][:, :, 3] > 0).all()
+    c.dev[1].upload(c.pool.bytes)
+    raw = c.dev[0].download(np.uint16).reshape(c.b.total, 4, d)
+    for r in (0, sum(rows) - 1):
+        raw[r, 1], raw[r, 1, 3] = 0, 0xFF80
+        c.q[r, 1], c.q[r, 1, 3] = 0.0, -np.inf
+    c.dev[0].upload(raw)
+    say("minus infinity", d, rows, sinks)
+    c.call()
+    lib.synchronize()
+    got = c.check()
+    want = np.zeros(got.shape[:2], bool)
+    want[0, 1] = want[-1, 1] = not sinks
+    np.testing.assert_array_equal(np.isnan(got).all(-1), want)
+    if sinks:
+        assert not got[0, 1].any() and not got[-1, 1].any()
