@@ -1005,27 +1005,39 @@ class CacheBatch:
     def append(self, k, v, q=None, q_out=None, positions=None, rotation=None, stride: int = 0, stream=None):
         """Keys (turned) and values into the pages, queries turned into q_out (q
         by default).  stride: between the rows of q, k and v where they lie
-        together, as one product writes them (q_out's stay head after head)."""
+        together, as one product writes them; q_out's stay head after head,
+        unless it is q."""
         p = self.p
         if stride:
             p = Cache.from_buffer_copy(p)
             p.k_stride = p.v_stride = stride
-            p.q_stride = stride if q is not None else 0
+            if q is not None:
+                p.q_stride = stride
+                if q_out is None or _addr(q_out) == _addr(q):
+                    p.out_stride = stride
         cache_append(self.cache.buffer, self.table, self.lengths, k, v, p, self.starts, q, q_out, positions, rotation, stream)
 
     def read(self, k, v, stream=None):
         """The rows' keys and values as the pages hold them."""
         cache_read(self.cache.buffer, self.table, self.lengths, k, v, self.p, self.starts, stream)
 
-    def attention(self, q, out, sinks=None, workspace=None, stream=None):
+    def attention(self, q, out, sinks=None, workspace=None, stream=None, stride: int = 0):
         """Causal attention of the rows.  Without a `workspace` (a DeviceBuffer
         of workspace_bytes()) a Stream keeps one, and the batch one for each
         stream that is given by its handle and for the default one; reserve()
-        draws it before a capture."""
+        draws it before a capture.  stride: between q's rows where they were
+        turned in their place among keys and values (out's stay head after
+        head, unless it is q)."""
         need = self.workspace_bytes()
         if need and workspace is None:
             workspace = self._scratch(stream).at_least(need)
-        cache_attention(q, self.cache.buffer, self.table, self.lengths, out, self.p, self.starts, sinks, workspace if need else None,
+        p = self.p
+        if stride:
+            p = Cache.from_buffer_copy(p)
+            p.q_stride = stride
+            if _addr(out) == _addr(q):
+                p.out_stride = stride
+        cache_attention(q, self.cache.buffer, self.table, self.lengths, out, p, self.starts, sinks, workspace if need else None,
                         workspace.nbytes if need else 0, stream)
 
     def workspace_bytes(self) -> int:

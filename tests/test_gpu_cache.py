@@ -270,3 +270,40 @@ def test_read(lib, dtype, d):
     np.testing.assert_array_equal(got_v.reshape(vals.shape), stored(vals, dtype)[1])
     tail = v.read(np.uint8).reshape(c.b.total, -1)[len(live):]
     assert np.all(np.ascontiguousarray(tail).reshape(-1).view(np.uint32) == 0x7FC12345)
+
+
+@pytest.mark.parametrize("named", [False, True])
+def test_append_packed_queries_in_place(lib, named):
+    """Queries turned where they lie, between the keys and values of one product's rows, through PagedCache: those turned into
+    rows of their own, and nothing else of the product changes; the attention reads them there, and may leave its rows there."""
+    rng = np.random.default_rng(3)
+    heads, kv, d, P, rows, lengths = 6, 2, 64, 16, [3, 1], [3, 1]
+    b, width = Batch(rng, rows, lengths, P), (heads + 2 * kv) * d + 6
+    raw, _ = stored(rng.normal(size=(b.total, width)), "bf16")
+    keep = []
+    r = rotation(lib, 100.0 ** (-np.arange(d // 2) * 2.0 / d), 1.0, d, False, keep)
+    table, lens, starts, apart = dev(lib, b.table), dev(lib, np.array(lengths, np.uint32)), dev(lib, b.starts), Guarded(lib, b.total * heads * d * 2)
+    pages, product = [], dev(lib, raw)
+    for place in (apart.ptr, product.ptr if named else None):
+        cache = lib.PagedCache(b.pages, d, kv, P)
+        cache.buffer.fill32(0)
+        batch = cache.batch(table, lens, len(rows), b.total, max(rows), max(lengths), b.stride, heads, starts=starts)
+        say("packed", named, place is None)
+        batch.append(product.ptr + heads * d * 2, product.ptr + (heads + kv) * d * 2, q=product.ptr, q_out=place, rotation=r, stride=width)
+        lib.synchronize()
+        pages.append(cache.buffer.download(np.uint8))
+    np.testing.assert_array_equal(*pages)
+    after = product.download(np.uint16).reshape(b.total, width)
+    np.testing.assert_array_equal(after[:, :heads * d], apart.read(np.uint16).reshape(b.total, heads * d))
+    np.testing.assert_array_equal(after[:, heads * d:], raw.view(np.uint16).reshape(b.total, width)[:, heads * d:])
+    out = [Guarded(lib, b.total * heads * d * 2) for _ in range(2)]
+    say("packed attention", named)
+    batch.attention(apart.ptr, out[0].ptr)
+    batch.attention(product, out[1].ptr, stride=width)
+    batch.attention(product.ptr, product, stride=width)
+    lib.synchronize()
+    want = out[0].read(np.uint16).reshape(b.total, heads * d)
+    np.testing.assert_array_equal(out[1].read(np.uint16).reshape(b.total, heads * d), want)
+    again = product.download(np.uint16).reshape(b.total, width)
+    np.testing.assert_array_equal(again[:, :heads * d], want)
+    np.testing.assert_array_equal(again[:, heads * d:], after[:, heads * d:])
