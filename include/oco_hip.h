@@ -630,8 +630,8 @@ int oco_draft_verify(const void *target, const void *draft, const uint32_t *draf
  * `dim` values (dim even) is (j, j + dim / 2) in halves or (2j, 2j + 1)
  * interleaved, and turns by position * frequencies[j] radians:
  *   a' = a cos - b sin,  b' = b cos + a sin,  both times magnitude,
- * angles, functions and products in 64 bits, rounded to the type once.  Values
- * from dim on stay.
+ * angles, functions and products in 64 bits, rounded to f32 and that to the
+ * type.  Values from dim on stay.
  *   frequencies: f64 [dim / 2] on the device (oco_rotation_frequencies) */
 typedef enum oco_rotation_layout { OCO_ROTATION_HALF = 0, OCO_ROTATION_INTERLEAVED = 1 } oco_rotation_layout;
 #define OCO_ROTATION_DIM 1024u

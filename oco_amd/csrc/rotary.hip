@@ -4,10 +4,11 @@
 // Angles are position * frequency in 64 bits, at most 2^-53 of themselves off
 // (1e-10 at a million radians, where f32 would be off by 0.06), their cosines
 // and sines by Taylor series on a quarter turn, and the products are 64-bit
-// too: a key next to a border between two codes falls where the exact one
-// does.  One token's pairs are the same for all its heads, so a wavefront
-// takes a token, or a part of its heads, keeps them in LDS and waits for no
-// other.
+// too.  They are rounded to f32 and from there to the type, so that a key next
+// to a border between two codes falls where the exact one does unless it is
+// within half a step of f32 of a middle between two numbers of the type.  One
+// token's pairs are the same for all its heads, so a wavefront takes a token,
+// or a part of its heads, keeps them in LDS and waits for no other.
 //
 // Bound by memory where there are many rows (8192 rows of 32 heads of 128 f16
 // 24 us, 5.6 TB/s; 8192 tokens of 32 + 2 * 8 heads appended 37 us, 4.5 TB/s,
