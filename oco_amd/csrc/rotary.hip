@@ -11,7 +11,7 @@
 // or a part of its heads, keeps them in LDS and waits for no other.
 //
 // Bound by memory where there are many rows (8192 rows of 32 heads of 128 f16
-// 24 us, 5.6 TB/s; 8192 tokens of 32 + 2 * 8 heads appended 37 us, 4.5 TB/s,
+// 22.6 us, 5.9 TB/s; 8192 tokens of 32 + 2 * 8 heads appended 37 us, 4.5 TB/s,
 // and read back 8.5), and by the loads that wait for each other where there are
 // few (a row 2.2 us, 64 tokens appended 6.0 and read back 3.1).
 #include "cache.h"
@@ -117,10 +117,14 @@ __device__ __forceinline__ void load_unit_tail(Unit &x, const T *head, const Uni
     load_run(head, p.first, p.pairs ? r.dim / 2 : p.turns ? r.dim : head_dim, x.a);
     if (p.pairs) load_run(head + r.dim / 2, p.first, r.dim / 2, x.b);
 }
+// To f32; the type's conversion is the second rounding, kept apart from the first by the empty statement: for a pair in eight
+// of f16 the compiler made one of the two, in integer code (8192 rows of 32 x 128 f16, half turned, 24.2 us, so 22.6; about
+// 1300 tokens of 64 wide heads appended and read back 13.0, 12.4).
 __device__ __forceinline__ void turn_pair(float &x, float &y, const double2 &t) {
     const double v = x, w = y;
     x = (float)__builtin_fma(v, t.x, -(w * t.y));
     y = (float)__builtin_fma(w, t.x, v * t.y);
+    asm("" : "+v"(x), "+v"(y));
 }
 template <bool INTERLEAVED, bool WHOLE>
 __device__ __forceinline__ void turn_unit(Unit &x, const UnitPlace &p, const Rotation &r, const double2 *table) {

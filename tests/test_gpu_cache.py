@@ -307,3 +307,22 @@ def test_append_packed_queries_in_place(lib, named):
     again = product.download(np.uint16).reshape(b.total, width)
     np.testing.assert_array_equal(again[:, :heads * d], want)
     np.testing.assert_array_equal(again[:, heads * d:], after[:, heads * d:])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim", [64, 50])
+def test_roundings_by_way_of_f32(lib, dtype, interleaved, dim):
+    """Products next to the middle between two numbers of the type, nearer to it than f32 tells apart, go where the middle goes: to
+    the even number. In f32 itself they go to the nearer one."""
+    half, tiny, d = HALF[dtype], 2.0 ** -45, 64
+    raw, x = stored(np.ldexp(1.0, np.arange(d) % 24 - 12) * np.where(np.arange(d) % 3, 1, -1), dtype)
+    once = dtype == "f32"
+    for factor, want in ((1 + half + tiny, 1 + 2 * half if once else 1.0), (1 + half - tiny, 1.0), (1 + 3 * half - tiny, 1 + 2 * half if once else 1 + 4 * half),
+                         (1 + 3 * half + tiny, 1 + 4 * half)):
+        keep, out = [], Guarded(lib, raw.nbytes)
+        say("roundings", dtype, interleaved, factor)
+        lib.rotate(dev(lib, raw), 1, 1, d, out.ptr, rotation(lib, np.zeros(dim // 2), factor, dim, interleaved, keep), dev(lib, np.array([7], np.uint32)),
+                   CODE[dtype])
+        lib.synchronize()
+        np.testing.assert_array_equal(values(out.read(np.uint8), dtype, (d,)), np.where(np.arange(d) < dim, x * want, x))
