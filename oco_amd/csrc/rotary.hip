@@ -52,7 +52,11 @@ struct Rotation {
     uint32_t dim;
 };
 
-// The pairs' cosines and sines of one position, by one wavefront for itself: what it writes to LDS it reads in order.
+// Between what a wavefront's lanes write to LDS and what other lanes of it read there. LDS takes a wavefront's accesses in
+// order; this keeps the compiler from moving them past each other, and is no instruction.
+__device__ __forceinline__ void lanes_wrote() { __builtin_amdgcn_wave_barrier(); }
+
+// The pairs' cosines and sines of one position, by one wavefront for itself.
 struct Angles {
     double first;  // a lane's first frequency, which can be read before the position is known
     __device__ __forceinline__ Angles(const Rotation &r) {
@@ -197,6 +201,7 @@ __device__ __forceinline__ bool turn_heads(uint32_t first, uint32_t step, uint32
             }
             if (first_time && !make_table()) return false;
             first_time = false;
+            lanes_wrote();  // in every turn: behind the condition, the same statement costs 22 spilled scalars and 2% of a prompt
 #pragma unroll
             for (int k = 0; k < N; k++) {
                 if (now.head < heads) {
@@ -212,6 +217,7 @@ __device__ __forceinline__ bool turn_heads(uint32_t first, uint32_t step, uint32
         } while (__any(now.head < heads));
     } else {
         if (!make_table()) return false;
+        lanes_wrote();
         for (; now.head < heads; now.advance(dh, du, n)) {
             const UnitPlace p = unit_place<INTERLEAVED>(now.unit, n, r);
             Unit x;
@@ -346,6 +352,7 @@ __global__ __launch_bounds__(256, 4) void append_kernel(AppendArgs a) {
             store_unit_tail<T>(keys + c.head * D, x, p, a.r, D);
         }
     }
+    lanes_wrote();  // the turned keys
     const uint32_t head_bytes = cache_head_bytes(a.b.page_size, D);
     uint8_t *const head = a.cache + ((uint64_t)page * a.b.kv_heads + h0) * head_bytes;
     // blocks of four words stay in four adjacent lanes
