@@ -618,3 +618,36 @@ def test_scores_that_are_all_minus_infinity(kernel, lib, d, rows, lengths, sinks
     np.testing.assert_array_equal(np.isnan(got).all(-1), want)
     if sinks:
         assert not got[0, 1].any() and not got[-1, 1].any()
+
+
+@pytest.mark.parametrize("sequences,d,group,kv,rows,longest,window",
+                         [(2, 64, 8, 2, 2, 45000, 0), (40, 128, 4, 2, 1, 8000, 2100), (20, 128, 8, 2, 3, 5000, 0), (64, 256, 4, 2, 2, 8000, 0), (64, 128, 8, 1, 5, 13000, 0),
+                          (65, 64, 8, 1, 2, 4000, 0), (65, 64, 8, 1, 5, 4000, 1500), (200, 128, 4, 1, 1, 8000, 0),  # tiles of 16 rows, four sequences per lane
+                          (100, 128, 8, 2, 3, 4096, 0), (130, 256, 8, 1, 3, 6000, 0), (200, 64, 8, 1, 3, 8000, 0), (65, 64, 8, 2, 9, 4000, 0),  # of 32
+                          (130, 128, 8, 1, 5, 6000, 0), (200, 64, 8, 2, 5, 8000, 0), (256, 64, 8, 1, 5, 8000, 0)])  # of 48
+def test_chunks_are_by_the_lengths(lib, sequences, d, group, kv, rows, longest, window):
+    """As the two tests above, at bounds where the tokens are split for certain: the workspace says so, and says that the kernel
+    sized the chunks itself. Sequences without rows and without tokens lie among a lane's four."""
+    rng = np.random.default_rng(d + sequences + rows)
+    n, lengths = rng.integers(1, rows + 1, sequences), rng.integers(rows, 90, sequences)
+    for i in rng.integers(0, sequences, min(sequences, 3)):
+        n[i], lengths[i] = rows, min(3000, longest - 3)
+    if sequences > 4:
+        n[1], n[-2], lengths[sequences // 2] = 0, 0, 0
+        n[5:13] = [0, rows, 0, 0, 0, 0, 0, rows]
+    c = Case(lib, rng, [int(i) for i in n], [int(i) for i in lengths], group * kv, kv, d, 16, "bf16", window=window, sinks=True, holes=sequences % 2, max_rows=rows,
+             extra_rows=2)
+    c.p.max_length = longest
+    stride = c.p.max_length // 16 + 1
+    c.p.table_stride = stride
+    c.dev[2] = dev(lib, np.ascontiguousarray(np.pad(c.b.table, ((0, 0), (0, stride - c.b.table.shape[1])))))
+    c.need = lib.cache_attention_workspace(c.p)
+    c.work = Guarded(lib, c.need)
+    say("by the lengths", sequences, d, group, rows)
+    assert c.need
+    c.call()
+    lib.synchronize()
+    size = int(c.work.read(np.uint8)[-16:].view(np.uint32)[0])  # where the join finds it
+    assert 0 < size < max(lengths) and size % 128 == 0
+    c.check()
+    assert np.all(np.ascontiguousarray(c.out.read(np.uint8)[int(n.sum()) * group * kv * d * 2:]).view(np.uint32) == 0x7FC12345)
