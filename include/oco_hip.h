@@ -647,7 +647,9 @@ typedef struct oco_rotation {
  *   LINEAR: all divided by `factor`
  *   YARN:   pairs that turn more than `fast` times over `original` positions
  *           stay, those that turn less than `slow` times are divided by
- *           factor, in between by their place between the two pairs;
+ *           factor, in between by their place between the two pairs, whose
+ *           indexes are rounded down and up (checkpoints that take them as
+ *           they are, gpt-oss among them, bring frequencies of their own);
  *           *magnitude = 0.1 ln(factor) + 1
  *   BANDS:  the same in between by the number of turns itself, and
  *           *magnitude = 1
@@ -677,7 +679,10 @@ int oco_rotate(const void *x, oco_dtype dtype, uint32_t rows, uint32_t heads, ui
  * A block's scale is 2^floor(log2(max |x|)) / 4, at least 2^-126; its codes
  * are x / scale rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4 and 6 (ties
  * to the even code, beyond 6 to 6).  A block with a NaN or an infinity has
- * scale 255 and reads as NaN.
+ * scale 255 and reads as NaN.  Normal values are off by 11% of their root mean
+ * square; attention over 2048 such tokens, with scores of unit deviation, by
+ * 17% of its result's (12% by the keys, 12% by the values), of deviation 2 by
+ * 25% (22% by the keys).
  *
  * Sequence s has rows starts[s] .. starts[s + 1] - 1 of the batch (starts
  * NULL: rows / sequences each), at most max_rows, and lengths[s] tokens (more
@@ -726,9 +731,10 @@ int oco_cache_read(const void *pages, const uint32_t *table, const uint32_t *sta
  * (a NaN among it) has no effect on it; a page that is not in the pool reads as
  * NaN, and so does, in f16, a block with a scale past 2^13 (append gives it
  * values past 65504 alone).  q and out are bf16 or f16; the probabilities are
- * rounded to that type, sums are f32.  out may be q where their strides agree.
- * How the tokens are split over workgroups, and with it the roundings, goes by
- * the whole batch; the same call gives the same bits.
+ * rounded to that type (in f16 those up to 2^-25 of the row's largest may be
+ * 0), sums are f32.  out may be q where their strides agree.  How the tokens
+ * are split over workgroups, and with it the roundings, goes by the whole
+ * batch; the same call gives the same bits.
  *   workspace: oco_cache_attention_workspace bytes (0 for a description that is
  *   refused, and where none is needed), 16-byte aligned; calls sharing one must be ordered */
 uint64_t oco_cache_attention_workspace(const oco_cache *p);
@@ -745,7 +751,9 @@ int oco_cache_attention(const void *q, const void *pages, const uint32_t *table,
  *   v in the row's biases:  x = x + its bias (of several the last one's)
  *   v not in the row's mask:  x = -Inf, whatever it was
  * `group` consecutive rows share a history, penalties and biases, mask_group
- * rows a mask (0: 1).  Ids past the vocabulary are passed over.
+ * rows a mask (0: 1).  Ids past the vocabulary are passed over.  Where the
+ * repetition counts other tokens than frequency and presence do, that is two
+ * calls, the first with frequency and presence 0, the second with repetition 1.
  *   history: u32 [groups][history_stride], history_lengths: u32 [groups] (NULL or more: history_stride)
  *   penalties: f32 [groups][3]: repetition (> 0), frequency, presence; with history
  *   bias_ids: u32 [groups][bias_stride], biases: f32 alike, bias_lengths as history_lengths

@@ -20,10 +20,14 @@
 //
 // Bound by memory for single tokens of many long sequences (32 of up to 16384,
 // 8 heads of 128: 338 MB in 75 us, 4.5 TB/s), by two launches and three loads
-// that wait for each other for one (4101 tokens 8.5 to 9), and by issue where
-// several tiles convert the same codes: per step of 16 rows and 64 columns
-// about 190 vector instructions of 4 clocks beside 128 clocks of products (8
-// sequences of up to 5 rows of 64 heads 20 us; 1700 rows 256 wide 55 us).
+// that wait for each other for one (4101 tokens 8.5 to 9).  A few drafted rows
+// wait half of the time (8 sequences of up to 5 rows of 64 heads of 64 20 us,
+// the join 4.7 of it): a wavefront has four or five steps behind lengths, chunk,
+// table and page, 39% of its time goes by for loads and 31% for its turn to
+// issue, and vector instructions take 18,000 of 37,000 clocks, a quarter of them
+// in the loop conversions and transposes.  Many rows of wide heads are bound by
+// the conversions that each tile makes for itself: per step of 32 rows 290
+// vector instructions beside 64 products (1700 rows 256 wide 56 us).
 #include "attention.h"
 
 namespace oco {
@@ -510,11 +514,14 @@ static AttentionPlan attention_split(const oco_cache *p, uint32_t tile, uint64_t
         if (part && (16ull << 20) / part < most) most = (16ull << 20) / part;
         if (chunks > most) chunks = most;
     }
-    // Whole where the join costs more than a split saves (us, split / whole, 128 wide, tokens x tiles: 505 x 8 8.8 / 6.7, 755 x 8
-    // 8.5 / 8.2, 1005 x 8 8.4 / 9.6; 505 x 256 12.2 / 7.9, 1255 x 256 15.8 / 13.1, 3005 x 256 28.6 / 29.8; 3005 x 512 47.8 /
-    // 41.6; up to 2005 x 256 17.2 / 18.0; 256 wide 755 x 32 10.0 / 11.1, 1255 x 128 19.4 / 16.6;
-    // up to 8005 x 1024 128 / 153, up to 4005 x 2048 164 / 138; tiles of 32 rows, which join more, 1304 x 104 19.7 / 16.5, 2200 x 200
-    // 31.1 / 23.9, 2505 x 256 37.5 / 30.8, up to 2505 x 256 26.6 / 28.5)
+    // Whole where the join costs more than a split saves: up to 6 tokens for each tile of 16 rows, 12 for each larger one, whose
+    // rows the join all reads, but no more than 512 tiles of 16 rows give; from 1024 tiles on, which fill the card by
+    // themselves, 3 for each, up to what 4096 of them give; and 768 tokens, 512 of 256 wide heads, however few tiles there
+    // are.  Fitted to these (us, split / whole, 128 wide, tokens x tiles):
+    // 505 x 8 8.8 / 6.7, 755 x 8 8.5 / 8.2, 1005 x 8 8.4 / 9.6; 505 x 256 12.2 / 7.9, 1255 x 256 15.8 / 13.1, 3005 x 256 28.6 /
+    // 29.8; 3005 x 512 47.8 / 41.6; up to 2005 x 256 17.2 / 18.0; 256 wide 755 x 32 10.0 / 11.1, 1255 x 128 19.4 / 16.6;
+    // up to 8005 x 1024 128 / 153, up to 4005 x 2048 164 / 138; tiles of 32 rows 1304 x 104 19.7 / 16.5, 2200 x 200
+    // 31.1 / 23.9, 2505 x 256 37.5 / 30.8, up to 2505 x 256 26.6 / 28.5.
     const uint64_t several = (tile == 1 ? 6 : 12) * blocks, whole = blocks < 1024 ? (several < 6 * 512 ? several : 6 * 512) : 3 * (blocks < 4096 ? blocks : 4096);
     if (!prompt && seen <= (whole > 768 ? whole : p->head_dim > 128 ? 512 : 768)) chunks = 1;
     if (chunks < 1) chunks = 1;
@@ -569,8 +576,9 @@ static AttentionPlan attention_plan(const oco_cache *p, bool starts) {
     // 4096 x 4 rows over 8192 (512 of 256) 715 / 567 / 376 / 365, 4096 from the start on 147 / 138, 8192 505 / 507, with a window
     // of 2048 252 / 272, 64 wide 328 / 339; 4 sequences of up to 1000 x 4 rows after 3000 142 / 150, 4 of up to 4096 after 4096
     // 1020 / 1047; 256 wide (16 heads) 623 / 443.
-    // Tiles of 16 / 48, 5 x 8 rows: 32 sequences of 4005 tokens, 64 wide 54 / 42, 128 wide 85 / 59, of up to 8192 64 wide 63 / 59,
-    // 128 wide 89 / 76; 8 of up to 8192, 64 wide 20.7 / 21.8; two of 2000 9.3 / 11.6.
+    // Tiles of 16 / 48, 5 x 8 rows: 32 sequences of 4005 tokens, 64 wide 52.6 / 42.3, 128 wide 71 / 56, of up to 8192 64 wide 63 /
+    // 59, 128 wide 89 / 76; 8 of up to 8192, 64 wide 19.9 / 21.8; two of 2005 9.6 / 11.5.  Where rows differ too, 32 sequences of
+    // up to 5 over up to 8192, 64 wide 50 / 54, 128 wide 77 / 69, and tiles of 32 would take 42 and 64.
     int32_t knob[4];
     const int set = plan_override(OCO_KNOB_ATTENTION, knob);
     const bool narrow = p->head_dim <= 128;
