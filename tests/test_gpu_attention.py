@@ -651,3 +651,30 @@ def test_chunks_are_by_the_lengths(lib, sequences, d, group, kv, rows, longest, 
     assert 0 < size < max(lengths) and size % 128 == 0
     c.check()
     assert np.all(np.ascontiguousarray(c.out.read(np.uint8)[int(n.sum()) * group * kv * d * 2:]).view(np.uint32) == 0x7FC12345)
+
+
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("rows,lengths,first", [([50, 1, 1, 2], [120, 900, 0, 1400], 1), ([1, 3, 140], [2000, 3, 200], 2), ([1] * 70 + [30], [90] * 70 + [700], 70)])
+def test_a_batch_in_two_calls(lib, d, rows, lengths, first):
+    """A prompt's rows and single tokens apart: each call has the whole batch's rows and its own sequences' starts, lengths and
+    tables, and leaves the other's rows as they were."""
+    rng = np.random.default_rng(d + len(rows))
+    c = Case(lib, rng, rows, lengths, 8, 2, d, 16, "bf16", sinks=True, extra_rows=2)
+    q, cache, table, lens, starts, sinks = c.dev
+    total, z = int(c.b.starts[-1]), 8 * d * 2
+    for at, n in ((0, first), (first, len(rows) - first)):
+        p = lib.Cache.from_buffer_copy(c.p)
+        p.sequences, p.max_rows, p.max_length = n, max(rows[at:at + n]), max(lengths[at:at + n])
+        need = lib.cache_attention_workspace(p)
+        work = Guarded(lib, need)
+        say("in two", d, rows[:5], at, n)
+        before = c.out.read(np.uint8).copy()
+        lib.cache_attention(q, cache, table.ptr + 4 * at * c.b.stride, lens.ptr + 4 * at, c.out.ptr, p, starts=starts.ptr + 4 * at, sinks=sinks,
+                            workspace=work.ptr if need else None, workspace_bytes=need)
+        lib.synchronize()
+        work.read(np.uint8)
+        after, mine = c.out.read(np.uint8), slice(int(c.b.starts[at]) * z, int(c.b.starts[at + n]) * z)
+        before[mine] = after[mine]
+        np.testing.assert_array_equal(after, before)
+    c.check()
+    assert np.all(np.ascontiguousarray(c.out.read(np.uint8)[total * z:]).view(np.uint32) == 0x7FC12345)
